@@ -1,0 +1,327 @@
+"""The operators at the end of a token-level training step, as they are measured: orthogonalised updates of weight matrices
+(`ssecg.ops.orthogonalize`, `ssecg.optim.FusedMuon`), layer norm with its backward pass (`ssecg.ops.layer_norm_fwd` / `_bwd`)
+and the classifier with softmax cross entropy over a large vocabulary, without the logits (`ssecg.ops.linear_ce_fwd` / `_bwd`).
+
+A case names its operator in ``op``; every case is one training-time pass: forward and backward, or one update.
+"""
+import math
+import os
+import sys
+
+import torch
+
+#: False: the plain form (elementary torch operations in 32 bits); True: the framework's calls.
+own = False
+
+_TYPES = {"fp32": torch.float32, "bf16": torch.bfloat16, "fp16": torch.float16}
+_COEF = (3.4445, -4.7750, 2.0315)   # the quintic of the Newton-Schulz iteration
+_ITERATIONS = 5
+_NORM_EPS = 1e-7
+_LN_EPS = 1e-5
+_LR, _DECAY, _MOMENTUM = 1e-3, 0.05, 0.95
+_THRESH = 0.95                      # confidence threshold of the pseudo-labels
+_IGNORE = -100
+
+#: The 1D ResNet18's convolutions and the head's as the matrices (out channels, in channels x taps) an optimiser sees.
+_RESNET18 = ([(64, 12, 7)] + [(64, 64, 3)] * 4
+             + [(128, 64, 3)] + [(128, 128, 3)] * 3 + [(128, 64, 1)]
+             + [(256, 128, 3)] + [(256, 256, 3)] * 3 + [(256, 128, 1)]
+             + [(512, 256, 3)] + [(512, 512, 3)] * 3 + [(512, 256, 1)]
+             + [(128, 512, 3)])
+
+
+def listed():
+    return [
+        # one filter bank of the first stage: the smallest update, where only latency counts
+        {"name": "ortho 64x192 fp32", "op": "ortho", "shapes": "64x192", "dtype": "fp32"},
+        # the whole optimiser step of the shipped model's convolutions
+        {"name": "muon resnet18 fp32", "op": "muon", "shapes": "resnet18", "dtype": "fp32"},
+        # 16-bit gradients of odd matrices, wide and tall, with a single row among them
+        {"name": "ortho ragged bf16", "op": "ortho", "shapes": "1000x2333,777x129,1x515,515x1", "dtype": "bf16"},
+        # a large square matrix
+        {"name": "ortho 4096x4096 fp32", "op": "ortho", "shapes": "4096x4096", "dtype": "fp32"},
+        # 16 windows of 63 positions with the encoder's 512 channels: the shipped batch size
+        {"name": "ln 1008x512 fp32", "op": "ln", "rows": 1008, "cols": 512, "dtype": "fp32"},
+        # a row that is no multiple of a vector, rows that are no multiple of anything
+        {"name": "ln 4097x777 fp16", "op": "ln", "rows": 4097, "cols": 777, "dtype": "fp16"},
+        # long activations of a wide model
+        {"name": "ln 32768x4096 bf16", "op": "ln", "rows": 32768, "cols": 4096, "dtype": "bf16"},
+        # two windows of 63 positions, a thousand codes
+        {"name": "ce 126x512x1000 fp32", "op": "ce", "rows": 126, "cols": 512, "vocab": 1000, "dtype": "fp32", "bias": True, "gate": False},
+        # a few rows against a whole vocabulary: bound by the weights
+        {"name": "ce 8x1024x32768 fp16", "op": "ce", "rows": 8, "cols": 1024, "vocab": 32768, "dtype": "fp16", "bias": False, "gate": False},
+        # pseudo-labels gated by their confidence, odd in every size
+        {"name": "ce 1999x771x32003 bf16", "op": "ce", "rows": 1999, "cols": 771, "vocab": 32003, "dtype": "bf16", "bias": True, "gate": True},
+        # one record of 2000 samples in 32 bits
+        {"name": "ce 2000x512x8192 fp32", "op": "ce", "rows": 2000, "cols": 512, "vocab": 8192, "dtype": "fp32", "bias": True, "gate": True},
+        # a large batch of tokens
+        {"name": "ce 8192x1024x65536 bf16", "op": "ce", "rows": 8192, "cols": 1024, "vocab": 65536, "dtype": "bf16", "bias": False, "gate": False},
+    ]
+
+
+def _spread(rng, lo, hi):
+    """A whole number of [lo, hi], even over its logarithm."""
+    return min(hi, max(lo, int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))))
+
+
+def draw(rng):
+    op = rng.choice(["ortho", "muon", "ln", "ce", "ce"])
+    dtype = rng.choice(["fp32", "bf16", "fp16"])
+    if op in ("ortho", "muon"):
+        while True:
+            shapes = [(_spread(rng, 1, 4096), _spread(rng, 1, 4096)) for _ in range(rng.randint(1, 6))]
+            if sum(_ortho_flops(m, n) for m, n in shapes) <= _ortho_flops(4096, 4096):
+                break
+        text = ",".join("%dx%d" % s for s in shapes)
+        return {"op": op, "shapes": text, "dtype": "fp32" if op == "muon" else dtype}
+    if op == "ln":
+        while True:
+            rows, cols = _spread(rng, 1, 65536), _spread(rng, 16, 16384)
+            if rows * cols <= 32768 * 4096:
+                return {"op": op, "rows": rows, "cols": cols, "dtype": dtype}
+    while True:
+        rows, cols, vocab = _spread(rng, 1, 16384), _spread(rng, 8, 2048), _spread(rng, 2, 131072)
+        if rows * cols * vocab <= 8192 * 1024 * 65536 and rows * vocab <= 8192 * 65536:
+            return {"op": op, "rows": rows, "cols": cols, "vocab": vocab, "dtype": dtype, "bias": rng.random() < 0.5, "gate": rng.random() < 0.5}
+
+
+def _shapes(case):
+    if case["shapes"] == "resnet18":
+        return list(_RESNET18)
+    return [tuple(int(v) for v in s.split("x")) for s in case["shapes"].split(",")]
+
+
+def _flat(shape):
+    """(rows, columns) of a weight as a matrix."""
+    return shape[0], math.prod(shape[1:])
+
+
+# ------------------------------------------------------------------------------------------------ inputs
+def prepare(case, seed):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+
+    def normal(*shape, scale=1.0):
+        return torch.randn(shape, generator=g, device="cuda") * scale
+
+    t = _TYPES[case["dtype"]]
+    s = {"op": case["op"]}
+    if case["op"] in ("ortho", "muon"):
+        # a gradient: a few strong directions over noise
+        def gradient(shape):
+            m, n = _flat(shape)
+            r = max(1, min(m, n) // 8)
+            low = normal(m, r) @ normal(r, n) / math.sqrt(r)
+            return ((low + normal(m, n, scale=0.5)) * 1e-3).to(t).reshape(shape).contiguous()
+
+        s["grads"] = [gradient(shape) for shape in _shapes(case)]
+        if case["op"] == "muon":
+            s["params"] = [normal(*x.shape, scale=1 / math.sqrt(_flat(x.shape)[1])) for x in s["grads"]]
+            s["moments"] = [gradient(x.shape) * 10 for x in s["grads"]]
+            if own:
+                s["optimizer"] = _optimizer(s)
+        return s
+    rows, cols = case["rows"], case["cols"]
+    if case["op"] == "ln":
+        s["x"] = (normal(rows, cols) * (0.5 + torch.rand((rows, 1), generator=g, device="cuda")) + normal(rows, 1, scale=0.5)).to(t)
+        s["dy"] = normal(rows, cols).to(t)
+        s["w"] = 1 + normal(cols, scale=0.1)
+        s["b"] = normal(cols, scale=0.1)
+        return s
+    vocab = case["vocab"]
+    s["x"] = normal(rows, cols).to(t)
+    s["w"] = normal(vocab, cols, scale=1 / math.sqrt(cols)).to(t)
+    s["bias"] = normal(vocab, scale=0.1) if case["bias"] else None
+    # few labels are frequent, many are rare; one in twenty positions carries none
+    u = torch.rand((rows,), generator=g, device="cuda", dtype=torch.float64)
+    label = (vocab * u ** 3).to(torch.int64).clamp_(0, vocab - 1)
+    none = torch.rand((rows,), generator=g, device="cuda") < 0.05
+    s["target"] = torch.where(none, torch.full_like(label, _IGNORE), label)
+    s["conf"] = 1 - 0.2 * torch.rand((rows,), generator=g, device="cuda") ** 2 if case["gate"] else None
+    # the loss scale that half precision is trained with
+    s["dloss"] = torch.full((), 65536.0 if t == torch.float16 else 1.0, device="cuda")
+    return s
+
+
+# ------------------------------------------------------------------------------------------------ one pass
+def run(state):
+    return {"ortho": _run_ortho, "muon": _run_muon, "ln": _run_ln, "ce": _run_ce}[state["op"]](state)
+
+
+def _ssecg():
+    src = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "semi-seg-ecg_amd")
+    if src not in sys.path:
+        sys.path.insert(1, src)
+    from ssecg import ops
+    return ops
+
+
+def _optimizer(s):
+    _ssecg()
+    from ssecg.optim import FusedMuon
+    params = [torch.nn.Parameter(p) for p in s["params"]]
+    for p, grad in zip(params, s["grads"]):
+        p.grad = grad
+    optimizer = FusedMuon(params, lr=_LR, momentum=_MOMENTUM, nesterov=True, weight_decay=_DECAY)
+    for p, v in zip(params, s["moments"]):
+        optimizer.state[p]["momentum_buffer"] = v
+    return optimizer
+
+
+def _orthogonal(x):
+    """Newton-Schulz in 32 bits: x (m, n) -> the iterate near the orthogonal factor of x."""
+    a, b, c = _COEF
+    tall = x.shape[0] > x.shape[1]
+    x = x.float().T if tall else x.float()
+    x = x / (x.square().sum().sqrt() + _NORM_EPS)
+    for _ in range(_ITERATIONS):
+        gram = x @ x.T
+        x = a * x + (b * gram + c * (gram @ gram)) @ x
+    return x.T if tall else x
+
+
+def _run_ortho(s):
+    if own:
+        return _ssecg().orthogonalize(s["grads"])
+    return [_orthogonal(x).to(x.dtype).contiguous() for x in s["grads"]]
+
+
+def _muon_update(p, grad, v):
+    m, n = _flat(p.shape)
+    v.mul_(_MOMENTUM).add_(grad)
+    u = _orthogonal((grad + _MOMENTUM * v).reshape(m, n))
+    p.mul_(1 - _LR * _DECAY).sub_(_LR * 0.2 * math.sqrt(max(m, n)) * u.reshape(p.shape))
+
+
+def _run_muon(s):
+    if own:
+        s["optimizer"].step()
+        return {"params": [p.data for p in s["optimizer"].param_groups[0]["params"]], "moments": s["moments"]}
+    [_muon_update(*row) for row in zip(s["params"], s["grads"], s["moments"])]
+    return {"params": s["params"], "moments": s["moments"]}
+
+
+def _run_ln(s):
+    x, dy, w, b = s["x"], s["dy"], s["w"], s["b"]
+    if own:
+        ops = _ssecg()
+        y, mean, rstd = ops.layer_norm_fwd(x, w, b, eps=_LN_EPS)
+        dx, dw, db = ops.layer_norm_bwd(dy, x, mean, rstd, w)
+        return {"y": y, "dx": dx, "dw": dw, "db": db}
+    xf, dyf = x.float(), dy.float()
+    centred = xf - xf.mean(1, keepdim=True)
+    rstd = torch.rsqrt(centred.square().mean(1, keepdim=True) + _LN_EPS)
+    hat = centred * rstd
+    y = hat * w + b
+    gw = dyf * w
+    dx = rstd * (gw - gw.mean(1, keepdim=True) - hat * (gw * hat).mean(1, keepdim=True))
+    return {"y": y.to(x.dtype), "dx": dx.to(x.dtype), "dw": (dyf * hat).sum(0), "db": dyf.sum(0)}
+
+
+def _run_ce(s):
+    x, w, bias, target, conf = s["x"], s["w"], s["bias"], s["target"], s["conf"]
+    if own:
+        ops = _ssecg()
+        loss, saved = ops.linear_ce_fwd(x, w, target, bias=bias, conf=conf, thresh=_THRESH, ignore_index=_IGNORE)
+        dx, dw, db = ops.linear_ce_bwd(saved, s["dloss"])
+        out = {"loss": loss, "dx": dx, "dw": dw}
+        return {**out, "db": db} if bias is not None else out
+    xf, wf = x.float(), w.float()
+    logits = xf @ wf.T
+    logits = logits if bias is None else logits + bias
+    valid = target != _IGNORE
+    label = torch.where(valid, target, torch.zeros_like(target))
+    top = logits.max(1, keepdim=True).values
+    e = (logits - top).exp()
+    total = e.sum(1, keepdim=True)
+    weight = valid.float() if conf is None else valid.float() * (conf >= _THRESH).float()
+    count = valid.float().sum().clamp(min=1)
+    row = top.squeeze(1) + total.squeeze(1).log() - logits.gather(1, label[:, None]).squeeze(1)
+    loss = (row * weight).sum() / count
+    grad = e / total
+    grad.scatter_add_(1, label[:, None], torch.full_like(total, -1.0))
+    grad = grad * (weight * s["dloss"] / count)[:, None]
+    out = {"loss": loss, "dx": (grad @ wf).to(x.dtype), "dw": (grad.T @ xf).to(w.dtype)}
+    return {**out, "db": grad.sum(0)} if bias is not None else out
+
+
+# ------------------------------------------------------------------------------------------------ work and exact values
+def _ortho_flops(m, n):
+    m, n = min(m, n), max(m, n)
+    # the Gram matrix and its square are symmetric: half of each; the product with X is whole
+    return _ITERATIONS * (m * (m + 1) * n + m * m * (m + 1) + 2 * m * m * n)
+
+
+def work(case):
+    e = _TYPES[case["dtype"]].itemsize
+    if case["op"] in ("ortho", "muon"):
+        flat = [_flat(s) for s in _shapes(case)]
+        # gradient in, update out; the optimiser reads and writes parameter and momentum and reads the gradient
+        return {"bytes": sum(m * n for m, n in flat) * e * (2 if case["op"] == "ortho" else 5), "flops": sum(_ortho_flops(m, n) for m, n in flat)}
+    rows, cols = case["rows"], case["cols"]
+    if case["op"] == "ln":
+        # x and dy in, y and dx out, four vectors of parameters and their gradients
+        return {"bytes": 4 * rows * cols * e + 16 * cols, "flops": 16 * rows * cols}
+    vocab = case["vocab"]
+    # logits, gradient of the rows, gradient of the weights: one product each; x, W in, their gradients out, the labels in
+    nbytes = 2 * (rows + vocab) * cols * e + 8 * rows + (4 * rows if case["gate"] else 0) + (8 * vocab if case["bias"] else 0)
+    return {"bytes": nbytes, "flops": 6 * rows * cols * vocab}
+
+
+def _polar64(matrix):
+    """The same five iterations in 64 bits, on the Frobenius-normalised matrix, always with the shorter side first."""
+    a, b, c = _COEF
+    x = matrix.double()
+    flip = x.size(0) > x.size(1)
+    if flip:
+        x = x.t().contiguous()
+    x = x / (torch.sqrt(torch.sum(x * x)) + _NORM_EPS)
+    eye = torch.eye(x.size(0), dtype=torch.float64, device=x.device)
+    for _ in range(_ITERATIONS):
+        g = torch.mm(x, x.t().contiguous())
+        x = torch.mm(a * eye + torch.mm(b * eye + c * g, g), x)
+    return x.t().contiguous() if flip else x
+
+
+def exact(case, seed):
+    s = prepare(case, seed)
+    if case["op"] == "ortho":
+        return [_polar64(x) for x in s["grads"]]
+    if case["op"] == "muon":
+        moments = [_MOMENTUM * v.double() + x.double() for v, x in zip(s["moments"], s["grads"])]
+        params = []
+        for p, x, v in zip(s["params"], s["grads"], moments):
+            p = p.detach().double()
+            m, n = _flat(p.shape)
+            o = _polar64((x.double() + _MOMENTUM * v).reshape(m, n)).reshape(p.shape)
+            params.append(p - _LR * (_DECAY * p + 0.2 * max(m, n) ** 0.5 * o))
+        return {"params": params, "moments": moments}
+    if case["op"] == "ln":
+        x, dy, w, b = (s[k].double() for k in ("x", "dy", "w", "b"))
+        var, mean = torch.var_mean(x, dim=1, unbiased=False, keepdim=True)
+        inv = 1 / torch.sqrt(var + _LN_EPS)
+        hat = (x - mean) * inv
+        k = torch.mean(dy * w * hat, dim=1, keepdim=True)
+        return {"y": torch.addcmul(b, hat, w), "dx": inv * (dy * w - torch.mean(dy * w, dim=1, keepdim=True) - k * hat),
+                "dw": torch.sum(dy * hat, dim=0), "db": torch.sum(dy, dim=0)}
+    x, w, target, dloss = s["x"].double(), s["w"].double(), s["target"], float(s["dloss"])
+    kept = target.ne(_IGNORE)
+    count = max(1, int(kept.sum()))
+    gate = kept if s["conf"] is None else kept & s["conf"].ge(_THRESH)
+    loss, dx, dw = 0.0, torch.zeros_like(x), torch.zeros_like(w)
+    db = torch.zeros(w.size(0), dtype=torch.float64, device=w.device)
+    for at in range(0, x.size(0), 1024):
+        rows = slice(at, at + 1024)
+        z = torch.mm(x[rows], w.t())
+        if s["bias"] is not None:
+            z = z + s["bias"].double()
+        logp = z - torch.logsumexp(z, dim=1, keepdim=True)
+        one = torch.zeros_like(z)
+        index = torch.arange(z.size(0), device=z.device)[gate[rows]]
+        one[index, target[rows][gate[rows]]] = 1.0
+        loss = loss - torch.sum(logp * one) / count
+        d = (torch.exp(logp) * gate[rows].double()[:, None] - one) * (dloss / count)
+        dx[rows] = torch.mm(d, w)
+        dw += torch.mm(d.t().contiguous(), x[rows])
+        db += torch.sum(d, dim=0)
+    out = {"loss": loss, "dx": dx, "dw": dw}
+    return {**out, "db": db} if s["bias"] is not None else out
