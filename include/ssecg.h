@@ -531,6 +531,51 @@ size_t ssecg_amp_wgrad_workspace(int N, int Cin, int Lx, int Cout, int Ldy, int 
 int ssecg_amp_wgrad(const void *dy, const void *x, float *dw, int N, int Cin, int Lx, int Cout, int Ldy, int K,
                     int stride, int pad, void *workspace, size_t workspace_bytes, void *stream);
 
+/* ------------------------------------------------------------------------
+ * Token-level operators: layer norm, a classifier with softmax cross entropy over a large vocabulary, orthogonalised updates.
+ * dtype: 0 = fp32, 1 = bf16, 2 = fp16 (the type of x, dy, y, dx, weight and dweight of the classifier, matrices and results of the
+ * orthogonalisation); parameters of the norm, biases, statistics and losses are fp32.  Tensors are contiguous; rows are counted in
+ * 64 bits.  Workspaces are 256-byte aligned.
+ * --------------------------------------------------------------------- */
+
+/* y = (x - mean) rstd weight + bias over the last axis of x (rows, C); weight / bias may be NULL (1 / 0); mean, rstd: (rows) */
+int ssecg_layer_norm_fwd(const void *x, const float *weight, const float *bias, int dtype, int64_t rows, int C, double eps, void *y,
+                         float *mean, float *rstd, void *stream);
+/* dx and, where not NULL, dweight[c] = sum_rows dy xhat, dbias[c] = sum_rows dy (deterministic; they need the workspace) */
+size_t ssecg_layer_norm_bwd_workspace(int dtype, int64_t rows, int C);
+int ssecg_layer_norm_bwd(const void *dy, const void *x, const float *mean, const float *rstd, const float *weight, int dtype,
+                         int64_t rows, int C, void *dx, float *dweight, float *dbias, float *workspace, size_t workspace_bytes,
+                         void *stream);
+
+/* z = x weight^T (+ bias), x (N, C), weight (V, C); the logits are never stored.
+ *   lse[n]  = log sum_v exp z_nv (NaN for a target outside [0, V) that is not ignore_index)
+ *   gate[n] = 0 for target == ignore_index or (conf given) conf[n] < thresh or NaN, else 1
+ *   count   = max(1, positions whose target is not ignore_index)
+ *   loss    : reduction 0: (N) gate (lse - z_target); 1: their sum / count; 2: their sum
+ * A position whose gate is 0 contributes nothing, whatever x holds there. */
+size_t ssecg_linear_ce_fwd_workspace(int dtype, int64_t N, int64_t C, int64_t V);
+int ssecg_linear_ce_fwd(const void *x, const void *weight, const float *bias, const int64_t *target, const float *conf, double thresh,
+                        int64_t ignore_index, int dtype, int64_t N, int64_t C, int64_t V, int reduction, float *loss, float *lse,
+                        float *gate, float *count, void *workspace, size_t workspace_bytes, void *stream);
+/* gradients of the above (each may be NULL, not all): dloss is a scalar on the device (reduction 1, 2) or (N) (reduction 0).  The
+ * vocabulary is taken in pieces that bound the workspace (about 1 GiB beside copies of the operands). */
+size_t ssecg_linear_ce_bwd_workspace(int dtype, int64_t N, int64_t C, int64_t V, int want_dx, int want_dweight, int want_dbias);
+int ssecg_linear_ce_bwd(const float *dloss, const void *x, const void *weight, const float *bias, const int64_t *target,
+                        const float *lse, const float *gate, const float *count, int dtype, int64_t N, int64_t C, int64_t V,
+                        int reduction, void *dx, void *dweight, float *dbias, void *workspace, size_t workspace_bytes, void *stream);
+
+/* Newton-Schulz orthogonalisation of `count` matrices.  mats is a HOST array of rows {source, result, momentum, rows, cols} (device
+ * pointers as integers; momentum unused here); it is read during the call only.  At most 2^20 rows / columns each. */
+size_t ssecg_orthogonalize_workspace(const int64_t *mats, int count);
+int ssecg_orthogonalize_multi(const int64_t *mats, int count, int dtype, int steps, double eps, void *workspace,
+                              size_t workspace_bytes, void *stream);
+/* One optimiser step on fp32 matrices, rows {gradient, parameter, momentum, rows, cols}: v = momentum v + g, u = g + momentum v
+ * (nesterov) or v, p = p (1 - lr weight_decay) - lr s O(u) with s = sqrt(max(1, rows / cols)) (adjust 0) or 0.2 sqrt(max(rows, cols))
+ * (adjust 1).  skip_flag: as in ssecg_adamw_multi (nothing is touched); lr_dev: this step's lr on the device (captured launches). */
+int ssecg_muon_multi(const int64_t *mats, int count, double lr, double momentum, int nesterov, double weight_decay, int adjust,
+                     int steps, double eps, const float *skip_flag, const double *lr_dev, void *workspace, size_t workspace_bytes,
+                     void *stream);
+
 #ifdef __cplusplus
 }
 #endif

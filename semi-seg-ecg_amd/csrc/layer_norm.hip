@@ -1,0 +1,463 @@
+// Layer norm over the last axis of (rows, C) and its backward pass.
+//
+//   mu = mean(x), r = 1 / sqrt(mean((x - mu)^2) + eps), xh = (x - mu) r, y = xh w + b
+//   g = dy w,  dx = r (g - mean(g) - xh mean(g xh)),  dw = sum_rows dy xh,  db = sum_rows dy
+//
+// Both passes are bound by HBM: forward reads x and writes y, backward reads x and dy and writes dx - each byte once.  A row
+// stays in the registers of the threads that own it (one wave up to 4 vectors per lane, otherwise 256 or 1024 threads), so the
+// variance is the two-pass one (the sum of squared differences from the mean, no cancellation) without a second read.  A thread
+// owns the same columns of every row its workgroup takes: w and b are loaded once, and the column sums dw / db grow in its
+// registers; the row groups of a workgroup are joined in LDS, the workgroups by a second launch in fixed order (no atomics:
+// results do not change from run to run).  Statistics, sums and parameter gradients are fp32; y and dx are rounded once.
+#include "lm_common.h"
+#include "ssecg.h"
+
+namespace {
+using namespace ssecg_lm;
+
+constexpr int kMaxBlocks = 512;   // workgroups of the backward pass = rows of its partial sums (2 of 1024 threads per CU)
+
+template <typename T>
+__device__ __forceinline__ typename Vec<T>::type load_vec(const T* __restrict__ p, int c0, int C) {
+    constexpr int V = Vec<T>::N;
+    typename Vec<T>::type v;
+    if (c0 + V <= C) {
+        v = *reinterpret_cast<const typename Vec<T>::type*>(p + c0);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] = c0 + i < C ? p[c0 + i] : (T)0.f;
+    }
+    return v;
+}
+
+template <typename T>
+__device__ __forceinline__ void store_vec(T* __restrict__ p, int c0, int C, typename Vec<T>::type v) {
+    constexpr int V = Vec<T>::N;
+    if (c0 + V <= C) {
+        *reinterpret_cast<typename Vec<T>::type*>(p + c0) = v;
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (c0 + i < C) p[c0 + i] = v[i];
+    }
+}
+
+// Sum over the TPR threads of a row; every thread gets it.  `sh` holds a slot per wave; two slots sets alternate by `flip`, so
+// one barrier per reduction is enough (a wave can be at most one reduction ahead of the others).
+template <int TPR, int K>
+__device__ __forceinline__ void row_sum(float (&v)[K], float* sh, int& flip) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] = wave_sum(v[k]);
+    if (TPR > 64) {
+        constexpr int W = TPR / 64;
+        const int wave = threadIdx.x >> 6, first = wave / W * W;
+        float* s = sh + flip * (16 * K);
+        flip ^= 1;
+        if ((threadIdx.x & 63) == 0)
+#pragma unroll
+            for (int k = 0; k < K; ++k) s[wave * K + k] = v[k];
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            float t = 0.f;
+#pragma unroll
+            for (int w = 0; w < W; ++w) t += s[(first + w) * K + k];
+            v[k] = t;
+        }
+    }
+}
+
+template <typename T, int TPR, int NT, int NCH>
+__global__ __launch_bounds__(NT) void ln_fwd_kernel(const T* __restrict__ x, const float* __restrict__ w, const float* __restrict__ b,
+                                                    T* __restrict__ y, float* __restrict__ mean, float* __restrict__ rstd,
+                                                    int64_t rows, int C, float eps) {
+    constexpr int V = Vec<T>::N, G = NT / TPR;
+    __shared__ float sh[2 * 16];
+    int flip = 0;
+    const int t = threadIdx.x % TPR, grp = threadIdx.x / TPR;
+    float wv[NCH][V], bv[NCH][V];
+#pragma unroll
+    for (int j = 0; j < NCH; ++j)
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const int c = (t + TPR * j) * V + i;
+            wv[j][i] = w && c < C ? w[c] : 1.f;
+            bv[j][i] = b && c < C ? b[c] : 0.f;
+        }
+    const float invC = 1.f / (float)C;
+    for (int64_t r0 = (int64_t)blockIdx.x * G; r0 < rows; r0 += (int64_t)gridDim.x * G) {   // uniform: every wave reaches each barrier
+        const int64_t row = r0 + grp;
+        const bool live = row < rows;
+        const T* xr = x + (live ? row : rows - 1) * C;
+        float v[NCH][V];
+        float s[1] = {0.f};
+#pragma unroll
+        for (int j = 0; j < NCH; ++j) {
+            const int c0 = (t + TPR * j) * V;
+            if (c0 < C) {
+                const auto q = load_vec(xr, c0, C);
+#pragma unroll
+                for (int i = 0; i < V; ++i) { v[j][i] = (float)q[i]; s[0] += v[j][i]; }
+            } else {
+#pragma unroll
+                for (int i = 0; i < V; ++i) v[j][i] = 0.f;
+            }
+        }
+        row_sum<TPR, 1>(s, sh, flip);
+        const float mu = s[0] * invC;
+        float q[1] = {0.f};
+#pragma unroll
+        for (int j = 0; j < NCH; ++j)
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const float d = v[j][i] - mu;
+                if ((t + TPR * j) * V + i < C) q[0] += d * d;
+            }
+        row_sum<TPR, 1>(q, sh, flip);
+        const float rs = 1.f / sqrtf(q[0] * invC + eps);
+        if (!live) continue;
+        if (t == 0) { mean[row] = mu; rstd[row] = rs; }
+#pragma unroll
+        for (int j = 0; j < NCH; ++j) {
+            const int c0 = (t + TPR * j) * V;
+            if (c0 < C) {
+                typename Vec<T>::type o;
+#pragma unroll
+                for (int i = 0; i < V; ++i) o[i] = (T)((v[j][i] - mu) * rs * wv[j][i] + bv[j][i]);
+                store_vec(y + row * C, c0, C, o);
+            }
+        }
+    }
+}
+
+// any C: a workgroup walks its row three times (the second and third read come from the caches)
+template <typename T>
+__global__ __launch_bounds__(1024) void ln_fwd_long_kernel(const T* __restrict__ x, const float* __restrict__ w, const float* __restrict__ b,
+                                                           T* __restrict__ y, float* __restrict__ mean, float* __restrict__ rstd,
+                                                           int64_t rows, int C, float eps) {
+    constexpr int V = Vec<T>::N;
+    __shared__ float sh[2 * 16];
+    int flip = 0;
+    for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+        const T* xr = x + row * C;
+        float s[1] = {0.f};
+        for (int64_t c0 = (int64_t)threadIdx.x * V; c0 < C; c0 += 1024 * V) {
+            const auto q = load_vec(xr, (int)c0, C);
+#pragma unroll
+            for (int i = 0; i < V; ++i) s[0] += (float)q[i];
+        }
+        row_sum<1024, 1>(s, sh, flip);
+        const float mu = s[0] / (float)C;
+        float d2[1] = {0.f};
+        for (int64_t c0 = (int64_t)threadIdx.x * V; c0 < C; c0 += 1024 * V) {
+            const auto q = load_vec(xr, (int)c0, C);
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const float d = (float)q[i] - mu;
+                if (c0 + i < C) d2[0] += d * d;
+            }
+        }
+        row_sum<1024, 1>(d2, sh, flip);
+        const float rs = 1.f / sqrtf(d2[0] / (float)C + eps);
+        if (threadIdx.x == 0) { mean[row] = mu; rstd[row] = rs; }
+        for (int64_t c0 = (int64_t)threadIdx.x * V; c0 < C; c0 += 1024 * V) {
+            const auto q = load_vec(xr, (int)c0, C);
+            typename Vec<T>::type o;
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const int c = (int)c0 + i;
+                const float wi = w && c < C ? w[c] : 1.f, bi = b && c < C ? b[c] : 0.f;
+                o[i] = (T)(((float)q[i] - mu) * rs * wi + bi);
+            }
+            store_vec(y + row * C, (int)c0, C, o);
+        }
+    }
+}
+
+// partial: [gridDim.x][2][C] column sums {dy xh, dy} of the workgroup's rows
+template <typename T, int TPR, int NT, int NCH>
+__global__ __launch_bounds__(NT) void ln_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ x, const float* __restrict__ mean,
+                                                    const float* __restrict__ rstd, const float* __restrict__ w, T* __restrict__ dx,
+                                                    float* __restrict__ partial, int64_t rows, int C) {
+    constexpr int V = Vec<T>::N, G = NT / TPR;
+    __shared__ float sh[2 * 32];
+    extern __shared__ float col[];                    // [2][C] when a workgroup has several row groups
+    int flip = 0;
+    const int t = threadIdx.x % TPR, grp = threadIdx.x / TPR;
+    float wv[NCH][V], aw[NCH][V], ab[NCH][V];
+#pragma unroll
+    for (int j = 0; j < NCH; ++j)
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const int c = (t + TPR * j) * V + i;
+            wv[j][i] = w && c < C ? w[c] : 1.f;
+            aw[j][i] = 0.f;
+            ab[j][i] = 0.f;
+        }
+    const float invC = 1.f / (float)C;
+    for (int64_t r0 = (int64_t)blockIdx.x * G; r0 < rows; r0 += (int64_t)gridDim.x * G) {
+        const int64_t row = r0 + grp;
+        const bool live = row < rows;
+        const int64_t at = (live ? row : rows - 1) * C;
+        const float mu = mean[live ? row : rows - 1], rs = rstd[live ? row : rows - 1];
+        typename Vec<T>::type xq[NCH], gq[NCH];
+        float s[2] = {0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < NCH; ++j) {
+            const int c0 = (t + TPR * j) * V;
+            if (c0 < C) {
+                xq[j] = load_vec(x + at, c0, C);
+                gq[j] = load_vec(dy + at, c0, C);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < NCH; ++j) {
+            const int c0 = (t + TPR * j) * V;
+            if (c0 < C) {
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    const float xh = ((float)xq[j][i] - mu) * rs, d = (float)gq[j][i], g = d * wv[j][i];   // beyond C: dy = 0
+                    s[0] += g;
+                    s[1] += g * xh;
+                    if (live) { aw[j][i] += d * xh; ab[j][i] += d; }
+                }
+            }
+        }
+        row_sum<TPR, 2>(s, sh, flip);
+        const float c1 = s[0] * invC, c2 = s[1] * invC;
+        if (live) {
+#pragma unroll
+            for (int j = 0; j < NCH; ++j) {
+                const int c0 = (t + TPR * j) * V;
+                if (c0 < C) {
+                    typename Vec<T>::type o;
+#pragma unroll
+                    for (int i = 0; i < V; ++i) {
+                        const float xh = ((float)xq[j][i] - mu) * rs, g = (float)gq[j][i] * wv[j][i];
+                        o[i] = (T)(rs * (g - c1 - xh * c2));
+                    }
+                    store_vec(dx + at, c0, C, o);
+                }
+            }
+        }
+    }
+    if (partial == nullptr) return;
+    float* out = partial + (size_t)blockIdx.x * 2 * C;
+    if (G > 1) {                                      // row groups one after the other: fixed order
+        for (int g = 0; g < G; ++g) {
+            __syncthreads();
+            if (grp == g) {
+#pragma unroll
+                for (int j = 0; j < NCH; ++j)
+#pragma unroll
+                    for (int i = 0; i < V; ++i) {
+                        const int c = (t + TPR * j) * V + i;
+                        if (c < C) {
+                            if (g > 0) { aw[j][i] += col[c]; ab[j][i] += col[C + c]; }
+                            if (g < G - 1) { col[c] = aw[j][i]; col[C + c] = ab[j][i]; }
+                        }
+                    }
+            }
+        }
+    }
+    if (grp == G - 1) {
+#pragma unroll
+        for (int j = 0; j < NCH; ++j)
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const int c = (t + TPR * j) * V + i;
+                if (c < C) { out[c] = aw[j][i]; out[C + c] = ab[j][i]; }
+            }
+    }
+}
+
+// any C: dx alone, two reads of the row
+template <typename T>
+__global__ __launch_bounds__(1024) void ln_bwd_long_kernel(const T* __restrict__ dy, const T* __restrict__ x, const float* __restrict__ mean,
+                                                           const float* __restrict__ rstd, const float* __restrict__ w,
+                                                           T* __restrict__ dx, int64_t rows, int C) {
+    constexpr int V = Vec<T>::N;
+    __shared__ float sh[2 * 32];
+    int flip = 0;
+    for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+        const int64_t at = row * C;
+        const float mu = mean[row], rs = rstd[row];
+        float s[2] = {0.f, 0.f};
+        for (int64_t c0 = (int64_t)threadIdx.x * V; c0 < C; c0 += 1024 * V) {
+            const auto xq = load_vec(x + at, (int)c0, C);
+            const auto gq = load_vec(dy + at, (int)c0, C);
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const int c = (int)c0 + i;
+                const float g = (float)gq[i] * (w && c < C ? w[c] : 1.f);
+                s[0] += g;
+                s[1] += g * (((float)xq[i] - mu) * rs);
+            }
+        }
+        row_sum<1024, 2>(s, sh, flip);
+        const float c1 = s[0] / (float)C, c2 = s[1] / (float)C;
+        for (int64_t c0 = (int64_t)threadIdx.x * V; c0 < C; c0 += 1024 * V) {
+            const auto xq = load_vec(x + at, (int)c0, C);
+            const auto gq = load_vec(dy + at, (int)c0, C);
+            typename Vec<T>::type o;
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const int c = (int)c0 + i;
+                const float g = (float)gq[i] * (w && c < C ? w[c] : 1.f);
+                o[i] = (T)(rs * (g - c1 - (((float)xq[i] - mu) * rs) * c2));
+            }
+            store_vec(dx + at, (int)c0, C, o);
+        }
+    }
+}
+
+// any C: the column sums of a slab of rows, one thread per column
+template <typename T>
+__global__ __launch_bounds__(256) void ln_bwd_cols_kernel(const T* __restrict__ dy, const T* __restrict__ x, const float* __restrict__ mean,
+                                                          const float* __restrict__ rstd, float* __restrict__ partial, int64_t rows, int C) {
+    const int64_t per = (rows + gridDim.y - 1) / gridDim.y;
+    const int64_t r0 = per * blockIdx.y, r1 = r0 + per < rows ? r0 + per : rows;
+    const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (c >= C) return;
+    float aw = 0.f, ab = 0.f;
+    for (int64_t r = r0; r < r1; ++r) {
+        const float d = (float)dy[r * C + c];
+        aw += d * (((float)x[r * C + c] - mean[r]) * rstd[r]);
+        ab += d;
+    }
+    float* out = partial + (size_t)blockIdx.y * 2 * C;
+    out[c] = aw;
+    out[C + c] = ab;
+}
+
+// dw / db: columns of partial [parts][2][C] in fixed order; 32 columns x 32 row strands per workgroup
+__global__ __launch_bounds__(1024) void ln_param_grads_kernel(const float* __restrict__ partial, int parts, int C, float* __restrict__ dw,
+                                                              float* __restrict__ db) {
+    __shared__ float sh[32][33];
+    const int lane = threadIdx.x & 31, strand = threadIdx.x >> 5;
+    const int64_t c = (int64_t)blockIdx.x * 32 + lane;       // column of the flattened [2][C]
+    const int64_t W = 2 * (int64_t)C;
+    float s = 0.f;
+    if (c < W)
+        for (int p = strand; p < parts; p += 32) s += partial[p * W + c];
+    sh[strand][lane] = s;
+    __syncthreads();
+    if (strand == 0 && c < W) {
+        float t = 0.f;
+#pragma unroll
+        for (int k = 0; k < 32; ++k) t += sh[k][lane];
+        float* out = c < C ? dw : db;
+        if (out) out[c < C ? c : c - C] = t;
+    }
+}
+
+// Threads per row and 16-byte vectors per thread.  One wave per row up to 4 vectors a lane: no barrier, and several rows are in
+// flight per SIMD.  Beyond that 256, then 1024 threads, so that a thread's share (row, parameters, column sums) stays in registers.
+struct LnShape { int tpr, nch; };
+inline LnShape ln_shape(int C, int V, bool bwd) {
+    const int64_t vecs = ((int64_t)C + V - 1) / V;
+    const int deep = V == 8 ? 2 : 4;                         // vectors per thread that the backward pass of 1024 threads can hold
+    auto fit = [&](int tpr, int most) {
+        for (int n = 1; n <= most; n *= 2)
+            if (vecs <= (int64_t)tpr * n) return n;
+        return 0;
+    };
+    if (int n = fit(64, bwd ? deep : 4)) return {64, n};
+    if (int n = fit(256, bwd ? 2 : 4)) return {256, n};
+    if (int n = fit(1024, deep)) return {1024, n};
+    return {0, 0};
+}
+
+template <typename T, int TPR, int NCH>
+int launch_fwd(const void* x, const float* w, const float* b, void* y, float* mean, float* rstd, int64_t rows, int C, float eps, hipStream_t st) {
+    constexpr int NT = TPR == 1024 ? 1024 : 256, G = NT / TPR;
+    const int64_t blocks = (rows + G - 1) / G, most = 256 * (2048 / NT);
+    hipLaunchKernelGGL((ln_fwd_kernel<T, TPR, NT, NCH>), dim3((unsigned)(blocks < most ? blocks : most)), dim3(NT), 0, st, (const T*)x, w, b,
+                       (T*)y, mean, rstd, rows, C, eps);
+    return (int)hipGetLastError();
+}
+
+template <typename T, int TPR, int NCH>
+int launch_bwd(const void* dy, const void* x, const float* mean, const float* rstd, const float* w, void* dx, float* partial, int64_t rows,
+               int C, int parts, hipStream_t st) {
+    constexpr int NT = 1024;
+    const size_t lds = partial && TPR < NT ? (size_t)2 * C * sizeof(float) : 0;
+    hipLaunchKernelGGL((ln_bwd_kernel<T, TPR, NT, NCH>), dim3((unsigned)parts), dim3(NT), lds, st, (const T*)dy, (const T*)x, mean, rstd, w,
+                       (T*)dx, partial, rows, C);
+    return (int)hipGetLastError();
+}
+
+inline int ln_parts(int64_t rows, int C, int dtype) {
+    const LnShape s = ln_shape(C, dtype == kF32 ? 4 : 8, true);
+    const int64_t g = s.tpr ? 1024 / s.tpr : 1;
+    const int64_t blocks = (rows + g - 1) / g, most = s.tpr ? kMaxBlocks : 32;   // very long rows: few slabs bound the workspace
+    return (int)(blocks < most ? blocks : most);
+}
+
+template <typename T>
+int ln_fwd(const void* x, const float* w, const float* b, void* y, float* mean, float* rstd, int64_t rows, int C, float eps, hipStream_t st) {
+    const LnShape s = ln_shape(C, Vec<T>::N, false);
+#define SSECG_LN_CASE(TPR, NCH) if (s.tpr == TPR && s.nch == NCH) return launch_fwd<T, TPR, NCH>(x, w, b, y, mean, rstd, rows, C, eps, st)
+    SSECG_LN_CASE(64, 1); SSECG_LN_CASE(64, 2); SSECG_LN_CASE(64, 4);
+    SSECG_LN_CASE(256, 2); SSECG_LN_CASE(256, 4);
+    SSECG_LN_CASE(1024, 2);
+    if constexpr (Vec<T>::N == 4) SSECG_LN_CASE(1024, 4);
+#undef SSECG_LN_CASE
+    hipLaunchKernelGGL((ln_fwd_long_kernel<T>), dim3((unsigned)(rows < 512 ? rows : 512)), dim3(1024), 0, st, (const T*)x, w, b, (T*)y, mean,
+                       rstd, rows, C, eps);
+    return (int)hipGetLastError();
+}
+
+template <typename T>
+int ln_bwd(const void* dy, const void* x, const float* mean, const float* rstd, const float* w, void* dx, float* partial, int64_t rows, int C,
+           int parts, hipStream_t st) {
+    const LnShape s = ln_shape(C, Vec<T>::N, true);
+#define SSECG_LN_CASE(TPR, NCH) if (s.tpr == TPR && s.nch == NCH) return launch_bwd<T, TPR, NCH>(dy, x, mean, rstd, w, dx, partial, rows, C, parts, st)
+    SSECG_LN_CASE(64, 1); SSECG_LN_CASE(64, 2);
+    SSECG_LN_CASE(256, 1); SSECG_LN_CASE(256, 2);
+    SSECG_LN_CASE(1024, 1); SSECG_LN_CASE(1024, 2);
+    if constexpr (Vec<T>::N == 4) {
+        SSECG_LN_CASE(64, 4); SSECG_LN_CASE(1024, 4);
+    }
+#undef SSECG_LN_CASE
+    hipLaunchKernelGGL((ln_bwd_long_kernel<T>), dim3((unsigned)(rows < 512 ? rows : 512)), dim3(1024), 0, st, (const T*)dy, (const T*)x, mean,
+                       rstd, w, (T*)dx, rows, C);
+    if (partial)
+        hipLaunchKernelGGL((ln_bwd_cols_kernel<T>), dim3((unsigned)((C + 255) / 256), (unsigned)parts), dim3(256), 0, st, (const T*)dy,
+                           (const T*)x, mean, rstd, partial, rows, C);
+    return (int)hipGetLastError();
+}
+
+constexpr int kMaxC = 1 << 24;
+
+}  // namespace
+
+extern "C" {
+
+int ssecg_layer_norm_fwd(const void* x, const float* weight, const float* bias, int dtype, int64_t rows, int C, double eps, void* y,
+                         float* mean, float* rstd, void* stream) {
+    if (!x || !y || !mean || !rstd || !dtype_ok(dtype) || rows <= 0 || C <= 0 || C > kMaxC || !(eps >= 0.0)) return SSECG_E_INVAL;
+    SSECG_LM_DTYPE(dtype, T, return ln_fwd<T>(x, weight, bias, y, mean, rstd, rows, C, (float)eps, (hipStream_t)stream));
+}
+
+size_t ssecg_layer_norm_bwd_workspace(int dtype, int64_t rows, int C) {
+    if (!dtype_ok(dtype) || rows <= 0 || C <= 0 || C > kMaxC) return 0;
+    return (size_t)ln_parts(rows, C, dtype) * 2 * C * sizeof(float);
+}
+
+int ssecg_layer_norm_bwd(const void* dy, const void* x, const float* mean, const float* rstd, const float* weight, int dtype, int64_t rows,
+                         int C, void* dx, float* dweight, float* dbias, float* workspace, size_t workspace_bytes, void* stream) {
+    if (!dy || !x || !mean || !rstd || !dx || !dtype_ok(dtype) || rows <= 0 || C <= 0 || C > kMaxC) return SSECG_E_INVAL;
+    const bool params = dweight || dbias;
+    if (params && (!workspace || workspace_bytes < ssecg_layer_norm_bwd_workspace(dtype, rows, C))) return SSECG_E_WORKSPACE;
+    const int parts = ln_parts(rows, C, dtype);
+    float* partial = params ? workspace : nullptr;
+    int rc = 0;
+    SSECG_LM_DTYPE(dtype, T, rc = ln_bwd<T>(dy, x, mean, rstd, weight, dx, partial, rows, C, parts, (hipStream_t)stream));
+    if (rc != 0 || !params) return rc;
+    hipLaunchKernelGGL(ln_param_grads_kernel, dim3((unsigned)((2 * (int64_t)C + 31) / 32)), dim3(1024), 0, (hipStream_t)stream, partial, parts,
+                       C, dweight, dbias);
+    return (int)hipGetLastError();
+}
+
+}  // extern "C"

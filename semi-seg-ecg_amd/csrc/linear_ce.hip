@@ -1,0 +1,801 @@
+// A classifier and its softmax cross entropy over a large vocabulary, in pieces of the vocabulary, without keeping the logits:
+//
+//   z_nv = x_n . w_v (+ b_v),  lse_n = log sum_v exp z_nv,  row loss = g_n (lse_n - z_{n,t_n})
+//   E_nv = g_n (exp(z_nv - lse_n) - [v = t_n]),  dx_n = f sum_v E_nv w_v,  dw_v = f sum_n E_nv x_n,  db_v = f sum_n E_nv
+//
+// g_n is 0 for an ignored position and for one whose confidence is below the threshold, else 1 (times the upstream gradient when
+// the loss is not reduced); f = upstream / number of positions that are not ignored (mean), upstream (sum).
+//
+// Forward: one product whose epilogue keeps, per tile, the maximum and the sum of exponentials of a row and its target's logit.
+// The vocabulary is the tile's register axis (operand A), so a lane reduces its own row without shuffles but one.  A second launch
+// joins the tiles.  Backward: the logits of a piece are computed again, E is written in 16 bits (both ways round, so that every
+// product reads k fastest) and two products take it up.  8 N V C multiplications and additions against the 6 N V C that keeping
+// N V logits would need.
+//
+// 32-bit inputs travel as two fp16 planes (mm_core.h), scaled by a power of two that the largest finite value sets: exact, and an
+// entry 2^-17 of the largest still has all its bits.  E lies in [-1, 1] and is held times 2^14 for fp16's sake.  Rows whose g_n is
+// zero enter nothing: neither their values (which may be infinite or NaN) nor their products.
+#include "mm_core.h"
+#include "ssecg.h"
+
+namespace {
+using namespace ssecg_lm;
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kEScale = 14;                       // E is held times 2^14
+constexpr int kAmaxParts = 256;
+
+__device__ __forceinline__ float exp2_fast(float v) { return __builtin_amdgcn_exp2f(v); }
+
+// ---------------------------------------------------------------- operands
+// Which rows count: by the gate of the forward pass, or (there) by target and confidence.
+struct Counts {
+    const float* gate;
+    const int64_t* target; int64_t ignore;
+    const float* conf; float thresh;
+    __device__ __forceinline__ bool operator()(int64_t r) const {
+        if (gate) return gate[r] != 0.f;
+        return target == nullptr || (target[r] != ignore && (conf == nullptr || conf[r] >= thresh));
+    }
+};
+
+// largest finite |x| of the rows that count, per workgroup (a maximum: any order gives the same); a wave per row
+__global__ __launch_bounds__(256) void ce_amax_kernel(const float* __restrict__ x, int64_t rows, int C, Counts counts, float* __restrict__ out) {
+    float m = 0.f;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (int64_t r = (int64_t)blockIdx.x * 4 + wave; r < rows; r += (int64_t)kAmaxParts * 4) {
+        if (!counts(r)) continue;
+        for (int c = lane; c < C; c += 64) {
+            const float v = fabsf(x[r * C + c]);
+            m = v < INFINITY ? fmaxf(m, v) : m;
+        }
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+    __shared__ float sh[4];
+    if (lane == 0) sh[wave] = m;
+    __syncthreads();
+    if (threadIdx.x == 0) out[blockIdx.x] = fmaxf(fmaxf(sh[0], sh[1]), fmaxf(sh[2], sh[3]));
+}
+
+// -> the scale's exponent, the same in every thread of a 256-thread workgroup
+__device__ __forceinline__ int amax_exp(const float* __restrict__ parts) {
+    __shared__ float sh[4];
+    float m = parts[threadIdx.x & (kAmaxParts - 1)];
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) sh[(threadIdx.x >> 6) & 3] = m;
+    __syncthreads();
+    return scale_exp(fmaxf(fmaxf(sh[0], sh[1]), fmaxf(sh[2], sh[3])));
+}
+
+// rows [r0, r0 + R) of src (.., C) as planes, as they lie (dst, may be null) and transposed (dstT, may be null); k is zero-filled
+// to the pitch.  gate: a row whose gate is 0 is written as zeros.  One workgroup: 64 rows x 64 columns.
+template <typename S, typename T, int P>
+__global__ __launch_bounds__(256) void ce_pack_kernel(const S* __restrict__ src, int64_t r0, int R, int C, const float* __restrict__ gate,
+                                                      const float* __restrict__ amax, char* __restrict__ dst, int64_t pitch, int64_t plane,
+                                                      char* __restrict__ dstT, int64_t pitchT, int64_t planeT) {
+    __shared__ uint32_t tile[64][65];
+    const int ex = P == 2 ? amax_exp(amax) : 0;
+    const int64_t rb = (int64_t)blockIdx.y * 64, cb = (int64_t)blockIdx.x * 64;
+    const int lane = threadIdx.x & 63, strand = threadIdx.x >> 6;
+    for (int i = strand; i < 64; i += 4) {
+        const int64_t r = rb + i, c = cb + lane;
+        uint32_t q = 0;
+        if (r < R && c < C && (gate == nullptr || gate[r0 + r] != 0.f)) {
+            const S v = src[(r0 + r) * C + c];
+            if constexpr (P == 2) {
+                _Float16 hi, lo;
+                split16(ldexpf((float)v, ex), hi, lo);
+                q = (uint32_t)__builtin_bit_cast(uint16_t, hi) | (uint32_t)__builtin_bit_cast(uint16_t, lo) << 16;
+            } else {
+                q = __builtin_bit_cast(uint16_t, v);
+            }
+        }
+        tile[i][lane] = q;
+    }
+    __syncthreads();
+    for (int u = threadIdx.x; u < 512; u += 256) {         // 64 rows x 8 chunks of 8 values
+        const int i = u >> 3, k = (u & 7) * 8;
+        if (dst && rb + i < R && (cb + k) * 2 < pitch) {
+            u32x4 a, b;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t p = tile[i][k + 2 * j], q = tile[i][k + 2 * j + 1];
+                a[j] = (p & 0xffffu) | q << 16;
+                b[j] = p >> 16 | (q & 0xffff0000u);
+            }
+            char* d = dst + (rb + i) * pitch + (cb + k) * 2;
+            *reinterpret_cast<u32x4*>(d) = a;
+            if (P == 2) *reinterpret_cast<u32x4*>(d + plane) = b;
+        }
+        if (dstT && cb + i < C && (rb + k) * 2 < pitchT) {
+            u32x4 a, b;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t p = tile[k + 2 * j][i], q = tile[k + 2 * j + 1][i];
+                a[j] = (p & 0xffffu) | q << 16;
+                b[j] = p >> 16 | (q & 0xffff0000u);
+            }
+            char* d = dstT + (cb + i) * pitchT + (rb + k) * 2;
+            *reinterpret_cast<u32x4*>(d) = a;
+            if (P == 2) *reinterpret_cast<u32x4*>(d + planeT) = b;
+        }
+    }
+}
+
+// ---------------------------------------------------------------- logits
+struct LogitArgs {
+    Operand W, X;                                // vocabulary rows (of the piece), position rows
+    const float* bias;                           // of the piece, or null
+    const float* amaxX; const float* amaxW;      // scale parts (two planes) or null
+    int V, N, tilesV, tilesN, stages;
+    const int64_t* target;                       // class indices; v0 is the piece's first class
+    int64_t v0;
+    // forward: partial maxima and sums [parts][N], target logits [N]
+    float* pm; float* ps; float* tl;
+    // gradient: lse and g per row, E [N][pitchE] and its transpose [V][pitchT], partial db [tilesN * WN][V]
+    const float* lse; const float* gate; const float* coef;
+    char* E; int64_t pitchE, planeE;
+    char* Et; int64_t pitchT, planeT;
+    float* pdb;
+};
+
+template <class M>
+__device__ __forceinline__ void tile_of(int tilesA, int tilesB, int& ta, int& tb) {
+    // operand A's tiles fastest within groups of 4 tiles of B: a group's rows of B stay in the L2 while A passes
+    const int t = xcd_tile(blockIdx.x, tilesA * tilesB);
+    const int grp = 4 * tilesA, g = t / grp, in = t - g * grp;
+    const int width = tilesB - 4 * g < 4 ? tilesB - 4 * g : 4;
+    ta = in / width;
+    tb = 4 * g + in - ta * width;
+}
+
+template <class M>
+__device__ __forceinline__ void logits_tile(const LogitArgs& p, int a0, int b0, char* lds, f32x16 (&acc)[M::TM][M::TN]) {
+    int ex = 0;
+    if constexpr (M::P == 2) {
+        // every thread reads the parts itself (256 words, cached); the wave's maximum is the workgroup's
+        float mx = 0.f, mw = 0.f;
+        const int lane = threadIdx.x & 63;
+#pragma unroll
+        for (int k = 0; k < kAmaxParts / 64; ++k) {
+            mx = fmaxf(mx, p.amaxX[lane + 64 * k]);
+            mw = fmaxf(mw, p.amaxW[lane + 64 * k]);
+        }
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) {
+            mx = fmaxf(mx, __shfl_xor(mx, o, 64));
+            mw = fmaxf(mw, __shfl_xor(mw, o, 64));
+        }
+        ex = -(scale_exp(mx) + scale_exp(mw));
+    }
+    M::zero(acc);
+    M::run(p.W, a0, p.X, b0, 0, p.stages, lds, acc);
+    if constexpr (M::P == 2) {
+#pragma unroll
+        for (int i = 0; i < M::TM; ++i)
+#pragma unroll
+            for (int j = 0; j < M::TN; ++j)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) acc[i][j][e] = ldexpf(acc[i][j][e], ex);
+    }
+    if (p.bias) {
+#pragma unroll
+        for (int i = 0; i < M::TM; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int v = a0 + M::arow(i, e);
+                const float b = p.bias[v < p.V ? v : p.V - 1];
+#pragma unroll
+                for (int j = 0; j < M::TN; ++j) acc[i][j][e] += b;
+            }
+    }
+    if (a0 + M::BM > p.V) {                       // the last tile: classes that do not exist
+#pragma unroll
+        for (int i = 0; i < M::TM; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const bool out = a0 + M::arow(i, e) >= p.V;
+#pragma unroll
+                for (int j = 0; j < M::TN; ++j) acc[i][j][e] = out ? -INFINITY : acc[i][j][e];
+            }
+    }
+}
+
+// the label of a position as an offset from the lane's first class: register (i, e) holds it where offset == 32 i + 8 (e / 4) + e % 4
+template <class M>
+__device__ __forceinline__ int label_offset(int64_t t, int a0) {
+    const int64_t off = t - a0 - M::arow(0, 0);
+    return off >= 0 && off < 32 * M::TM ? (int)off : -1;
+}
+__device__ __forceinline__ constexpr int reg_offset(int i, int e) { return 32 * i + 8 * (e >> 2) + (e & 3); }
+
+template <class M>
+__global__ __launch_bounds__(M::NT) void ce_lse_kernel(LogitArgs p) {
+    __shared__ __attribute__((aligned(16))) char lds[M::LDS];
+    int ta, tb;
+    tile_of<M>(p.tilesV, p.tilesN, ta, tb);
+    const int a0 = ta * M::BM, b0 = tb * M::BN;
+    f32x16 acc[M::TM][M::TN];
+    logits_tile<M>(p, a0, b0, lds, acc);
+    const int wm = (threadIdx.x >> 6) / M::WN, h = (threadIdx.x >> 5) & 1;
+#pragma unroll
+    for (int j = 0; j < M::TN; ++j) {
+        const int n = b0 + M::bcol(j);
+        const int off = n < p.N ? label_offset<M>(p.target[n], a0) : -1;
+        float m = -INFINITY, hit = 0.f;
+#pragma unroll
+        for (int i = 0; i < M::TM; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                m = fmaxf(m, acc[i][j][e]);
+                hit = reg_offset(i, e) == off ? acc[i][j][e] : hit;
+            }
+        const float mm = m == -INFINITY ? 0.f : m;
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < M::TM; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s += exp2_fast((acc[i][j][e] - mm) * kLog2e);
+        if (off >= 0 && (off & 4) == 0 && a0 + M::arow(0, 0) + off < p.V) p.tl[n] = hit;
+        // the lane's other half of the rows
+        const float m2 = __shfl_xor(m, 32, 64), s2 = __shfl_xor(s, 32, 64);
+        const float mt = fmaxf(m, m2), mz = mt == -INFINITY ? 0.f : mt;
+        const float mm2 = m2 == -INFINITY ? 0.f : m2;
+        s = s * exp2_fast((mm - mz) * kLog2e) + s2 * exp2_fast((mm2 - mz) * kLog2e);
+        if (h == 0 && n < p.N) {
+            const int64_t part = (int64_t)ta * M::WM + wm;
+            p.pm[part * p.N + n] = mt;
+            p.ps[part * p.N + n] = s;
+        }
+    }
+}
+
+// joins the parts of a row: lse, g and the row's loss.  A strand of 64 / .. lanes would not pay: rows are the long axis.
+__global__ __launch_bounds__(256) void ce_join_kernel(const float* __restrict__ pm, const float* __restrict__ ps, const float* __restrict__ tl,
+                                                      int parts, int N, int V, const int64_t* __restrict__ target, const float* __restrict__ conf,
+                                                      float thresh, int64_t ignore, float* __restrict__ lse, float* __restrict__ gate,
+                                                      float* __restrict__ row_loss) {
+    // 16 rows x 16 strands of parts per workgroup
+    __shared__ float sm[16][17], ss[16][17];
+    const int c = threadIdx.x & 15, k = threadIdx.x >> 4, n = blockIdx.x * 16 + c;
+    float m = -INFINITY, s = 0.f;
+    if (n < N)
+        for (int p = k; p < parts; p += 16) {
+            const float m2 = pm[(int64_t)p * N + n], s2 = ps[(int64_t)p * N + n];
+            const float mt = fmaxf(m, m2), mz = mt == -INFINITY ? 0.f : mt;
+            s = s * exp2_fast(((m == -INFINITY ? 0.f : m) - mz) * kLog2e) + s2 * exp2_fast(((m2 == -INFINITY ? 0.f : m2) - mz) * kLog2e);
+            m = mt;
+        }
+    sm[k][c] = m;
+    ss[k][c] = s;
+    __syncthreads();
+    if (k != 0 || n >= N) return;
+    for (int q = 1; q < 16; ++q) {
+        const float m2 = sm[q][c], s2 = ss[q][c];
+        const float mt = fmaxf(m, m2), mz = mt == -INFINITY ? 0.f : mt;
+        s = s * exp2_fast(((m == -INFINITY ? 0.f : m) - mz) * kLog2e) + s2 * exp2_fast(((m2 == -INFINITY ? 0.f : m2) - mz) * kLog2e);
+        m = mt;
+    }
+    const int64_t t = target[n];
+    const bool kept = t != ignore, bad = kept && (t < 0 || t >= V);
+    const float l = bad || m == -INFINITY ? NAN : m + logf(s);     // a label outside the vocabulary poisons its row: no silent loss
+    const float g = kept && (conf == nullptr || conf[n] >= thresh) ? 1.f : 0.f;
+    lse[n] = l;
+    gate[n] = g;
+    row_loss[n] = g != 0.f ? l - (bad ? 0.f : tl[n]) : 0.f;
+}
+
+// out[0] = sum of the row losses (/ count for the mean), count[0] = max(1, positions that are not ignored); fixed order, fp64
+__global__ __launch_bounds__(1024) void ce_total_kernel(const float* __restrict__ row_loss, const int64_t* __restrict__ target, int64_t ignore,
+                                                        int N, int mean, float* __restrict__ out, float* __restrict__ count) {
+    __shared__ double sh[1024];
+    __shared__ int shc[1024];
+    double s = 0.0;
+    int k = 0;
+    for (int i = threadIdx.x; i < N; i += 1024) {
+        s += (double)row_loss[i];
+        k += target[i] != ignore ? 1 : 0;
+    }
+    sh[threadIdx.x] = s;
+    shc[threadIdx.x] = k;
+    for (int o = 512; o > 0; o >>= 1) {
+        __syncthreads();
+        if (threadIdx.x < o) { sh[threadIdx.x] += sh[threadIdx.x + o]; shc[threadIdx.x] += shc[threadIdx.x + o]; }
+    }
+    if (threadIdx.x == 0) {
+        const int c = shc[0] > 0 ? shc[0] : 1;
+        count[0] = (float)c;
+        if (out) out[0] = (float)(mean ? sh[0] / (double)c : sh[0]);
+    }
+}
+
+// ---------------------------------------------------------------- gradient
+// Not reduced: coef[n] = g_n dloss[n] / s with s a power of two >= max |g dloss| (so that E stays in [-1, 1]); fscale[0] = s.
+// Reduced: fscale[0] = dloss / count (mean) or dloss (sum), coef is not used.
+__global__ __launch_bounds__(1024) void ce_coef_kernel(const float* __restrict__ dloss, const float* __restrict__ gate,
+                                                       const float* __restrict__ count, int N, int reduction, float* __restrict__ coef,
+                                                       float* __restrict__ fscale) {
+    if (reduction != 0) {
+        if (threadIdx.x == 0) fscale[0] = reduction == 1 ? dloss[0] / count[0] : dloss[0];
+        return;
+    }
+    __shared__ float sh[16];
+    float m = 0.f;
+    for (int i = threadIdx.x; i < N; i += 1024) {
+        const float v = gate[i] != 0.f ? fabsf(dloss[i]) : 0.f;
+        if (v < INFINITY) m = fmaxf(m, v);
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = m;
+    __syncthreads();
+    m = sh[0];
+    for (int k = 1; k < 16; ++k) m = fmaxf(m, sh[k]);
+    int e = 0;
+    if (m > 0.f) frexpf(m, &e);                        // m <= 2^e
+    e = e > 127 ? 127 : (e < -126 ? -126 : e);
+    for (int i = threadIdx.x; i < N; i += 1024) coef[i] = gate[i] != 0.f ? ldexpf(dloss[i], -e) : 0.f;
+    if (threadIdx.x == 0) fscale[0] = ldexpf(1.f, e);
+}
+
+template <class M, bool DB>
+__global__ __launch_bounds__(M::NT) void ce_grad_kernel(LogitArgs p) {
+    __shared__ __attribute__((aligned(16))) char lds[M::LDS];
+    int ta, tb;
+    tile_of<M>(p.tilesV, p.tilesN, ta, tb);
+    const int a0 = ta * M::BM, b0 = tb * M::BN;
+    using T = typename M::T;
+    f32x16 acc[M::TM][M::TN];
+    logits_tile<M>(p, a0, b0, lds, acc);
+    const int lane = threadIdx.x & 63, wn = (threadIdx.x >> 6) % M::WN;
+    float lse[M::TN], g[M::TN];
+    int off[M::TN];
+#pragma unroll
+    for (int j = 0; j < M::TN; ++j) {
+        const int n = b0 + M::bcol(j);
+        const bool in = n < p.N;
+        g[j] = in ? p.gate[n] : 0.f;
+        if (in && p.coef) g[j] = p.coef[n];
+        lse[j] = in ? p.lse[n] : 0.f;
+        off[j] = in ? label_offset<M>(p.target[n] - p.v0, a0) : -1;
+    }
+#pragma unroll
+    for (int i = 0; i < M::TM; ++i) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const int v = a0 + M::arow(i, e);
+            float sum = 0.f;
+#pragma unroll
+            for (int j = 0; j < M::TN; ++j) {
+                const float pr = exp2_fast((acc[i][j][e] - lse[j]) * kLog2e) - (reg_offset(i, e) == off[j] ? 1.f : 0.f);
+                const float q = g[j] != 0.f ? pr * g[j] : 0.f;      // a row that does not count enters as zero, whatever it holds
+                acc[i][j][e] = q * (float)(1 << kEScale);
+                sum += q;
+            }
+            if (DB) {                                                          // column sum over the wave's positions
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+                if ((lane & 31) == 0 && v < p.V) p.pdb[(int64_t)(tb * M::WN + wn) * p.V + v] = sum;
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < M::TN; ++j) {
+            const int n = b0 + M::bcol(j);
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+                const int v = a0 + M::arow(i, e);                              // 4 consecutive classes
+                T hi[4], lo[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    if constexpr (M::P == 2) split16(acc[i][j][e + k], hi[k], lo[k]);
+                    else hi[k] = (T)acc[i][j][e + k];
+                }
+                if (p.E && n < p.N) {
+                    char* d = p.E + n * p.pitchE + (int64_t)v * 2;
+                    u32x2 q;
+                    __builtin_memcpy(&q, hi, 8);
+                    *reinterpret_cast<u32x2*>(d) = q;
+                    if constexpr (M::P == 2) {
+                        __builtin_memcpy(&q, lo, 8);
+                        *reinterpret_cast<u32x2*>(d + p.planeE) = q;
+                    }
+                }
+                if (p.Et) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        if (v + k < p.V) {
+                            char* d = p.Et + (v + k) * p.pitchT + (int64_t)n * 2;
+                            *reinterpret_cast<T*>(d) = hi[k];
+                            if constexpr (M::P == 2) *reinterpret_cast<T*>(d + p.planeT) = lo[k];
+                        }
+                }
+            }
+        }
+    }
+}
+
+// ---------------------------------------------------------------- products with E
+struct ProdArgs {
+    Operand A, B;
+    int rows, cols, tilesA, tilesB, stages, splits;
+    float* plane;                                // partial planes [splits][rows][cols], or null: write out
+    int add;                                     // plane += instead of plane =
+    void* out;                                   // (rows, cols) of the result's type
+    const float* amax;                           // scale parts of operand B, or null
+    const float* fscale;
+};
+
+template <typename O>
+__device__ __forceinline__ O finish(float v, float f, int ex) { return (O)ldexpf(v * f, ex); }
+
+template <class M, typename O>
+__global__ __launch_bounds__(M::NT) void ce_prod_kernel(ProdArgs p) {
+    __shared__ __attribute__((aligned(16))) char lds[M::LDS];
+    int ta, tb;
+    tile_of<M>(p.tilesA, p.tilesB, ta, tb);
+    const int a0 = ta * M::BM, b0 = tb * M::BN;
+    const int z = blockIdx.y, s0 = (int)((int64_t)p.stages * z / p.splits), s1 = (int)((int64_t)p.stages * (z + 1) / p.splits);
+    f32x16 acc[M::TM][M::TN];
+    M::zero(acc);
+    M::run(p.A, a0, p.B, b0, s0, s1 - s0, lds, acc);
+    int ex = -kEScale;
+    float f = 0.f;
+    if (!p.plane) {
+        f = p.fscale[0];
+        if constexpr (M::P == 2) {
+            float m = 0.f;
+            const int lane = threadIdx.x & 63;
+#pragma unroll
+            for (int k = 0; k < kAmaxParts / 64; ++k) m = fmaxf(m, p.amax[lane + 64 * k]);
+#pragma unroll
+            for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+            ex -= scale_exp(m);
+        }
+    }
+    float* plane = p.plane ? p.plane + (int64_t)z * p.rows * p.cols : nullptr;
+#pragma unroll
+    for (int i = 0; i < M::TM; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const int64_t r = a0 + M::arow(i, e);
+            if (r >= p.rows) continue;
+#pragma unroll
+            for (int j = 0; j < M::TN; ++j) {
+                const int c = b0 + M::bcol(j);
+                if (c >= p.cols) continue;
+                const int64_t at = r * p.cols + c;
+                if (plane) plane[at] = p.add ? plane[at] + acc[i][j][e] : acc[i][j][e];
+                else reinterpret_cast<O*>(p.out)[at] = finish<O>(acc[i][j][e], f, ex);
+            }
+        }
+}
+
+// out = f 2^ex sum of the planes, in their order
+template <typename O>
+__global__ __launch_bounds__(256) void ce_sum_planes_kernel(const float* __restrict__ planes, int splits, int64_t n, const float* __restrict__ amax,
+                                                            const float* __restrict__ fscale, O* __restrict__ out) {
+    int ex = -kEScale;
+    if (amax) ex -= amax_exp(amax);
+    const float f = fscale[0];
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+        float s = planes[i];
+        for (int k = 1; k < splits; ++k) s += planes[(int64_t)k * n + i];
+        out[i] = finish<O>(s, f, ex);
+    }
+}
+
+__global__ __launch_bounds__(256) void ce_db_kernel(const float* __restrict__ pdb, int parts, int V, const float* __restrict__ fscale,
+                                                    float* __restrict__ db) {
+    const int v = blockIdx.x * 256 + threadIdx.x;
+    if (v >= V) return;
+    float s = 0.f;
+    for (int p = 0; p < parts; ++p) s += pdb[(int64_t)p * V + v];
+    db[v] = s * fscale[0];
+}
+
+template <typename O>
+__global__ __launch_bounds__(256) void ce_zero_kernel(O* __restrict__ out, int64_t n) {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) out[i] = (O)0.f;
+}
+
+// ---------------------------------------------------------------- host side
+template <typename S> struct Inner { using T = S; static constexpr int P = 1; };
+template <> struct Inner<float> { using T = _Float16; static constexpr int P = 2; };
+
+template <typename T, int P> using Big = MmTile<T, P, 256, 256, 2, 4, 2>;
+template <typename T, int P> using Mid = MmTile<T, P, 128, 128, 2, 2, 2>;
+
+inline int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
+
+struct Blob {                                    // carves a workspace; a first pass with base 0 sizes it
+    char* base; size_t at = 0;
+    explicit Blob(void* p) : base((char*)p) {}
+    template <typename T> T* take(size_t n) {
+        char* q = base + at;
+        at += (n * sizeof(T) + 255) & ~(size_t)255;
+        return (T*)q;
+    }
+};
+
+constexpr int64_t kMaxN = 1 << 24, kMaxV = 1 << 24, kMaxC = 1 << 16;
+inline bool shape_ok(int64_t N, int64_t C, int64_t V) {
+    return N > 0 && C > 0 && V > 0 && N <= kMaxN && V <= kMaxV && C <= kMaxC && (N / 128 + 1) * (V / 128 + 1) < INT32_MAX;
+}
+
+// Is the matrix an operand as it lies (16-bit, whole stages of k, aligned)?
+inline bool direct(int dtype, const void* p, int64_t C) { return dtype != kF32 && C % 64 == 0 && ((uintptr_t)p & 15) == 0; }
+
+struct FwdPlan {
+    int64_t Cp; int BMt, WMt, tilesV, tilesN, parts;
+    float *amaxX, *amaxW, *pm, *ps, *tl, *row;
+    char *Xp, *Wp;
+};
+
+inline bool use_big(int64_t a, int64_t b) { return ((a + 255) / 256) * ((b + 255) / 256) >= 256; }
+
+FwdPlan plan_fwd(Blob& ws, int dtype, int64_t N, int64_t C, int64_t V, bool dx, bool dw) {
+    FwdPlan p;
+    const int P = dtype == kF32 ? 2 : 1;
+    p.Cp = up(C, 64);
+    const bool big = use_big(V, N);
+    p.BMt = big ? 256 : 128;
+    p.WMt = 2;
+    p.tilesV = (int)((V + p.BMt - 1) / p.BMt);
+    p.tilesN = (int)((N + p.BMt - 1) / p.BMt);
+    p.parts = p.tilesV * p.WMt;
+    p.amaxX = ws.take<float>(P == 2 ? kAmaxParts : 0);
+    p.amaxW = ws.take<float>(P == 2 ? kAmaxParts : 0);
+    p.pm = ws.take<float>((size_t)p.parts * N);
+    p.ps = ws.take<float>((size_t)p.parts * N);
+    p.tl = ws.take<float>((size_t)N);
+    p.row = ws.take<float>((size_t)N);
+    p.Xp = ws.take<char>(dx ? 0 : (size_t)N * p.Cp * 2 * P);
+    p.Wp = ws.take<char>(dw ? 0 : (size_t)V * p.Cp * 2 * P);
+    return p;
+}
+
+template <typename S>
+int pack(const void* src, int64_t r0, int64_t R, int64_t C, const float* gate, const float* amax, char* dst, int64_t pitch, int64_t plane, char* dstT,
+         int64_t pitchT, int64_t planeT, hipStream_t st) {
+    const int64_t wide = dst && pitch / 2 > C ? pitch / 2 : C, tall = dstT && pitchT / 2 > R ? pitchT / 2 : R;
+    hipLaunchKernelGGL((ce_pack_kernel<S, typename Inner<S>::T, Inner<S>::P>), dim3((unsigned)((wide + 63) / 64), (unsigned)((tall + 63) / 64)),
+                       dim3(256), 0, st, (const S*)src, r0, (int)R, (int)C, gate, amax, dst, pitch, plane, dstT, pitchT, planeT);
+    return (int)hipGetLastError();
+}
+
+#define SSECG_CE_LAUNCH(M, kernel, grid, st, args)                                                                              \
+    do {                                                                                                                        \
+        hipLaunchKernelGGL(kernel, grid, dim3(M::NT), 0, st, args);                                                        \
+        const int rc_ = (int)hipGetLastError();                                                                                 \
+        if (rc_ != 0) return rc_;                                                                                               \
+    } while (0)
+
+template <typename S>
+int ce_fwd(const void* x, const void* w, const float* bias, const int64_t* target, const float* conf, float thresh, int64_t ignore, int dtype,
+           int64_t N, int64_t C, int64_t V, int reduction, float* loss, float* lse, float* gate, float* count, void* ws, hipStream_t st) {
+    using T = typename Inner<S>::T;
+    constexpr int P = Inner<S>::P;
+    Blob blob(ws);
+    const bool dX = direct(dtype, x, C), dW = direct(dtype, w, C);
+    const FwdPlan p = plan_fwd(blob, dtype, N, C, V, dX, dW);
+    LogitArgs a = {};
+    int rc = 0;
+    if constexpr (P == 2) {
+        hipLaunchKernelGGL(ce_amax_kernel, dim3(kAmaxParts), dim3(256), 0, st, (const float*)x, N, (int)C,
+                           Counts{nullptr, target, ignore, conf, thresh}, p.amaxX);
+        hipLaunchKernelGGL(ce_amax_kernel, dim3(kAmaxParts), dim3(256), 0, st, (const float*)w, V, (int)C, Counts{}, p.amaxW);
+        a.amaxX = p.amaxX;
+        a.amaxW = p.amaxW;
+    }
+    if (!dX && (rc = pack<S>(x, 0, N, C, nullptr, p.amaxX, p.Xp, p.Cp * 2, N * p.Cp * 2, nullptr, 0, 0, st)) != 0) return rc;
+    if (!dW && (rc = pack<S>(w, 0, V, C, nullptr, p.amaxW, p.Wp, p.Cp * 2, V * p.Cp * 2, nullptr, 0, 0, st)) != 0) return rc;
+    a.X = {dX ? (const char*)x : p.Xp, p.Cp * 2, N * p.Cp * 2, (int)N};
+    a.W = {dW ? (const char*)w : p.Wp, p.Cp * 2, V * p.Cp * 2, (int)V};
+    a.bias = bias;
+    a.V = (int)V; a.N = (int)N; a.tilesV = p.tilesV; a.tilesN = p.tilesN;
+    a.stages = (int)(p.Cp / (P == 1 ? 64 : 32));
+    a.target = target; a.v0 = 0;
+    a.pm = p.pm; a.ps = p.ps; a.tl = p.tl;
+    if (p.BMt == 256) { using M = Big<T, P>; SSECG_CE_LAUNCH(M, ce_lse_kernel<M>, dim3(p.tilesV * p.tilesN), st, a); }
+    else { using M = Mid<T, P>; SSECG_CE_LAUNCH(M, ce_lse_kernel<M>, dim3(p.tilesV * p.tilesN), st, a); }
+    float* row = reduction == 0 ? loss : p.row;
+    hipLaunchKernelGGL(ce_join_kernel, dim3((unsigned)((N + 15) / 16)), dim3(256), 0, st, p.pm, p.ps, p.tl, p.parts, (int)N, (int)V, target, conf, thresh,
+                       ignore, lse, gate, row);
+    hipLaunchKernelGGL(ce_total_kernel, dim3(1), dim3(1024), 0, st, row, target, ignore, (int)N, reduction == 1 ? 1 : 0,
+                       reduction == 0 ? nullptr : loss, count);
+    return (int)hipGetLastError();
+}
+
+constexpr size_t kPieceBytes = (size_t)1 << 30;  // E, its transpose and the piece's W^T
+
+struct BwdPlan {
+    int64_t Cp, Np, Vc;                          // padded sizes, classes per piece (multiple of 256 unless one piece)
+    int pieces, splitX, splitW;
+    bool bigL, bigX, bigW;
+    float *amaxX, *amaxW, *coef, *fscale, *pdb, *planeX, *planeW;
+    char *Xp, *Wp, *Xt, *Wt, *E, *Et;
+    int64_t pitchE, pitchT, pitchWt;
+};
+
+// How many workgroups share the k of one tile: enough to give each of the 256 CUs one, each at least 8 stages long.
+inline int split_of(int64_t tiles, int64_t stages) {
+    int64_t s = 256 / (tiles > 0 ? tiles : 1);
+    if (s > stages / 8) s = stages / 8;
+    return (int)(s < 1 ? 1 : (s > 64 ? 64 : s));
+}
+
+BwdPlan plan_bwd(Blob& ws, int dtype, int64_t N, int64_t C, int64_t V, bool dX, bool dW, bool want_x, bool want_w, bool want_b) {
+    BwdPlan p;
+    const int P = dtype == kF32 ? 2 : 1, BK = P == 1 ? 64 : 32;
+    p.Cp = up(C, 64);
+    p.Np = up(N, 256);
+    const size_t per = (size_t)(p.Np * (want_w ? 2 : 0) + N * (want_x ? 2 : 0) + C * (want_x ? 2 : 0)) * P + 1;
+    int64_t most = (int64_t)(kPieceBytes / per) / 256 * 256;
+    if (most < 256) most = 256;
+    const int64_t pieces = (V + most - 1) / most;
+    p.Vc = pieces == 1 ? V : up((V + pieces - 1) / pieces, 256);
+    p.pieces = (int)((V + p.Vc - 1) / p.Vc);
+    p.bigL = use_big(p.Vc, N);
+    p.bigX = use_big(N, C);
+    p.bigW = use_big(p.Vc, C);
+    p.pitchE = up(p.Vc, 256) * 2;
+    p.pitchWt = p.pitchE;
+    p.pitchT = p.Np * 2;
+    const int bx = p.bigX ? 256 : 128, bw = p.bigW ? 256 : 128;
+    p.splitX = split_of(((N + bx - 1) / bx) * ((C + bx - 1) / bx), up(p.Vc, BK) / BK);
+    p.splitW = split_of(((p.Vc + bw - 1) / bw) * ((C + bw - 1) / bw), up(N, BK) / BK);
+    p.amaxX = ws.take<float>(P == 2 ? kAmaxParts : 0);
+    p.amaxW = ws.take<float>(P == 2 ? kAmaxParts : 0);
+    p.coef = ws.take<float>((size_t)N);
+    p.fscale = ws.take<float>(1);
+    const int bl = p.bigL ? 256 : 128, wn = p.bigL ? 4 : 2;
+    p.pdb = ws.take<float>(want_b ? (size_t)((N + bl - 1) / bl) * wn * p.Vc : 0);
+    p.planeX = ws.take<float>(want_x && (p.splitX > 1 || p.pieces > 1) ? (size_t)p.splitX * N * C : 0);
+    p.planeW = ws.take<float>(want_w && p.splitW > 1 ? (size_t)p.splitW * p.Vc * C : 0);
+    p.Xp = ws.take<char>(dX ? 0 : (size_t)N * p.Cp * 2 * P);
+    p.Wp = ws.take<char>(dW ? 0 : (size_t)V * p.Cp * 2 * P);
+    p.Xt = ws.take<char>(want_w ? (size_t)C * p.pitchT * P : 0);
+    p.Wt = ws.take<char>(want_x ? (size_t)C * p.pitchWt * P : 0);
+    p.E = ws.take<char>(want_x ? (size_t)N * p.pitchE * P : 0);
+    p.Et = ws.take<char>(want_w ? (size_t)p.Vc * p.pitchT * P : 0);
+    return p;
+}
+
+inline unsigned grid_for(int64_t n) {
+    const int64_t b = (n + 255) / 256;
+    return (unsigned)(b < 2048 ? b : 2048);
+}
+
+template <typename S>
+int ce_bwd(const float* dloss, const void* x, const void* w, const float* bias, const int64_t* target, const float* lse, const float* gate,
+           const float* count, int dtype, int64_t N, int64_t C, int64_t V, int reduction, void* dx, void* dw, float* db, void* ws, hipStream_t st) {
+    using T = typename Inner<S>::T;
+    constexpr int P = Inner<S>::P;
+    constexpr int BK = P == 1 ? 64 : 32;
+    Blob blob(ws);
+    const bool dX = direct(dtype, x, C), dW = direct(dtype, w, C);
+    const BwdPlan p = plan_bwd(blob, dtype, N, C, V, dX, dW, dx != nullptr, dw != nullptr, db != nullptr);
+    int rc = 0;
+    if constexpr (P == 2) {
+        // X's scale: over the rows that count (a row that does not may hold anything)
+        hipLaunchKernelGGL(ce_amax_kernel, dim3(kAmaxParts), dim3(256), 0, st, (const float*)x, N, (int)C, Counts{gate, nullptr, 0, nullptr, 0.f},
+                           p.amaxX);
+        hipLaunchKernelGGL(ce_amax_kernel, dim3(kAmaxParts), dim3(256), 0, st, (const float*)w, V, (int)C, Counts{}, p.amaxW);
+    }
+    hipLaunchKernelGGL(ce_coef_kernel, dim3(1), dim3(1024), 0, st, dloss, gate, count, (int)N, reduction, p.coef, p.fscale);
+    if (!dX || dw) {
+        rc = pack<S>(x, 0, N, C, gate, p.amaxX, dX ? nullptr : p.Xp, p.Cp * 2, N * p.Cp * 2, dw ? p.Xt : nullptr, p.pitchT, C * p.pitchT, st);
+        if (rc != 0) return rc;
+    }
+    if (!dW && (rc = pack<S>(w, 0, V, C, nullptr, p.amaxW, p.Wp, p.Cp * 2, V * p.Cp * 2, nullptr, 0, 0, st)) != 0) return rc;
+    for (int i = 0; i < p.pieces; ++i) {
+        const int64_t v0 = i * p.Vc, vn = V - v0 < p.Vc ? V - v0 : p.Vc;
+        LogitArgs a = {};
+        a.X = {dX ? (const char*)x : p.Xp, p.Cp * 2, N * p.Cp * 2, (int)N};
+        a.W = {(dW ? (const char*)w : p.Wp) + v0 * p.Cp * 2, p.Cp * 2, V * p.Cp * 2, (int)vn};
+        a.bias = bias ? bias + v0 : nullptr;
+        a.amaxX = p.amaxX; a.amaxW = p.amaxW;
+        a.V = (int)vn; a.N = (int)N;
+        const int bl = p.bigL ? 256 : 128, wn = p.bigL ? 4 : 2;
+        a.tilesV = (int)((vn + bl - 1) / bl); a.tilesN = (int)((N + bl - 1) / bl);
+        a.stages = (int)(p.Cp / BK);
+        a.target = target; a.v0 = v0;
+        a.lse = lse; a.gate = gate; a.coef = reduction == 0 ? p.coef : nullptr;
+        a.E = dx ? p.E : nullptr; a.pitchE = p.pitchE; a.planeE = N * p.pitchE;
+        a.Et = dw ? p.Et : nullptr; a.pitchT = p.pitchT; a.planeT = p.Vc * p.pitchT;
+        a.pdb = p.pdb;
+        const dim3 grid(a.tilesV * a.tilesN);
+        if (p.bigL) {
+            using M = Big<T, P>;
+            if (db) SSECG_CE_LAUNCH(M, (ce_grad_kernel<M, true>), grid, st, a);
+            else SSECG_CE_LAUNCH(M, (ce_grad_kernel<M, false>), grid, st, a);
+        } else {
+            using M = Mid<T, P>;
+            if (db) SSECG_CE_LAUNCH(M, (ce_grad_kernel<M, true>), grid, st, a);
+            else SSECG_CE_LAUNCH(M, (ce_grad_kernel<M, false>), grid, st, a);
+        }
+        if (db) hipLaunchKernelGGL(ce_db_kernel, dim3((unsigned)((vn + 255) / 256)), dim3(256), 0, st, p.pdb, a.tilesN * wn, (int)vn, p.fscale, db + v0);
+        if (dx) {
+            if ((rc = pack<S>(w, v0, vn, C, nullptr, p.amaxW, nullptr, 0, 0, p.Wt, up(vn, 64) * 2 < p.pitchWt ? up(vn, 64) * 2 : p.pitchWt, C * p.pitchWt, st)) != 0) return rc;
+            ProdArgs q = {};
+            const int64_t wp = up(vn, 64) * 2 < p.pitchWt ? up(vn, 64) * 2 : p.pitchWt;
+            q.A = {p.E, p.pitchE, N * p.pitchE, (int)N};
+            q.B = {p.Wt, wp, C * p.pitchWt, (int)C};
+            q.rows = (int)N; q.cols = (int)C;
+            const int bx = p.bigX ? 256 : 128;
+            q.tilesA = (int)((N + bx - 1) / bx); q.tilesB = (int)((C + bx - 1) / bx);
+            q.stages = (int)(up(vn, BK) / BK); q.splits = p.splitX;
+            q.plane = p.splitX > 1 || p.pieces > 1 ? p.planeX : nullptr;
+            q.add = i > 0; q.out = dx; q.amax = p.amaxW; q.fscale = p.fscale;
+            const dim3 g2(q.tilesA * q.tilesB, q.splits);
+            if (p.bigX) { using M = Big<T, P>; SSECG_CE_LAUNCH(M, (ce_prod_kernel<M, S>), g2, st, q); }
+            else { using M = Mid<T, P>; SSECG_CE_LAUNCH(M, (ce_prod_kernel<M, S>), g2, st, q); }
+        }
+        if (dw) {
+            ProdArgs q = {};
+            q.A = {p.Et, p.pitchT, p.Vc * p.pitchT, (int)vn};
+            q.B = {p.Xt, p.pitchT, C * p.pitchT, (int)C};
+            q.rows = (int)vn; q.cols = (int)C;
+            const int bw = p.bigW ? 256 : 128;
+            q.tilesA = (int)((vn + bw - 1) / bw); q.tilesB = (int)((C + bw - 1) / bw);
+            q.stages = (int)(up(N, BK) / BK); q.splits = p.splitW;
+            q.plane = p.splitW > 1 ? p.planeW : nullptr;
+            q.out = (S*)dw + v0 * C; q.amax = p.amaxX; q.fscale = p.fscale;
+            const dim3 g2(q.tilesA * q.tilesB, q.splits);
+            if (p.bigW) { using M = Big<T, P>; SSECG_CE_LAUNCH(M, (ce_prod_kernel<M, S>), g2, st, q); }
+            else { using M = Mid<T, P>; SSECG_CE_LAUNCH(M, (ce_prod_kernel<M, S>), g2, st, q); }
+            if (q.plane)
+                hipLaunchKernelGGL((ce_sum_planes_kernel<S>), dim3(grid_for(vn * C)), dim3(256), 0, st, p.planeW, p.splitW, vn * C,
+                                   P == 2 ? p.amaxX : nullptr, p.fscale, (S*)dw + v0 * C);
+        }
+    }
+    if (dx && (p.splitX > 1 || p.pieces > 1))
+        hipLaunchKernelGGL((ce_sum_planes_kernel<S>), dim3(grid_for(N * C)), dim3(256), 0, st, p.planeX, p.splitX, N * C, P == 2 ? p.amaxW : nullptr,
+                           p.fscale, (S*)dx);
+    return (int)hipGetLastError();
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t ssecg_linear_ce_fwd_workspace(int dtype, int64_t N, int64_t C, int64_t V) {
+    if (!dtype_ok(dtype) || !shape_ok(N, C, V)) return 0;
+    Blob b(nullptr);
+    plan_fwd(b, dtype, N, C, V, false, false);
+    return b.at;
+}
+
+int ssecg_linear_ce_fwd(const void* x, const void* weight, const float* bias, const int64_t* target, const float* conf, double thresh,
+                        int64_t ignore_index, int dtype, int64_t N, int64_t C, int64_t V, int reduction, float* loss, float* lse, float* gate,
+                        float* count, void* workspace, size_t workspace_bytes, void* stream) {
+    if (!x || !weight || !target || !loss || !lse || !gate || !count || !workspace || !dtype_ok(dtype) || !shape_ok(N, C, V) || reduction < 0 ||
+        reduction > 2 || ((uintptr_t)workspace & 255))
+        return SSECG_E_INVAL;
+    if (workspace_bytes < ssecg_linear_ce_fwd_workspace(dtype, N, C, V)) return SSECG_E_WORKSPACE;
+    SSECG_LM_DTYPE(dtype, S, return ce_fwd<S>(x, weight, bias, target, conf, (float)thresh, ignore_index, dtype, N, C, V, reduction, loss, lse, gate,
+                                              count, workspace, (hipStream_t)stream));
+}
+
+size_t ssecg_linear_ce_bwd_workspace(int dtype, int64_t N, int64_t C, int64_t V, int want_dx, int want_dw, int want_db) {
+    if (!dtype_ok(dtype) || !shape_ok(N, C, V)) return 0;
+    Blob b(nullptr);
+    plan_bwd(b, dtype, N, C, V, false, false, want_dx != 0, want_dw != 0, want_db != 0);
+    return b.at;
+}
+
+int ssecg_linear_ce_bwd(const float* dloss, const void* x, const void* weight, const float* bias, const int64_t* target, const float* lse,
+                        const float* gate, const float* count, int dtype, int64_t N, int64_t C, int64_t V, int reduction, void* dx, void* dweight,
+                        float* dbias, void* workspace, size_t workspace_bytes, void* stream) {
+    if (!dloss || !x || !weight || !target || !lse || !gate || !count || !workspace || (!dx && !dweight && !dbias) || !dtype_ok(dtype) ||
+        !shape_ok(N, C, V) || reduction < 0 || reduction > 2 || ((uintptr_t)workspace & 255))
+        return SSECG_E_INVAL;
+    if (workspace_bytes < ssecg_linear_ce_bwd_workspace(dtype, N, C, V, dx != nullptr, dweight != nullptr, dbias != nullptr)) return SSECG_E_WORKSPACE;
+    SSECG_LM_DTYPE(dtype, S, return ce_bwd<S>(dloss, x, weight, bias, target, lse, gate, count, dtype, N, C, V, reduction, dx, dweight, dbias, workspace,
+                                              (hipStream_t)stream));
+}
+
+}  // extern "C"

@@ -1,0 +1,41 @@
+// What the token-level operators (layer_norm.hip, linear_ce.hip, muon.hip) share: element types, their conversions and the
+// reductions of a wave.  Element types of the C ABI: 0 = fp32, 1 = bf16, 2 = fp16.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+namespace ssecg_lm {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+enum { kF32 = 0, kB16 = 1, kF16 = 2 };
+inline bool dtype_ok(int t) { return t == kF32 || t == kB16 || t == kF16; }
+inline size_t dtype_size(int t) { return t == kF32 ? 4 : 2; }
+
+// 16 bytes of elements, at any alignment that the element itself has (the hardware takes unaligned global accesses)
+template <typename T> struct Vec;
+template <> struct Vec<float> { static constexpr int N = 4; typedef float type __attribute__((ext_vector_type(4), aligned(4))); };
+template <> struct Vec<__bf16> { static constexpr int N = 8; typedef __bf16 type __attribute__((ext_vector_type(8), aligned(2))); };
+template <> struct Vec<_Float16> { static constexpr int N = 8; typedef _Float16 type __attribute__((ext_vector_type(8), aligned(2))); };
+
+__device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    return v;
+}
+
+// calls f.template operator()<T>() with the element type of the ABI code
+#define SSECG_LM_DTYPE(code, T, ...)                                   \
+    do {                                                               \
+        if ((code) == ssecg_lm::kF32) { using T = float; __VA_ARGS__; }      \
+        else if ((code) == ssecg_lm::kB16) { using T = __bf16; __VA_ARGS__; } \
+        else { using T = _Float16; __VA_ARGS__; }                      \
+    } while (0)
+
+}  // namespace ssecg_lm

@@ -1,0 +1,482 @@
+// Orthogonalised updates of weight matrices: the quintic Newton-Schulz iteration and the optimiser step built on it, for many
+// matrices of any sizes in one chain of launches.
+//
+//   X = U / (|U|_F + eps), the shorter side first (m <= n);   repeat:  A = X X^T,  P = a I + b A + c A A,  X = P X
+//   optimiser: v = mu v + g,  U = g + mu v (Nesterov) or v,  p = p (1 - lr wd) - lr s X,  s = 0.2 sqrt(max(rows, cols)) or
+//   sqrt(max(1, rows / cols))
+//
+// Every product is mm_core.h's with k fastest in both operands.  A and P are symmetric, so they are their own transposes (and only
+// the tiles on and below the diagonal are computed); X is kept both ways round, X for A and X^T for the update, and the update's
+// epilogue writes both.  The identity is folded into P, so the update needs no third operand.
+//
+// Precision: the iteration multiplies errors along weak directions by up to a = 3.44 per step (485 over five), so 16-bit iterates
+// would lose them.  All matrices are two fp16 planes times 2^13 - singular values stay below 1.21 and P's below 3.45, far inside
+// fp16's range, and an entry keeps 22 bits down to 2^-16 of the largest possible one - with fp32 accumulators.
+#include "mm_core.h"
+#include "ssecg.h"
+
+namespace {
+using namespace ssecg_lm;
+
+constexpr float kA = 3.4445f, kB = -4.7750f, kC = 2.0315f;
+constexpr int kScale = 13;
+constexpr int kNormParts = 128;                   // workgroups that share one matrix's norm
+constexpr int kMost = 32;                         // matrices of one chain of launches: their table travels in the kernel arguments
+
+// By value in the kernel arguments (1.9 KB): no upload, nothing to keep for a captured launch.  first[w][k]: the first workgroup
+// of matrix k in the launch of kind w.
+enum { wPrep, wGram, wUpd };
+struct Table {
+    const void* src[kMost]; void* dst[kMost]; float* mom[kMost];
+    int64_t offset[kMost];                        // of the matrix's planes in the workspace
+    int rows[kMost], cols[kMost], first[3][kMost];
+    int count;
+};
+
+struct Mat {
+    const void* src; void* dst; float* mom;
+    int rows, cols, m, n;
+    int64_t pn, pm;                               // bytes of a row of X; of X^T, A and P
+    char *X, *Xt0, *Xt1, *A, *P;
+    int64_t planeX, planeXt, planeA;
+};
+
+inline __host__ __device__ int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
+
+// planes of one matrix in the workspace: X, X^T twice (read one, write the other), A, P
+inline __host__ __device__ int64_t mat_bytes(int64_t rows, int64_t cols) {
+    const int64_t m = rows < cols ? rows : cols, n = rows < cols ? cols : rows;
+    const int64_t pn = up(n, 32) * 2, pm = up(m, 32) * 2;
+    return up(2 * (m * pn + 2 * n * pm + 2 * m * pm), 256);
+}
+
+__device__ __forceinline__ Mat load_mat(const Table& table, int k, char* ws) {
+    Mat t;
+    t.src = table.src[k];
+    t.dst = table.dst[k];
+    t.mom = table.mom[k];
+    t.rows = table.rows[k];
+    t.cols = table.cols[k];
+    t.m = t.rows < t.cols ? t.rows : t.cols;
+    t.n = t.rows < t.cols ? t.cols : t.rows;
+    t.pn = up(t.n, 32) * 2;
+    t.pm = up(t.m, 32) * 2;
+    t.planeX = t.m * t.pn;
+    t.planeXt = t.n * t.pm;
+    t.planeA = t.m * t.pm;
+    t.X = ws + table.offset[k];
+    t.Xt0 = t.X + 2 * t.planeX;
+    t.Xt1 = t.Xt0 + 2 * t.planeXt;
+    t.A = t.Xt1 + 2 * t.planeXt;
+    t.P = t.A + 2 * t.planeA;
+    return t;
+}
+
+// the matrix whose workgroups of kind w hold workgroup q; every wave finds it by itself
+__device__ __forceinline__ int find_mat(const Table& table, int w, int q, int& first) {
+    const int lane = threadIdx.x & (kMost - 1);
+    const unsigned long long le = __ballot((threadIdx.x & 63) < kMost && lane < table.count && table.first[w][lane] <= q);
+    const int k = __builtin_amdgcn_readfirstlane(__popcll(le) - 1);
+    first = table.first[w][k];
+    return k;
+}
+
+// U of element i (momentum already advanced): Nesterov g + mu v, else v; without momentum g
+template <typename S, bool MUON>
+__device__ __forceinline__ float update_of(const Mat& t, int64_t i, float mu, int nesterov) {
+    const float g = (float)reinterpret_cast<const S*>(t.src)[i];
+    if (!MUON) return g;
+    const float v = t.mom[i];
+    return nesterov ? g + mu * v : v;
+}
+
+// momentum and the partial sums of |U|^2 (fp64: no gradient's scale overflows it); partial [count][kNormParts]
+template <typename S, bool MUON>
+__global__ __launch_bounds__(256) void ns_norm_kernel(Table table, float mu, int nesterov, const float* __restrict__ skip,
+                                                      double* __restrict__ partial) {
+    if (MUON && skip != nullptr && skip[0] != 0.f) return;
+    const Mat t = load_mat(table, blockIdx.y, nullptr);
+    const int64_t n = (int64_t)t.rows * t.cols;
+    double s = 0.0;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+        float u;
+        if (MUON) {
+            const float g = (float)reinterpret_cast<const S*>(t.src)[i], v = mu * t.mom[i] + g;
+            t.mom[i] = v;
+            u = nesterov ? g + mu * v : v;
+        } else {
+            u = (float)reinterpret_cast<const S*>(t.src)[i];
+        }
+        s += (double)u * (double)u;
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+    __shared__ double sh[4];
+    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) partial[(int64_t)blockIdx.y * kNormParts + blockIdx.x] = (sh[0] + sh[1]) + (sh[2] + sh[3]);
+}
+
+// U / (norm + eps) as planes, X and X^T; one workgroup: 64 x 64 elements, zeros up to the pitch
+template <typename S, bool MUON>
+__global__ __launch_bounds__(256) void ns_prep_kernel(Table table, char* __restrict__ ws, float mu, int nesterov,
+                                                      int parts, double eps, const float* __restrict__ skip, const double* __restrict__ partial) {
+    if (MUON && skip != nullptr && skip[0] != 0.f) return;
+    __shared__ uint32_t tile[64][65];
+    int first;
+    const int k = find_mat(table, wPrep, blockIdx.x, first);
+    const Mat t = load_mat(table, k, ws);
+    double s = 0.0;
+    const int lane = threadIdx.x & 63, strand = threadIdx.x >> 6;
+    for (int p = lane; p < parts; p += 64) s += partial[(int64_t)k * kNormParts + p];
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+    const float f = (float)((double)(1 << kScale) / (sqrt(s) + eps));
+    const int tiles = (int)((up(t.cols, 32) + 63) / 64), q0 = blockIdx.x - first;
+    const int64_t rb = (int64_t)(q0 / tiles) * 64, cb = (int64_t)(q0 % tiles) * 64;
+    for (int i = strand; i < 64; i += 4) {
+        const int64_t r = rb + i, c = cb + lane;
+        uint32_t q = 0;
+        if (r < t.rows && c < t.cols) {
+            _Float16 hi, lo;
+            split16(update_of<S, MUON>(t, r * t.cols + c, mu, nesterov) * f, hi, lo);
+            q = (uint32_t)__builtin_bit_cast(uint16_t, hi) | (uint32_t)__builtin_bit_cast(uint16_t, lo) << 16;
+        }
+        tile[i][lane] = q;
+    }
+    __syncthreads();
+    const bool tall = t.rows > t.cols;
+    char* D = tall ? t.Xt0 : t.X;               // as the matrix lies: rows x cols
+    char* Dt = tall ? t.X : t.Xt0;              // transposed: cols x rows
+    const int64_t pd = tall ? t.pm : t.pn, pt = tall ? t.pn : t.pm;
+    const int64_t ld = tall ? t.planeXt : t.planeX, lt = tall ? t.planeX : t.planeXt;
+    for (int u = threadIdx.x; u < 512; u += 256) {
+        const int i = u >> 3, c8 = (u & 7) * 8;
+        u32x4 a, b, ta, tb;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t p = tile[i][c8 + 2 * j], q = tile[i][c8 + 2 * j + 1];
+            a[j] = (p & 0xffffu) | q << 16;
+            b[j] = p >> 16 | (q & 0xffff0000u);
+            const uint32_t pp = tile[c8 + 2 * j][i], qq = tile[c8 + 2 * j + 1][i];
+            ta[j] = (pp & 0xffffu) | qq << 16;
+            tb[j] = pp >> 16 | (qq & 0xffff0000u);
+        }
+        if (rb + i < t.rows && (cb + c8) * 2 < pd) {
+            char* d = D + (rb + i) * pd + (cb + c8) * 2;
+            *reinterpret_cast<u32x4*>(d) = a;
+            *reinterpret_cast<u32x4*>(d + ld) = b;
+        }
+        if (cb + i < t.cols && (rb + c8) * 2 < pt) {
+            char* d = Dt + (cb + i) * pt + (rb + c8) * 2;
+            *reinterpret_cast<u32x4*>(d) = ta;
+            *reinterpret_cast<u32x4*>(d + lt) = tb;
+        }
+    }
+}
+
+__device__ __forceinline__ void store4(char* d, int64_t plane, const float (&v)[4]) {   // 4 values along k
+    _Float16 hi[4], lo[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) split16(v[k], hi[k], lo[k]);
+    u32x2 q;
+    __builtin_memcpy(&q, hi, 8);
+    *reinterpret_cast<u32x2*>(d) = q;
+    __builtin_memcpy(&q, lo, 8);
+    *reinterpret_cast<u32x2*>(d + plane) = q;
+}
+__device__ __forceinline__ void store1(char* d, int64_t plane, float v) {
+    _Float16 hi, lo;
+    split16(v, hi, lo);
+    *reinterpret_cast<_Float16*>(d) = hi;
+    *reinterpret_cast<_Float16*>(d + plane) = lo;
+}
+
+// Tile q of the lower triangle of a square of tiles: row ti >= column tj
+__device__ __forceinline__ void tri_tile(int q, int& ti, int& tj) {
+    ti = (int)((sqrtf(8.f * (float)q + 1.f) - 1.f) * 0.5f);
+    while (ti * (ti + 1) / 2 > q) --ti;
+    while ((ti + 1) * (ti + 2) / 2 <= q) ++ti;
+    tj = q - ti * (ti + 1) / 2;
+}
+
+// POLY = false: A = X X^T.  POLY = true: P = a I + b A + c A A.
+template <class M, bool POLY>
+__global__ __launch_bounds__(M::NT) void ns_gram_kernel(Table table, char* __restrict__ ws,
+                                                        const float* __restrict__ skip) {
+    if (skip != nullptr && skip[0] != 0.f) return;
+    __shared__ __attribute__((aligned(16))) char lds[M::LDS];
+    int first, ti, tj;
+    const int tile = xcd_tile(blockIdx.x, gridDim.x);
+    const Mat t = load_mat(table, find_mat(table, wGram, tile, first), ws);
+    tri_tile(tile - first, ti, tj);
+    const int a0 = ti * M::BM, b0 = tj * M::BN;
+    const int64_t pitch = POLY ? t.pm : t.pn, plane = POLY ? t.planeA : t.planeX;
+    const Operand op = {POLY ? t.A : t.X, pitch, plane, t.m};
+    f32x16 acc[M::TM][M::TN];
+    M::zero(acc);
+    M::run(op, a0, op, b0, 0, (int)(pitch / M::STEP), lds, acc);
+    char* out = POLY ? t.P : t.A;
+    constexpr float down = 1.f / (float)(1 << kScale);
+#pragma unroll
+    for (int j = 0; j < M::TN; ++j) {
+        const int c = b0 + M::bcol(j);
+#pragma unroll
+        for (int i = 0; i < M::TM; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+                const int r = a0 + M::arow(i, e);            // 4 consecutive rows
+                float v[4], w[4] = {0.f, 0.f, 0.f, 0.f};
+                if (POLY && c < t.m && r * 2 < t.pm) {       // A[r..r+3][c] = A[c][r..r+3]
+                    const char* s = t.A + (int64_t)c * t.pm + (int64_t)r * 2;
+                    _Float16 hi[4], lo[4];
+                    u32x2 q = *reinterpret_cast<const u32x2*>(s);
+                    __builtin_memcpy(hi, &q, 8);
+                    q = *reinterpret_cast<const u32x2*>(s + t.planeA);
+                    __builtin_memcpy(lo, &q, 8);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) w[k] = (float)hi[k] + (float)lo[k];
+                }
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    float d = acc[i][j][e + k] * down;
+                    if (POLY) d = kC * d + (kB * w[k] + (r + k == c ? kA * (float)(1 << kScale) : 0.f));
+                    v[k] = r + k < t.m && c < t.m ? d : 0.f;
+                }
+                if (c < t.m && r * 2 < t.pm) {
+                    // below the diagonal: the mirrored tile as well, rows and columns exchanged
+                    if (ti != tj) {
+                        store4(out + (int64_t)c * t.pm + (int64_t)r * 2, t.planeA, v);
+                    }
+                }
+                if (c * 2 < t.pm) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        if (r + k < t.m) store1(out + (int64_t)(r + k) * t.pm + (int64_t)c * 2, t.planeA, v[k]);
+                }
+            }
+    }
+}
+
+struct Apply {                                    // the optimiser's half of the last product
+    double lr, weight_decay;
+    int adjust;                                   // 0: sqrt(max(1, rows / cols)); 1: 0.2 sqrt(max(rows, cols))
+    const double* lr_dev;
+};
+
+// X = P X: planes both ways round (from X^T number `from` to the other), or the last one: the result / the parameter's update
+template <class M, typename S, int LAST>          // LAST: 0 = planes, 1 = result, 2 = optimiser
+__global__ __launch_bounds__(M::NT) void ns_update_kernel(Table table, char* __restrict__ ws, int from, Apply ap,
+                                                          const float* __restrict__ skip) {
+    if (skip != nullptr && skip[0] != 0.f) return;
+    __shared__ __attribute__((aligned(16))) char lds[M::LDS];
+    int first;
+    const int tile = xcd_tile(blockIdx.x, gridDim.x);
+    const Mat t = load_mat(table, find_mat(table, wUpd, tile, first), ws);
+    const int tm = (t.m + M::BM - 1) / M::BM, q = tile - first;
+    const int a0 = q % tm * M::BM, b0 = q / tm * M::BN;
+    const Operand P = {t.P, t.pm, t.planeA, t.m}, Xt = {(from ? t.Xt1 : t.Xt0), t.pm, t.planeXt, t.n};
+    f32x16 acc[M::TM][M::TN];
+    M::zero(acc);
+    M::run(P, a0, Xt, b0, 0, (int)(t.pm / M::STEP), lds, acc);
+    constexpr float down = 1.f / (float)(1 << kScale);
+    char* to = from ? t.Xt0 : t.Xt1;
+    const bool tall = t.rows > t.cols;
+    float step = 0.f, keep = 0.f;
+    if (LAST == 2) {
+        const double lr = ap.lr_dev != nullptr ? ap.lr_dev[0] : ap.lr;
+        const double s = ap.adjust == 1 ? 0.2 * sqrt((double)t.n) : sqrt(t.rows > t.cols ? (double)t.rows / (double)t.cols : 1.0);
+        step = (float)(lr * s);
+        keep = (float)(1.0 - lr * ap.weight_decay);
+    }
+#pragma unroll
+    for (int j = 0; j < M::TN; ++j) {
+        const int c = b0 + M::bcol(j);
+#pragma unroll
+        for (int i = 0; i < M::TM; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+                const int r = a0 + M::arow(i, e);
+                if (LAST == 0) {
+                    float v[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) v[k] = r + k < t.m && c < t.n ? acc[i][j][e + k] * down : 0.f;
+                    if (c < t.n && r * 2 < t.pm) store4(to + (int64_t)c * t.pm + (int64_t)r * 2, t.planeXt, v);
+                    if (c * 2 < t.pn) {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            if (r + k < t.m) store1(t.X + (int64_t)(r + k) * t.pn + (int64_t)c * 2, t.planeX, v[k]);
+                    }
+                } else if (c < t.n) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        if (r + k < t.m) {
+                            const float v = acc[i][j][e + k] * (down * down);
+                            const int64_t at = tall ? (int64_t)c * t.cols + r + k : (int64_t)(r + k) * t.cols + c;
+                            if (LAST == 1) {
+                                reinterpret_cast<S*>(t.dst)[at] = (S)v;
+                            } else {
+                                float* p = reinterpret_cast<float*>(t.dst) + at;
+                                *p = *p * keep - step * v;
+                            }
+                        }
+                }
+            }
+    }
+}
+
+using Big = MmTile<_Float16, 2, 256, 256, 2, 4, 2>;
+using Mid = MmTile<_Float16, 2, 128, 128, 2, 2, 2>;
+using Small = MmTile<_Float16, 2, 64, 64, 2, 2, 4>;
+
+#define SSECG_NS_LAUNCH(M, kernel, grid, st, ...)                                                                               \
+    do {                                                                                                                        \
+        hipLaunchKernelGGL(kernel, dim3((unsigned)(grid)), dim3(M::NT), 0, st, __VA_ARGS__);                               \
+        const int rc_ = (int)hipGetLastError();                                                                                 \
+        if (rc_ != 0) return rc_;                                                                                               \
+    } while (0)
+
+struct Plan {
+    size_t bytes;
+    int prep, gram, upd, gramTile, updTile;       // workgroups of the launches and tile sides
+};
+
+template <bool POLY>
+int launch_gram(const Table& t, const Plan& p, char* ws, const float* skip, hipStream_t st) {
+    if (p.gramTile == 256) SSECG_NS_LAUNCH(Big, (ns_gram_kernel<Big, POLY>), p.gram, st, t, ws, skip);
+    else if (p.gramTile == 128) SSECG_NS_LAUNCH(Mid, (ns_gram_kernel<Mid, POLY>), p.gram, st, t, ws, skip);
+    else SSECG_NS_LAUNCH(Small, (ns_gram_kernel<Small, POLY>), p.gram, st, t, ws, skip);
+    return 0;
+}
+
+template <typename S, int LAST>
+int launch_update(const Table& t, const Plan& p, char* ws, int from, const Apply& ap, const float* skip, hipStream_t st) {
+    if (p.updTile == 256) SSECG_NS_LAUNCH(Big, (ns_update_kernel<Big, S, LAST>), p.upd, st, t, ws, from, ap, skip);
+    else if (p.updTile == 128) SSECG_NS_LAUNCH(Mid, (ns_update_kernel<Mid, S, LAST>), p.upd, st, t, ws, from, ap, skip);
+    else SSECG_NS_LAUNCH(Small, (ns_update_kernel<Small, S, LAST>), p.upd, st, t, ws, from, ap, skip);
+    return 0;
+}
+
+// mats: host rows {source, result or parameter, momentum, rows, cols} of at most kMost matrices
+int make_plan(const int64_t* mats, int count, Table& t, Plan& p) {
+    auto tiles = [&](int64_t side, bool gram) {
+        int64_t s = 0;
+        for (int k = 0; k < count; ++k) {
+            const int64_t a = mats[5 * k + 3], b = mats[5 * k + 4], m = a < b ? a : b, n = a < b ? b : a;
+            const int64_t tm = (m + side - 1) / side, tn = (n + side - 1) / side;
+            s += gram ? tm * (tm + 1) / 2 : tm * tn;
+        }
+        return s;
+    };
+    // the largest tile that still gives each of the 256 CUs one
+    auto pick = [&](bool gram) { return tiles(256, gram) >= 256 ? 256 : (tiles(128, gram) >= 256 ? 128 : 64); };
+    p.gramTile = pick(true);
+    p.updTile = pick(false);
+    t.count = count;
+    int64_t at = up((int64_t)kMost * kNormParts * 8, 256), prep = 0, gram = 0, upd = 0;
+    for (int k = 0; k < kMost; ++k) {
+        const int64_t a = k < count ? mats[5 * k + 3] : 0, b = k < count ? mats[5 * k + 4] : 0, m = a < b ? a : b, n = a < b ? b : a;
+        t.src[k] = k < count ? (const void*)mats[5 * k] : nullptr;
+        t.dst[k] = k < count ? (void*)mats[5 * k + 1] : nullptr;
+        t.mom[k] = k < count ? (float*)mats[5 * k + 2] : nullptr;
+        t.rows[k] = (int)a;
+        t.cols[k] = (int)b;
+        t.offset[k] = at;
+        t.first[wPrep][k] = (int)prep;
+        t.first[wGram][k] = (int)gram;
+        t.first[wUpd][k] = (int)upd;
+        if (k >= count) continue;
+        const int64_t tg = (m + p.gramTile - 1) / p.gramTile;
+        at += mat_bytes(a, b);
+        prep += ((up(a, 32) + 63) / 64) * ((up(b, 32) + 63) / 64);
+        gram += tg * (tg + 1) / 2;
+        upd += ((m + p.updTile - 1) / p.updTile) * ((n + p.updTile - 1) / p.updTile);
+        if (prep >= INT32_MAX || gram >= INT32_MAX || upd >= INT32_MAX) return SSECG_E_INVAL;
+    }
+    p.bytes = (size_t)at;
+    p.prep = (int)prep;
+    p.gram = (int)gram;
+    p.upd = (int)upd;
+    return 0;
+}
+
+template <typename S, bool MUON>
+int run_chain(const int64_t* mats, int count, float mu, int nesterov, int steps, double eps, const Apply& ap, const float* skip, char* ws,
+              hipStream_t st) {
+    Table t;
+    Plan p;
+    int rc = make_plan(mats, count, t, p);
+    if (rc != 0) return rc;
+    double* partial = reinterpret_cast<double*>(ws);
+    hipLaunchKernelGGL((ns_norm_kernel<S, MUON>), dim3(kNormParts, count), dim3(256), 0, st, t, mu, nesterov, skip, partial);
+    hipLaunchKernelGGL((ns_prep_kernel<S, MUON>), dim3((unsigned)p.prep), dim3(256), 0, st, t, ws, mu, nesterov, kNormParts, eps, skip, partial);
+    rc = (int)hipGetLastError();
+    for (int k = 0; k < steps && rc == 0; ++k) {
+        if ((rc = launch_gram<false>(t, p, ws, skip, st)) != 0) break;
+        if ((rc = launch_gram<true>(t, p, ws, skip, st)) != 0) break;
+        if (k + 1 < steps) rc = launch_update<S, 0>(t, p, ws, k & 1, ap, skip, st);
+        else rc = launch_update<S, MUON ? 2 : 1>(t, p, ws, k & 1, ap, skip, st);
+    }
+    return rc;
+}
+
+constexpr int64_t kMaxSide = 1 << 20;
+
+bool mats_ok(const int64_t* mats, int count, bool pointers, bool muon) {
+    if (!mats || count <= 0) return false;
+    for (int k = 0; k < count; ++k) {
+        const int64_t* r = mats + 5 * (size_t)k;
+        if (r[3] <= 0 || r[4] <= 0 || r[3] > kMaxSide || r[4] > kMaxSide) return false;
+        if (pointers && (!r[0] || !r[1] || (muon && !r[2]))) return false;
+    }
+    return true;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t ssecg_orthogonalize_workspace(const int64_t* mats, int count) {
+    if (!mats_ok(mats, count, false, false)) return 0;
+    size_t most = 0;
+    for (int k = 0; k < count; k += kMost) {
+        Table t;
+        Plan p;
+        if (make_plan(mats + 5 * (size_t)k, count - k < kMost ? count - k : kMost, t, p) != 0) return 0;
+        most = p.bytes > most ? p.bytes : most;
+    }
+    return most;
+}
+
+int ssecg_orthogonalize_multi(const int64_t* mats, int count, int dtype, int steps, double eps, void* workspace, size_t workspace_bytes,
+                              void* stream) {
+    if (!mats_ok(mats, count, true, false) || !dtype_ok(dtype) || steps < 1 || steps > 100 || !(eps >= 0.0) || !workspace ||
+        ((uintptr_t)workspace & 255))
+        return SSECG_E_INVAL;
+    if (workspace_bytes < ssecg_orthogonalize_workspace(mats, count)) return SSECG_E_WORKSPACE;
+    const Apply ap = {};
+    for (int k = 0; k < count; k += kMost) {
+        int rc = 0;
+        SSECG_LM_DTYPE(dtype, S, rc = (run_chain<S, false>(mats + 5 * (size_t)k, count - k < kMost ? count - k : kMost, 0.f, 0, steps, eps, ap, nullptr,
+                                                          (char*)workspace, (hipStream_t)stream)));
+        if (rc != 0) return rc;
+    }
+    return 0;
+}
+
+int ssecg_muon_multi(const int64_t* mats, int count, double lr, double momentum, int nesterov, double weight_decay, int adjust, int steps, double eps,
+                     const float* skip_flag, const double* lr_dev, void* workspace, size_t workspace_bytes, void* stream) {
+    if (!mats_ok(mats, count, true, true) || steps < 1 || steps > 100 || !(eps >= 0.0) || !(momentum >= 0.0 && momentum < 1.0) || adjust < 0 ||
+        adjust > 1 || !workspace || ((uintptr_t)workspace & 255))
+        return SSECG_E_INVAL;
+    if (workspace_bytes < ssecg_orthogonalize_workspace(mats, count)) return SSECG_E_WORKSPACE;
+    const Apply ap = {lr, weight_decay, adjust, lr_dev};
+    for (int k = 0; k < count; k += kMost) {
+        const int rc = run_chain<float, true>(mats + 5 * (size_t)k, count - k < kMost ? count - k : kMost, (float)momentum, nesterov != 0, steps, eps, ap,
+                                              skip_flag, (char*)workspace, (hipStream_t)stream);
+        if (rc != 0) return rc;
+    }
+    return 0;
+}
+
+}  // extern "C"

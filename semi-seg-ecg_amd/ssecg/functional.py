@@ -21,6 +21,7 @@ from typing import Optional
 
 import torch
 import torch.distributed as dist
+from torch.autograd.function import once_differentiable
 
 from . import config, ops
 
@@ -681,6 +682,31 @@ def batch_norm(x, bn_module):
     return BatchNormFn.apply(x, bn_module.weight, bn_module.bias, BNState.of(bn_module), bn_module.training)
 
 
+class LayerNormFn(torch.autograd.Function):
+    """Layer norm over the last axis (``ops.layer_norm_fwd`` / ``_bwd``); the row's mean and 1 / deviation are kept, not xhat."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps):
+        y, mean, rstd = ops.layer_norm_fwd(x, weight, bias, eps)
+        ctx.save_for_backward(x, mean, rstd, weight, bias)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, mean, rstd, weight, bias = ctx.saved_tensors
+        params = ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
+        dx, dw, db = ops.layer_norm_bwd(dy, x, mean, rstd, weight, want_params=params)
+        dw = dw.to(weight.dtype) if ctx.needs_input_grad[1] else None
+        db = db.to(bias.dtype) if ctx.needs_input_grad[2] else None
+        return dx, dw, db, None
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5):
+    """x (..., C) fp32 / bf16 / fp16, weight / bias (C,) or None -> y of x's type; statistics and parameter gradients in fp32."""
+    return LayerNormFn.apply(x, weight, bias, float(eps))
+
+
 class ReLUFn(torch.autograd.Function):
     """Standalone ReLU (any shape) through the BN kernels with identity coefficients; off the hot path (see BatchNormFn)."""
 
@@ -773,6 +799,39 @@ def masked_cross_entropy(logits, target, conf, thresh):
     """(F.cross_entropy(.., reduction='none') * (conf >= thresh)).mean()  (fixmatch.py:114-116).
     -> (loss, stat) with stat = [loss, mask_ratio] on device."""
     return _CEHardFn.apply(logits, target, conf, float(thresh), float(logits.shape[0] * logits.shape[2]))
+
+
+class _LinearCEFn(torch.autograd.Function):
+    """Classifier and cross entropy in one node: the logits exist in neither pass (``ops.linear_ce_fwd`` / ``_bwd``)."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, target, conf, thresh, ignore_index, reduction):
+        loss, saved = ops.linear_ce_fwd(x, weight, target, bias, conf, thresh, ignore_index, reduction)
+        ctx.save_for_backward(x, weight, bias, *saved[3:7])
+        ctx.reduction = saved.reduction
+        return loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dloss):
+        x, weight, bias, target, lse, gate, count = ctx.saved_tensors
+        f32_bias = None if bias is None else bias.float().contiguous()
+        saved = ops.LinearCE(x.contiguous(), weight.contiguous(), f32_bias, target, lse, gate, count, ctx.reduction)
+        need = ctx.needs_input_grad
+        dx, dw, db = ops.linear_ce_bwd(saved, dloss, need[0], need[1], need[2])
+        return dx, dw, db.to(bias.dtype) if db is not None else None, None, None, None, None, None
+
+
+def linear_cross_entropy(x, weight, target, bias=None, ignore_index=-100, reduction="mean"):
+    """``cross_entropy(x @ weight.T + bias, target)`` for any number of classes, without the logits: x (..., C), weight (V, C) of one
+    type (fp32, bf16, fp16), target (...) int64."""
+    return _LinearCEFn.apply(x, weight, bias, target, None, 0.0, int(ignore_index), reduction)
+
+
+def masked_linear_cross_entropy(x, weight, target, conf, thresh, bias=None, ignore_index=-100, reduction="mean"):
+    """``linear_cross_entropy`` whose rows are weighted by (conf >= thresh), as FixMatch weights its pseudo-labels
+    (fixmatch.py:114-116); the mean divides by the number of positions that are not ignored."""
+    return _LinearCEFn.apply(x, weight, bias, target, conf, float(thresh), int(ignore_index), reduction)
 
 
 class _CESoftFn(torch.autograd.Function):

@@ -77,6 +77,29 @@ class BatchNorm1d(nn.BatchNorm1d):
         return SF.batch_norm(x, self)
 
 
+class LayerNorm(nn.Module):
+    """nn.LayerNorm over the last axis: its parameters (``weight``, ``bias``), its init (ones, zeros)."""
+
+    def __init__(self, normalized_shape, eps=1e-5, elementwise_affine=True, bias=True, device=None, dtype=None):
+        super().__init__()
+        shape = (normalized_shape,) if isinstance(normalized_shape, int) else tuple(normalized_shape)
+        if len(shape) != 1:
+            raise NotImplementedError("LayerNorm: the last axis only")
+        self.normalized_shape, self.eps, self.elementwise_affine = shape, eps, elementwise_affine
+        kw = {"device": device, "dtype": dtype}
+        self.weight = nn.Parameter(torch.ones(shape, **kw)) if elementwise_affine else None
+        self.bias = nn.Parameter(torch.zeros(shape, **kw)) if elementwise_affine and bias else None
+
+    def extra_repr(self):
+        return f"{self.normalized_shape}, eps={self.eps}, elementwise_affine={self.elementwise_affine}, bias={self.bias is not None}"
+
+    def forward(self, x):
+        from . import functional as SF
+        if tuple(x.shape[-1:]) != self.normalized_shape:
+            raise ValueError(f"LayerNorm: expected (..., {self.normalized_shape[0]}), got {tuple(x.shape)}")
+        return SF.layer_norm(x, self.weight, self.bias, self.eps)
+
+
 class ReLU(nn.Module):
     """Keeps the reference's module indices (stem.2, convs.0.2); fused into the units on the hot path, a standalone call
     runs ``functional.relu``."""

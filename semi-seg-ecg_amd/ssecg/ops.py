@@ -7,7 +7,10 @@ product path has no CPU implementation.
 """
 from __future__ import annotations
 
+import contextlib
+import ctypes
 import weakref
+from typing import NamedTuple, Optional
 
 import torch
 
@@ -1310,6 +1313,228 @@ def pack_scaled_multi(table, ntensors, max_numel, dst, scale):
     trace("pack_scaled_multi", (ntensors,))
     dst = _req(dst, "dst")
     check(lib().ssecg_pack_scaled_multi(_p(table), ntensors, max_numel, _p(dst), float(scale), _stream()), "ssecg_pack_scaled_multi")
+
+
+# ----------------------------------------------------------------------------- token-level operators
+_LM_DTYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_REDUCTION = {"none": 0, "mean": 1, "sum": 2}
+
+
+def _lm(t, name, dtype=None):
+    """A contiguous fp32 / bf16 / fp16 device tensor (of type ``dtype`` where given)."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise SsecgError(f"{name}: expected a HIP device tensor (the MI355X hot path has no CPU fallback)")
+    if t.dtype not in _LM_DTYPE:
+        raise SsecgError(f"{name}: expected fp32, bf16 or fp16, got {t.dtype}")
+    if dtype is not None and t.dtype != dtype:
+        raise SsecgError(f"{name}: expected dtype {dtype}, got {t.dtype}")
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _lm_vec(t, name, n, like):
+    """A parameter vector of ``n`` values as fp32 on ``like``'s device; None stays None."""
+    if t is None:
+        return None
+    t = _lm(t, name)
+    if t.numel() != n or t.dim() != 1:
+        raise SsecgError(f"{name}: expected ({n},), got {tuple(t.shape)}")
+    _lm_device(like, **{name: t})
+    return t.float()
+
+
+def _lm_device(ref, **tensors):
+    for name, t in tensors.items():
+        if t is not None and t.device != ref.device:
+            raise SsecgError(f"{name}: on {t.device}, expected {ref.device}")
+
+
+def _lm_guard(t):
+    """The launches of a call go to the current stream of ITS tensors' device."""
+    return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+def layer_norm_fwd(x, weight=None, bias=None, eps=1e-5):
+    """Layer norm over the last axis of x (..., C) -> (y of x's type, mean, rstd); mean and rstd are fp32, one per row.
+    ``weight`` / ``bias``: (C,), None = 1 / 0."""
+    trace("layer_norm_fwd", tuple(getattr(x, "shape", ())))
+    x = _lm(x, "x")
+    if x.dim() < 1 or x.shape[-1] == 0:
+        raise SsecgError("layer_norm: x must be (..., C) with C > 0")
+    if not eps >= 0:
+        raise SsecgError("layer_norm: eps must not be negative")
+    C = x.shape[-1]
+    rows = x.numel() // C
+    weight, bias = _lm_vec(weight, "weight", C, x), _lm_vec(bias, "bias", C, x)
+    y = torch.empty_like(x)
+    mean, rstd = torch.empty((2, rows), device=x.device, dtype=torch.float32).unbind(0)
+    if rows:
+        with _lm_guard(x), _Timed("ln_fwd_kernel", 0.0, 2.0 * x.numel() * x.element_size()):
+            check(lib().ssecg_layer_norm_fwd(_p(x), _p(weight), _p(bias), _LM_DTYPE[x.dtype], rows, C, float(eps), _p(y), _p(mean),
+                                             _p(rstd), _stream()), "ssecg_layer_norm_fwd")
+    return y, mean, rstd
+
+
+def layer_norm_bwd(dy, x, mean, rstd, weight=None, want_params=True):
+    """-> (dx of x's type, dweight, dbias in fp32 or None): the backward pass of ``layer_norm_fwd``."""
+    trace("layer_norm_bwd", tuple(getattr(x, "shape", ())))
+    x = _lm(x, "x")
+    dy = _lm(dy, "dy", x.dtype)
+    if dy.shape != x.shape or x.dim() < 1 or x.shape[-1] == 0:
+        raise SsecgError("layer_norm_bwd: dy and x must both be (..., C)")
+    C = x.shape[-1]
+    rows = x.numel() // C
+    mean, rstd = _req(mean, "mean"), _req(rstd, "rstd")
+    if mean.numel() != rows or rstd.numel() != rows:
+        raise SsecgError("layer_norm_bwd: mean and rstd must hold one value per row")
+    _lm_device(x, dy=dy, mean=mean, rstd=rstd)
+    weight = _lm_vec(weight, "weight", C, x)
+    dx = torch.empty_like(x)
+    dw = db = ws = None
+    if want_params:
+        dw, db = (torch.empty if rows else torch.zeros)((2, C), device=x.device, dtype=torch.float32).unbind(0)
+    if rows:
+        Lb, code = lib(), _LM_DTYPE[x.dtype]
+        with _lm_guard(x), _Timed("ln_bwd_kernel", 0.0, 3.0 * x.numel() * x.element_size()):
+            if want_params:
+                ws = torch.empty((Lb.ssecg_layer_norm_bwd_workspace(code, rows, C),), device=x.device, dtype=torch.uint8)
+            check(Lb.ssecg_layer_norm_bwd(_p(dy), _p(x), _p(mean), _p(rstd), _p(weight), code, rows, C, _p(dx), _p(dw), _p(db), _p(ws),
+                                          ws.numel() if ws is not None else 0, _stream()), "ssecg_layer_norm_bwd")
+    return dx, dw, db
+
+
+class LinearCE(NamedTuple):
+    """What ``linear_ce_bwd`` needs of ``linear_ce_fwd``: the operands and, per position, log-sum-exp and gate."""
+    x: torch.Tensor
+    weight: torch.Tensor
+    bias: Optional[torch.Tensor]
+    target: torch.Tensor
+    lse: torch.Tensor
+    gate: torch.Tensor
+    count: torch.Tensor
+    reduction: int
+
+
+def linear_ce_fwd(x, weight, target, bias=None, conf=None, thresh=0.0, ignore_index=-100, reduction="mean"):
+    """Cross entropy of the classifier ``x @ weight.T + bias`` without its logits -> (loss, LinearCE).
+
+    x (..., C) and weight (V, C) of one type (fp32, bf16, fp16), target (...) int64, bias (V,).  A position counts if its target is
+    not ``ignore_index`` and, with ``conf`` (...) given, its confidence reaches ``thresh`` (FixMatch's mask); what x holds at the
+    others does not matter.  reduction "mean": over the positions that are not ignored (the confidence does not change the divisor; 0
+    if there is none), "sum", or "none": one value per position.  A target outside [0, V) makes its loss and gradient NaN."""
+    trace("linear_ce_fwd", tuple(getattr(x, "shape", ())), tuple(getattr(weight, "shape", ())))
+    x = _lm(x, "x")
+    weight = _lm(weight, "weight", x.dtype)
+    target = _req(target, "target", torch.int64)
+    if reduction not in _REDUCTION:
+        raise SsecgError(f"linear_ce: reduction {reduction!r}, expected one of {tuple(_REDUCTION)}")
+    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1] or x.shape[-1] == 0 or weight.shape[0] == 0:
+        raise SsecgError("linear_ce: x must be (..., C) and weight (V, C)")
+    if target.shape != x.shape[:-1]:
+        raise SsecgError("linear_ce: target must have x's shape without its last axis")
+    (V, C), N, mode = weight.shape, target.numel(), _REDUCTION[reduction]
+    bias = _lm_vec(bias, "bias", V, x)
+    if conf is not None:
+        conf = _req(conf, "conf")
+        if conf.shape != target.shape:
+            raise SsecgError("linear_ce: conf must have target's shape")
+    _lm_device(x, weight=weight, target=target, conf=conf)
+    loss = torch.empty(target.shape if mode == 0 else (), device=x.device, dtype=torch.float32)
+    lse, gate = torch.empty((2, N), device=x.device, dtype=torch.float32).unbind(0)
+    count = torch.empty((1,), device=x.device, dtype=torch.float32)
+    if N:
+        Lb, code = lib(), _LM_DTYPE[x.dtype]
+        with _lm_guard(x), _Timed("ce_lse_kernel", 2.0 * N * C * V, (N + V) * C * x.element_size()):
+            ws = torch.empty((Lb.ssecg_linear_ce_fwd_workspace(code, N, C, V),), device=x.device, dtype=torch.uint8)
+            check(Lb.ssecg_linear_ce_fwd(_p(x), _p(weight), _p(bias), _p(target), _p(conf), float(thresh), int(ignore_index), code, N, C, V,
+                                         mode, _p(loss), _p(lse), _p(gate), _p(count), _p(ws), ws.numel(), _stream()), "ssecg_linear_ce_fwd")
+    else:
+        loss.zero_()
+        count.fill_(1)
+    return loss, LinearCE(x, weight, bias, target, lse, gate, count, mode)
+
+
+def linear_ce_bwd(saved, dloss=None, want_dx=True, want_dweight=True, want_dbias=True):
+    """-> (dx, dweight of their operands' type, dbias in fp32): gradients of ``linear_ce_fwd``'s loss times ``dloss`` (a device scalar,
+    or one value per position for reduction "none"; None = 1).  What is not wanted (or has no bias) is None."""
+    x, weight, bias, target, lse, gate, count, mode = saved
+    trace("linear_ce_bwd", tuple(x.shape), tuple(weight.shape))
+    (V, C), N = weight.shape, target.numel()
+    shape = target.shape if mode == 0 else ()
+    if dloss is None:
+        dloss = torch.ones(shape, device=x.device, dtype=torch.float32)
+    dloss = _req(dloss, "dloss")
+    if dloss.numel() != (N if mode == 0 else 1):
+        raise SsecgError(f"linear_ce_bwd: dloss must be {tuple(shape)}, got {tuple(dloss.shape)}")
+    _lm_device(x, dloss=dloss)
+    want_dbias = want_dbias and bias is not None
+    make = torch.empty if N else torch.zeros
+    dx = torch.empty_like(x) if want_dx else None
+    dw = make(weight.shape, device=x.device, dtype=weight.dtype) if want_dweight else None
+    db = make((V,), device=x.device, dtype=torch.float32) if want_dbias else None
+    if N and (want_dx or want_dweight or want_dbias):
+        Lb, code = lib(), _LM_DTYPE[x.dtype]
+        flops = 2.0 * N * C * V * (1 + bool(want_dx) + bool(want_dweight))
+        with _lm_guard(x), _Timed("ce_grad_kernel + ce_prod_kernel", flops, 2.0 * (N + V) * C * x.element_size()):
+            ws = torch.empty((Lb.ssecg_linear_ce_bwd_workspace(code, N, C, V, int(want_dx), int(want_dweight), int(want_dbias)),),
+                             device=x.device, dtype=torch.uint8)
+            check(Lb.ssecg_linear_ce_bwd(_p(dloss), _p(x), _p(weight), _p(bias), _p(target), _p(lse), _p(gate), _p(count), code, N, C, V, mode,
+                                         _p(dx), _p(dw), _p(db), _p(ws), ws.numel(), _stream()), "ssecg_linear_ce_bwd")
+    return dx, dw, db
+
+
+def _mats(rows):
+    """Rows {source, result, momentum, rows, cols} as the host array the library reads during the call."""
+    flat = [v for r in rows for v in r]
+    return (ctypes.c_int64 * len(flat))(*flat)
+
+
+def orthogonalize(matrices, steps=5, eps=1e-7):
+    """The Newton-Schulz iterate of each matrix near its orthogonal factor (singular values about 0.7 .. 1.2), of the matrix's type.
+    ``matrices``: one (m, n) tensor or a list of them, all of one type on one device; a list is one chain of launches per 32
+    matrices.  X = G / (|G|_F + eps), ``steps`` times X = a X + (b A + c A A) X with A = X X^T."""
+    one = isinstance(matrices, torch.Tensor)
+    mats = [matrices] if one else list(matrices)
+    trace("orthogonalize", [tuple(getattr(m, "shape", ())) for m in mats])
+    if not 1 <= int(steps) <= 100 or not eps >= 0:
+        raise SsecgError("orthogonalize: steps must lie in 1 .. 100 and eps must not be negative")
+    if not mats:
+        return []
+    mats = [_lm(m, "matrix", mats[0].dtype if i else None) for i, m in enumerate(mats)]
+    for m in mats:
+        if m.dim() != 2:
+            raise SsecgError(f"orthogonalize: expected matrices, got {tuple(m.shape)}")
+        _lm_device(mats[0], matrix=m)
+    out = [torch.empty_like(m) for m in mats]
+    rows = [(m.data_ptr(), o.data_ptr(), 0, m.shape[0], m.shape[1]) for m, o in zip(mats, out) if m.numel()]
+    if rows:
+        Lb, arr = lib(), _mats(rows)
+        with _lm_guard(mats[0]), _Timed("ns_gram_kernel + ns_update_kernel", _ortho_flops(rows, steps),
+                                        2.0 * mats[0].element_size() * sum(m.numel() for m in mats)):
+            nbytes = Lb.ssecg_orthogonalize_workspace(arr, len(rows))
+            ws = torch.empty((max(nbytes, 256),), device=mats[0].device, dtype=torch.uint8)
+            check(Lb.ssecg_orthogonalize_multi(arr, len(rows), _LM_DTYPE[mats[0].dtype], int(steps), float(eps), _p(ws), ws.numel(),
+                                               _stream()), "ssecg_orthogonalize_multi")
+    return out[0] if one else out
+
+
+def _ortho_flops(rows, steps):
+    if PROFILE is None:
+        return 0.0
+    sizes = [(min(r[3], r[4]), max(r[3], r[4])) for r in rows]
+    return float(steps * sum(m * (m + 1) * n + m * m * (m + 1) + 2 * m * m * n for m, n in sizes))
+
+
+def muon_multi(rows, device, lr, momentum, nesterov, weight_decay, adjust, steps, eps, skip_flag=None, refresh=None):
+    """One step of ``ssecg_muon_multi`` on rows {gradient, parameter, momentum, rows, cols} (fp32, contiguous).  ``skip_flag``: as in
+    ``adamw_multi``."""
+    weights_changed()
+    trace("muon_multi", len(rows))
+    Lb, arr = lib(), _mats(rows)
+    lr_dev = STEP_SCALARS.lr_slot(lr, refresh) if STEP_SCALARS is not None else None
+    ws = torch.empty((max(Lb.ssecg_orthogonalize_workspace(arr, len(rows)), 256),), device=device, dtype=torch.uint8)
+    with _Timed("ns_gram_kernel + ns_update_kernel", _ortho_flops(rows, steps), 20.0 * sum(r[3] * r[4] for r in rows)):
+        check(Lb.ssecg_muon_multi(arr, len(rows), float(lr), float(momentum), int(bool(nesterov)), float(weight_decay), int(adjust), int(steps),
+                                  float(eps), _p(skip_flag), lr_dev, _p(ws), ws.numel(), _stream()), "ssecg_muon_multi")
 
 
 # ----------------------------------------------------------------------------- record pipeline (SURVEY.md 8f N1)

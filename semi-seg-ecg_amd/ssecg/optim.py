@@ -1,4 +1,4 @@
-"""Multi-tensor AdamW and EMA on the HIP kernels.
+"""Multi-tensor AdamW, SGD, Muon and EMA on the HIP kernels.
 
 ``FusedAdamW`` is a ``torch.optim.Optimizer`` whose ``state_dict`` has the layout
 of ``torch.optim.AdamW`` (per-parameter ``step`` / ``exp_avg`` / ``exp_avg_sq``) so
@@ -138,40 +138,106 @@ class FusedAdamW(_FusedOptimizer):
                 loss = closure()
         for gi, group in enumerate(self.param_groups):
             plist = self._plist(group)
-            if not plist:
-                continue
+            if plist:
+                self._adamw_group(gi, group, plist, found_inf)
+        return loss
+
+    def _adamw_group(self, gi, group, plist, found_inf):
+        """One launch: AdamW on ``plist``, parameters of group ``gi``."""
+        for p in plist:
+            st = self.state[p]
+            if len(st) == 0:
+                st["step"] = torch.tensor(0.0, dtype=torch.float32)
+                st["exp_avg"] = torch.zeros_like(p, memory_format=torch.preserve_format)
+                st["exp_avg_sq"] = torch.zeros_like(p, memory_format=torch.preserve_format)
+        table, max_numel = self._table(gi, plist)
+        skipped = self._skipped_counter(plist[0].device) if found_inf is not None else self._skipped
+        if skipped is not None and len(self._skips_applied) != len(self.param_groups):
+            skipped = self._skipped_counter(plist[0].device)     # a param group was added
+
+        def host_step(gi=gi, group=group, plist=plist, counted=skipped is not None):
+            """The host half of one step of this group: advance the per-parameter ``step`` -> the launch's scalars.  Also
+            the refresh hook of a step captured in a HIP graph (ssecg/graph.py): a replay runs this and nothing else."""
+            steps = {int(self.state[p]["step"].item()) for p in plist}  # CPU scalars: no device sync
+            if len(steps) != 1:
+                raise SsecgError(f"{type(self).__name__}: parameters of one group must share a step count")
+            t = steps.pop() + 1
             for p in plist:
+                self.state[p]["step"] += 1
+            b1, b2 = group["betas"]
+            # ``t`` counts launches; the ones the device skipped are subtracted in the kernel (bias corrections) and, at
+            # checkpoint time, from the per-parameter ``step`` (reconcile_skips)
+            return (float(group["lr"]), float(b1), float(b2), float(group["weight_decay"]),
+                    t + (self._skips_applied[gi] if counted else 0))
+
+        lr, b1, b2, wd, t = host_step()
+        if ops.STEP_SCALARS is not None:   # a capture that fails must leave the host bookkeeping where it found it
+            ops.STEP_SCALARS.aborts.append(lambda plist=plist: [self.state[p]["step"].sub_(1) for p in plist])
+        ops.adamw_multi(table, len(plist), max_numel, lr, b1, b2, float(group["eps"]), wd, t,
+                        total_numel=sum(p.numel() for p in plist), skip_flag=found_inf,
+                        skipped_count=(skipped[gi:gi + 1] if skipped is not None else None), refresh=host_step)
+
+
+class FusedMuon(FusedAdamW):
+    """Orthogonalised momentum for weight matrices, AdamW for the rest, in one optimiser.
+
+    Parameters of two or more dimensions are matrices (out channels, everything else): v = momentum v + g, u = g + momentum v
+    (nesterov) or v, p = p (1 - lr weight_decay) - lr s O(u), O = ``ns_steps`` Newton-Schulz steps (``ops.orthogonalize``).
+    ``adjust_lr`` "match_rms_adamw" (default): s = 0.2 sqrt(max(rows, cols)) - an update of AdamW's usual size, so that both kinds of
+    parameters share lr and weight_decay -, "original": s = sqrt(max(1, rows / cols)).  Vectors (norms, biases) take AdamW's update
+    with ``betas`` and ``eps``.  A group with ``muon: False`` takes AdamW for everything (a classifier, an embedding).
+
+    State: ``momentum_buffer`` per matrix, torch.optim.AdamW's entries for the others.  Skipped steps (``found_inf``), checkpoints and
+    captured steps behave as in ``FusedAdamW``."""
+
+    ADJUST = {"original": 0, "match_rms_adamw": 1}
+
+    def __init__(self, params, lr=1e-3, momentum=0.95, nesterov=True, weight_decay=0.1, ns_steps=5, ns_eps=1e-7,
+                 adjust_lr="match_rms_adamw", betas=(0.9, 0.999), eps=1e-8):
+        if not 0.0 <= momentum < 1.0 or not 1 <= int(ns_steps) <= 100 or not ns_eps >= 0.0 or adjust_lr not in self.ADJUST:
+            raise ValueError("invalid Muon hyper-parameter")
+        self._muon_defaults = dict(momentum=momentum, nesterov=bool(nesterov), ns_steps=int(ns_steps), ns_eps=ns_eps, adjust_lr=adjust_lr,
+                                   muon=True)
+        super().__init__(params, lr=lr, betas=betas, eps=eps, weight_decay=weight_decay)
+
+    def add_param_group(self, param_group):
+        for k, v in self._muon_defaults.items():
+            param_group.setdefault(k, v)
+        if param_group["adjust_lr"] not in self.ADJUST:
+            raise ValueError("invalid Muon hyper-parameter")
+        super().add_param_group(param_group)
+
+    @torch.no_grad()
+    def step(self, closure=None, found_inf=None):
+        """``found_inf``: device float tensor; non-zero -> this update is skipped inside the kernels (no host sync)."""
+        loss = None
+        _drop_grads_if_capture_fails(self.param_groups)
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for gi, group in enumerate(self.param_groups):
+            plist = [p for p in self._plist(group) if p.numel()]
+            matrices = [p for p in plist if p.dim() >= 2] if group["muon"] else []
+            others = [p for p in plist if p.dim() < 2] if group["muon"] else plist
+            if others:
+                self._adamw_group(gi, group, others, found_inf)
+            if not matrices:
+                continue
+            rows = []
+            for p in matrices:
                 st = self.state[p]
-                if len(st) == 0:
-                    st["step"] = torch.tensor(0.0, dtype=torch.float32)
-                    st["exp_avg"] = torch.zeros_like(p, memory_format=torch.preserve_format)
-                    st["exp_avg_sq"] = torch.zeros_like(p, memory_format=torch.preserve_format)
-            table, max_numel = self._table(gi, plist)
-            skipped = self._skipped_counter(plist[0].device) if found_inf is not None else self._skipped
-            if skipped is not None and len(self._skips_applied) != len(self.param_groups):
-                skipped = self._skipped_counter(plist[0].device)     # a param group was added
-
-            def host_step(gi=gi, group=group, plist=plist, counted=skipped is not None):
-                """The host half of one step of this group: advance the per-parameter ``step`` -> the launch's scalars.  Also
-                the refresh hook of a step captured in a HIP graph (ssecg/graph.py): a replay runs this and nothing else."""
-                steps = {int(self.state[p]["step"].item()) for p in plist}  # CPU scalars: no device sync
-                if len(steps) != 1:
-                    raise SsecgError("FusedAdamW: parameters of one group must share a step count")
-                t = steps.pop() + 1
-                for p in plist:
-                    self.state[p]["step"] += 1
-                b1, b2 = group["betas"]
-                # ``t`` counts launches; the ones the device skipped are subtracted in the kernel (bias corrections) and, at
-                # checkpoint time, from the per-parameter ``step`` (reconcile_skips)
-                return (float(group["lr"]), float(b1), float(b2), float(group["weight_decay"]),
-                        t + (self._skips_applied[gi] if counted else 0))
-
-            lr, b1, b2, wd, t = host_step()
-            if ops.STEP_SCALARS is not None:   # a capture that fails must leave the host bookkeeping where it found it
-                ops.STEP_SCALARS.aborts.append(lambda plist=plist: [self.state[p]["step"].sub_(1) for p in plist])
-            ops.adamw_multi(table, len(plist), max_numel, lr, b1, b2, float(group["eps"]), wd, t,
-                            total_numel=sum(p.numel() for p in plist), skip_flag=found_inf,
-                            skipped_count=(skipped[gi:gi + 1] if skipped is not None else None), refresh=host_step)
+                if "momentum_buffer" not in st:
+                    st["momentum_buffer"] = torch.zeros_like(p, memory_format=torch.preserve_format)
+                v = st["momentum_buffer"]
+                if v.dtype != torch.float32 or v.device != p.device or not v.is_contiguous():
+                    raise SsecgError("FusedMuon: a momentum buffer must be a contiguous fp32 tensor on its parameter's device")
+                rows.append((p.grad.data_ptr(), p.data_ptr(), v.data_ptr(), p.shape[0], p.numel() // p.shape[0]))
+            if len({p.device for p in matrices}) != 1:
+                raise SsecgError("FusedMuon: the matrices of one group must live on one device")
+            with torch.cuda.device(matrices[0].device):
+                ops.muon_multi(rows, matrices[0].device, group["lr"], group["momentum"], group["nesterov"], group["weight_decay"],
+                               self.ADJUST[group["adjust_lr"]], group["ns_steps"], group["ns_eps"], skip_flag=found_inf,
+                               refresh=lambda group=group: float(group["lr"]))
         return loss
 
 

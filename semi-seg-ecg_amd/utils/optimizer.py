@@ -1,6 +1,7 @@
 """Optimizer factory (``src/utils/optimizer.py:8-37``): ``adamw`` and ``sgd``, both fused multi-tensor HIP updates
-with ``torch.optim``-compatible ``state_dict`` layouts."""
-from ssecg.optim import FusedAdamW, FusedSGD
+with ``torch.optim``-compatible ``state_dict`` layouts; beyond the reference ``muon``: orthogonalised momentum for every weight of
+two or more dimensions, AdamW for the rest."""
+from ssecg.optim import FusedAdamW, FusedMuon, FusedSGD
 
 
 def get_optimizer_from_config(config: dict, param_groups):
@@ -15,4 +16,7 @@ def get_optimizer_from_config(config: dict, param_groups):
         if isinstance(betas, list):
             betas = tuple(betas)
         return FusedAdamW(param_groups, lr=lr, betas=betas, eps=kwargs.get('eps', 1e-8), weight_decay=weight_decay)
+    if opt_name == "muon":
+        known = {k: kwargs[k] for k in ('momentum', 'nesterov', 'ns_steps', 'ns_eps', 'adjust_lr', 'eps') if k in kwargs}
+        return FusedMuon(param_groups, lr=lr, weight_decay=weight_decay, betas=tuple(kwargs.get('betas', (0.9, 0.999))), **known)
     raise ValueError(f"Unknown optimizer: {opt_name}")
