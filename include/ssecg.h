@@ -552,17 +552,23 @@ int ssecg_layer_norm_bwd(const void *dy, const void *x, const float *mean, const
  *   gate[n] = 0 for target == ignore_index or (conf given) conf[n] < thresh or NaN, else 1
  *   count   = max(1, positions whose target is not ignore_index)
  *   loss    : reduction 0: (N) gate (lse - z_target); 1: their sum / count; 2: their sum
- * A position whose gate is 0 contributes nothing, whatever x holds there. */
+ * A position whose gate is 0 contributes nothing, whatever x holds there.
+ *  packed: what the backward pass reuses - the scales and copies of operands that are none as they lie (fp32, C not a multiple of
+ *  64, not 16-byte aligned); 0 bytes otherwise.  x and weight must stay where they are until then.
+ */
+size_t ssecg_linear_ce_packed_bytes(const void *x, const void *weight, int dtype, int64_t N, int64_t C, int64_t V);
 size_t ssecg_linear_ce_fwd_workspace(int dtype, int64_t N, int64_t C, int64_t V);
 int ssecg_linear_ce_fwd(const void *x, const void *weight, const float *bias, const int64_t *target, const float *conf, double thresh,
                         int64_t ignore_index, int dtype, int64_t N, int64_t C, int64_t V, int reduction, float *loss, float *lse,
-                        float *gate, float *count, void *workspace, size_t workspace_bytes, void *stream);
+                        float *gate, float *count, void *packed, size_t packed_bytes, void *workspace, size_t workspace_bytes,
+                        void *stream);
 /* gradients of the above (each may be NULL, not all): dloss is a scalar on the device (reduction 1, 2) or (N) (reduction 0).  The
  * vocabulary is taken in pieces that bound the workspace (about 1 GiB beside copies of the operands). */
 size_t ssecg_linear_ce_bwd_workspace(int dtype, int64_t N, int64_t C, int64_t V, int want_dx, int want_dweight, int want_dbias);
 int ssecg_linear_ce_bwd(const float *dloss, const void *x, const void *weight, const float *bias, const int64_t *target,
                         const float *lse, const float *gate, const float *count, int dtype, int64_t N, int64_t C, int64_t V,
-                        int reduction, void *dx, void *dweight, float *dbias, void *workspace, size_t workspace_bytes, void *stream);
+                        int reduction, void *dx, void *dweight, float *dbias, const void *packed, size_t packed_bytes, void *workspace,
+                        size_t workspace_bytes, void *stream);
 
 /* Newton-Schulz orthogonalisation of `count` matrices.  mats is a HOST array of rows {source, result, momentum, rows, cols} (device
  * pointers as integers; momentum unused here); it is read during the call only.  At most 2^20 rows / columns each. */

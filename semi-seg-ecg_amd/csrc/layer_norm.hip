@@ -4,7 +4,7 @@
 //   g = dy w,  dx = r (g - mean(g) - xh mean(g xh)),  dw = sum_rows dy xh,  db = sum_rows dy
 //
 // Both passes are bound by HBM: forward reads x and writes y, backward reads x and dy and writes dx - each byte once.  A row
-// stays in the registers of the threads that own it (one wave up to 4 vectors per lane, otherwise 256 or 1024 threads), so the
+// stays in the registers of the threads that own it (64 to 1024 of them), so the
 // variance is the two-pass one (the sum of squared differences from the mean, no cancellation) without a second read.  A thread
 // owns the same columns of every row its workgroup takes: w and b are loaded once, and the column sums dw / db grow in its
 // registers; the row groups of a workgroup are joined in LDS, the workgroups by a second launch in fixed order (no atomics:
@@ -14,33 +14,6 @@
 
 namespace {
 using namespace ssecg_lm;
-
-constexpr int kMaxBlocks = 512;   // workgroups of the backward pass = rows of its partial sums (2 of 1024 threads per CU)
-
-template <typename T>
-__device__ __forceinline__ typename Vec<T>::type load_vec(const T* __restrict__ p, int c0, int C) {
-    constexpr int V = Vec<T>::N;
-    typename Vec<T>::type v;
-    if (c0 + V <= C) {
-        v = *reinterpret_cast<const typename Vec<T>::type*>(p + c0);
-    } else {
-#pragma unroll
-        for (int i = 0; i < V; ++i) v[i] = c0 + i < C ? p[c0 + i] : (T)0.f;
-    }
-    return v;
-}
-
-template <typename T>
-__device__ __forceinline__ void store_vec(T* __restrict__ p, int c0, int C, typename Vec<T>::type v) {
-    constexpr int V = Vec<T>::N;
-    if (c0 + V <= C) {
-        *reinterpret_cast<typename Vec<T>::type*>(p + c0) = v;
-    } else {
-#pragma unroll
-        for (int i = 0; i < V; ++i)
-            if (c0 + i < C) p[c0 + i] = v[i];
-    }
-}
 
 // Sum over the TPR threads of a row; every thread gets it.  `sh` holds a slot per wave; two slots sets alternate by `flip`, so
 // one barrier per reduction is enough (a wave can be at most one reduction ahead of the others).
@@ -67,6 +40,39 @@ __device__ __forceinline__ void row_sum(float (&v)[K], float* sh, int& flip) {
     }
 }
 
+// a thread's share of a parameter vector (absent or beyond C: `none`)
+template <typename T, int TPR, int NCH>
+__device__ __forceinline__ void load_params(const float* __restrict__ p, int t, int C, float none, float (&v)[NCH][Vec<T>::N]) {
+    constexpr int V = Vec<T>::N;
+#pragma unroll
+    for (int j = 0; j < NCH; ++j)
+#pragma unroll
+        for (int i = 0; i < V; i += 4) {
+            const int c = (t + TPR * j) * V + i;
+            Vec<float>::type q = {none, none, none, none};
+            if (p && c < C) q = load_vec(p, c, C);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[j][i + k] = q[k];
+        }
+}
+
+// a thread's share of a row
+template <typename T, int TPR, int NCH>
+__device__ __forceinline__ void load_row(const T* __restrict__ p, int t, int C, typename Vec<T>::type (&v)[NCH]) {
+#pragma unroll
+    for (int j = 0; j < NCH; ++j) {
+        const int c0 = (t + TPR * j) * Vec<T>::N;
+        if (c0 < C) {
+            v[j] = load_vec(p, c0, C);
+        } else {
+#pragma unroll
+            for (int i = 0; i < Vec<T>::N; ++i) v[j][i] = (T)0.f;
+        }
+    }
+}
+
+// A row group takes every gridDim-th row; the next row is requested before the current one is reduced, so that loads travel
+// through the two reductions.
 template <typename T, int TPR, int NT, int NCH>
 __global__ __launch_bounds__(NT) void ln_fwd_kernel(const T* __restrict__ x, const float* __restrict__ w, const float* __restrict__ b,
                                                     T* __restrict__ y, float* __restrict__ mean, float* __restrict__ rstd,
@@ -75,34 +81,25 @@ __global__ __launch_bounds__(NT) void ln_fwd_kernel(const T* __restrict__ x, con
     __shared__ float sh[2 * 16];
     int flip = 0;
     const int t = threadIdx.x % TPR, grp = threadIdx.x / TPR;
+    const int64_t step = (int64_t)gridDim.x * G;
+    typename Vec<T>::type cur[NCH], nxt[NCH];
+    {
+        const int64_t row = (int64_t)blockIdx.x * G + grp;
+        load_row<T, TPR, NCH>(x + (row < rows ? row : rows - 1) * C, t, C, cur);
+    }
     float wv[NCH][V], bv[NCH][V];
-#pragma unroll
-    for (int j = 0; j < NCH; ++j)
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const int c = (t + TPR * j) * V + i;
-            wv[j][i] = w && c < C ? w[c] : 1.f;
-            bv[j][i] = b && c < C ? b[c] : 0.f;
-        }
+    load_params<T, TPR, NCH>(w, t, C, 1.f, wv);
+    load_params<T, TPR, NCH>(b, t, C, 0.f, bv);
     const float invC = 1.f / (float)C;
-    for (int64_t r0 = (int64_t)blockIdx.x * G; r0 < rows; r0 += (int64_t)gridDim.x * G) {   // uniform: every wave reaches each barrier
-        const int64_t row = r0 + grp;
+    for (int64_t r0 = (int64_t)blockIdx.x * G; r0 < rows; r0 += step) {   // uniform: every wave reaches each barrier
+        const int64_t row = r0 + grp, after = row + step;
         const bool live = row < rows;
-        const T* xr = x + (live ? row : rows - 1) * C;
-        float v[NCH][V];
+        if (r0 + step < rows) load_row<T, TPR, NCH>(x + (after < rows ? after : rows - 1) * C, t, C, nxt);
         float s[1] = {0.f};
 #pragma unroll
-        for (int j = 0; j < NCH; ++j) {
-            const int c0 = (t + TPR * j) * V;
-            if (c0 < C) {
-                const auto q = load_vec(xr, c0, C);
+        for (int j = 0; j < NCH; ++j)
 #pragma unroll
-                for (int i = 0; i < V; ++i) { v[j][i] = (float)q[i]; s[0] += v[j][i]; }
-            } else {
-#pragma unroll
-                for (int i = 0; i < V; ++i) v[j][i] = 0.f;
-            }
-        }
+            for (int i = 0; i < V; ++i) s[0] += (float)cur[j][i];
         row_sum<TPR, 1>(s, sh, flip);
         const float mu = s[0] * invC;
         float q[1] = {0.f};
@@ -110,23 +107,26 @@ __global__ __launch_bounds__(NT) void ln_fwd_kernel(const T* __restrict__ x, con
         for (int j = 0; j < NCH; ++j)
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                const float d = v[j][i] - mu;
+                const float d = (float)cur[j][i] - mu;
                 if ((t + TPR * j) * V + i < C) q[0] += d * d;
             }
         row_sum<TPR, 1>(q, sh, flip);
         const float rs = 1.f / sqrtf(q[0] * invC + eps);
-        if (!live) continue;
-        if (t == 0) { mean[row] = mu; rstd[row] = rs; }
+        if (live) {
+            if (t == 0) { mean[row] = mu; rstd[row] = rs; }
 #pragma unroll
-        for (int j = 0; j < NCH; ++j) {
-            const int c0 = (t + TPR * j) * V;
-            if (c0 < C) {
-                typename Vec<T>::type o;
+            for (int j = 0; j < NCH; ++j) {
+                const int c0 = (t + TPR * j) * V;
+                if (c0 < C) {
+                    typename Vec<T>::type o;
 #pragma unroll
-                for (int i = 0; i < V; ++i) o[i] = (T)((v[j][i] - mu) * rs * wv[j][i] + bv[j][i]);
-                store_vec(y + row * C, c0, C, o);
+                    for (int i = 0; i < V; ++i) o[i] = (T)(((float)cur[j][i] - mu) * rs * wv[j][i] + bv[j][i]);
+                    store_vec(y + row * C, c0, C, o);
+                }
             }
         }
+#pragma unroll
+        for (int j = 0; j < NCH; ++j) cur[j] = nxt[j];
     }
 }
 
@@ -174,55 +174,54 @@ __global__ __launch_bounds__(1024) void ln_fwd_long_kernel(const T* __restrict__
     }
 }
 
-// partial: [gridDim.x][2][C] column sums {dy xh, dy} of the workgroup's rows
+// partial: [gridDim.x][2][C] column sums {dy xh, dy} of the workgroup's rows, or null
 template <typename T, int TPR, int NT, int NCH>
 __global__ __launch_bounds__(NT) void ln_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ x, const float* __restrict__ mean,
                                                     const float* __restrict__ rstd, const float* __restrict__ w, T* __restrict__ dx,
                                                     float* __restrict__ partial, int64_t rows, int C) {
     constexpr int V = Vec<T>::N, G = NT / TPR;
     __shared__ float sh[2 * 32];
-    extern __shared__ float col[];                    // [2][C] when a workgroup has several row groups
+    extern __shared__ float col[];                    // [G / 2][C]: the join of the row groups
     int flip = 0;
     const int t = threadIdx.x % TPR, grp = threadIdx.x / TPR;
+    const int64_t step = (int64_t)gridDim.x * G;
+    typename Vec<T>::type xq[NCH], gq[NCH], xn[NCH], gn[NCH];
+    float mu, rs, mun = 0.f, rsn = 0.f;
+    {
+        int64_t row = (int64_t)blockIdx.x * G + grp;
+        row = row < rows ? row : rows - 1;
+        load_row<T, TPR, NCH>(x + row * C, t, C, xq);
+        load_row<T, TPR, NCH>(dy + row * C, t, C, gq);
+        mu = mean[row];
+        rs = rstd[row];
+    }
     float wv[NCH][V], aw[NCH][V], ab[NCH][V];
+    load_params<T, TPR, NCH>(w, t, C, 1.f, wv);
 #pragma unroll
     for (int j = 0; j < NCH; ++j)
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const int c = (t + TPR * j) * V + i;
-            wv[j][i] = w && c < C ? w[c] : 1.f;
-            aw[j][i] = 0.f;
-            ab[j][i] = 0.f;
-        }
+        for (int i = 0; i < V; ++i) { aw[j][i] = 0.f; ab[j][i] = 0.f; }
     const float invC = 1.f / (float)C;
-    for (int64_t r0 = (int64_t)blockIdx.x * G; r0 < rows; r0 += (int64_t)gridDim.x * G) {
+    for (int64_t r0 = (int64_t)blockIdx.x * G; r0 < rows; r0 += step) {
         const int64_t row = r0 + grp;
         const bool live = row < rows;
-        const int64_t at = (live ? row : rows - 1) * C;
-        const float mu = mean[live ? row : rows - 1], rs = rstd[live ? row : rows - 1];
-        typename Vec<T>::type xq[NCH], gq[NCH];
+        if (r0 + step < rows) {
+            const int64_t after = row + step < rows ? row + step : rows - 1;
+            load_row<T, TPR, NCH>(x + after * C, t, C, xn);
+            load_row<T, TPR, NCH>(dy + after * C, t, C, gn);
+            mun = mean[after];
+            rsn = rstd[after];
+        }
         float s[2] = {0.f, 0.f};
 #pragma unroll
-        for (int j = 0; j < NCH; ++j) {
-            const int c0 = (t + TPR * j) * V;
-            if (c0 < C) {
-                xq[j] = load_vec(x + at, c0, C);
-                gq[j] = load_vec(dy + at, c0, C);
-            }
-        }
+        for (int j = 0; j < NCH; ++j)
 #pragma unroll
-        for (int j = 0; j < NCH; ++j) {
-            const int c0 = (t + TPR * j) * V;
-            if (c0 < C) {
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    const float xh = ((float)xq[j][i] - mu) * rs, d = (float)gq[j][i], g = d * wv[j][i];   // beyond C: dy = 0
-                    s[0] += g;
-                    s[1] += g * xh;
-                    if (live) { aw[j][i] += d * xh; ab[j][i] += d; }
-                }
+            for (int i = 0; i < V; ++i) {
+                const float xh = ((float)xq[j][i] - mu) * rs, d = (float)gq[j][i], g = d * wv[j][i];   // beyond C: dy = 0
+                s[0] += g;
+                s[1] += g * xh;
+                if (live) { aw[j][i] += d * xh; ab[j][i] += d; }
             }
-        }
         row_sum<TPR, 2>(s, sh, flip);
         const float c1 = s[0] * invC, c2 = s[1] * invC;
         if (live) {
@@ -236,37 +235,55 @@ __global__ __launch_bounds__(NT) void ln_bwd_kernel(const T* __restrict__ dy, co
                         const float xh = ((float)xq[j][i] - mu) * rs, g = (float)gq[j][i] * wv[j][i];
                         o[i] = (T)(rs * (g - c1 - xh * c2));
                     }
-                    store_vec(dx + at, c0, C, o);
+                    store_vec(dx + row * C, c0, C, o);
                 }
             }
         }
+#pragma unroll
+        for (int j = 0; j < NCH; ++j) { xq[j] = xn[j]; gq[j] = gn[j]; }
+        mu = mun;
+        rs = rsn;
     }
     if (partial == nullptr) return;
-    float* out = partial + (size_t)blockIdx.x * 2 * C;
-    if (G > 1) {                                      // row groups one after the other: fixed order
-        for (int g = 0; g < G; ++g) {
-            __syncthreads();
-            if (grp == g) {
+    if (G > 1) {                                      // the upper half of the groups to the lower half, down to one: fixed order
+        auto join = [&](float (&a)[NCH][V]) {
 #pragma unroll
-                for (int j = 0; j < NCH; ++j)
+            for (int half = G / 2; half > 0; half /= 2) {
+                __syncthreads();
+                if (grp >= half && grp < 2 * half)
 #pragma unroll
-                    for (int i = 0; i < V; ++i) {
-                        const int c = (t + TPR * j) * V + i;
-                        if (c < C) {
-                            if (g > 0) { aw[j][i] += col[c]; ab[j][i] += col[C + c]; }
-                            if (g < G - 1) { col[c] = aw[j][i]; col[C + c] = ab[j][i]; }
-                        }
-                    }
+                    for (int j = 0; j < NCH; ++j)
+                        if ((t + TPR * j) * V < C)
+#pragma unroll
+                            for (int i = 0; i < V; ++i)
+                                if ((t + TPR * j) * V + i < C) col[(grp - half) * C + (t + TPR * j) * V + i] = a[j][i];
+                __syncthreads();
+                if (grp < half)
+#pragma unroll
+                    for (int j = 0; j < NCH; ++j)
+                        if ((t + TPR * j) * V < C)
+#pragma unroll
+                            for (int i = 0; i < V; ++i)
+                                if ((t + TPR * j) * V + i < C) a[j][i] += col[grp * C + (t + TPR * j) * V + i];
             }
-        }
+        };
+        join(aw);
+        join(ab);
     }
-    if (grp == G - 1) {
+    if (grp == 0) {
+        float* out = partial + (size_t)blockIdx.x * 2 * C;
 #pragma unroll
         for (int j = 0; j < NCH; ++j)
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
+            for (int i = 0; i < V; i += 4) {
                 const int c = (t + TPR * j) * V + i;
-                if (c < C) { out[c] = aw[j][i]; out[C + c] = ab[j][i]; }
+                if (c < C) {
+                    Vec<float>::type p, q;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) { p[k] = aw[j][i + k]; q[k] = ab[j][i + k]; }
+                    store_vec(out, c, C, p);
+                    store_vec(out + C, c, C, q);
+                }
             }
     }
 }
@@ -351,57 +368,67 @@ __global__ __launch_bounds__(1024) void ln_param_grads_kernel(const float* __res
     }
 }
 
-// Threads per row and 16-byte vectors per thread.  One wave per row up to 4 vectors a lane: no barrier, and several rows are in
-// flight per SIMD.  Beyond that 256, then 1024 threads, so that a thread's share (row, parameters, column sums) stays in registers.
+// Threads per row and 16-byte vectors per thread: the fewest threads whose registers hold the row beside the parameters (and, in the
+// backward pass, the column sums and the next row: 128 registers a thread at 1024 threads).  One wave per row needs no barrier.
 struct LnShape { int tpr, nch; };
 inline LnShape ln_shape(int C, int V, bool bwd) {
     const int64_t vecs = ((int64_t)C + V - 1) / V;
-    const int deep = V == 8 ? 2 : 4;                         // vectors per thread that the backward pass of 1024 threads can hold
-    auto fit = [&](int tpr, int most) {
+    const int most = bwd ? (V == 8 ? 1 : 2) : (V == 8 ? 2 : 4);
+    for (int tpr = 64; tpr <= 1024; tpr *= V == 8 || bwd ? 2 : 4)
         for (int n = 1; n <= most; n *= 2)
-            if (vecs <= (int64_t)tpr * n) return n;
-        return 0;
-    };
-    if (int n = fit(64, bwd ? deep : 4)) return {64, n};
-    if (int n = fit(256, bwd ? 2 : 4)) return {256, n};
-    if (int n = fit(1024, deep)) return {1024, n};
+            if (vecs <= (int64_t)tpr * n) return {tpr, n};
+    if (bwd && vecs <= 2048 * most) return {1024, 2 * most};
     return {0, 0};
 }
 
 template <typename T, int TPR, int NCH>
 int launch_fwd(const void* x, const float* w, const float* b, void* y, float* mean, float* rstd, int64_t rows, int C, float eps, hipStream_t st) {
-    constexpr int NT = TPR == 1024 ? 1024 : 256, G = NT / TPR;
-    const int64_t blocks = (rows + G - 1) / G, most = 256 * (2048 / NT);
+    constexpr int NT = TPR > 256 ? TPR : 256, G = NT / TPR;
+    const int64_t blocks = (rows + G - 1) / G, most = 256 * (1024 / NT);
     hipLaunchKernelGGL((ln_fwd_kernel<T, TPR, NT, NCH>), dim3((unsigned)(blocks < most ? blocks : most)), dim3(NT), 0, st, (const T*)x, w, b,
                        (T*)y, mean, rstd, rows, C, eps);
     return (int)hipGetLastError();
 }
 
-template <typename T, int TPR, int NCH>
-int launch_bwd(const void* dy, const void* x, const float* mean, const float* rstd, const float* w, void* dx, float* partial, int64_t rows,
-               int C, int parts, hipStream_t st) {
-    constexpr int NT = 1024;
-    const size_t lds = partial && TPR < NT ? (size_t)2 * C * sizeof(float) : 0;
-    hipLaunchKernelGGL((ln_bwd_kernel<T, TPR, NT, NCH>), dim3((unsigned)parts), dim3(NT), lds, st, (const T*)dy, (const T*)x, mean, rstd, w,
-                       (T*)dx, partial, rows, C);
-    return (int)hipGetLastError();
+// Workgroups of the backward pass: 1024 threads, one per CU, if that gives every CU one; else as few threads as a row takes (256 at
+// least), so that few rows still reach many CUs.
+struct LnGrid { int nt, parts; };
+inline LnGrid ln_grid(int64_t rows, int C, int dtype) {
+    const LnShape s = ln_shape(C, dtype == kF32 ? 4 : 8, true);
+    if (!s.tpr) return {1024, (int)(rows < 32 ? rows : 32)};           // very long rows: few slabs bound the workspace
+    const int64_t g = 1024 / s.tpr, wide = (rows + g - 1) / g;
+    if (s.tpr == 1024 || wide >= 256) return {1024, (int)(wide < 256 ? wide : 256)};
+    const int nt = s.tpr < 256 ? 256 : s.tpr;
+    return {nt, (int)((rows * s.tpr + nt - 1) / nt)};
 }
 
-inline int ln_parts(int64_t rows, int C, int dtype) {
-    const LnShape s = ln_shape(C, dtype == kF32 ? 4 : 8, true);
-    const int64_t g = s.tpr ? 1024 / s.tpr : 1;
-    const int64_t blocks = (rows + g - 1) / g, most = s.tpr ? kMaxBlocks : 32;   // very long rows: few slabs bound the workspace
-    return (int)(blocks < most ? blocks : most);
+template <typename T, int TPR, int NCH>
+int launch_bwd(const void* dy, const void* x, const float* mean, const float* rstd, const float* w, void* dx, float* partial, int64_t rows,
+               int C, const LnGrid& g, hipStream_t st) {
+    if (TPR < 1024 && g.nt < 1024) {
+        constexpr int NT = TPR < 256 ? 256 : TPR;
+        const size_t lds = partial && TPR < NT ? (size_t)(NT / TPR / 2) * C * sizeof(float) : 0;
+        hipLaunchKernelGGL((ln_bwd_kernel<T, TPR, NT, NCH>), dim3((unsigned)g.parts), dim3(NT), lds, st, (const T*)dy, (const T*)x, mean, rstd, w,
+                           (T*)dx, partial, rows, C);
+    } else {
+        constexpr int NT = 1024;
+        const size_t lds = partial && TPR < NT ? (size_t)(NT / TPR / 2) * C * sizeof(float) : 0;
+        hipLaunchKernelGGL((ln_bwd_kernel<T, TPR, NT, NCH>), dim3((unsigned)g.parts), dim3(NT), lds, st, (const T*)dy, (const T*)x, mean, rstd, w,
+                           (T*)dx, partial, rows, C);
+    }
+    return (int)hipGetLastError();
 }
 
 template <typename T>
 int ln_fwd(const void* x, const float* w, const float* b, void* y, float* mean, float* rstd, int64_t rows, int C, float eps, hipStream_t st) {
     const LnShape s = ln_shape(C, Vec<T>::N, false);
 #define SSECG_LN_CASE(TPR, NCH) if (s.tpr == TPR && s.nch == NCH) return launch_fwd<T, TPR, NCH>(x, w, b, y, mean, rstd, rows, C, eps, st)
-    SSECG_LN_CASE(64, 1); SSECG_LN_CASE(64, 2); SSECG_LN_CASE(64, 4);
-    SSECG_LN_CASE(256, 2); SSECG_LN_CASE(256, 4);
-    SSECG_LN_CASE(1024, 2);
-    if constexpr (Vec<T>::N == 4) SSECG_LN_CASE(1024, 4);
+    SSECG_LN_CASE(64, 1); SSECG_LN_CASE(64, 2); SSECG_LN_CASE(256, 2); SSECG_LN_CASE(1024, 2);
+    if constexpr (Vec<T>::N == 4) {
+        SSECG_LN_CASE(64, 4); SSECG_LN_CASE(256, 4); SSECG_LN_CASE(1024, 4);
+    } else {
+        SSECG_LN_CASE(128, 2); SSECG_LN_CASE(512, 2);
+    }
 #undef SSECG_LN_CASE
     hipLaunchKernelGGL((ln_fwd_long_kernel<T>), dim3((unsigned)(rows < 512 ? rows : 512)), dim3(1024), 0, st, (const T*)x, w, b, (T*)y, mean,
                        rstd, rows, C, eps);
@@ -410,20 +437,20 @@ int ln_fwd(const void* x, const float* w, const float* b, void* y, float* mean, 
 
 template <typename T>
 int ln_bwd(const void* dy, const void* x, const float* mean, const float* rstd, const float* w, void* dx, float* partial, int64_t rows, int C,
-           int parts, hipStream_t st) {
+           const LnGrid& g, hipStream_t st) {
     const LnShape s = ln_shape(C, Vec<T>::N, true);
-#define SSECG_LN_CASE(TPR, NCH) if (s.tpr == TPR && s.nch == NCH) return launch_bwd<T, TPR, NCH>(dy, x, mean, rstd, w, dx, partial, rows, C, parts, st)
-    SSECG_LN_CASE(64, 1); SSECG_LN_CASE(64, 2);
-    SSECG_LN_CASE(256, 1); SSECG_LN_CASE(256, 2);
-    SSECG_LN_CASE(1024, 1); SSECG_LN_CASE(1024, 2);
+#define SSECG_LN_CASE(TPR, NCH) if (s.tpr == TPR && s.nch == NCH) return launch_bwd<T, TPR, NCH>(dy, x, mean, rstd, w, dx, partial, rows, C, g, st)
+    SSECG_LN_CASE(64, 1); SSECG_LN_CASE(1024, 2);
     if constexpr (Vec<T>::N == 4) {
-        SSECG_LN_CASE(64, 4); SSECG_LN_CASE(1024, 4);
+        SSECG_LN_CASE(64, 2); SSECG_LN_CASE(128, 2); SSECG_LN_CASE(256, 2); SSECG_LN_CASE(512, 2); SSECG_LN_CASE(1024, 4);
+    } else {
+        SSECG_LN_CASE(128, 1); SSECG_LN_CASE(256, 1); SSECG_LN_CASE(512, 1); SSECG_LN_CASE(1024, 1);
     }
 #undef SSECG_LN_CASE
     hipLaunchKernelGGL((ln_bwd_long_kernel<T>), dim3((unsigned)(rows < 512 ? rows : 512)), dim3(1024), 0, st, (const T*)dy, (const T*)x, mean,
                        rstd, w, (T*)dx, rows, C);
     if (partial)
-        hipLaunchKernelGGL((ln_bwd_cols_kernel<T>), dim3((unsigned)((C + 255) / 256), (unsigned)parts), dim3(256), 0, st, (const T*)dy,
+        hipLaunchKernelGGL((ln_bwd_cols_kernel<T>), dim3((unsigned)((C + 255) / 256), (unsigned)g.parts), dim3(256), 0, st, (const T*)dy,
                            (const T*)x, mean, rstd, partial, rows, C);
     return (int)hipGetLastError();
 }
@@ -442,7 +469,7 @@ int ssecg_layer_norm_fwd(const void* x, const float* weight, const float* bias, 
 
 size_t ssecg_layer_norm_bwd_workspace(int dtype, int64_t rows, int C) {
     if (!dtype_ok(dtype) || rows <= 0 || C <= 0 || C > kMaxC) return 0;
-    return (size_t)ln_parts(rows, C, dtype) * 2 * C * sizeof(float);
+    return (size_t)ln_grid(rows, C, dtype).parts * 2 * C * sizeof(float);
 }
 
 int ssecg_layer_norm_bwd(const void* dy, const void* x, const float* mean, const float* rstd, const float* weight, int dtype, int64_t rows,
@@ -450,12 +477,12 @@ int ssecg_layer_norm_bwd(const void* dy, const void* x, const float* mean, const
     if (!dy || !x || !mean || !rstd || !dx || !dtype_ok(dtype) || rows <= 0 || C <= 0 || C > kMaxC) return SSECG_E_INVAL;
     const bool params = dweight || dbias;
     if (params && (!workspace || workspace_bytes < ssecg_layer_norm_bwd_workspace(dtype, rows, C))) return SSECG_E_WORKSPACE;
-    const int parts = ln_parts(rows, C, dtype);
+    const LnGrid g = ln_grid(rows, C, dtype);
     float* partial = params ? workspace : nullptr;
     int rc = 0;
-    SSECG_LM_DTYPE(dtype, T, rc = ln_bwd<T>(dy, x, mean, rstd, weight, dx, partial, rows, C, parts, (hipStream_t)stream));
+    SSECG_LM_DTYPE(dtype, T, rc = ln_bwd<T>(dy, x, mean, rstd, weight, dx, partial, rows, C, g, (hipStream_t)stream));
     if (rc != 0 || !params) return rc;
-    hipLaunchKernelGGL(ln_param_grads_kernel, dim3((unsigned)((2 * (int64_t)C + 31) / 32)), dim3(1024), 0, (hipStream_t)stream, partial, parts,
+    hipLaunchKernelGGL(ln_param_grads_kernel, dim3((unsigned)((2 * (int64_t)C + 31) / 32)), dim3(1024), 0, (hipStream_t)stream, partial, g.parts,
                        C, dweight, dbias);
     return (int)hipGetLastError();
 }

@@ -28,34 +28,41 @@ constexpr int kAmaxParts = 256;
 __device__ __forceinline__ float exp2_fast(float v) { return __builtin_amdgcn_exp2f(v); }
 
 // ---------------------------------------------------------------- operands
-// Which rows count: by the gate of the forward pass, or (there) by target and confidence.
-struct Counts {
-    const float* gate;
+struct Counts {                                   // which rows count
     const int64_t* target; int64_t ignore;
     const float* conf; float thresh;
-    __device__ __forceinline__ bool operator()(int64_t r) const {
-        if (gate) return gate[r] != 0.f;
-        return target == nullptr || (target[r] != ignore && (conf == nullptr || conf[r] >= thresh));
-    }
+    __device__ __forceinline__ bool operator()(int64_t r) const { return target[r] != ignore && (conf == nullptr || conf[r] >= thresh); }
 };
 
-// largest finite |x| of the rows that count, per workgroup (a maximum: any order gives the same); a wave per row
-__global__ __launch_bounds__(256) void ce_amax_kernel(const float* __restrict__ x, int64_t rows, int C, Counts counts, float* __restrict__ out) {
+// largest finite |x| of the rows that count (blockIdx.y = 0) and of W (1), per workgroup (a maximum: any order gives the same); a
+// wave per row
+__global__ __launch_bounds__(1024) void ce_amax_kernel(const float* __restrict__ x, int64_t N, const float* __restrict__ w, int64_t V, int C,
+                                                       Counts counts, float* __restrict__ out) {
     float m = 0.f;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (int64_t r = (int64_t)blockIdx.x * 4 + wave; r < rows; r += (int64_t)kAmaxParts * 4) {
-        if (!counts(r)) continue;
-        for (int c = lane; c < C; c += 64) {
-            const float v = fabsf(x[r * C + c]);
-            m = v < INFINITY ? fmaxf(m, v) : m;
+    const bool first = blockIdx.y == 0;
+    const float* src = first ? x : w;
+    const int64_t rows = first ? N : V;
+    for (int64_t r = (int64_t)blockIdx.x * 16 + wave; r < rows; r += (int64_t)kAmaxParts * 16) {
+        if (first && !counts(r)) continue;
+        for (int c = lane * 4; c < C; c += 256) {
+            const auto q = load_vec(src + r * C, c, C);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float v = fabsf(q[k]);
+                m = v < INFINITY ? fmaxf(m, v) : m;
+            }
         }
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-    __shared__ float sh[4];
+    __shared__ float sh[16];
     if (lane == 0) sh[wave] = m;
     __syncthreads();
-    if (threadIdx.x == 0) out[blockIdx.x] = fmaxf(fmaxf(sh[0], sh[1]), fmaxf(sh[2], sh[3]));
+    if (threadIdx.x == 0) {
+        for (int k = 1; k < 16; ++k) m = fmaxf(m, sh[k]);
+        out[blockIdx.y * kAmaxParts + blockIdx.x] = m;
+    }
 }
 
 // -> the scale's exponent, the same in every thread of a 256-thread workgroup
@@ -70,12 +77,12 @@ __device__ __forceinline__ int amax_exp(const float* __restrict__ parts) {
     return scale_exp(fmaxf(fmaxf(sh[0], sh[1]), fmaxf(sh[2], sh[3])));
 }
 
-// rows [r0, r0 + R) of src (.., C) as planes, as they lie (dst, may be null) and transposed (dstT, may be null); k is zero-filled
+// rows [r0, r0 + R) of src (.., C) as an operand, as they lie (dst, may be null) and transposed (dstT, may be null); k is zero-filled
 // to the pitch.  gate: a row whose gate is 0 is written as zeros.  One workgroup: 64 rows x 64 columns.
 template <typename S, typename T, int P>
 __global__ __launch_bounds__(256) void ce_pack_kernel(const S* __restrict__ src, int64_t r0, int R, int C, const float* __restrict__ gate,
-                                                      const float* __restrict__ amax, char* __restrict__ dst, int64_t pitch, int64_t plane,
-                                                      char* __restrict__ dstT, int64_t pitchT, int64_t planeT) {
+                                                      const float* __restrict__ amax, char* __restrict__ dst, int64_t pitch,
+                                                      char* __restrict__ dstT, int64_t pitchT) {
     __shared__ uint32_t tile[64][65];
     const int ex = P == 2 ? amax_exp(amax) : 0;
     const int64_t rb = (int64_t)blockIdx.y * 64, cb = (int64_t)blockIdx.x * 64;
@@ -86,11 +93,10 @@ __global__ __launch_bounds__(256) void ce_pack_kernel(const S* __restrict__ src,
         if (r < R && c < C && (gate == nullptr || gate[r0 + r] != 0.f)) {
             const S v = src[(r0 + r) * C + c];
             if constexpr (P == 2) {
-                _Float16 hi, lo;
-                split16(ldexpf((float)v, ex), hi, lo);
-                q = (uint32_t)__builtin_bit_cast(uint16_t, hi) | (uint32_t)__builtin_bit_cast(uint16_t, lo) << 16;
+                const float f = ldexpf((float)v, ex);
+                q = (uint32_t)plane16(f, 0) | (uint32_t)plane16(f, 1) << 16;
             } else {
-                q = __builtin_bit_cast(uint16_t, v);
+                q = bits16(v);
             }
         }
         tile[i][lane] = q;
@@ -98,29 +104,20 @@ __global__ __launch_bounds__(256) void ce_pack_kernel(const S* __restrict__ src,
     __syncthreads();
     for (int u = threadIdx.x; u < 512; u += 256) {         // 64 rows x 8 chunks of 8 values
         const int i = u >> 3, k = (u & 7) * 8;
-        if (dst && rb + i < R && (cb + k) * 2 < pitch) {
-            u32x4 a, b;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const uint32_t p = tile[i][k + 2 * j], q = tile[i][k + 2 * j + 1];
-                a[j] = (p & 0xffffu) | q << 16;
-                b[j] = p >> 16 | (q & 0xffff0000u);
-            }
-            char* d = dst + (rb + i) * pitch + (cb + k) * 2;
-            *reinterpret_cast<u32x4*>(d) = a;
-            if (P == 2) *reinterpret_cast<u32x4*>(d + plane) = b;
-        }
-        if (dstT && cb + i < C && (rb + k) * 2 < pitchT) {
-            u32x4 a, b;
+        for (int q = 0; q < P; ++q) {
+            if (dst && rb + i < R && kbyte<P>(cb + k) < pitch) {
+                u32x4 a;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const uint32_t p = tile[k + 2 * j][i], q = tile[k + 2 * j + 1][i];
-                a[j] = (p & 0xffffu) | q << 16;
-                b[j] = p >> 16 | (q & 0xffff0000u);
+                for (int j = 0; j < 4; ++j) a[j] = (tile[i][k + 2 * j] >> 16 * q & 0xffffu) | tile[i][k + 2 * j + 1] >> 16 * q << 16;
+                *reinterpret_cast<u32x4*>(dst + (rb + i) * pitch + kbyte<P>(cb + k, q)) = a;
             }
-            char* d = dstT + (cb + i) * pitchT + (rb + k) * 2;
-            *reinterpret_cast<u32x4*>(d) = a;
-            if (P == 2) *reinterpret_cast<u32x4*>(d + planeT) = b;
+            if (dstT && cb + i < C && kbyte<P>(rb + k) < pitchT) {
+                u32x4 a;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) a[j] = (tile[k + 2 * j][i] >> 16 * q & 0xffffu) | tile[k + 2 * j + 1][i] >> 16 * q << 16;
+                *reinterpret_cast<u32x4*>(dstT + (cb + i) * pitchT + kbyte<P>(rb + k, q)) = a;
+            }
         }
     }
 }
@@ -137,8 +134,8 @@ struct LogitArgs {
     float* pm; float* ps; float* tl;
     // gradient: lse and g per row, E [N][pitchE] and its transpose [V][pitchT], partial db [tilesN * WN][V]
     const float* lse; const float* gate; const float* coef;
-    char* E; int64_t pitchE, planeE;
-    char* Et; int64_t pitchT, planeT;
+    char* E; int64_t pitchE;
+    char* Et; int64_t pitchT;
     float* pdb;
 };
 
@@ -183,7 +180,7 @@ __device__ __forceinline__ void logits_tile(const LogitArgs& p, int a0, int b0, 
     }
     if (p.bias) {
 #pragma unroll
-        for (int i = 0; i < M::TM; ++i)
+        for (int i = 0; i < M::TM; ++i) {
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
                 const int v = a0 + M::arow(i, e);
@@ -191,6 +188,8 @@ __device__ __forceinline__ void logits_tile(const LogitArgs& p, int a0, int b0, 
 #pragma unroll
                 for (int j = 0; j < M::TN; ++j) acc[i][j][e] += b;
             }
+            __builtin_amdgcn_sched_barrier(0);    // 16 loads at a time: all of them at once would spill the accumulators
+        }
     }
     if (a0 + M::BM > p.V) {                       // the last tile: classes that do not exist
 #pragma unroll
@@ -202,6 +201,7 @@ __device__ __forceinline__ void logits_tile(const LogitArgs& p, int a0, int b0, 
                 for (int j = 0; j < M::TN; ++j) acc[i][j][e] = out ? -INFINITY : acc[i][j][e];
             }
     }
+    __builtin_amdgcn_sched_barrier(0);
 }
 
 // the label of a position as an offset from the lane's first class: register (i, e) holds it where offset == 32 i + 8 (e / 4) + e % 4
@@ -213,7 +213,7 @@ __device__ __forceinline__ int label_offset(int64_t t, int a0) {
 __device__ __forceinline__ constexpr int reg_offset(int i, int e) { return 32 * i + 8 * (e >> 2) + (e & 3); }
 
 template <class M>
-__global__ __launch_bounds__(M::NT) void ce_lse_kernel(LogitArgs p) {
+__global__ __launch_bounds__(M::NT, 2) void ce_lse_kernel(LogitArgs p) {
     __shared__ __attribute__((aligned(16))) char lds[M::LDS];
     int ta, tb;
     tile_of<M>(p.tilesV, p.tilesN, ta, tb);
@@ -227,18 +227,22 @@ __global__ __launch_bounds__(M::NT) void ce_lse_kernel(LogitArgs p) {
         const int off = n < p.N ? label_offset<M>(p.target[n], a0) : -1;
         float m = -INFINITY, hit = 0.f;
 #pragma unroll
-        for (int i = 0; i < M::TM; ++i)
+        for (int i = 0; i < M::TM; ++i) {
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
                 m = fmaxf(m, acc[i][j][e]);
                 hit = reg_offset(i, e) == off ? acc[i][j][e] : hit;
             }
+            __builtin_amdgcn_sched_barrier(0);
+        }
         const float mm = m == -INFINITY ? 0.f : m;
         float s = 0.f;
 #pragma unroll
-        for (int i = 0; i < M::TM; ++i)
+        for (int i = 0; i < M::TM; ++i) {
 #pragma unroll
             for (int e = 0; e < 16; ++e) s += exp2_fast((acc[i][j][e] - mm) * kLog2e);
+            __builtin_amdgcn_sched_barrier(0);
+        }
         if (off >= 0 && (off & 4) == 0 && a0 + M::arow(0, 0) + off < p.V) p.tl[n] = hit;
         // the lane's other half of the rows
         const float m2 = __shfl_xor(m, 32, 64), s2 = __shfl_xor(s, 32, 64);
@@ -342,7 +346,7 @@ __global__ __launch_bounds__(1024) void ce_coef_kernel(const float* __restrict__
 }
 
 template <class M, bool DB>
-__global__ __launch_bounds__(M::NT) void ce_grad_kernel(LogitArgs p) {
+__global__ __launch_bounds__(M::NT, 2) void ce_grad_kernel(LogitArgs p) {
     __shared__ __attribute__((aligned(16))) char lds[M::LDS];
     int ta, tb;
     tile_of<M>(p.tilesV, p.tilesN, ta, tb);
@@ -381,39 +385,25 @@ __global__ __launch_bounds__(M::NT) void ce_grad_kernel(LogitArgs p) {
                 if ((lane & 31) == 0 && v < p.V) p.pdb[(int64_t)(tb * M::WN + wn) * p.V + v] = sum;
             }
         }
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    using W = WaveStore<M>;
+    char* reg = W::region(lds);
+    const int v0 = a0 + M::wave_row(), n0 = b0 + M::wave_col();
 #pragma unroll
-        for (int j = 0; j < M::TN; ++j) {
-            const int n = b0 + M::bcol(j);
-#pragma unroll
-            for (int e = 0; e < 16; e += 4) {
-                const int v = a0 + M::arow(i, e);                              // 4 consecutive classes
-                T hi[4], lo[4];
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    if constexpr (M::P == 2) split16(acc[i][j][e + k], hi[k], lo[k]);
-                    else hi[k] = (T)acc[i][j][e + k];
-                }
-                if (p.E && n < p.N) {
-                    char* d = p.E + n * p.pitchE + (int64_t)v * 2;
-                    u32x2 q;
-                    __builtin_memcpy(&q, hi, 8);
-                    *reinterpret_cast<u32x2*>(d) = q;
-                    if constexpr (M::P == 2) {
-                        __builtin_memcpy(&q, lo, 8);
-                        *reinterpret_cast<u32x2*>(d + p.planeE) = q;
-                    }
-                }
-                if (p.Et) {
-#pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        if (v + k < p.V) {
-                            char* d = p.Et + (v + k) * p.pitchT + (int64_t)n * 2;
-                            *reinterpret_cast<T*>(d) = hi[k];
-                            if constexpr (M::P == 2) *reinterpret_cast<T*>(d + p.planeT) = lo[k];
-                        }
-                }
-            }
-        }
+    for (int q = 0; q < M::P; ++q) {
+        auto val = [&](int i, int j, int e) -> uint16_t {
+            if constexpr (M::P == 2) return plane16(acc[i][j][e], q);
+            else return bits16((T)acc[i][j][e]);
+        };
+        if (p.E)                                           // the pitch covers the whole tile: no condition on the class
+            W::store_cols(reg, val, [&](int n, int v, u32x4 d) {
+                if (n0 + n < p.N) *reinterpret_cast<u32x4*>(p.E + (n0 + n) * p.pitchE + kbyte<M::P>(v0 + v, q)) = d;
+            });
+        if (p.Et)
+            W::store_rows(reg, val, [&](int v, int n, u32x4 d) {
+                if (v0 + v < p.V) *reinterpret_cast<u32x4*>(p.Et + (v0 + v) * p.pitchT + kbyte<M::P>(n0 + n, q)) = d;
+            });
     }
 }
 
@@ -432,7 +422,7 @@ template <typename O>
 __device__ __forceinline__ O finish(float v, float f, int ex) { return (O)ldexpf(v * f, ex); }
 
 template <class M, typename O>
-__global__ __launch_bounds__(M::NT) void ce_prod_kernel(ProdArgs p) {
+__global__ __launch_bounds__(M::NT, 2) void ce_prod_kernel(ProdArgs p) {
     __shared__ __attribute__((aligned(16))) char lds[M::LDS];
     int ta, tb;
     tile_of<M>(p.tilesA, p.tilesB, ta, tb);
@@ -456,6 +446,19 @@ __global__ __launch_bounds__(M::NT) void ce_prod_kernel(ProdArgs p) {
         }
     }
     float* plane = p.plane ? p.plane + (int64_t)z * p.rows * p.cols : nullptr;
+    if constexpr (sizeof(O) == 2) {
+        if (!plane) {
+            using W = WaveStore<M>;
+            const int r0 = a0 + M::wave_row(), c0 = b0 + M::wave_col();
+            W::store_rows(W::region(lds), [&](int i, int j, int e) -> uint16_t { return bits16(finish<O>(acc[i][j][e], f, ex)); },
+                          [&](int r, int c, u32x4 d) {
+                              if (r0 + r < p.rows && c0 + c < p.cols)
+                                  store_vec(reinterpret_cast<O*>(p.out) + (int64_t)(r0 + r) * p.cols, c0 + c, p.cols,
+                                            __builtin_bit_cast(typename Vec<O>::type, d));
+                          });
+            return;
+        }
+    }
 #pragma unroll
     for (int i = 0; i < M::TM; ++i)
 #pragma unroll
@@ -520,7 +523,7 @@ struct Blob {                                    // carves a workspace; a first 
     }
 };
 
-constexpr int64_t kMaxN = 1 << 24, kMaxV = 1 << 24, kMaxC = 1 << 16;
+constexpr int64_t kMaxN = 1 << 21, kMaxV = 1 << 24, kMaxC = 1 << 16;   // rows of operands stay below kMaxPitch
 inline bool shape_ok(int64_t N, int64_t C, int64_t V) {
     return N > 0 && C > 0 && V > 0 && N <= kMaxN && V <= kMaxV && C <= kMaxC && (N / 128 + 1) * (V / 128 + 1) < INT32_MAX;
 }
@@ -528,41 +531,57 @@ inline bool shape_ok(int64_t N, int64_t C, int64_t V) {
 // Is the matrix an operand as it lies (16-bit, whole stages of k, aligned)?
 inline bool direct(int dtype, const void* p, int64_t C) { return dtype != kF32 && C % 64 == 0 && ((uintptr_t)p & 15) == 0; }
 
+// What forward leaves for backward beside the statistics: the scales' parts and the operands that had to be copied (two planes, or
+// k padded to a stage).
+struct Packed {
+    float *amaxX, *amaxW;                        // null for 16-bit types
+    char *Xp, *Wp;                               // null where the tensor is an operand as it lies
+    int64_t pitch;
+    size_t bytes;
+};
+
+Packed plan_packed(void* base, const void* x, const void* w, int dtype, int64_t N, int64_t C, int64_t V) {
+    Blob b(base);
+    Packed p = {};
+    const int P = dtype == kF32 ? 2 : 1;
+    p.pitch = up(C, 64) * 2 * P;
+    if (P == 2) {
+        p.amaxX = b.take<float>(2 * kAmaxParts);
+        p.amaxW = p.amaxX + kAmaxParts;
+    }
+    if (!direct(dtype, x, C)) p.Xp = b.take<char>((size_t)(N * p.pitch));
+    if (!direct(dtype, w, C)) p.Wp = b.take<char>((size_t)(V * p.pitch));
+    p.bytes = b.at;
+    return p;
+}
+
 struct FwdPlan {
-    int64_t Cp; int BMt, WMt, tilesV, tilesN, parts;
-    float *amaxX, *amaxW, *pm, *ps, *tl, *row;
-    char *Xp, *Wp;
+    int tile, tilesV, tilesN, parts;
+    float *pm, *ps, *tl, *row;
 };
 
 inline bool use_big(int64_t a, int64_t b) { return ((a + 255) / 256) * ((b + 255) / 256) >= 256; }
 
-FwdPlan plan_fwd(Blob& ws, int dtype, int64_t N, int64_t C, int64_t V, bool dx, bool dw) {
+FwdPlan plan_fwd(Blob& ws, int64_t N, int64_t V) {
     FwdPlan p;
-    const int P = dtype == kF32 ? 2 : 1;
-    p.Cp = up(C, 64);
-    const bool big = use_big(V, N);
-    p.BMt = big ? 256 : 128;
-    p.WMt = 2;
-    p.tilesV = (int)((V + p.BMt - 1) / p.BMt);
-    p.tilesN = (int)((N + p.BMt - 1) / p.BMt);
-    p.parts = p.tilesV * p.WMt;
-    p.amaxX = ws.take<float>(P == 2 ? kAmaxParts : 0);
-    p.amaxW = ws.take<float>(P == 2 ? kAmaxParts : 0);
+    p.tile = use_big(V, N) ? 256 : 128;
+    p.tilesV = (int)((V + p.tile - 1) / p.tile);
+    p.tilesN = (int)((N + p.tile - 1) / p.tile);
+    p.parts = p.tilesV * 2;                      // two waves of a tile along the classes
     p.pm = ws.take<float>((size_t)p.parts * N);
     p.ps = ws.take<float>((size_t)p.parts * N);
     p.tl = ws.take<float>((size_t)N);
     p.row = ws.take<float>((size_t)N);
-    p.Xp = ws.take<char>(dx ? 0 : (size_t)N * p.Cp * 2 * P);
-    p.Wp = ws.take<char>(dw ? 0 : (size_t)V * p.Cp * 2 * P);
     return p;
 }
 
 template <typename S>
-int pack(const void* src, int64_t r0, int64_t R, int64_t C, const float* gate, const float* amax, char* dst, int64_t pitch, int64_t plane, char* dstT,
-         int64_t pitchT, int64_t planeT, hipStream_t st) {
-    const int64_t wide = dst && pitch / 2 > C ? pitch / 2 : C, tall = dstT && pitchT / 2 > R ? pitchT / 2 : R;
-    hipLaunchKernelGGL((ce_pack_kernel<S, typename Inner<S>::T, Inner<S>::P>), dim3((unsigned)((wide + 63) / 64), (unsigned)((tall + 63) / 64)),
-                       dim3(256), 0, st, (const S*)src, r0, (int)R, (int)C, gate, amax, dst, pitch, plane, dstT, pitchT, planeT);
+int pack(const void* src, int64_t r0, int64_t R, int64_t C, const float* gate, const float* amax, char* dst, int64_t pitch, char* dstT,
+         int64_t pitchT, hipStream_t st) {
+    constexpr int P = Inner<S>::P;
+    const int64_t wide = dst ? pitch / (2 * P) : C, tall = dstT ? pitchT / (2 * P) : R;
+    hipLaunchKernelGGL((ce_pack_kernel<S, typename Inner<S>::T, P>), dim3((unsigned)((wide + 63) / 64), (unsigned)((tall + 63) / 64)), dim3(256), 0, st,
+                       (const S*)src, r0, (int)R, (int)C, gate, amax, dst, pitch, dstT, pitchT);
     return (int)hipGetLastError();
 }
 
@@ -575,31 +594,31 @@ int pack(const void* src, int64_t r0, int64_t R, int64_t C, const float* gate, c
 
 template <typename S>
 int ce_fwd(const void* x, const void* w, const float* bias, const int64_t* target, const float* conf, float thresh, int64_t ignore, int dtype,
-           int64_t N, int64_t C, int64_t V, int reduction, float* loss, float* lse, float* gate, float* count, void* ws, hipStream_t st) {
+           int64_t N, int64_t C, int64_t V, int reduction, float* loss, float* lse, float* gate, float* count, void* packed, void* ws,
+           hipStream_t st) {
     using T = typename Inner<S>::T;
     constexpr int P = Inner<S>::P;
     Blob blob(ws);
-    const bool dX = direct(dtype, x, C), dW = direct(dtype, w, C);
-    const FwdPlan p = plan_fwd(blob, dtype, N, C, V, dX, dW);
+    const Packed k = plan_packed(packed, x, w, dtype, N, C, V);
+    const FwdPlan p = plan_fwd(blob, N, V);
     LogitArgs a = {};
     int rc = 0;
     if constexpr (P == 2) {
-        hipLaunchKernelGGL(ce_amax_kernel, dim3(kAmaxParts), dim3(256), 0, st, (const float*)x, N, (int)C,
-                           Counts{nullptr, target, ignore, conf, thresh}, p.amaxX);
-        hipLaunchKernelGGL(ce_amax_kernel, dim3(kAmaxParts), dim3(256), 0, st, (const float*)w, V, (int)C, Counts{}, p.amaxW);
-        a.amaxX = p.amaxX;
-        a.amaxW = p.amaxW;
+        hipLaunchKernelGGL(ce_amax_kernel, dim3(kAmaxParts, 2), dim3(1024), 0, st, (const float*)x, N, (const float*)w, V, (int)C,
+                           Counts{target, ignore, conf, thresh}, k.amaxX);
+        a.amaxX = k.amaxX;
+        a.amaxW = k.amaxW;
     }
-    if (!dX && (rc = pack<S>(x, 0, N, C, nullptr, p.amaxX, p.Xp, p.Cp * 2, N * p.Cp * 2, nullptr, 0, 0, st)) != 0) return rc;
-    if (!dW && (rc = pack<S>(w, 0, V, C, nullptr, p.amaxW, p.Wp, p.Cp * 2, V * p.Cp * 2, nullptr, 0, 0, st)) != 0) return rc;
-    a.X = {dX ? (const char*)x : p.Xp, p.Cp * 2, N * p.Cp * 2, (int)N};
-    a.W = {dW ? (const char*)w : p.Wp, p.Cp * 2, V * p.Cp * 2, (int)V};
+    if (k.Xp && (rc = pack<S>(x, 0, N, C, nullptr, k.amaxX, k.Xp, k.pitch, nullptr, 0, st)) != 0) return rc;
+    if (k.Wp && (rc = pack<S>(w, 0, V, C, nullptr, k.amaxW, k.Wp, k.pitch, nullptr, 0, st)) != 0) return rc;
+    a.X = {k.Xp ? k.Xp : (const char*)x, k.pitch, (int)N};
+    a.W = {k.Wp ? k.Wp : (const char*)w, k.pitch, (int)V};
     a.bias = bias;
     a.V = (int)V; a.N = (int)N; a.tilesV = p.tilesV; a.tilesN = p.tilesN;
-    a.stages = (int)(p.Cp / (P == 1 ? 64 : 32));
+    a.stages = (int)(k.pitch / 128);
     a.target = target; a.v0 = 0;
     a.pm = p.pm; a.ps = p.ps; a.tl = p.tl;
-    if (p.BMt == 256) { using M = Big<T, P>; SSECG_CE_LAUNCH(M, ce_lse_kernel<M>, dim3(p.tilesV * p.tilesN), st, a); }
+    if (p.tile == 256) { using M = Big<T, P>; SSECG_CE_LAUNCH(M, ce_lse_kernel<M>, dim3(p.tilesV * p.tilesN), st, a); }
     else { using M = Mid<T, P>; SSECG_CE_LAUNCH(M, ce_lse_kernel<M>, dim3(p.tilesV * p.tilesN), st, a); }
     float* row = reduction == 0 ? loss : p.row;
     hipLaunchKernelGGL(ce_join_kernel, dim3((unsigned)((N + 15) / 16)), dim3(256), 0, st, p.pm, p.ps, p.tl, p.parts, (int)N, (int)V, target, conf, thresh,
@@ -612,12 +631,12 @@ int ce_fwd(const void* x, const void* w, const float* bias, const int64_t* targe
 constexpr size_t kPieceBytes = (size_t)1 << 30;  // E, its transpose and the piece's W^T
 
 struct BwdPlan {
-    int64_t Cp, Np, Vc;                          // padded sizes, classes per piece (multiple of 256 unless one piece)
+    int64_t Vc;                                  // classes per piece (a multiple of 256 unless there is one piece)
     int pieces, splitX, splitW;
     bool bigL, bigX, bigW;
-    float *amaxX, *amaxW, *coef, *fscale, *pdb, *planeX, *planeW;
-    char *Xp, *Wp, *Xt, *Wt, *E, *Et;
-    int64_t pitchE, pitchT, pitchWt;
+    float *coef, *fscale, *pdb, *planeX, *planeW;
+    char *Xt, *Wt, *E, *Et;
+    int64_t pitchE, pitchT;                      // bytes of a row of E and W^T; of E^T and X^T
 };
 
 // How many workgroups share the k of one tile: enough to give each of the 256 CUs one, each at least 8 stages long.
@@ -627,40 +646,35 @@ inline int split_of(int64_t tiles, int64_t stages) {
     return (int)(s < 1 ? 1 : (s > 64 ? 64 : s));
 }
 
-BwdPlan plan_bwd(Blob& ws, int dtype, int64_t N, int64_t C, int64_t V, bool dX, bool dW, bool want_x, bool want_w, bool want_b) {
+BwdPlan plan_bwd(Blob& ws, int dtype, int64_t N, int64_t C, int64_t V, bool want_x, bool want_w, bool want_b) {
     BwdPlan p;
     const int P = dtype == kF32 ? 2 : 1, BK = P == 1 ? 64 : 32;
-    p.Cp = up(C, 64);
-    p.Np = up(N, 256);
-    const size_t per = (size_t)(p.Np * (want_w ? 2 : 0) + N * (want_x ? 2 : 0) + C * (want_x ? 2 : 0)) * P + 1;
+    const int64_t Np = up(N, 256);
+    const size_t per = (size_t)(Np * (want_w ? 2 : 0) + N * (want_x ? 2 : 0) + C * (want_x ? 2 : 0)) * P + 1;
     int64_t most = (int64_t)(kPieceBytes / per) / 256 * 256;
     if (most < 256) most = 256;
+    if (most > (1 << 21)) most = 1 << 21;        // a row of E stays below the operand's largest pitch
     const int64_t pieces = (V + most - 1) / most;
     p.Vc = pieces == 1 ? V : up((V + pieces - 1) / pieces, 256);
     p.pieces = (int)((V + p.Vc - 1) / p.Vc);
     p.bigL = use_big(p.Vc, N);
     p.bigX = use_big(N, C);
     p.bigW = use_big(p.Vc, C);
-    p.pitchE = up(p.Vc, 256) * 2;
-    p.pitchWt = p.pitchE;
-    p.pitchT = p.Np * 2;
+    p.pitchE = up(p.Vc, 256) * 2 * P;
+    p.pitchT = Np * 2 * P;
     const int bx = p.bigX ? 256 : 128, bw = p.bigW ? 256 : 128;
     p.splitX = split_of(((N + bx - 1) / bx) * ((C + bx - 1) / bx), up(p.Vc, BK) / BK);
     p.splitW = split_of(((p.Vc + bw - 1) / bw) * ((C + bw - 1) / bw), up(N, BK) / BK);
-    p.amaxX = ws.take<float>(P == 2 ? kAmaxParts : 0);
-    p.amaxW = ws.take<float>(P == 2 ? kAmaxParts : 0);
     p.coef = ws.take<float>((size_t)N);
     p.fscale = ws.take<float>(1);
     const int bl = p.bigL ? 256 : 128, wn = p.bigL ? 4 : 2;
     p.pdb = ws.take<float>(want_b ? (size_t)((N + bl - 1) / bl) * wn * p.Vc : 0);
     p.planeX = ws.take<float>(want_x && (p.splitX > 1 || p.pieces > 1) ? (size_t)p.splitX * N * C : 0);
     p.planeW = ws.take<float>(want_w && p.splitW > 1 ? (size_t)p.splitW * p.Vc * C : 0);
-    p.Xp = ws.take<char>(dX ? 0 : (size_t)N * p.Cp * 2 * P);
-    p.Wp = ws.take<char>(dW ? 0 : (size_t)V * p.Cp * 2 * P);
-    p.Xt = ws.take<char>(want_w ? (size_t)C * p.pitchT * P : 0);
-    p.Wt = ws.take<char>(want_x ? (size_t)C * p.pitchWt * P : 0);
-    p.E = ws.take<char>(want_x ? (size_t)N * p.pitchE * P : 0);
-    p.Et = ws.take<char>(want_w ? (size_t)p.Vc * p.pitchT * P : 0);
+    p.Xt = ws.take<char>(want_w ? (size_t)C * p.pitchT : 0);
+    p.Wt = ws.take<char>(want_x ? (size_t)C * p.pitchE : 0);
+    p.E = ws.take<char>(want_x ? (size_t)N * p.pitchE : 0);
+    p.Et = ws.take<char>(want_w ? (size_t)p.Vc * p.pitchT : 0);
     return p;
 }
 
@@ -671,41 +685,32 @@ inline unsigned grid_for(int64_t n) {
 
 template <typename S>
 int ce_bwd(const float* dloss, const void* x, const void* w, const float* bias, const int64_t* target, const float* lse, const float* gate,
-           const float* count, int dtype, int64_t N, int64_t C, int64_t V, int reduction, void* dx, void* dw, float* db, void* ws, hipStream_t st) {
+           const float* count, int dtype, int64_t N, int64_t C, int64_t V, int reduction, void* dx, void* dw, float* db, void* packed, void* ws,
+           hipStream_t st) {
     using T = typename Inner<S>::T;
     constexpr int P = Inner<S>::P;
     constexpr int BK = P == 1 ? 64 : 32;
     Blob blob(ws);
-    const bool dX = direct(dtype, x, C), dW = direct(dtype, w, C);
-    const BwdPlan p = plan_bwd(blob, dtype, N, C, V, dX, dW, dx != nullptr, dw != nullptr, db != nullptr);
+    const Packed k = plan_packed(packed, x, w, dtype, N, C, V);
+    const BwdPlan p = plan_bwd(blob, dtype, N, C, V, dx != nullptr, dw != nullptr, db != nullptr);
     int rc = 0;
-    if constexpr (P == 2) {
-        // X's scale: over the rows that count (a row that does not may hold anything)
-        hipLaunchKernelGGL(ce_amax_kernel, dim3(kAmaxParts), dim3(256), 0, st, (const float*)x, N, (int)C, Counts{gate, nullptr, 0, nullptr, 0.f},
-                           p.amaxX);
-        hipLaunchKernelGGL(ce_amax_kernel, dim3(kAmaxParts), dim3(256), 0, st, (const float*)w, V, (int)C, Counts{}, p.amaxW);
-    }
     hipLaunchKernelGGL(ce_coef_kernel, dim3(1), dim3(1024), 0, st, dloss, gate, count, (int)N, reduction, p.coef, p.fscale);
-    if (!dX || dw) {
-        rc = pack<S>(x, 0, N, C, gate, p.amaxX, dX ? nullptr : p.Xp, p.Cp * 2, N * p.Cp * 2, dw ? p.Xt : nullptr, p.pitchT, C * p.pitchT, st);
-        if (rc != 0) return rc;
-    }
-    if (!dW && (rc = pack<S>(w, 0, V, C, nullptr, p.amaxW, p.Wp, p.Cp * 2, V * p.Cp * 2, nullptr, 0, 0, st)) != 0) return rc;
+    if (dw && (rc = pack<S>(x, 0, N, C, gate, k.amaxX, nullptr, 0, p.Xt, p.pitchT, st)) != 0) return rc;
     for (int i = 0; i < p.pieces; ++i) {
         const int64_t v0 = i * p.Vc, vn = V - v0 < p.Vc ? V - v0 : p.Vc;
         LogitArgs a = {};
-        a.X = {dX ? (const char*)x : p.Xp, p.Cp * 2, N * p.Cp * 2, (int)N};
-        a.W = {(dW ? (const char*)w : p.Wp) + v0 * p.Cp * 2, p.Cp * 2, V * p.Cp * 2, (int)vn};
+        a.X = {k.Xp ? k.Xp : (const char*)x, k.pitch, (int)N};
+        a.W = {(k.Wp ? k.Wp : (const char*)w) + v0 * k.pitch, k.pitch, (int)vn};
         a.bias = bias ? bias + v0 : nullptr;
-        a.amaxX = p.amaxX; a.amaxW = p.amaxW;
+        a.amaxX = k.amaxX; a.amaxW = k.amaxW;
         a.V = (int)vn; a.N = (int)N;
         const int bl = p.bigL ? 256 : 128, wn = p.bigL ? 4 : 2;
         a.tilesV = (int)((vn + bl - 1) / bl); a.tilesN = (int)((N + bl - 1) / bl);
-        a.stages = (int)(p.Cp / BK);
+        a.stages = (int)(k.pitch / 128);
         a.target = target; a.v0 = v0;
         a.lse = lse; a.gate = gate; a.coef = reduction == 0 ? p.coef : nullptr;
-        a.E = dx ? p.E : nullptr; a.pitchE = p.pitchE; a.planeE = N * p.pitchE;
-        a.Et = dw ? p.Et : nullptr; a.pitchT = p.pitchT; a.planeT = p.Vc * p.pitchT;
+        a.E = dx ? p.E : nullptr; a.pitchE = p.pitchE;
+        a.Et = dw ? p.Et : nullptr; a.pitchT = p.pitchT;
         a.pdb = p.pdb;
         const dim3 grid(a.tilesV * a.tilesN);
         if (p.bigL) {
@@ -719,41 +724,41 @@ int ce_bwd(const float* dloss, const void* x, const void* w, const float* bias, 
         }
         if (db) hipLaunchKernelGGL(ce_db_kernel, dim3((unsigned)((vn + 255) / 256)), dim3(256), 0, st, p.pdb, a.tilesN * wn, (int)vn, p.fscale, db + v0);
         if (dx) {
-            if ((rc = pack<S>(w, v0, vn, C, nullptr, p.amaxW, nullptr, 0, 0, p.Wt, up(vn, 64) * 2 < p.pitchWt ? up(vn, 64) * 2 : p.pitchWt, C * p.pitchWt, st)) != 0) return rc;
+            const int64_t pitch = up(vn, 64) * 2 * P;
+            if ((rc = pack<S>(w, v0, vn, C, nullptr, k.amaxW, nullptr, 0, p.Wt, pitch, st)) != 0) return rc;
             ProdArgs q = {};
-            const int64_t wp = up(vn, 64) * 2 < p.pitchWt ? up(vn, 64) * 2 : p.pitchWt;
-            q.A = {p.E, p.pitchE, N * p.pitchE, (int)N};
-            q.B = {p.Wt, wp, C * p.pitchWt, (int)C};
+            q.A = {p.E, p.pitchE, (int)N};
+            q.B = {p.Wt, pitch, (int)C};
             q.rows = (int)N; q.cols = (int)C;
             const int bx = p.bigX ? 256 : 128;
             q.tilesA = (int)((N + bx - 1) / bx); q.tilesB = (int)((C + bx - 1) / bx);
             q.stages = (int)(up(vn, BK) / BK); q.splits = p.splitX;
             q.plane = p.splitX > 1 || p.pieces > 1 ? p.planeX : nullptr;
-            q.add = i > 0; q.out = dx; q.amax = p.amaxW; q.fscale = p.fscale;
+            q.add = i > 0; q.out = dx; q.amax = k.amaxW; q.fscale = p.fscale;
             const dim3 g2(q.tilesA * q.tilesB, q.splits);
             if (p.bigX) { using M = Big<T, P>; SSECG_CE_LAUNCH(M, (ce_prod_kernel<M, S>), g2, st, q); }
             else { using M = Mid<T, P>; SSECG_CE_LAUNCH(M, (ce_prod_kernel<M, S>), g2, st, q); }
         }
         if (dw) {
             ProdArgs q = {};
-            q.A = {p.Et, p.pitchT, p.Vc * p.pitchT, (int)vn};
-            q.B = {p.Xt, p.pitchT, C * p.pitchT, (int)C};
+            q.A = {p.Et, p.pitchT, (int)vn};
+            q.B = {p.Xt, p.pitchT, (int)C};
             q.rows = (int)vn; q.cols = (int)C;
             const int bw = p.bigW ? 256 : 128;
             q.tilesA = (int)((vn + bw - 1) / bw); q.tilesB = (int)((C + bw - 1) / bw);
             q.stages = (int)(up(N, BK) / BK); q.splits = p.splitW;
             q.plane = p.splitW > 1 ? p.planeW : nullptr;
-            q.out = (S*)dw + v0 * C; q.amax = p.amaxX; q.fscale = p.fscale;
+            q.out = (S*)dw + v0 * C; q.amax = k.amaxX; q.fscale = p.fscale;
             const dim3 g2(q.tilesA * q.tilesB, q.splits);
             if (p.bigW) { using M = Big<T, P>; SSECG_CE_LAUNCH(M, (ce_prod_kernel<M, S>), g2, st, q); }
             else { using M = Mid<T, P>; SSECG_CE_LAUNCH(M, (ce_prod_kernel<M, S>), g2, st, q); }
             if (q.plane)
                 hipLaunchKernelGGL((ce_sum_planes_kernel<S>), dim3(grid_for(vn * C)), dim3(256), 0, st, p.planeW, p.splitW, vn * C,
-                                   P == 2 ? p.amaxX : nullptr, p.fscale, (S*)dw + v0 * C);
+                                   P == 2 ? k.amaxX : nullptr, p.fscale, (S*)dw + v0 * C);
         }
     }
     if (dx && (p.splitX > 1 || p.pieces > 1))
-        hipLaunchKernelGGL((ce_sum_planes_kernel<S>), dim3(grid_for(N * C)), dim3(256), 0, st, p.planeX, p.splitX, N * C, P == 2 ? p.amaxW : nullptr,
+        hipLaunchKernelGGL((ce_sum_planes_kernel<S>), dim3(grid_for(N * C)), dim3(256), 0, st, p.planeX, p.splitX, N * C, P == 2 ? k.amaxW : nullptr,
                            p.fscale, (S*)dx);
     return (int)hipGetLastError();
 }
@@ -762,40 +767,49 @@ int ce_bwd(const float* dloss, const void* x, const void* w, const float* bias, 
 
 extern "C" {
 
+size_t ssecg_linear_ce_packed_bytes(const void* x, const void* weight, int dtype, int64_t N, int64_t C, int64_t V) {
+    if (!x || !weight || !dtype_ok(dtype) || !shape_ok(N, C, V)) return 0;
+    return plan_packed(nullptr, x, weight, dtype, N, C, V).bytes;
+}
+
 size_t ssecg_linear_ce_fwd_workspace(int dtype, int64_t N, int64_t C, int64_t V) {
     if (!dtype_ok(dtype) || !shape_ok(N, C, V)) return 0;
     Blob b(nullptr);
-    plan_fwd(b, dtype, N, C, V, false, false);
+    plan_fwd(b, N, V);
     return b.at;
 }
 
 int ssecg_linear_ce_fwd(const void* x, const void* weight, const float* bias, const int64_t* target, const float* conf, double thresh,
                         int64_t ignore_index, int dtype, int64_t N, int64_t C, int64_t V, int reduction, float* loss, float* lse, float* gate,
-                        float* count, void* workspace, size_t workspace_bytes, void* stream) {
+                        float* count, void* packed, size_t packed_bytes, void* workspace, size_t workspace_bytes, void* stream) {
     if (!x || !weight || !target || !loss || !lse || !gate || !count || !workspace || !dtype_ok(dtype) || !shape_ok(N, C, V) || reduction < 0 ||
-        reduction > 2 || ((uintptr_t)workspace & 255))
+        reduction > 2 || ((uintptr_t)workspace & 255) || ((uintptr_t)packed & 255))
         return SSECG_E_INVAL;
     if (workspace_bytes < ssecg_linear_ce_fwd_workspace(dtype, N, C, V)) return SSECG_E_WORKSPACE;
+    const size_t keep = ssecg_linear_ce_packed_bytes(x, weight, dtype, N, C, V);
+    if (packed_bytes < keep || (keep && !packed)) return SSECG_E_WORKSPACE;
     SSECG_LM_DTYPE(dtype, S, return ce_fwd<S>(x, weight, bias, target, conf, (float)thresh, ignore_index, dtype, N, C, V, reduction, loss, lse, gate,
-                                              count, workspace, (hipStream_t)stream));
+                                              count, packed, workspace, (hipStream_t)stream));
 }
 
 size_t ssecg_linear_ce_bwd_workspace(int dtype, int64_t N, int64_t C, int64_t V, int want_dx, int want_dw, int want_db) {
     if (!dtype_ok(dtype) || !shape_ok(N, C, V)) return 0;
     Blob b(nullptr);
-    plan_bwd(b, dtype, N, C, V, false, false, want_dx != 0, want_dw != 0, want_db != 0);
+    plan_bwd(b, dtype, N, C, V, want_dx != 0, want_dw != 0, want_db != 0);
     return b.at;
 }
 
 int ssecg_linear_ce_bwd(const float* dloss, const void* x, const void* weight, const float* bias, const int64_t* target, const float* lse,
                         const float* gate, const float* count, int dtype, int64_t N, int64_t C, int64_t V, int reduction, void* dx, void* dweight,
-                        float* dbias, void* workspace, size_t workspace_bytes, void* stream) {
+                        float* dbias, const void* packed, size_t packed_bytes, void* workspace, size_t workspace_bytes, void* stream) {
     if (!dloss || !x || !weight || !target || !lse || !gate || !count || !workspace || (!dx && !dweight && !dbias) || !dtype_ok(dtype) ||
-        !shape_ok(N, C, V) || reduction < 0 || reduction > 2 || ((uintptr_t)workspace & 255))
+        !shape_ok(N, C, V) || reduction < 0 || reduction > 2 || ((uintptr_t)workspace & 255) || ((uintptr_t)packed & 255))
         return SSECG_E_INVAL;
     if (workspace_bytes < ssecg_linear_ce_bwd_workspace(dtype, N, C, V, dx != nullptr, dweight != nullptr, dbias != nullptr)) return SSECG_E_WORKSPACE;
-    SSECG_LM_DTYPE(dtype, S, return ce_bwd<S>(dloss, x, weight, bias, target, lse, gate, count, dtype, N, C, V, reduction, dx, dweight, dbias, workspace,
-                                              (hipStream_t)stream));
+    const size_t keep = ssecg_linear_ce_packed_bytes(x, weight, dtype, N, C, V);
+    if (packed_bytes < keep || (keep && !packed)) return SSECG_E_WORKSPACE;
+    SSECG_LM_DTYPE(dtype, S, return ce_bwd<S>(dloss, x, weight, bias, target, lse, gate, count, dtype, N, C, V, reduction, dx, dweight, dbias,
+                                              (void*)packed, workspace, (hipStream_t)stream));
 }
 
 }  // extern "C"

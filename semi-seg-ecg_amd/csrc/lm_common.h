@@ -30,7 +30,33 @@ __device__ __forceinline__ float wave_sum(float v) {
     return v;
 }
 
-// calls f.template operator()<T>() with the element type of the ABI code
+// elements [c0, c0 + 16 bytes) of a row of C; beyond C: zeros, and nothing is written there
+template <typename T>
+__device__ __forceinline__ typename Vec<T>::type load_vec(const T* __restrict__ p, int c0, int C) {
+    constexpr int V = Vec<T>::N;
+    typename Vec<T>::type v;
+    if (c0 + V <= C) {
+        v = *reinterpret_cast<const typename Vec<T>::type*>(p + c0);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] = c0 + i < C ? p[c0 + i] : (T)0.f;
+    }
+    return v;
+}
+
+template <typename T>
+__device__ __forceinline__ void store_vec(T* __restrict__ p, int c0, int C, typename Vec<T>::type v) {
+    constexpr int V = Vec<T>::N;
+    if (c0 + V <= C) {
+        *reinterpret_cast<typename Vec<T>::type*>(p + c0) = v;
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (c0 + i < C) p[c0 + i] = v[i];
+    }
+}
+
+// runs the statements with T = the element type of the ABI code
 #define SSECG_LM_DTYPE(code, T, ...)                                   \
     do {                                                               \
         if ((code) == ssecg_lm::kF32) { using T = float; __VA_ARGS__; }      \

@@ -37,8 +37,7 @@ struct Mat {
     const void* src; void* dst; float* mom;
     int rows, cols, m, n;
     int64_t pn, pm;                               // bytes of a row of X; of X^T, A and P
-    char *X, *Xt0, *Xt1, *A, *P;
-    int64_t planeX, planeXt, planeA;
+    char *X, *Xt0, *Xt1, *A, *P;                  // operands of two planes (mm_core.h)
 };
 
 inline __host__ __device__ int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
@@ -46,8 +45,8 @@ inline __host__ __device__ int64_t up(int64_t v, int64_t to) { return (v + to - 
 // planes of one matrix in the workspace: X, X^T twice (read one, write the other), A, P
 inline __host__ __device__ int64_t mat_bytes(int64_t rows, int64_t cols) {
     const int64_t m = rows < cols ? rows : cols, n = rows < cols ? cols : rows;
-    const int64_t pn = up(n, 32) * 2, pm = up(m, 32) * 2;
-    return up(2 * (m * pn + 2 * n * pm + 2 * m * pm), 256);
+    const int64_t pn = up(n, 32) * 4, pm = up(m, 32) * 4;
+    return up(m * pn + 2 * n * pm + 2 * m * pm, 256);
 }
 
 __device__ __forceinline__ Mat load_mat(const Table& table, int k, char* ws) {
@@ -59,16 +58,13 @@ __device__ __forceinline__ Mat load_mat(const Table& table, int k, char* ws) {
     t.cols = table.cols[k];
     t.m = t.rows < t.cols ? t.rows : t.cols;
     t.n = t.rows < t.cols ? t.cols : t.rows;
-    t.pn = up(t.n, 32) * 2;
-    t.pm = up(t.m, 32) * 2;
-    t.planeX = t.m * t.pn;
-    t.planeXt = t.n * t.pm;
-    t.planeA = t.m * t.pm;
+    t.pn = up(t.n, 32) * 4;
+    t.pm = up(t.m, 32) * 4;
     t.X = ws + table.offset[k];
-    t.Xt0 = t.X + 2 * t.planeX;
-    t.Xt1 = t.Xt0 + 2 * t.planeXt;
-    t.A = t.Xt1 + 2 * t.planeXt;
-    t.P = t.A + 2 * t.planeA;
+    t.Xt0 = t.X + t.m * t.pn;
+    t.Xt1 = t.Xt0 + t.n * t.pm;
+    t.A = t.Xt1 + t.n * t.pm;
+    t.P = t.A + t.m * t.pm;
     return t;
 }
 
@@ -138,9 +134,8 @@ __global__ __launch_bounds__(256) void ns_prep_kernel(Table table, char* __restr
         const int64_t r = rb + i, c = cb + lane;
         uint32_t q = 0;
         if (r < t.rows && c < t.cols) {
-            _Float16 hi, lo;
-            split16(update_of<S, MUON>(t, r * t.cols + c, mu, nesterov) * f, hi, lo);
-            q = (uint32_t)__builtin_bit_cast(uint16_t, hi) | (uint32_t)__builtin_bit_cast(uint16_t, lo) << 16;
+            const float u = update_of<S, MUON>(t, r * t.cols + c, mu, nesterov) * f;
+            q = (uint32_t)plane16(u, 0) | (uint32_t)plane16(u, 1) << 16;
         }
         tile[i][lane] = q;
     }
@@ -149,47 +144,20 @@ __global__ __launch_bounds__(256) void ns_prep_kernel(Table table, char* __restr
     char* D = tall ? t.Xt0 : t.X;               // as the matrix lies: rows x cols
     char* Dt = tall ? t.X : t.Xt0;              // transposed: cols x rows
     const int64_t pd = tall ? t.pm : t.pn, pt = tall ? t.pn : t.pm;
-    const int64_t ld = tall ? t.planeXt : t.planeX, lt = tall ? t.planeX : t.planeXt;
     for (int u = threadIdx.x; u < 512; u += 256) {
         const int i = u >> 3, c8 = (u & 7) * 8;
-        u32x4 a, b, ta, tb;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const uint32_t p = tile[i][c8 + 2 * j], q = tile[i][c8 + 2 * j + 1];
-            a[j] = (p & 0xffffu) | q << 16;
-            b[j] = p >> 16 | (q & 0xffff0000u);
-            const uint32_t pp = tile[c8 + 2 * j][i], qq = tile[c8 + 2 * j + 1][i];
-            ta[j] = (pp & 0xffffu) | qq << 16;
-            tb[j] = pp >> 16 | (qq & 0xffff0000u);
-        }
-        if (rb + i < t.rows && (cb + c8) * 2 < pd) {
-            char* d = D + (rb + i) * pd + (cb + c8) * 2;
-            *reinterpret_cast<u32x4*>(d) = a;
-            *reinterpret_cast<u32x4*>(d + ld) = b;
-        }
-        if (cb + i < t.cols && (rb + c8) * 2 < pt) {
-            char* d = Dt + (cb + i) * pt + (rb + c8) * 2;
-            *reinterpret_cast<u32x4*>(d) = ta;
-            *reinterpret_cast<u32x4*>(d + lt) = tb;
+        for (int q = 0; q < 2; ++q) {
+            u32x4 a, ta;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                a[j] = (tile[i][c8 + 2 * j] >> 16 * q & 0xffffu) | tile[i][c8 + 2 * j + 1] >> 16 * q << 16;
+                ta[j] = (tile[c8 + 2 * j][i] >> 16 * q & 0xffffu) | tile[c8 + 2 * j + 1][i] >> 16 * q << 16;
+            }
+            if (rb + i < t.rows && kbyte<2>(cb + c8) < pd) *reinterpret_cast<u32x4*>(D + (rb + i) * pd + kbyte<2>(cb + c8, q)) = a;
+            if (cb + i < t.cols && kbyte<2>(rb + c8) < pt) *reinterpret_cast<u32x4*>(Dt + (cb + i) * pt + kbyte<2>(rb + c8, q)) = ta;
         }
     }
-}
-
-__device__ __forceinline__ void store4(char* d, int64_t plane, const float (&v)[4]) {   // 4 values along k
-    _Float16 hi[4], lo[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) split16(v[k], hi[k], lo[k]);
-    u32x2 q;
-    __builtin_memcpy(&q, hi, 8);
-    *reinterpret_cast<u32x2*>(d) = q;
-    __builtin_memcpy(&q, lo, 8);
-    *reinterpret_cast<u32x2*>(d + plane) = q;
-}
-__device__ __forceinline__ void store1(char* d, int64_t plane, float v) {
-    _Float16 hi, lo;
-    split16(v, hi, lo);
-    *reinterpret_cast<_Float16*>(d) = hi;
-    *reinterpret_cast<_Float16*>(d + plane) = lo;
 }
 
 // Tile q of the lower triangle of a square of tiles: row ti >= column tj
@@ -202,7 +170,7 @@ __device__ __forceinline__ void tri_tile(int q, int& ti, int& tj) {
 
 // POLY = false: A = X X^T.  POLY = true: P = a I + b A + c A A.
 template <class M, bool POLY>
-__global__ __launch_bounds__(M::NT) void ns_gram_kernel(Table table, char* __restrict__ ws,
+__global__ __launch_bounds__(M::NT, 2) void ns_gram_kernel(Table table, char* __restrict__ ws,
                                                         const float* __restrict__ skip) {
     if (skip != nullptr && skip[0] != 0.f) return;
     __shared__ __attribute__((aligned(16))) char lds[M::LDS];
@@ -211,8 +179,8 @@ __global__ __launch_bounds__(M::NT) void ns_gram_kernel(Table table, char* __res
     const Mat t = load_mat(table, find_mat(table, wGram, tile, first), ws);
     tri_tile(tile - first, ti, tj);
     const int a0 = ti * M::BM, b0 = tj * M::BN;
-    const int64_t pitch = POLY ? t.pm : t.pn, plane = POLY ? t.planeA : t.planeX;
-    const Operand op = {POLY ? t.A : t.X, pitch, plane, t.m};
+    const int64_t pitch = POLY ? t.pm : t.pn;
+    const Operand op = {POLY ? t.A : t.X, pitch, t.m};
     f32x16 acc[M::TM][M::TN];
     M::zero(acc);
     M::run(op, a0, op, b0, 0, (int)(pitch / M::STEP), lds, acc);
@@ -226,13 +194,13 @@ __global__ __launch_bounds__(M::NT) void ns_gram_kernel(Table table, char* __res
 #pragma unroll
             for (int e = 0; e < 16; e += 4) {
                 const int r = a0 + M::arow(i, e);            // 4 consecutive rows
-                float v[4], w[4] = {0.f, 0.f, 0.f, 0.f};
-                if (POLY && c < t.m && r * 2 < t.pm) {       // A[r..r+3][c] = A[c][r..r+3]
-                    const char* s = t.A + (int64_t)c * t.pm + (int64_t)r * 2;
+                float w[4] = {0.f, 0.f, 0.f, 0.f};
+                if (POLY && c < t.m && r < t.m) {            // A[r..r+3][c] = A[c][r..r+3]
+                    const char* s = t.A + (int64_t)c * t.pm;
                     _Float16 hi[4], lo[4];
-                    u32x2 q = *reinterpret_cast<const u32x2*>(s);
+                    u32x2 q = *reinterpret_cast<const u32x2*>(s + kbyte<2>(r));
                     __builtin_memcpy(hi, &q, 8);
-                    q = *reinterpret_cast<const u32x2*>(s + t.planeA);
+                    q = *reinterpret_cast<const u32x2*>(s + kbyte<2>(r, 1));
                     __builtin_memcpy(lo, &q, 8);
 #pragma unroll
                     for (int k = 0; k < 4; ++k) w[k] = (float)hi[k] + (float)lo[k];
@@ -241,20 +209,22 @@ __global__ __launch_bounds__(M::NT) void ns_gram_kernel(Table table, char* __res
                 for (int k = 0; k < 4; ++k) {
                     float d = acc[i][j][e + k] * down;
                     if (POLY) d = kC * d + (kB * w[k] + (r + k == c ? kA * (float)(1 << kScale) : 0.f));
-                    v[k] = r + k < t.m && c < t.m ? d : 0.f;
-                }
-                if (c < t.m && r * 2 < t.pm) {
-                    // below the diagonal: the mirrored tile as well, rows and columns exchanged
-                    if (ti != tj) {
-                        store4(out + (int64_t)c * t.pm + (int64_t)r * 2, t.planeA, v);
-                    }
-                }
-                if (c * 2 < t.pm) {
-#pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        if (r + k < t.m) store1(out + (int64_t)(r + k) * t.pm + (int64_t)c * 2, t.planeA, v[k]);
+                    acc[i][j][e + k] = r + k < t.m && c < t.m ? d : 0.f;
                 }
             }
+    }
+    using W = WaveStore<M>;
+    char* reg = W::region(lds);
+    const int r0 = a0 + M::wave_row(), c0 = b0 + M::wave_col();
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+        auto val = [&](int i, int j, int e) -> uint16_t { return plane16(acc[i][j][e], q); };
+        auto put = [&](int r, int c, u32x4 d) {
+            if (r < t.m && kbyte<2>(c) < t.pm) *reinterpret_cast<u32x4*>(out + (int64_t)r * t.pm + kbyte<2>(c, q)) = d;
+        };
+        W::store_rows(reg, val, [&](int r, int c, u32x4 d) { put(r0 + r, c0 + c, d); });
+        // below the diagonal: the mirrored tile as well
+        if (ti != tj) W::store_cols(reg, val, [&](int c, int r, u32x4 d) { put(c0 + c, r0 + r, d); });
     }
 }
 
@@ -266,7 +236,7 @@ struct Apply {                                    // the optimiser's half of the
 
 // X = P X: planes both ways round (from X^T number `from` to the other), or the last one: the result / the parameter's update
 template <class M, typename S, int LAST>          // LAST: 0 = planes, 1 = result, 2 = optimiser
-__global__ __launch_bounds__(M::NT) void ns_update_kernel(Table table, char* __restrict__ ws, int from, Apply ap,
+__global__ __launch_bounds__(M::NT, 2) void ns_update_kernel(Table table, char* __restrict__ ws, int from, Apply ap,
                                                           const float* __restrict__ skip) {
     if (skip != nullptr && skip[0] != 0.f) return;
     __shared__ __attribute__((aligned(16))) char lds[M::LDS];
@@ -275,13 +245,47 @@ __global__ __launch_bounds__(M::NT) void ns_update_kernel(Table table, char* __r
     const Mat t = load_mat(table, find_mat(table, wUpd, tile, first), ws);
     const int tm = (t.m + M::BM - 1) / M::BM, q = tile - first;
     const int a0 = q % tm * M::BM, b0 = q / tm * M::BN;
-    const Operand P = {t.P, t.pm, t.planeA, t.m}, Xt = {(from ? t.Xt1 : t.Xt0), t.pm, t.planeXt, t.n};
+    const Operand P = {t.P, t.pm, t.m}, Xt = {from ? t.Xt1 : t.Xt0, t.pm, t.n};
     f32x16 acc[M::TM][M::TN];
     M::zero(acc);
     M::run(P, a0, Xt, b0, 0, (int)(t.pm / M::STEP), lds, acc);
     constexpr float down = 1.f / (float)(1 << kScale);
-    char* to = from ? t.Xt0 : t.Xt1;
+    using W = WaveStore<M>;
+    char* reg = W::region(lds);
+    const int r0 = a0 + M::wave_row(), c0 = b0 + M::wave_col();
+    if constexpr (LAST == 0) {
+        char* to = from ? t.Xt0 : t.Xt1;
+#pragma unroll
+        for (int j = 0; j < M::TN; ++j) {
+            const int c = b0 + M::bcol(j);
+#pragma unroll
+            for (int i = 0; i < M::TM; ++i)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) acc[i][j][e] = a0 + M::arow(i, e) < t.m && c < t.n ? acc[i][j][e] * down : 0.f;
+        }
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            auto val = [&](int i, int j, int e) -> uint16_t { return plane16(acc[i][j][e], q); };
+            W::store_cols(reg, val, [&](int c, int r, u32x4 d) {
+                if (c0 + c < t.n && kbyte<2>(r0 + r) < t.pm) *reinterpret_cast<u32x4*>(to + (int64_t)(c0 + c) * t.pm + kbyte<2>(r0 + r, q)) = d;
+            });
+            W::store_rows(reg, val, [&](int r, int c, u32x4 d) {
+                if (r0 + r < t.m && kbyte<2>(c0 + c) < t.pn) *reinterpret_cast<u32x4*>(t.X + (int64_t)(r0 + r) * t.pn + kbyte<2>(c0 + c, q)) = d;
+            });
+        }
+        return;
+    }
     const bool tall = t.rows > t.cols;
+    if constexpr (LAST == 1 && sizeof(S) == 2) {
+        auto val = [&](int i, int j, int e) -> uint16_t { return bits16((S)(acc[i][j][e] * (down * down))); };
+        S* out = reinterpret_cast<S*>(t.dst);
+        auto put = [&](int r, int c, u32x4 d) {
+            if (r < t.rows && c < t.cols) store_vec(out + (int64_t)r * t.cols, c, t.cols, __builtin_bit_cast(typename Vec<S>::type, d));
+        };
+        if (tall) W::store_cols(reg, val, [&](int c, int r, u32x4 d) { put(c0 + c, r0 + r, d); });
+        else W::store_rows(reg, val, [&](int r, int c, u32x4 d) { put(r0 + r, c0 + c, d); });
+        return;
+    }
     float step = 0.f, keep = 0.f;
     if (LAST == 2) {
         const double lr = ap.lr_dev != nullptr ? ap.lr_dev[0] : ap.lr;
@@ -292,35 +296,16 @@ __global__ __launch_bounds__(M::NT) void ns_update_kernel(Table table, char* __r
 #pragma unroll
     for (int j = 0; j < M::TN; ++j) {
         const int c = b0 + M::bcol(j);
+        if (c >= t.n) continue;
 #pragma unroll
         for (int i = 0; i < M::TM; ++i)
 #pragma unroll
-            for (int e = 0; e < 16; e += 4) {
+            for (int e = 0; e < 16; ++e) {
                 const int r = a0 + M::arow(i, e);
-                if (LAST == 0) {
-                    float v[4];
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) v[k] = r + k < t.m && c < t.n ? acc[i][j][e + k] * down : 0.f;
-                    if (c < t.n && r * 2 < t.pm) store4(to + (int64_t)c * t.pm + (int64_t)r * 2, t.planeXt, v);
-                    if (c * 2 < t.pn) {
-#pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            if (r + k < t.m) store1(t.X + (int64_t)(r + k) * t.pn + (int64_t)c * 2, t.planeX, v[k]);
-                    }
-                } else if (c < t.n) {
-#pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        if (r + k < t.m) {
-                            const float v = acc[i][j][e + k] * (down * down);
-                            const int64_t at = tall ? (int64_t)c * t.cols + r + k : (int64_t)(r + k) * t.cols + c;
-                            if (LAST == 1) {
-                                reinterpret_cast<S*>(t.dst)[at] = (S)v;
-                            } else {
-                                float* p = reinterpret_cast<float*>(t.dst) + at;
-                                *p = *p * keep - step * v;
-                            }
-                        }
-                }
+                if (r >= t.m) continue;
+                const float v = acc[i][j][e] * (down * down);
+                float* d = reinterpret_cast<float*>(t.dst) + (tall ? (int64_t)c * t.cols + r : (int64_t)r * t.cols + c);
+                *d = LAST == 1 ? v : *d * keep - step * v;
             }
     }
 }

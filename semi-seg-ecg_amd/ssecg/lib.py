@@ -114,10 +114,11 @@ SIGNATURES = {
     "ssecg_layer_norm_fwd": (_i, [_vp, _vp, _vp, _i, _i64, _i, _d, _vp, _vp, _vp, _vp]),
     "ssecg_layer_norm_bwd_workspace": (_sz, [_i, _i64, _i]),
     "ssecg_layer_norm_bwd": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i64, _i, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "ssecg_linear_ce_packed_bytes": (_sz, [_vp, _vp, _i, _i64, _i64, _i64]),
     "ssecg_linear_ce_fwd_workspace": (_sz, [_i, _i64, _i64, _i64]),
-    "ssecg_linear_ce_fwd": (_i, [_vp, _vp, _vp, _vp, _vp, _d, _i64, _i, _i64, _i64, _i64, _i, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "ssecg_linear_ce_fwd": (_i, [_vp, _vp, _vp, _vp, _vp, _d, _i64, _i, _i64, _i64, _i64, _i, _vp, _vp, _vp, _vp, _vp, _sz, _vp, _sz, _vp]),
     "ssecg_linear_ce_bwd_workspace": (_sz, [_i, _i64, _i64, _i64, _i, _i, _i]),
-    "ssecg_linear_ce_bwd": (_i, [_vp] * 8 + [_i, _i64, _i64, _i64, _i, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "ssecg_linear_ce_bwd": (_i, [_vp] * 8 + [_i, _i64, _i64, _i64, _i, _vp, _vp, _vp, _vp, _sz, _vp, _sz, _vp]),
     "ssecg_orthogonalize_workspace": (_sz, [_vp, _i]),
     "ssecg_orthogonalize_multi": (_i, [_vp, _i, _i, _i, _d, _vp, _sz, _vp]),
     "ssecg_muon_multi": (_i, [_vp, _i, _d, _d, _i, _d, _i, _i, _d, _vp, _vp, _vp, _sz, _vp]),

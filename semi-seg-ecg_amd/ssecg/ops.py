@@ -1403,7 +1403,8 @@ def layer_norm_bwd(dy, x, mean, rstd, weight=None, want_params=True):
 
 
 class LinearCE(NamedTuple):
-    """What ``linear_ce_bwd`` needs of ``linear_ce_fwd``: the operands and, per position, log-sum-exp and gate."""
+    """What ``linear_ce_bwd`` needs of ``linear_ce_fwd``: the operands, log-sum-exp and gate per position, and (fp32, or C not a
+    multiple of 64) the operands as the matrix pipe reads them."""
     x: torch.Tensor
     weight: torch.Tensor
     bias: Optional[torch.Tensor]
@@ -1411,6 +1412,7 @@ class LinearCE(NamedTuple):
     lse: torch.Tensor
     gate: torch.Tensor
     count: torch.Tensor
+    packed: Optional[torch.Tensor]
     reduction: int
 
 
@@ -1441,22 +1443,26 @@ def linear_ce_fwd(x, weight, target, bias=None, conf=None, thresh=0.0, ignore_in
     loss = torch.empty(target.shape if mode == 0 else (), device=x.device, dtype=torch.float32)
     lse, gate = torch.empty((2, N), device=x.device, dtype=torch.float32).unbind(0)
     count = torch.empty((1,), device=x.device, dtype=torch.float32)
+    packed = None
     if N:
         Lb, code = lib(), _LM_DTYPE[x.dtype]
         with _lm_guard(x), _Timed("ce_lse_kernel", 2.0 * N * C * V, (N + V) * C * x.element_size()):
+            keep = Lb.ssecg_linear_ce_packed_bytes(_p(x), _p(weight), code, N, C, V)
+            packed = torch.empty((keep,), device=x.device, dtype=torch.uint8) if keep else None
             ws = torch.empty((Lb.ssecg_linear_ce_fwd_workspace(code, N, C, V),), device=x.device, dtype=torch.uint8)
             check(Lb.ssecg_linear_ce_fwd(_p(x), _p(weight), _p(bias), _p(target), _p(conf), float(thresh), int(ignore_index), code, N, C, V,
-                                         mode, _p(loss), _p(lse), _p(gate), _p(count), _p(ws), ws.numel(), _stream()), "ssecg_linear_ce_fwd")
+                                         mode, _p(loss), _p(lse), _p(gate), _p(count), _p(packed), keep, _p(ws), ws.numel(), _stream()),
+                  "ssecg_linear_ce_fwd")
     else:
         loss.zero_()
         count.fill_(1)
-    return loss, LinearCE(x, weight, bias, target, lse, gate, count, mode)
+    return loss, LinearCE(x, weight, bias, target, lse, gate, count, packed, mode)
 
 
 def linear_ce_bwd(saved, dloss=None, want_dx=True, want_dweight=True, want_dbias=True):
     """-> (dx, dweight of their operands' type, dbias in fp32): gradients of ``linear_ce_fwd``'s loss times ``dloss`` (a device scalar,
     or one value per position for reduction "none"; None = 1).  What is not wanted (or has no bias) is None."""
-    x, weight, bias, target, lse, gate, count, mode = saved
+    x, weight, bias, target, lse, gate, count, packed, mode = saved
     trace("linear_ce_bwd", tuple(x.shape), tuple(weight.shape))
     (V, C), N = weight.shape, target.numel()
     shape = target.shape if mode == 0 else ()
@@ -1478,7 +1484,8 @@ def linear_ce_bwd(saved, dloss=None, want_dx=True, want_dweight=True, want_dbias
             ws = torch.empty((Lb.ssecg_linear_ce_bwd_workspace(code, N, C, V, int(want_dx), int(want_dweight), int(want_dbias)),),
                              device=x.device, dtype=torch.uint8)
             check(Lb.ssecg_linear_ce_bwd(_p(dloss), _p(x), _p(weight), _p(bias), _p(target), _p(lse), _p(gate), _p(count), code, N, C, V, mode,
-                                         _p(dx), _p(dw), _p(db), _p(ws), ws.numel(), _stream()), "ssecg_linear_ce_bwd")
+                                         _p(dx), _p(dw), _p(db), _p(packed), packed.numel() if packed is not None else 0, _p(ws), ws.numel(),
+                                         _stream()), "ssecg_linear_ce_bwd")
     return dx, dw, db
 
 

@@ -21,20 +21,22 @@ def test_c_entries_refuse_bad_arguments():
     assert L.ssecg_layer_norm_bwd_workspace(0, 4, 8) > 0 and L.ssecg_layer_norm_bwd_workspace(0, 0, 8) == 0
     n = L.ssecg_linear_ce_fwd_workspace(1, 100, 64, 1000)
     assert n > 0 and L.ssecg_linear_ce_fwd_workspace(1, 0, 64, 1000) == 0
-    ok = [256, 256, None, 256, None, 0.0, -100, 1, 100, 64, 1000, 1, 256, 256, 256, 256, 256, n, None]
-    for at, bad in ((0, None), (1, None), (3, None), (7, 5), (8, 0), (9, 0), (10, 0), (11, 3), (12, None), (16, None), (16, 264)):
+    ok = [256, 256, None, 256, None, 0.0, -100, 1, 100, 64, 1000, 1, 256, 256, 256, 256, None, 0, 256, n, None]
+    for at, bad in ((0, None), (1, None), (3, None), (7, 5), (8, 0), (9, 0), (10, 0), (11, 3), (12, None), (16, 8), (18, None), (18, 264)):
         args = list(ok)
         args[at] = bad
         assert L.ssecg_linear_ce_fwd(*args) == -1, at
-    assert L.ssecg_linear_ce_fwd(*(ok[:17] + [n - 1, None])) == -2
+    assert L.ssecg_linear_ce_fwd(*(ok[:19] + [n - 1, None])) == -2
+    assert L.ssecg_linear_ce_fwd(*([264] + ok[1:])) == -2            # x is not 16-byte aligned: its copy has no place
+    assert L.ssecg_linear_ce_packed_bytes(256, 256, 1, 100, 64, 1000) == 0 < L.ssecg_linear_ce_packed_bytes(256, 256, 0, 100, 64, 1000)
     n = L.ssecg_linear_ce_bwd_workspace(1, 100, 64, 1000, 1, 1, 0)
-    ok = [256, 256, 256, None, 256, 256, 256, 256, 1, 100, 64, 1000, 1, 256, 256, None, 256, n, None]
-    for at, bad in ((0, None), (5, None), (8, 7), (9, -1), (12, -1), (16, None)):
+    ok = [256, 256, 256, None, 256, 256, 256, 256, 1, 100, 64, 1000, 1, 256, 256, None, None, 0, 256, n, None]
+    for at, bad in ((0, None), (5, None), (8, 7), (9, -1), (12, -1), (18, None)):
         args = list(ok)
         args[at] = bad
         assert L.ssecg_linear_ce_bwd(*args) == -1, at
-    assert L.ssecg_linear_ce_bwd(*(ok[:13] + [None, None, None, 256, n, None])) == -1          # nothing wanted
-    assert L.ssecg_linear_ce_bwd(*(ok[:17] + [n - 1, None])) == -2
+    assert L.ssecg_linear_ce_bwd(*(ok[:13] + [None, None, None, None, 0, 256, n, None])) == -1          # nothing wanted
+    assert L.ssecg_linear_ce_bwd(*(ok[:19] + [n - 1, None])) == -2
     one = _i64(256, 256, 256, 64, 192)
     n = L.ssecg_orthogonalize_workspace(one, 1)
     assert n > 0 and L.ssecg_orthogonalize_workspace(_i64(0, 0, 0, 0, 4), 1) == 0
