@@ -8,9 +8,9 @@
 //
 // Forward: one product whose epilogue keeps, per tile, the maximum and the sum of exponentials of a row and its target's logit.
 // The vocabulary is the tile's register axis (operand A), so a lane reduces its own row without shuffles but one.  A second launch
-// joins the tiles.  Backward: the logits of a piece are computed again, E is written in 16 bits (both ways round, so that every
-// product reads k fastest) and two products take it up.  8 N V C multiplications and additions against the 6 N V C that keeping
-// N V logits would need.
+// joins the tiles.  Backward: the logits of a piece are computed again, E is written in 16 bits and two products take it up, one
+// along its rows, one across (mm_core.h reads an operand either way, so no operand is transposed in memory).  8 N V C
+// multiplications and additions against the 6 N V C that keeping N V logits would need.
 //
 // 32-bit inputs travel as two fp16 planes (mm_core.h), scaled by a power of two that the largest finite value sets: exact, and an
 // entry 2^-17 of the largest still has all its bits.  E lies in [-1, 1] and is held times 2^14 for fp16's sake.  Rows whose g_n is
@@ -28,10 +28,14 @@ constexpr int kAmaxParts = 256;
 __device__ __forceinline__ float exp2_fast(float v) { return __builtin_amdgcn_exp2f(v); }
 
 // ---------------------------------------------------------------- operands
-struct Counts {                                   // which rows count
+struct Counts {                                   // which rows count: by the gate of the forward pass, by target and confidence, or all
+    const float* gate;
     const int64_t* target; int64_t ignore;
     const float* conf; float thresh;
-    __device__ __forceinline__ bool operator()(int64_t r) const { return target[r] != ignore && (conf == nullptr || conf[r] >= thresh); }
+    __device__ __forceinline__ bool operator()(int64_t r) const {
+        if (gate) return gate[r] != 0.f;
+        return target == nullptr || (target[r] != ignore && (conf == nullptr || conf[r] >= thresh));
+    }
 };
 
 // largest finite |x| of the rows that count (blockIdx.y = 0) and of W (1), per workgroup (a maximum: any order gives the same); a
@@ -77,47 +81,40 @@ __device__ __forceinline__ int amax_exp(const float* __restrict__ parts) {
     return scale_exp(fmaxf(fmaxf(sh[0], sh[1]), fmaxf(sh[2], sh[3])));
 }
 
-// rows [r0, r0 + R) of src (.., C) as an operand, as they lie (dst, may be null) and transposed (dstT, may be null); k is zero-filled
-// to the pitch.  gate: a row whose gate is 0 is written as zeros.  One workgroup: 64 rows x 64 columns.
+// src (R, C) as an operand: its planes, zeros up to the pitch, and zeros for a row that does not count.  One thread: 8 values.
 template <typename S, typename T, int P>
-__global__ __launch_bounds__(256) void ce_pack_kernel(const S* __restrict__ src, int64_t r0, int R, int C, const float* __restrict__ gate,
-                                                      const float* __restrict__ amax, char* __restrict__ dst, int64_t pitch,
-                                                      char* __restrict__ dstT, int64_t pitchT) {
-    __shared__ uint32_t tile[64][65];
+__global__ __launch_bounds__(256) void ce_pack_kernel(const S* __restrict__ src, int64_t R, int C, Counts counts, const float* __restrict__ amax,
+                                                      char* __restrict__ dst, int64_t pitch) {
     const int ex = P == 2 ? amax_exp(amax) : 0;
-    const int64_t rb = (int64_t)blockIdx.y * 64, cb = (int64_t)blockIdx.x * 64;
-    const int lane = threadIdx.x & 63, strand = threadIdx.x >> 6;
-    for (int i = strand; i < 64; i += 4) {
-        const int64_t r = rb + i, c = cb + lane;
-        uint32_t q = 0;
-        if (r < R && c < C && (gate == nullptr || gate[r0 + r] != 0.f)) {
-            const S v = src[(r0 + r) * C + c];
-            if constexpr (P == 2) {
-                const float f = ldexpf((float)v, ex);
-                q = (uint32_t)plane16(f, 0) | (uint32_t)plane16(f, 1) << 16;
-            } else {
-                q = bits16(v);
+    const int per = (int)(pitch / (16 * P));               // threads of a row
+    for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < R * per; at += (int64_t)gridDim.x * 256) {
+        const int64_t r = at / per;
+        const int k = (int)(at - r * per) * 8;
+        const bool live = counts(r);
+        float v[8];
+        uint16_t q[2][8];
+        constexpr int V = Vec<S>::N;
+#pragma unroll
+        for (int i = 0; i < 8; i += V) {
+            typename Vec<S>::type t = {};
+            if (live && k + i < C) t = load_vec(src + r * C, k + i, C);
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                if constexpr (P == 2) {
+                    v[i + j] = ldexpf((float)t[j], ex);
+                    q[0][i + j] = plane16(v[i + j], 0);
+                    q[1][i + j] = plane16(v[i + j], 1);
+                } else {
+                    q[0][i + j] = bits16(t[j]);
+                }
             }
         }
-        tile[i][lane] = q;
-    }
-    __syncthreads();
-    for (int u = threadIdx.x; u < 512; u += 256) {         // 64 rows x 8 chunks of 8 values
-        const int i = u >> 3, k = (u & 7) * 8;
 #pragma unroll
-        for (int q = 0; q < P; ++q) {
-            if (dst && rb + i < R && kbyte<P>(cb + k) < pitch) {
-                u32x4 a;
+        for (int p = 0; p < P; ++p) {
+            u32x4 d;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) a[j] = (tile[i][k + 2 * j] >> 16 * q & 0xffffu) | tile[i][k + 2 * j + 1] >> 16 * q << 16;
-                *reinterpret_cast<u32x4*>(dst + (rb + i) * pitch + kbyte<P>(cb + k, q)) = a;
-            }
-            if (dstT && cb + i < C && kbyte<P>(rb + k) < pitchT) {
-                u32x4 a;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) a[j] = (tile[k + 2 * j][i] >> 16 * q & 0xffffu) | tile[k + 2 * j + 1][i] >> 16 * q << 16;
-                *reinterpret_cast<u32x4*>(dstT + (cb + i) * pitchT + kbyte<P>(rb + k, q)) = a;
-            }
+            for (int j = 0; j < 4; ++j) d[j] = (unsigned)q[p][2 * j] | (unsigned)q[p][2 * j + 1] << 16;
+            *reinterpret_cast<u32x4*>(dst + r * pitch + kbyte<P>(k, p)) = d;
         }
     }
 }
@@ -132,10 +129,10 @@ struct LogitArgs {
     int64_t v0;
     // forward: partial maxima and sums [parts][N], target logits [N]
     float* pm; float* ps; float* tl;
-    // gradient: lse and g per row, E [N][pitchE] and its transpose [V][pitchT], partial db [tilesN * WN][V]
+    // gradient: lse and g per row, E [rowsE][pitchE] (rows from N on are zeros), partial db [tilesN][V]
     const float* lse; const float* gate; const float* coef;
     char* E; int64_t pitchE;
-    char* Et; int64_t pitchT;
+    int rowsE;
     float* pdb;
 };
 
@@ -257,36 +254,34 @@ __global__ __launch_bounds__(M::NT, 2) void ce_lse_kernel(LogitArgs p) {
     }
 }
 
-// joins the parts of a row: lse, g and the row's loss.  A strand of 64 / .. lanes would not pay: rows are the long axis.
-__global__ __launch_bounds__(256) void ce_join_kernel(const float* __restrict__ pm, const float* __restrict__ ps, const float* __restrict__ tl,
-                                                      int parts, int N, int V, const int64_t* __restrict__ target, const float* __restrict__ conf,
-                                                      float thresh, int64_t ignore, float* __restrict__ lse, float* __restrict__ gate,
-                                                      float* __restrict__ row_loss) {
-    // 16 rows x 16 strands of parts per workgroup
+__device__ __forceinline__ void join_lse(float& m, float& s, float m2, float s2) {
+    const float mt = fmaxf(m, m2), mz = mt == -INFINITY ? 0.f : mt;
+    s = s * exp2_fast(((m == -INFINITY ? 0.f : m) - mz) * kLog2e) + s2 * exp2_fast(((m2 == -INFINITY ? 0.f : m2) - mz) * kLog2e);
+    m = mt;
+}
+
+// joins the parts of a row: lse, g and the row's loss.  A workgroup: 16 rows x 64 strands of parts.
+__global__ __launch_bounds__(1024) void ce_join_kernel(const float* __restrict__ pm, const float* __restrict__ ps, const float* __restrict__ tl,
+                                                       int parts, int N, int V, const int64_t* __restrict__ target, Counts counts,
+                                                       float* __restrict__ lse, float* __restrict__ gate, float* __restrict__ row_loss) {
     __shared__ float sm[16][17], ss[16][17];
     const int c = threadIdx.x & 15, k = threadIdx.x >> 4, n = blockIdx.x * 16 + c;
     float m = -INFINITY, s = 0.f;
     if (n < N)
-        for (int p = k; p < parts; p += 16) {
-            const float m2 = pm[(int64_t)p * N + n], s2 = ps[(int64_t)p * N + n];
-            const float mt = fmaxf(m, m2), mz = mt == -INFINITY ? 0.f : mt;
-            s = s * exp2_fast(((m == -INFINITY ? 0.f : m) - mz) * kLog2e) + s2 * exp2_fast(((m2 == -INFINITY ? 0.f : m2) - mz) * kLog2e);
-            m = mt;
-        }
-    sm[k][c] = m;
-    ss[k][c] = s;
+        for (int p = k; p < parts; p += 64) join_lse(m, s, pm[(int64_t)p * N + n], ps[(int64_t)p * N + n]);
+#pragma unroll
+    for (int o = 16; o < 64; o *= 2) {                    // the wave's 4 strands
+        const float m2 = __shfl_xor(m, o, 64), s2 = __shfl_xor(s, o, 64);
+        join_lse(m, s, m2, s2);
+    }
+    if ((threadIdx.x & 63) < 16) { sm[threadIdx.x >> 6][c] = m; ss[threadIdx.x >> 6][c] = s; }
     __syncthreads();
     if (k != 0 || n >= N) return;
-    for (int q = 1; q < 16; ++q) {
-        const float m2 = sm[q][c], s2 = ss[q][c];
-        const float mt = fmaxf(m, m2), mz = mt == -INFINITY ? 0.f : mt;
-        s = s * exp2_fast(((m == -INFINITY ? 0.f : m) - mz) * kLog2e) + s2 * exp2_fast(((m2 == -INFINITY ? 0.f : m2) - mz) * kLog2e);
-        m = mt;
-    }
+    for (int q = 1; q < 16; ++q) join_lse(m, s, sm[q][c], ss[q][c]);
     const int64_t t = target[n];
-    const bool kept = t != ignore, bad = kept && (t < 0 || t >= V);
+    const bool bad = t != counts.ignore && (t < 0 || t >= V);
     const float l = bad || m == -INFINITY ? NAN : m + logf(s);     // a label outside the vocabulary poisons its row: no silent loss
-    const float g = kept && (conf == nullptr || conf[n] >= thresh) ? 1.f : 0.f;
+    const float g = counts(n) ? 1.f : 0.f;
     lse[n] = l;
     gate[n] = g;
     row_loss[n] = g != 0.f ? l - (bad ? 0.f : tl[n]) : 0.f;
@@ -295,37 +290,36 @@ __global__ __launch_bounds__(256) void ce_join_kernel(const float* __restrict__ 
 // out[0] = sum of the row losses (/ count for the mean), count[0] = max(1, positions that are not ignored); fixed order, fp64
 __global__ __launch_bounds__(1024) void ce_total_kernel(const float* __restrict__ row_loss, const int64_t* __restrict__ target, int64_t ignore,
                                                         int N, int mean, float* __restrict__ out, float* __restrict__ count) {
-    __shared__ double sh[1024];
-    __shared__ int shc[1024];
+    __shared__ double sh[16];
+    __shared__ int shc[16];
     double s = 0.0;
     int k = 0;
     for (int i = threadIdx.x; i < N; i += 1024) {
         s += (double)row_loss[i];
         k += target[i] != ignore ? 1 : 0;
     }
-    sh[threadIdx.x] = s;
-    shc[threadIdx.x] = k;
-    for (int o = 512; o > 0; o >>= 1) {
-        __syncthreads();
-        if (threadIdx.x < o) { sh[threadIdx.x] += sh[threadIdx.x + o]; shc[threadIdx.x] += shc[threadIdx.x + o]; }
-    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) { s += __shfl_xor(s, o, 64); k += __shfl_xor(k, o, 64); }
+    if ((threadIdx.x & 63) == 0) { sh[threadIdx.x >> 6] = s; shc[threadIdx.x >> 6] = k; }
+    __syncthreads();
     if (threadIdx.x == 0) {
-        const int c = shc[0] > 0 ? shc[0] : 1;
+        for (int w = 1; w < 16; ++w) { s += sh[w]; k += shc[w]; }
+        const int c = k > 0 ? k : 1;
         count[0] = (float)c;
-        if (out) out[0] = (float)(mean ? sh[0] / (double)c : sh[0]);
+        if (out) out[0] = (float)(mean ? s / (double)c : s);
     }
 }
 
 // ---------------------------------------------------------------- gradient
+// f: upstream / count (mean), upstream (sum), or the power of two that ce_coef_kernel chose
+struct Factor {
+    const float* up; const float* count;
+    __device__ __forceinline__ float operator()() const { return count ? up[0] / count[0] : up[0]; }
+};
+
 // Not reduced: coef[n] = g_n dloss[n] / s with s a power of two >= max |g dloss| (so that E stays in [-1, 1]); fscale[0] = s.
-// Reduced: fscale[0] = dloss / count (mean) or dloss (sum), coef is not used.
-__global__ __launch_bounds__(1024) void ce_coef_kernel(const float* __restrict__ dloss, const float* __restrict__ gate,
-                                                       const float* __restrict__ count, int N, int reduction, float* __restrict__ coef,
-                                                       float* __restrict__ fscale) {
-    if (reduction != 0) {
-        if (threadIdx.x == 0) fscale[0] = reduction == 1 ? dloss[0] / count[0] : dloss[0];
-        return;
-    }
+__global__ __launch_bounds__(1024) void ce_coef_kernel(const float* __restrict__ dloss, const float* __restrict__ gate, int N,
+                                                       float* __restrict__ coef, float* __restrict__ fscale) {
     __shared__ float sh[16];
     float m = 0.f;
     for (int i = threadIdx.x; i < N; i += 1024) {
@@ -366,11 +360,11 @@ __global__ __launch_bounds__(M::NT, 2) void ce_grad_kernel(LogitArgs p) {
         lse[j] = in ? p.lse[n] : 0.f;
         off[j] = in ? label_offset<M>(p.target[n] - p.v0, a0) : -1;
     }
+    float* part = reinterpret_cast<float*>(lds);          // DB: column sums [WN][BM] of the waves
 #pragma unroll
     for (int i = 0; i < M::TM; ++i) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-            const int v = a0 + M::arow(i, e);
             float sum = 0.f;
 #pragma unroll
             for (int j = 0; j < M::TN; ++j) {
@@ -379,14 +373,25 @@ __global__ __launch_bounds__(M::NT, 2) void ce_grad_kernel(LogitArgs p) {
                 acc[i][j][e] = q * (float)(1 << kEScale);
                 sum += q;
             }
-            if (DB) {                                                          // column sum over the wave's positions
+            if (DB) {                                                // column sum over the wave's positions
 #pragma unroll
                 for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
-                if ((lane & 31) == 0 && v < p.V) p.pdb[(int64_t)(tb * M::WN + wn) * p.V + v] = sum;
+                if ((lane & 31) == 0) part[wn * M::BM + M::arow(i, e)] = sum;
             }
         }
         __builtin_amdgcn_sched_barrier(0);
     }
+    if (DB) {
+        __syncthreads();
+        for (int r = threadIdx.x; r < M::BM; r += M::NT) {
+            float sum = 0.f;
+#pragma unroll
+            for (int k = 0; k < M::WN; ++k) sum += part[k * M::BM + r];
+            if (a0 + r < p.V) p.pdb[(int64_t)tb * p.V + a0 + r] = sum;
+        }
+        __syncthreads();
+    }
+    if (p.E == nullptr) return;
     using W = WaveStore<M>;
     char* reg = W::region(lds);
     const int v0 = a0 + M::wave_row(), n0 = b0 + M::wave_col();
@@ -396,14 +401,10 @@ __global__ __launch_bounds__(M::NT, 2) void ce_grad_kernel(LogitArgs p) {
             if constexpr (M::P == 2) return plane16(acc[i][j][e], q);
             else return bits16((T)acc[i][j][e]);
         };
-        if (p.E)                                           // the pitch covers the whole tile: no condition on the class
-            W::store_cols(reg, val, [&](int n, int v, u32x4 d) {
-                if (n0 + n < p.N) *reinterpret_cast<u32x4*>(p.E + (n0 + n) * p.pitchE + kbyte<M::P>(v0 + v, q)) = d;
-            });
-        if (p.Et)
-            W::store_rows(reg, val, [&](int v, int n, u32x4 d) {
-                if (v0 + v < p.V) *reinterpret_cast<u32x4*>(p.Et + (v0 + v) * p.pitchT + kbyte<M::P>(n0 + n, q)) = d;
-            });
+        // the pitch covers the whole tile: no condition on the class
+        W::store_cols(reg, val, [&](int n, int v, u32x4 d) {
+            if (n0 + n < p.rowsE) *reinterpret_cast<u32x4*>(p.E + (n0 + n) * p.pitchE + kbyte<M::P>(v0 + v, q)) = d;
+        });
     }
 }
 
@@ -415,7 +416,7 @@ struct ProdArgs {
     int add;                                     // plane += instead of plane =
     void* out;                                   // (rows, cols) of the result's type
     const float* amax;                           // scale parts of operand B, or null
-    const float* fscale;
+    Factor f;
 };
 
 template <typename O>
@@ -434,7 +435,7 @@ __global__ __launch_bounds__(M::NT, 2) void ce_prod_kernel(ProdArgs p) {
     int ex = -kEScale;
     float f = 0.f;
     if (!p.plane) {
-        f = p.fscale[0];
+        f = p.f();
         if constexpr (M::P == 2) {
             float m = 0.f;
             const int lane = threadIdx.x & 63;
@@ -479,37 +480,40 @@ __global__ __launch_bounds__(M::NT, 2) void ce_prod_kernel(ProdArgs p) {
 // out = f 2^ex sum of the planes, in their order
 template <typename O>
 __global__ __launch_bounds__(256) void ce_sum_planes_kernel(const float* __restrict__ planes, int splits, int64_t n, const float* __restrict__ amax,
-                                                            const float* __restrict__ fscale, O* __restrict__ out) {
+                                                            Factor factor, O* __restrict__ out) {
     int ex = -kEScale;
     if (amax) ex -= amax_exp(amax);
-    const float f = fscale[0];
+    const float f = factor();
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-        float s = planes[i];
-        for (int k = 1; k < splits; ++k) s += planes[(int64_t)k * n + i];
+        float s = 0.f;
+        int k = 0;
+        for (; k + 8 <= splits; k += 8) {                 // 8 loads in flight
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = planes[(int64_t)(k + j) * n + i];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) s += v[j];
+        }
+        for (; k < splits; ++k) s += planes[(int64_t)k * n + i];
         out[i] = finish<O>(s, f, ex);
     }
 }
 
-__global__ __launch_bounds__(256) void ce_db_kernel(const float* __restrict__ pdb, int parts, int V, const float* __restrict__ fscale,
-                                                    float* __restrict__ db) {
+__global__ __launch_bounds__(256) void ce_db_kernel(const float* __restrict__ pdb, int parts, int V, Factor factor, float* __restrict__ db) {
     const int v = blockIdx.x * 256 + threadIdx.x;
     if (v >= V) return;
     float s = 0.f;
     for (int p = 0; p < parts; ++p) s += pdb[(int64_t)p * V + v];
-    db[v] = s * fscale[0];
-}
-
-template <typename O>
-__global__ __launch_bounds__(256) void ce_zero_kernel(O* __restrict__ out, int64_t n) {
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) out[i] = (O)0.f;
+    db[v] = s * factor();
 }
 
 // ---------------------------------------------------------------- host side
 template <typename S> struct Inner { using T = S; static constexpr int P = 1; };
 template <> struct Inner<float> { using T = _Float16; static constexpr int P = 2; };
 
-template <typename T, int P> using Big = MmTile<T, P, 256, 256, 2, 4, 2>;
-template <typename T, int P> using Mid = MmTile<T, P, 128, 128, 2, 2, 2>;
+template <typename T, int P, bool TA = false, bool TB = false> using Big = MmTile<T, P, 256, 256, 2, 4, 2, TA, TB>;
+template <typename T, int P, bool TA = false, bool TB = false> using Mid = MmTile<T, P, 128, 128, 2, 2, 2, TA, TB>;
+template <typename T, int P, bool TA = false, bool TB = false> using Small = MmTile<T, P, 64, 64, 2, 2, 4, TA, TB>;
 
 inline int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
@@ -555,18 +559,38 @@ Packed plan_packed(void* base, const void* x, const void* w, int dtype, int64_t 
     return p;
 }
 
+inline int64_t tiles_of(int64_t n, int side) { return (n + side - 1) / side; }
+
+// the tile side (256, 128, 64) of a product of a x b tiles with `stages` stages, and how many workgroups share the k of a tile
+struct Choice { int side, splits; };
+inline Choice choose(int64_t a, int64_t b, int64_t stages, int P, bool split) {
+    Choice best = {256, 1};
+    double least = 0.0;
+    for (int side = 256; side >= 64; side /= 2)
+        for (int s = 1; s <= (split ? 64 : 1) && (s == 1 || stages / s >= 4); s += s < 8 ? 1 : s < 16 ? 2 : 8) {
+            MmWork w;
+            w.add(tiles_of(a, side) * tiles_of(b, side) * s, (stages + s - 1) / s);
+            // the planes of the parts are written and read again (4 TB/s), and a launch sums them
+            const double t = mm_time(side, P, w) + (s > 1 ? 4.0 + (double)a * b * s * 8 / 4e6 : 0.0);
+            if (least == 0.0 || t < least) {
+                least = t;
+                best = {side, s};
+            }
+        }
+    return best;
+}
+
 struct FwdPlan {
-    int tile, tilesV, tilesN, parts;
+    int side, tilesV, tilesN, parts;
     float *pm, *ps, *tl, *row;
 };
 
-inline bool use_big(int64_t a, int64_t b) { return ((a + 255) / 256) * ((b + 255) / 256) >= 256; }
-
-FwdPlan plan_fwd(Blob& ws, int64_t N, int64_t V) {
+FwdPlan plan_fwd(Blob& ws, int dtype, int64_t N, int64_t C, int64_t V) {
     FwdPlan p;
-    p.tile = use_big(V, N) ? 256 : 128;
-    p.tilesV = (int)((V + p.tile - 1) / p.tile);
-    p.tilesN = (int)((N + p.tile - 1) / p.tile);
+    const int P = dtype == kF32 ? 2 : 1;
+    p.side = choose(V, N, up(C, 64) * P / 64, P, false).side;
+    p.tilesV = (int)tiles_of(V, p.side);
+    p.tilesN = (int)tiles_of(N, p.side);
     p.parts = p.tilesV * 2;                      // two waves of a tile along the classes
     p.pm = ws.take<float>((size_t)p.parts * N);
     p.ps = ws.take<float>((size_t)p.parts * N);
@@ -575,13 +599,16 @@ FwdPlan plan_fwd(Blob& ws, int64_t N, int64_t V) {
     return p;
 }
 
+inline unsigned grid_for(int64_t n) {
+    const int64_t b = (n + 255) / 256;
+    return (unsigned)(b < 2048 ? b : 2048);
+}
+
 template <typename S>
-int pack(const void* src, int64_t r0, int64_t R, int64_t C, const float* gate, const float* amax, char* dst, int64_t pitch, char* dstT,
-         int64_t pitchT, hipStream_t st) {
+int pack(const void* src, int64_t R, int64_t C, const Counts& counts, const float* amax, char* dst, int64_t pitch, hipStream_t st) {
     constexpr int P = Inner<S>::P;
-    const int64_t wide = dst ? pitch / (2 * P) : C, tall = dstT ? pitchT / (2 * P) : R;
-    hipLaunchKernelGGL((ce_pack_kernel<S, typename Inner<S>::T, P>), dim3((unsigned)((wide + 63) / 64), (unsigned)((tall + 63) / 64)), dim3(256), 0, st,
-                       (const S*)src, r0, (int)R, (int)C, gate, amax, dst, pitch, dstT, pitchT);
+    hipLaunchKernelGGL((ce_pack_kernel<S, typename Inner<S>::T, P>), dim3(grid_for(R * (pitch / (16 * P)))), dim3(256), 0, st, (const S*)src, R, (int)C,
+                       counts, amax, dst, pitch);
     return (int)hipGetLastError();
 }
 
@@ -600,17 +627,18 @@ int ce_fwd(const void* x, const void* w, const float* bias, const int64_t* targe
     constexpr int P = Inner<S>::P;
     Blob blob(ws);
     const Packed k = plan_packed(packed, x, w, dtype, N, C, V);
-    const FwdPlan p = plan_fwd(blob, N, V);
+    const FwdPlan p = plan_fwd(blob, dtype, N, C, V);
+    const Counts counts = {nullptr, target, ignore, conf, thresh};
     LogitArgs a = {};
     int rc = 0;
     if constexpr (P == 2) {
         hipLaunchKernelGGL(ce_amax_kernel, dim3(kAmaxParts, 2), dim3(1024), 0, st, (const float*)x, N, (const float*)w, V, (int)C,
-                           Counts{target, ignore, conf, thresh}, k.amaxX);
+                           counts, k.amaxX);
         a.amaxX = k.amaxX;
         a.amaxW = k.amaxW;
     }
-    if (k.Xp && (rc = pack<S>(x, 0, N, C, nullptr, k.amaxX, k.Xp, k.pitch, nullptr, 0, st)) != 0) return rc;
-    if (k.Wp && (rc = pack<S>(w, 0, V, C, nullptr, k.amaxW, k.Wp, k.pitch, nullptr, 0, st)) != 0) return rc;
+    if (k.Xp && (rc = pack<S>(x, N, C, counts, k.amaxX, k.Xp, k.pitch, st)) != 0) return rc;
+    if (k.Wp && (rc = pack<S>(w, V, C, Counts{}, k.amaxW, k.Wp, k.pitch, st)) != 0) return rc;
     a.X = {k.Xp ? k.Xp : (const char*)x, k.pitch, (int)N};
     a.W = {k.Wp ? k.Wp : (const char*)w, k.pitch, (int)V};
     a.bias = bias;
@@ -618,69 +646,65 @@ int ce_fwd(const void* x, const void* w, const float* bias, const int64_t* targe
     a.stages = (int)(k.pitch / 128);
     a.target = target; a.v0 = 0;
     a.pm = p.pm; a.ps = p.ps; a.tl = p.tl;
-    if (p.tile == 256) { using M = Big<T, P>; SSECG_CE_LAUNCH(M, ce_lse_kernel<M>, dim3(p.tilesV * p.tilesN), st, a); }
-    else { using M = Mid<T, P>; SSECG_CE_LAUNCH(M, ce_lse_kernel<M>, dim3(p.tilesV * p.tilesN), st, a); }
+#define SSECG_CE_LSE(TILE) do { using M = TILE<T, P>; SSECG_CE_LAUNCH(M, ce_lse_kernel<M>, dim3(p.tilesV * p.tilesN), st, a); } while (0)
+    if (p.side == 256) SSECG_CE_LSE(Big);
+    else if (p.side == 128) SSECG_CE_LSE(Mid);
+    else SSECG_CE_LSE(Small);
+#undef SSECG_CE_LSE
     float* row = reduction == 0 ? loss : p.row;
-    hipLaunchKernelGGL(ce_join_kernel, dim3((unsigned)((N + 15) / 16)), dim3(256), 0, st, p.pm, p.ps, p.tl, p.parts, (int)N, (int)V, target, conf, thresh,
-                       ignore, lse, gate, row);
+    hipLaunchKernelGGL(ce_join_kernel, dim3((unsigned)((N + 15) / 16)), dim3(1024), 0, st, p.pm, p.ps, p.tl, p.parts, (int)N, (int)V, target, counts,
+                       lse, gate, row);
     hipLaunchKernelGGL(ce_total_kernel, dim3(1), dim3(1024), 0, st, row, target, ignore, (int)N, reduction == 1 ? 1 : 0,
                        reduction == 0 ? nullptr : loss, count);
     return (int)hipGetLastError();
 }
 
-constexpr size_t kPieceBytes = (size_t)1 << 30;  // E, its transpose and the piece's W^T
+constexpr size_t kPieceBytes = (size_t)1 << 30;  // of E
 
 struct BwdPlan {
-    int64_t Vc;                                  // classes per piece (a multiple of 256 unless there is one piece)
-    int pieces, splitX, splitW;
-    bool bigL, bigX, bigW;
+    int64_t Vc, rowsE, pitchE;                   // classes per piece (a multiple of 256 unless there is one piece); E's rows and bytes
+    int pieces;
+    int sideL;
+    Choice cx, cw;                               // dx, dw
     float *coef, *fscale, *pdb, *planeX, *planeW;
-    char *Xt, *Wt, *E, *Et;
-    int64_t pitchE, pitchT;                      // bytes of a row of E and W^T; of E^T and X^T
+    char *Xg, *E;
 };
 
-// How many workgroups share the k of one tile: enough to give each of the 256 CUs one, each at least 8 stages long.
-inline int split_of(int64_t tiles, int64_t stages) {
-    int64_t s = 256 / (tiles > 0 ? tiles : 1);
-    if (s > stages / 8) s = stages / 8;
-    return (int)(s < 1 ? 1 : (s > 64 ? 64 : s));
-}
-
-BwdPlan plan_bwd(Blob& ws, int dtype, int64_t N, int64_t C, int64_t V, bool want_x, bool want_w, bool want_b) {
+BwdPlan plan_bwd(Blob& ws, int dtype, int64_t N, int64_t C, int64_t V, bool want_x, bool want_w, bool want_b, bool x_direct) {
     BwdPlan p;
     const int P = dtype == kF32 ? 2 : 1, BK = P == 1 ? 64 : 32;
-    const int64_t Np = up(N, 256);
-    const size_t per = (size_t)(Np * (want_w ? 2 : 0) + N * (want_x ? 2 : 0) + C * (want_x ? 2 : 0)) * P + 1;
-    int64_t most = (int64_t)(kPieceBytes / per) / 256 * 256;
+    p.rowsE = up(N, 64);
+    int64_t most = (int64_t)(kPieceBytes / (size_t)(p.rowsE * 2 * P)) / 256 * 256;
     if (most < 256) most = 256;
     if (most > (1 << 21)) most = 1 << 21;        // a row of E stays below the operand's largest pitch
     const int64_t pieces = (V + most - 1) / most;
     p.Vc = pieces == 1 ? V : up((V + pieces - 1) / pieces, 256);
     p.pieces = (int)((V + p.Vc - 1) / p.Vc);
-    p.bigL = use_big(p.Vc, N);
-    p.bigX = use_big(N, C);
-    p.bigW = use_big(p.Vc, C);
     p.pitchE = up(p.Vc, 256) * 2 * P;
-    p.pitchT = Np * 2 * P;
-    const int bx = p.bigX ? 256 : 128, bw = p.bigW ? 256 : 128;
-    p.splitX = split_of(((N + bx - 1) / bx) * ((C + bx - 1) / bx), up(p.Vc, BK) / BK);
-    p.splitW = split_of(((p.Vc + bw - 1) / bw) * ((C + bw - 1) / bw), up(N, BK) / BK);
+    p.sideL = choose(p.Vc, N, up(C, 64) * P / 64, P, false).side;
+    p.cx = choose(N, C, up(p.Vc, BK) / BK, P, true);
+    p.cw = choose(p.Vc, C, up(N, BK) / BK, P, true);
     p.coef = ws.take<float>((size_t)N);
     p.fscale = ws.take<float>(1);
-    const int bl = p.bigL ? 256 : 128, wn = p.bigL ? 4 : 2;
-    p.pdb = ws.take<float>(want_b ? (size_t)((N + bl - 1) / bl) * wn * p.Vc : 0);
-    p.planeX = ws.take<float>(want_x && (p.splitX > 1 || p.pieces > 1) ? (size_t)p.splitX * N * C : 0);
-    p.planeW = ws.take<float>(want_w && p.splitW > 1 ? (size_t)p.splitW * p.Vc * C : 0);
-    p.Xt = ws.take<char>(want_w ? (size_t)C * p.pitchT : 0);
-    p.Wt = ws.take<char>(want_x ? (size_t)C * p.pitchE : 0);
-    p.E = ws.take<char>(want_x ? (size_t)N * p.pitchE : 0);
-    p.Et = ws.take<char>(want_w ? (size_t)p.Vc * p.pitchT : 0);
+    p.pdb = ws.take<float>(want_b ? (size_t)(tiles_of(N, p.sideL) * p.Vc) : 0);
+    p.planeX = ws.take<float>(want_x && (p.cx.splits > 1 || p.pieces > 1) ? (size_t)p.cx.splits * N * C : 0);
+    p.planeW = ws.take<float>(want_w && p.cw.splits > 1 ? (size_t)p.cw.splits * p.Vc * C : 0);
+    p.Xg = ws.take<char>(want_w && x_direct ? (size_t)(N * C * 2) : 0);
+    p.E = ws.take<char>(want_x || want_w ? (size_t)(p.rowsE * p.pitchE) : 0);
     return p;
 }
 
-inline unsigned grid_for(int64_t n) {
-    const int64_t b = (n + 255) / 256;
-    return (unsigned)(b < 2048 ? b : 2048);
+template <typename S, bool TA>
+int product(const ProdArgs& q, int side, hipStream_t st) {
+    using T = typename Inner<S>::T;
+    constexpr int P = Inner<S>::P;
+    const dim3 grid((unsigned)(q.tilesA * q.tilesB), (unsigned)q.splits);
+#define SSECG_CE_PROD(TILE) do { using M = TILE<T, P, TA, true>; SSECG_CE_LAUNCH(M, (ce_prod_kernel<M, S>), grid, st, q); } while (0)
+    if (side == 256) SSECG_CE_PROD(Big);
+    else if (side == 128) SSECG_CE_PROD(Mid);
+    else SSECG_CE_PROD(Small);
+#undef SSECG_CE_PROD
+    return 0;
 }
 
 template <typename S>
@@ -688,78 +712,77 @@ int ce_bwd(const float* dloss, const void* x, const void* w, const float* bias, 
            const float* count, int dtype, int64_t N, int64_t C, int64_t V, int reduction, void* dx, void* dw, float* db, void* packed, void* ws,
            hipStream_t st) {
     using T = typename Inner<S>::T;
-    constexpr int P = Inner<S>::P;
-    constexpr int BK = P == 1 ? 64 : 32;
+    constexpr int P = Inner<S>::P, BK = P == 1 ? 64 : 32;
     Blob blob(ws);
     const Packed k = plan_packed(packed, x, w, dtype, N, C, V);
-    const BwdPlan p = plan_bwd(blob, dtype, N, C, V, dx != nullptr, dw != nullptr, db != nullptr);
+    const BwdPlan p = plan_bwd(blob, dtype, N, C, V, dx != nullptr, dw != nullptr, db != nullptr, !k.Xp);
+    const char *X = k.Xp ? k.Xp : (const char*)x, *W = k.Wp ? k.Wp : (const char*)w;
     int rc = 0;
-    hipLaunchKernelGGL(ce_coef_kernel, dim3(1), dim3(1024), 0, st, dloss, gate, count, (int)N, reduction, p.coef, p.fscale);
-    if (dw && (rc = pack<S>(x, 0, N, C, gate, k.amaxX, nullptr, 0, p.Xt, p.pitchT, st)) != 0) return rc;
+    Factor f = {dloss, reduction == 1 ? count : nullptr};
+    if (reduction == 0) {
+        hipLaunchKernelGGL(ce_coef_kernel, dim3(1), dim3(1024), 0, st, dloss, gate, (int)N, p.coef, p.fscale);
+        f = {p.fscale, nullptr};
+    }
+    const char* Xw = X;                          // of dw: rows that do not count are zeros (a copy made by the forward pass has them so)
+    if (dw && !k.Xp) {
+        if ((rc = pack<S>(x, N, C, Counts{gate, nullptr, 0, nullptr, 0.f}, nullptr, p.Xg, k.pitch, st)) != 0) return rc;
+        Xw = p.Xg;
+    }
     for (int i = 0; i < p.pieces; ++i) {
         const int64_t v0 = i * p.Vc, vn = V - v0 < p.Vc ? V - v0 : p.Vc;
         LogitArgs a = {};
-        a.X = {k.Xp ? k.Xp : (const char*)x, k.pitch, (int)N};
-        a.W = {(k.Wp ? k.Wp : (const char*)w) + v0 * k.pitch, k.pitch, (int)vn};
+        a.X = {X, k.pitch, (int)N};
+        a.W = {W + v0 * k.pitch, k.pitch, (int)vn};
         a.bias = bias ? bias + v0 : nullptr;
         a.amaxX = k.amaxX; a.amaxW = k.amaxW;
         a.V = (int)vn; a.N = (int)N;
-        const int bl = p.bigL ? 256 : 128, wn = p.bigL ? 4 : 2;
-        a.tilesV = (int)((vn + bl - 1) / bl); a.tilesN = (int)((N + bl - 1) / bl);
+        a.tilesV = (int)tiles_of(vn, p.sideL); a.tilesN = (int)tiles_of(N, p.sideL);
         a.stages = (int)(k.pitch / 128);
         a.target = target; a.v0 = v0;
         a.lse = lse; a.gate = gate; a.coef = reduction == 0 ? p.coef : nullptr;
-        a.E = dx ? p.E : nullptr; a.pitchE = p.pitchE;
-        a.Et = dw ? p.Et : nullptr; a.pitchT = p.pitchT;
+        a.E = dx || dw ? p.E : nullptr; a.pitchE = p.pitchE; a.rowsE = (int)p.rowsE;
         a.pdb = p.pdb;
         const dim3 grid(a.tilesV * a.tilesN);
-        if (p.bigL) {
-            using M = Big<T, P>;
-            if (db) SSECG_CE_LAUNCH(M, (ce_grad_kernel<M, true>), grid, st, a);
-            else SSECG_CE_LAUNCH(M, (ce_grad_kernel<M, false>), grid, st, a);
-        } else {
-            using M = Mid<T, P>;
-            if (db) SSECG_CE_LAUNCH(M, (ce_grad_kernel<M, true>), grid, st, a);
-            else SSECG_CE_LAUNCH(M, (ce_grad_kernel<M, false>), grid, st, a);
-        }
-        if (db) hipLaunchKernelGGL(ce_db_kernel, dim3((unsigned)((vn + 255) / 256)), dim3(256), 0, st, p.pdb, a.tilesN * wn, (int)vn, p.fscale, db + v0);
-        if (dx) {
-            const int64_t pitch = up(vn, 64) * 2 * P;
-            if ((rc = pack<S>(w, v0, vn, C, nullptr, k.amaxW, nullptr, 0, p.Wt, pitch, st)) != 0) return rc;
+#define SSECG_CE_GRAD(TILE)                                                             \
+    do {                                                                                \
+        using M = TILE<T, P>;                                                           \
+        if (db) SSECG_CE_LAUNCH(M, (ce_grad_kernel<M, true>), grid, st, a);             \
+        else SSECG_CE_LAUNCH(M, (ce_grad_kernel<M, false>), grid, st, a);               \
+    } while (0)
+        if (p.sideL == 256) SSECG_CE_GRAD(Big);
+        else if (p.sideL == 128) SSECG_CE_GRAD(Mid);
+        else SSECG_CE_GRAD(Small);
+#undef SSECG_CE_GRAD
+        if (db) hipLaunchKernelGGL(ce_db_kernel, dim3((unsigned)((vn + 255) / 256)), dim3(256), 0, st, p.pdb, a.tilesN, (int)vn, f, db + v0);
+        if (dx) {                                // E along its rows, W across
             ProdArgs q = {};
             q.A = {p.E, p.pitchE, (int)N};
-            q.B = {p.Wt, pitch, (int)C};
+            q.B = {W + v0 * k.pitch, k.pitch, (int)vn};
             q.rows = (int)N; q.cols = (int)C;
-            const int bx = p.bigX ? 256 : 128;
-            q.tilesA = (int)((N + bx - 1) / bx); q.tilesB = (int)((C + bx - 1) / bx);
-            q.stages = (int)(up(vn, BK) / BK); q.splits = p.splitX;
-            q.plane = p.splitX > 1 || p.pieces > 1 ? p.planeX : nullptr;
-            q.add = i > 0; q.out = dx; q.amax = k.amaxW; q.fscale = p.fscale;
-            const dim3 g2(q.tilesA * q.tilesB, q.splits);
-            if (p.bigX) { using M = Big<T, P>; SSECG_CE_LAUNCH(M, (ce_prod_kernel<M, S>), g2, st, q); }
-            else { using M = Mid<T, P>; SSECG_CE_LAUNCH(M, (ce_prod_kernel<M, S>), g2, st, q); }
+            q.tilesA = (int)tiles_of(N, p.cx.side); q.tilesB = (int)tiles_of(C, p.cx.side);
+            q.stages = (int)(up(vn, BK) / BK); q.splits = p.cx.splits;
+            q.plane = p.cx.splits > 1 || p.pieces > 1 ? p.planeX : nullptr;
+            q.add = i > 0; q.out = dx; q.amax = k.amaxW; q.f = f;
+            if ((rc = product<S, false>(q, p.cx.side, st)) != 0) return rc;
         }
-        if (dw) {
+        if (dw) {                                // both across
             ProdArgs q = {};
-            q.A = {p.Et, p.pitchT, (int)vn};
-            q.B = {p.Xt, p.pitchT, (int)C};
+            q.A = {p.E, p.pitchE, (int)p.rowsE};
+            q.B = {Xw, k.pitch, (int)N};
             q.rows = (int)vn; q.cols = (int)C;
-            const int bw = p.bigW ? 256 : 128;
-            q.tilesA = (int)((vn + bw - 1) / bw); q.tilesB = (int)((C + bw - 1) / bw);
-            q.stages = (int)(up(N, BK) / BK); q.splits = p.splitW;
-            q.plane = p.splitW > 1 ? p.planeW : nullptr;
-            q.out = (S*)dw + v0 * C; q.amax = k.amaxX; q.fscale = p.fscale;
-            const dim3 g2(q.tilesA * q.tilesB, q.splits);
-            if (p.bigW) { using M = Big<T, P>; SSECG_CE_LAUNCH(M, (ce_prod_kernel<M, S>), g2, st, q); }
-            else { using M = Mid<T, P>; SSECG_CE_LAUNCH(M, (ce_prod_kernel<M, S>), g2, st, q); }
+            q.tilesA = (int)tiles_of(vn, p.cw.side); q.tilesB = (int)tiles_of(C, p.cw.side);
+            q.stages = (int)(up(N, BK) / BK); q.splits = p.cw.splits;
+            q.plane = p.cw.splits > 1 ? p.planeW : nullptr;
+            q.out = (S*)dw + v0 * C; q.amax = k.amaxX; q.f = f;
+            if ((rc = product<S, true>(q, p.cw.side, st)) != 0) return rc;
             if (q.plane)
-                hipLaunchKernelGGL((ce_sum_planes_kernel<S>), dim3(grid_for(vn * C)), dim3(256), 0, st, p.planeW, p.splitW, vn * C,
-                                   P == 2 ? k.amaxX : nullptr, p.fscale, (S*)dw + v0 * C);
+                hipLaunchKernelGGL((ce_sum_planes_kernel<S>), dim3(grid_for(vn * C)), dim3(256), 0, st, p.planeW, p.cw.splits, vn * C,
+                                   P == 2 ? k.amaxX : nullptr, f, (S*)dw + v0 * C);
         }
     }
-    if (dx && (p.splitX > 1 || p.pieces > 1))
-        hipLaunchKernelGGL((ce_sum_planes_kernel<S>), dim3(grid_for(N * C)), dim3(256), 0, st, p.planeX, p.splitX, N * C, P == 2 ? k.amaxW : nullptr,
-                           p.fscale, (S*)dx);
+    if (dx && (p.cx.splits > 1 || p.pieces > 1))
+        hipLaunchKernelGGL((ce_sum_planes_kernel<S>), dim3(grid_for(N * C)), dim3(256), 0, st, p.planeX, p.cx.splits, N * C,
+                           P == 2 ? k.amaxW : nullptr, f, (S*)dx);
     return (int)hipGetLastError();
 }
 
@@ -775,7 +798,7 @@ size_t ssecg_linear_ce_packed_bytes(const void* x, const void* weight, int dtype
 size_t ssecg_linear_ce_fwd_workspace(int dtype, int64_t N, int64_t C, int64_t V) {
     if (!dtype_ok(dtype) || !shape_ok(N, C, V)) return 0;
     Blob b(nullptr);
-    plan_fwd(b, N, V);
+    plan_fwd(b, dtype, N, C, V);
     return b.at;
 }
 
@@ -795,7 +818,7 @@ int ssecg_linear_ce_fwd(const void* x, const void* weight, const float* bias, co
 size_t ssecg_linear_ce_bwd_workspace(int dtype, int64_t N, int64_t C, int64_t V, int want_dx, int want_dw, int want_db) {
     if (!dtype_ok(dtype) || !shape_ok(N, C, V)) return 0;
     Blob b(nullptr);
-    plan_bwd(b, dtype, N, C, V, want_dx != 0, want_dw != 0, want_db != 0);
+    plan_bwd(b, dtype, N, C, V, want_dx != 0, want_dw != 0, want_db != 0, true);
     return b.at;
 }
 

@@ -10,11 +10,16 @@
 // Tile BM x BN by WM x WN waves, v_mfma_f32_32x32x16.  Stages travel by LDS-DMA (16 bytes a lane, no registers) into a ring of R
 // slots, requested R - 1 stages ahead with counted waits and one barrier per stage; the fragments of a k step are read while the
 // step before it is multiplied, across the barrier too.  A stage's LDS row is 8 chunks of 16 bytes.  Chunk c of row r lies at
-// position c ^ (r & 7): the DMA writes positions in lane order, so the lane fetches the permuted chunk, and 8 rows read at one k by
-// 8 lanes fall into 8 different bank groups.
+// position c ^ (r / 2 % 8): the DMA writes positions in lane order, so the lane fetches the permuted chunk, and the 16 rows that 16
+// lanes read at one k cover the 64 banks once (two rows of 128 bytes are one pass over the banks).
 //
-// Bounds: a row index beyond the operand is clamped to its last row (the caller masks the result); k is padded with zeros in
-// memory to a whole stage, so the loads have no other condition.  Offsets within a tile are 32 bits: 256 pitch < 2^32.
+// An operand may also lie with k SLOW (TA / TB): [k][index], its index padded in memory to whole chunks of 64.  Its stage in LDS is
+// BK rows of the tile's indices; ds_read_b64_tr_b16 gives a lane 4 consecutive k of its index, so two of them are a fragment.  The
+// chunks of a row are permuted by its row so that the 8 rows of a read fall into different banks.
+//
+// Bounds: an index beyond a k-fast operand is clamped to its last row, a chunk beyond a k-slow one to its row's last chunk (the
+// caller masks the result).  k-fast operands are padded with zeros to a whole stage; of a k-slow operand rows beyond the last are
+// read as the last one, and the other operand holds zeros there.  Offsets within a tile are 32 bits: 256 pitch < 2^32.
 #pragma once
 #include "lm_common.h"
 
@@ -23,7 +28,7 @@ namespace ssecg_lm {
 struct Operand {
     const char* base;    // 16-byte aligned
     int64_t pitch;       // bytes of a row, a multiple of 128, below 2^24
-    int rows;
+    int rows;            // rows in memory: indices, or k of a k-slow operand
 };
 constexpr int64_t kMaxPitch = (1 << 24) - 1;
 
@@ -40,6 +45,13 @@ __device__ __forceinline__ void lds_dma16(const char* base, unsigned off, unsign
                  : "=&s"(keep) : "v"(off), "s"(base), "s"(lds_wave_base) : "memory");
 }
 
+// a pointer that is the same in every lane, in scalar registers
+__device__ __forceinline__ const char* uniform(const char* p) {
+    const uint64_t v = (uint64_t)p;
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v), hi = __builtin_amdgcn_readfirstlane((uint32_t)(v >> 32));
+    return (const char*)((uint64_t)hi << 32 | lo);
+}
+
 template <typename T> struct Frag;
 template <> struct Frag<__bf16> {
     typedef bf16x8 type;
@@ -50,68 +62,149 @@ template <> struct Frag<_Float16> {
     static __device__ __forceinline__ f32x16 mfma(type a, type b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 };
 
-template <typename T_, int P_, int BM_, int BN_, int WM_, int WN_, int R_>
+template <typename T_, int P_, int BM_, int BN_, int WM_, int WN_, int R_, bool TA_ = false, bool TB_ = false>
 struct MmTile {
     using T = T_;
     using F = Frag<T>;
     using V8 = typename F::type;
     static constexpr int P = P_, BM = BM_, BN = BN_, WM = WM_, WN = WN_, R = R_;
+    static constexpr bool TA = TA_, TB = TB_;
     static constexpr int NW = WM * WN, NT = NW * 64;
     static constexpr int TM = BM / WM / 32, TN = BN / WN / 32;
     static constexpr int BK = P == 1 ? 64 : 32;                 // k of a stage
-    static constexpr int STEP = 128;                            // bytes a row advances per stage
+    static constexpr int STEP = 128;                            // bytes of a k-fast row in a stage
     static constexpr int PA = BM / 8 / NW, PB = BN / 8 / NW, PPW = PA + PB;   // 1 KB pieces (8 rows) per wave and stage
     static constexpr int SLOT = (BM + BN) * 128;
     static constexpr int LDS = R * SLOT;
     static_assert(PA * NW * 8 == BM && PB * NW * 8 == BN, "every wave requests the same number of pieces");
     static_assert(R >= 2 && (R - 2) * PPW <= 63, "vmcnt counts to 63");
 
-    template <int N> static __device__ __forceinline__ void stage_wait() {
-        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+    // waits for every piece of this wave but those of `ahead` (uniform, at most AHEAD) stages, and for the other waves
+    template <int AHEAD> static __device__ __forceinline__ void stage_wait(int ahead) {
+        if constexpr (AHEAD > 0)
+            if (ahead < AHEAD) return stage_wait<AHEAD - 1>(ahead);
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(AHEAD * PPW) : "memory");
     }
 
-    // acc += the tile at rows a0 of A and b0 of B over stages [s0, s0 + n); all waves of the workgroup call it together
+    // k-slow stage: BK rows of ROW bytes (SIDE indices); position of chunk c of row k
+    template <int SIDE> struct Slow {
+        static constexpr int ROW = SIDE * 2 * P, CH = ROW / 16;
+        static __device__ __forceinline__ int swz(int k) { return ((k & 3) << 2 | (k >> 2 & 3)) & (CH - 1); }
+        // lane's 4 indices x 4 k of the read that gives lane (r, h) the k 16 kk + 8 h + 4 part .. + 3 of index 32 blk + r, plane q
+        static __device__ __forceinline__ int at(int lane, int blk, int kk, int part, int q) {
+            const int l = lane & 15, g = lane >> 4;
+            const int k = kk * 16 + 8 * (g >> 1) + 4 * part + (l >> 2);
+            const int c = (blk * P + q) * 4 + 2 * (g & 1) + ((l & 3) >> 1);
+            return k * ROW + ((c ^ swz(k)) << 4) + 8 * (l & 1);
+        }
+    };
+    typedef short s16x4 __attribute__((ext_vector_type(4)));
+    typedef short s16x8 __attribute__((ext_vector_type(8)));
+    static __device__ __forceinline__ V8 read_tr(const char* lo, const char* hi) {
+        const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)lo);
+        const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)hi);
+        return __builtin_bit_cast(V8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+    }
+
+    // one operand's pieces of a stage: this wave's PC pieces of 1 KB, SIDE indices from i0
+    template <int SIDE, int PC, bool SLOW> struct Loader {
+        unsigned off[PC];
+        const char* base;                      // of the stage that is requested next
+        unsigned dst;
+        int64_t step;
+        int left;                              // k-slow: rows from the stage that is requested next
+        unsigned pitch;
+        int row0;                              // k-slow: row of the lane in its first piece
+        static constexpr int RPP = SLOW ? 1024 / Slow<SIDE>::ROW : 8;     // rows of a piece
+        __device__ __forceinline__ Loader(const Operand& o, int i0, int s0, int lane, int wave, unsigned lds) {
+            dst = lds + wave * PC * 1024;
+            pitch = (unsigned)o.pitch;
+            if constexpr (!SLOW) {
+                base = o.base + i0 * o.pitch + (int64_t)s0 * STEP;
+                step = STEP;
+                const int last = o.rows - 1 - i0;
+#pragma unroll
+                for (int i = 0; i < PC; ++i) {
+                    int row = (wave * PC + i) * 8 + (lane >> 3);
+                    const int chunk = (lane & 7) ^ (row >> 1 & 7);
+                    row = row < last ? row : last;
+                    off[i] = (unsigned)row * pitch + (chunk << 4);
+                }
+            } else {
+                using S = Slow<SIDE>;
+                step = BK * o.pitch;
+                base = o.base + s0 * step;
+                left = o.rows - s0 * BK;
+                const unsigned first = (unsigned)i0 * 2 * P, most = pitch - 16;
+                row0 = wave * PC * RPP + lane * 16 / S::ROW;
+#pragma unroll
+                for (int i = 0; i < PC; ++i) {
+                    const int k = row0 + i * RPP;
+                    const unsigned c = first + (((lane * 16 % S::ROW >> 4) ^ S::swz(k)) << 4);
+                    off[i] = (unsigned)k * pitch + (c < most ? c : most);
+                }
+            }
+        }
+        __device__ __forceinline__ void issue(int slot) {
+            const char* u = uniform(base);
+            if (SLOW && left < BK) {           // the last stage: rows that do not exist are read as the last one
+#pragma unroll
+                for (int i = 0; i < PC; ++i) {
+                    const int k = row0 + i * RPP;
+                    const unsigned back = k < left ? 0u : (unsigned)(k - left + 1) * pitch;
+                    lds_dma16(u, off[i] - back, __builtin_amdgcn_readfirstlane(dst + i * 1024 + slot * SLOT));
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < PC; ++i) lds_dma16(u, off[i], __builtin_amdgcn_readfirstlane(dst + i * 1024 + slot * SLOT));
+            }
+            base += step;
+            if (SLOW) left -= BK;
+        }
+    };
+
+    // acc += the tile at indices a0 of A and b0 of B over stages [s0, s0 + n); all waves of the workgroup call it together
     static __device__ __forceinline__ void run(const Operand& A, int a0, const Operand& B, int b0, int s0, int n, char* lds,
                                                f32x16 (&acc)[TM][TN]) {
         const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
         const int wm = wave / WN, wn = wave % WN, r = lane & 31, h = lane >> 5;
         const unsigned ldsbase = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
-        unsigned off[PPW];
-        const int chunk = (lane & 7) ^ (lane >> 3);
-#pragma unroll
-        for (int i = 0; i < PPW; ++i) {
-            int row = (i < PA ? (wave * PA + i) * 8 : (wave * PB + i - PA) * 8) + (lane >> 3);
-            const int last = i < PA ? A.rows - 1 - a0 : B.rows - 1 - b0;
-            row = row < last ? row : last;
-            off[i] = (unsigned)row * (unsigned)(i < PA ? A.pitch : B.pitch) + chunk * 16;
-        }
-        const char* pA = A.base + a0 * A.pitch + (int64_t)s0 * STEP;   // of the stage that is requested next
-        const char* pB = B.base + b0 * B.pitch + (int64_t)s0 * STEP;
-        const unsigned dstA = ldsbase + wave * PA * 1024, dstB = ldsbase + BM * 128 + wave * PB * 1024;
+        Loader<BM, PA, TA> la(A, a0, s0, lane, wave, ldsbase);
+        Loader<BN, PB, TB> lb(B, b0, s0, lane, wave, ldsbase + BM * 128);
         auto issue = [&](int slot) {
-#pragma unroll
-            for (int i = 0; i < PPW; ++i)
-                lds_dma16(i < PA ? pA : pB, off[i], (i < PA ? dstA + i * 1024 : dstB + (i - PA) * 1024) + slot * SLOT);
-            pA += STEP;
-            pB += STEP;
+            la.issue(slot);
+            lb.issue(slot);
         };
 #pragma unroll
         for (int s = 0; s < R - 1; ++s)
             if (s < n) issue(s);
-        // fragment offsets: row (wave tile + 32 i + r), chunk (2 kk + h) of this lane
-        const int swz = r & 7;
-        const char* fa = lds + (wm * TM * 32 + r) * 128;
-        const char* fb = lds + BM * 128 + (wn * TN * 32 + r) * 128;
+        // fragment offsets, k fast: row (wave tile + 32 i + r), chunk (2 kk + h) of this lane
+        const int swz = r >> 1 & 7;
+        const char* fa = lds + (TA ? 0 : (wm * TM * 32 + r) * 128);
+        const char* fb = lds + BM * 128 + (TB ? 0 : (wn * TN * 32 + r) * 128);
         constexpr int KK = P == 1 ? 4 : 2;                      // k steps of 16 in a stage
+        constexpr bool AHEAD = !(P == 2 && TA && TB && TM * TN > 4);   // (there a second set of fragments would spill)
         V8 a[2][P][TM], b[2][P][TN];                            // two sets: one is multiplied while the other is read
         auto frags = [&](int set, int slot, int kk) {
 #pragma unroll
             for (int q = 0; q < P; ++q) {
                 const int c = slot * SLOT + ((4 * q + 2 * kk + h) ^ swz) * 16;
 #pragma unroll
-                for (int i = 0; i < TM; ++i) a[set][q][i] = *reinterpret_cast<const V8*>(fa + i * 4096 + c);
+                for (int i = 0; i < TM; ++i) {
+                    if constexpr (TA)
+                        a[set][q][i] = read_tr(fa + slot * SLOT + Slow<BM>::at(lane, wm * TM + i, kk, 0, q),
+                                               fa + slot * SLOT + Slow<BM>::at(lane, wm * TM + i, kk, 1, q));
+                    else
+                        a[set][q][i] = *reinterpret_cast<const V8*>(fa + i * 4096 + c);
+                }
 #pragma unroll
-                for (int j = 0; j < TN; ++j) b[set][q][j] = *reinterpret_cast<const V8*>(fb + j * 4096 + c);
+                for (int j = 0; j < TN; ++j) {
+                    if constexpr (TB)
+                        b[set][q][j] = read_tr(fb + slot * SLOT + Slow<BN>::at(lane, wn * TN + j, kk, 0, q),
+                                               fb + slot * SLOT + Slow<BN>::at(lane, wn * TN + j, kk, 1, q));
+                    else
+                        b[set][q][j] = *reinterpret_cast<const V8*>(fb + j * 4096 + c);
+                }
             }
         };
         auto multiply = [&](int set) {
@@ -125,10 +218,8 @@ struct MmTile {
                         acc[i][j] = F::mfma(a[set][q == 0 ? P - 1 : 0][i], b[set][q == 1 ? P - 1 : 0][j], acc[i][j]);
         };
         if (n > 0) {
-            if (R > 3 && n > 2) stage_wait<(R > 3 ? 2 * PPW : 0)>();
-            else if (R > 2 && n > 1) stage_wait<(R > 2 ? PPW : 0)>();
-            else stage_wait<0>();
-            frags(0, 0, 0);
+            stage_wait<R - 2>(n - 1 < R - 2 ? n - 1 : R - 2);
+            if (AHEAD) frags(0, 0, 0);
         }
         int slot = 0;
         for (int s = 0; s < n; ++s) {
@@ -138,15 +229,14 @@ struct MmTile {
             if (s + R - 1 < n) issue(slot == 0 ? R - 1 : slot - 1);
 #pragma unroll
             for (int kk = 0; kk < KK; ++kk) {
+                if (!AHEAD) frags(kk & 1, slot, kk);
                 if (kk + 1 < KK) {
-                    frags((kk + 1) & 1, slot, kk + 1);
+                    if (AHEAD) frags((kk + 1) & 1, slot, kk + 1);
                 } else if (s + 1 < n) {
                     // the next stage has landed when only the pieces of the stages requested after it are outstanding
                     const int ahead = n - 2 - s < R - 2 ? n - 2 - s : R - 2;
-                    if (R > 3 && ahead == 2) stage_wait<(R > 3 ? 2 * PPW : 0)>();
-                    else if (R > 2 && ahead == 1) stage_wait<(R > 2 ? PPW : 0)>();
-                    else stage_wait<0>();
-                    frags((kk + 1) & 1, next, 0);
+                    stage_wait<R - 2>(ahead);
+                    if (AHEAD) frags((kk + 1) & 1, next, 0);
                 }
                 __builtin_amdgcn_sched_barrier(0);   // the reads above travel under the products below
                 multiply(kk & 1);
@@ -236,6 +326,28 @@ template <class M> struct WaveStore {
         }
     }
 };
+
+// The time of a launch in microseconds, to choose a tile side by.  One stage of one workgroup takes `alone` us where it has its CU to
+// itself and `full` us where the chip is full (two workgroups a CU up to 128); measured on products of 4096 x 4096 x 4096 (full:
+// 120 / 155 / 200 us with one plane, 308 / 344 / 466 us with two, for sides of 256 / 128 / 64) and 512 x 1536 x 512 (alone).
+struct MmWork {
+    int64_t tiles = 0, stages = 0, longest = 0;      // workgroups, their stages together, the most stages of one
+    void add(int64_t n, int64_t per) {
+        tiles += n;
+        stages += n * per;
+        longest = longest < per ? per : longest;
+    }
+};
+inline double mm_time(int side, int planes, const MmWork& w) {
+    const bool two = planes == 2;
+    const double full = side == 256 ? (two ? 2.4 : 1.87) : side == 192 ? (two ? 1.4 : 1.1) : side == 128 ? (two ? 1.34 : 1.2) : (two ? 0.46 : 0.39);
+    const double alone = side == 256 ? (two ? 1.9 : 1.5) : side == 192 ? (two ? 1.2 : 0.9) : side == 128 ? (two ? 0.75 : 0.6) : 0.3;
+    const int64_t slots = side > 128 ? 256 : 512;
+    if (w.tiles <= 256) return 3.0 + w.longest * alone;
+    const double rounds = (double)((w.tiles + slots - 1) / slots), mean = (double)w.stages / (double)w.tiles;
+    const double busy = rounds * mean * full, chain = w.longest * alone;
+    return 3.0 + (busy > chain ? busy : chain);
+}
 
 // Consecutive workgroups run on different XCDs (8, round robin), each with an L2 of its own: give every XCD a contiguous range of
 // tiles, so that neighbours share operand rows in one L2.  A permutation of [0, n).

@@ -5,9 +5,9 @@
 //   optimiser: v = mu v + g,  U = g + mu v (Nesterov) or v,  p = p (1 - lr wd) - lr s X,  s = 0.2 sqrt(max(rows, cols)) or
 //   sqrt(max(1, rows / cols))
 //
-// Every product is mm_core.h's with k fastest in both operands.  A and P are symmetric, so they are their own transposes (and only
-// the tiles on and below the diagonal are computed); X is kept both ways round, X for A and X^T for the update, and the update's
-// epilogue writes both.  The identity is folded into P, so the update needs no third operand.
+// Every product is mm_core.h's.  A and P are symmetric: only the tiles on and below the diagonal are computed, and the epilogue
+// writes the mirrored tile too.  X is read along its rows for A and across for the update.  The identity is folded into P, so the
+// update needs no third operand.
 //
 // Precision: the iteration multiplies errors along weak directions by up to a = 3.44 per step (485 over five), so 16-bit iterates
 // would lose them.  All matrices are two fp16 planes times 2^13 - singular values stay below 1.21 and P's below 3.45, far inside
@@ -20,7 +20,7 @@ using namespace ssecg_lm;
 
 constexpr float kA = 3.4445f, kB = -4.7750f, kC = 2.0315f;
 constexpr int kScale = 13;
-constexpr int kNormParts = 128;                   // workgroups that share one matrix's norm
+constexpr int kNormParts = 1024;                  // most workgroups that share one matrix's norm
 constexpr int kMost = 32;                         // matrices of one chain of launches: their table travels in the kernel arguments
 
 // By value in the kernel arguments (1.9 KB): no upload, nothing to keep for a captured launch.  first[w][k]: the first workgroup
@@ -36,20 +36,20 @@ struct Table {
 struct Mat {
     const void* src; void* dst; float* mom;
     int rows, cols, m, n;
-    int64_t pn, pm;                               // bytes of a row of X; of X^T, A and P
-    char *X, *Xt0, *Xt1, *A, *P;                  // operands of two planes (mm_core.h)
+    int64_t pn, pm;                               // bytes of a row of X; of A and P
+    char *X[2], *A, *P;                           // operands of two planes (mm_core.h); an update reads one X and writes the other
 };
 
 inline __host__ __device__ int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
-// planes of one matrix in the workspace: X, X^T twice (read one, write the other), A, P
+// of one matrix in the workspace
 inline __host__ __device__ int64_t mat_bytes(int64_t rows, int64_t cols) {
     const int64_t m = rows < cols ? rows : cols, n = rows < cols ? cols : rows;
     const int64_t pn = up(n, 32) * 4, pm = up(m, 32) * 4;
-    return up(m * pn + 2 * n * pm + 2 * m * pm, 256);
+    return up(2 * m * pn + 2 * m * pm, 256);
 }
 
-__device__ __forceinline__ Mat load_mat(const Table& table, int k, char* ws) {
+__device__ __forceinline__ Mat load_mat(const Table& table, int k, char* ws, int from) {   // X[0] is number `from`
     Mat t;
     t.src = table.src[k];
     t.dst = table.dst[k];
@@ -60,10 +60,10 @@ __device__ __forceinline__ Mat load_mat(const Table& table, int k, char* ws) {
     t.n = t.rows < t.cols ? t.cols : t.rows;
     t.pn = up(t.n, 32) * 4;
     t.pm = up(t.m, 32) * 4;
-    t.X = ws + table.offset[k];
-    t.Xt0 = t.X + t.m * t.pn;
-    t.Xt1 = t.Xt0 + t.n * t.pm;
-    t.A = t.Xt1 + t.n * t.pm;
+    char* base = ws + table.offset[k];
+    t.X[0] = base + from * (t.m * t.pn);
+    t.X[1] = base + (1 - from) * (t.m * t.pn);
+    t.A = base + 2 * t.m * t.pn;
     t.P = t.A + t.m * t.pm;
     return t;
 }
@@ -86,34 +86,42 @@ __device__ __forceinline__ float update_of(const Mat& t, int64_t i, float mu, in
     return nesterov ? g + mu * v : v;
 }
 
-// momentum and the partial sums of |U|^2 (fp64: no gradient's scale overflows it); partial [count][kNormParts]
+// momentum and the partial sums of |U|^2 (fp64: no gradient's scale overflows it); partial [count][gridDim.x]
 template <typename S, bool MUON>
 __global__ __launch_bounds__(256) void ns_norm_kernel(Table table, float mu, int nesterov, const float* __restrict__ skip,
                                                       double* __restrict__ partial) {
     if (MUON && skip != nullptr && skip[0] != 0.f) return;
-    const Mat t = load_mat(table, blockIdx.y, nullptr);
+    const Mat t = load_mat(table, blockIdx.y, nullptr, 0);
     const int64_t n = (int64_t)t.rows * t.cols;
+    constexpr int V = Vec<S>::N;
+    const S* src = reinterpret_cast<const S*>(t.src);
     double s = 0.0;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-        float u;
-        if (MUON) {
-            const float g = (float)reinterpret_cast<const S*>(t.src)[i], v = mu * t.mom[i] + g;
-            t.mom[i] = v;
-            u = nesterov ? g + mu * v : v;
+    for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * V; i < n; i += (int64_t)gridDim.x * 256 * V) {
+        const int left = n - i < V ? (int)(n - i) : V;
+        const auto g = load_vec(src + i, 0, left);
+        if constexpr (MUON) {
+            auto v = load_vec(t.mom + i, 0, left);
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                v[j] = mu * v[j] + g[j];
+                const float u = nesterov ? g[j] + mu * v[j] : v[j];
+                s += (double)u * (double)u;               // beyond the end: zeros
+            }
+            store_vec(t.mom + i, 0, left, v);
         } else {
-            u = (float)reinterpret_cast<const S*>(t.src)[i];
+#pragma unroll
+            for (int j = 0; j < V; ++j) s += (double)(float)g[j] * (double)(float)g[j];
         }
-        s += (double)u * (double)u;
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
     __shared__ double sh[4];
     if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = s;
     __syncthreads();
-    if (threadIdx.x == 0) partial[(int64_t)blockIdx.y * kNormParts + blockIdx.x] = (sh[0] + sh[1]) + (sh[2] + sh[3]);
+    if (threadIdx.x == 0) partial[(int64_t)blockIdx.y * gridDim.x + blockIdx.x] = (sh[0] + sh[1]) + (sh[2] + sh[3]);
 }
 
-// U / (norm + eps) as planes, X and X^T; one workgroup: 64 x 64 elements, zeros up to the pitch
+// U / (norm + eps) as an operand, the shorter side first; one workgroup: 64 x 64 elements, zeros up to the pitch
 template <typename S, bool MUON>
 __global__ __launch_bounds__(256) void ns_prep_kernel(Table table, char* __restrict__ ws, float mu, int nesterov,
                                                       int parts, double eps, const float* __restrict__ skip, const double* __restrict__ partial) {
@@ -121,10 +129,10 @@ __global__ __launch_bounds__(256) void ns_prep_kernel(Table table, char* __restr
     __shared__ uint32_t tile[64][65];
     int first;
     const int k = find_mat(table, wPrep, blockIdx.x, first);
-    const Mat t = load_mat(table, k, ws);
+    const Mat t = load_mat(table, k, ws, 0);
     double s = 0.0;
     const int lane = threadIdx.x & 63, strand = threadIdx.x >> 6;
-    for (int p = lane; p < parts; p += 64) s += partial[(int64_t)k * kNormParts + p];
+    for (int p = lane; p < parts; p += 64) s += partial[(int64_t)k * parts + p];
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
     const float f = (float)((double)(1 << kScale) / (sqrt(s) + eps));
@@ -141,21 +149,19 @@ __global__ __launch_bounds__(256) void ns_prep_kernel(Table table, char* __restr
     }
     __syncthreads();
     const bool tall = t.rows > t.cols;
-    char* D = tall ? t.Xt0 : t.X;               // as the matrix lies: rows x cols
-    char* Dt = tall ? t.X : t.Xt0;              // transposed: cols x rows
-    const int64_t pd = tall ? t.pm : t.pn, pt = tall ? t.pn : t.pm;
+    const int64_t row0 = tall ? cb : rb, k0 = tall ? rb : cb;
     for (int u = threadIdx.x; u < 512; u += 256) {
         const int i = u >> 3, c8 = (u & 7) * 8;
+        if (row0 + i >= t.m || kbyte<2>(k0 + c8) >= t.pn) continue;
+        uint32_t w[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) w[j] = tall ? tile[c8 + j][i] : tile[i][c8 + j];
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
-            u32x4 a, ta;
+            u32x4 a;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                a[j] = (tile[i][c8 + 2 * j] >> 16 * q & 0xffffu) | tile[i][c8 + 2 * j + 1] >> 16 * q << 16;
-                ta[j] = (tile[c8 + 2 * j][i] >> 16 * q & 0xffffu) | tile[c8 + 2 * j + 1][i] >> 16 * q << 16;
-            }
-            if (rb + i < t.rows && kbyte<2>(cb + c8) < pd) *reinterpret_cast<u32x4*>(D + (rb + i) * pd + kbyte<2>(cb + c8, q)) = a;
-            if (cb + i < t.cols && kbyte<2>(rb + c8) < pt) *reinterpret_cast<u32x4*>(Dt + (cb + i) * pt + kbyte<2>(rb + c8, q)) = ta;
+            for (int j = 0; j < 4; ++j) a[j] = (w[2 * j] >> 16 * q & 0xffffu) | w[2 * j + 1] >> 16 * q << 16;
+            *reinterpret_cast<u32x4*>(t.X[0] + (row0 + i) * t.pn + kbyte<2>(k0 + c8, q)) = a;
         }
     }
 }
@@ -170,17 +176,17 @@ __device__ __forceinline__ void tri_tile(int q, int& ti, int& tj) {
 
 // POLY = false: A = X X^T.  POLY = true: P = a I + b A + c A A.
 template <class M, bool POLY>
-__global__ __launch_bounds__(M::NT, 2) void ns_gram_kernel(Table table, char* __restrict__ ws,
+__global__ __launch_bounds__(M::NT, 2) void ns_gram_kernel(Table table, char* __restrict__ ws, int from,
                                                         const float* __restrict__ skip) {
     if (skip != nullptr && skip[0] != 0.f) return;
     __shared__ __attribute__((aligned(16))) char lds[M::LDS];
     int first, ti, tj;
     const int tile = xcd_tile(blockIdx.x, gridDim.x);
-    const Mat t = load_mat(table, find_mat(table, wGram, tile, first), ws);
+    const Mat t = load_mat(table, find_mat(table, wGram, tile, first), ws, from);
     tri_tile(tile - first, ti, tj);
     const int a0 = ti * M::BM, b0 = tj * M::BN;
     const int64_t pitch = POLY ? t.pm : t.pn;
-    const Operand op = {POLY ? t.A : t.X, pitch, t.m};
+    const Operand op = {POLY ? t.A : t.X[0], pitch, t.m};
     f32x16 acc[M::TM][M::TN];
     M::zero(acc);
     M::run(op, a0, op, b0, 0, (int)(pitch / M::STEP), lds, acc);
@@ -234,7 +240,7 @@ struct Apply {                                    // the optimiser's half of the
     const double* lr_dev;
 };
 
-// X = P X: planes both ways round (from X^T number `from` to the other), or the last one: the result / the parameter's update
+// X = P X, from X number `from` to the other, or the last one: the result / the parameter's update
 template <class M, typename S, int LAST>          // LAST: 0 = planes, 1 = result, 2 = optimiser
 __global__ __launch_bounds__(M::NT, 2) void ns_update_kernel(Table table, char* __restrict__ ws, int from, Apply ap,
                                                           const float* __restrict__ skip) {
@@ -242,19 +248,18 @@ __global__ __launch_bounds__(M::NT, 2) void ns_update_kernel(Table table, char* 
     __shared__ __attribute__((aligned(16))) char lds[M::LDS];
     int first;
     const int tile = xcd_tile(blockIdx.x, gridDim.x);
-    const Mat t = load_mat(table, find_mat(table, wUpd, tile, first), ws);
+    const Mat t = load_mat(table, find_mat(table, wUpd, tile, first), ws, from);
     const int tm = (t.m + M::BM - 1) / M::BM, q = tile - first;
     const int a0 = q % tm * M::BM, b0 = q / tm * M::BN;
-    const Operand P = {t.P, t.pm, t.m}, Xt = {from ? t.Xt1 : t.Xt0, t.pm, t.n};
+    const Operand P = {t.P, t.pm, t.m}, X = {t.X[0], t.pn, t.m};
     f32x16 acc[M::TM][M::TN];
     M::zero(acc);
-    M::run(P, a0, Xt, b0, 0, (int)(t.pm / M::STEP), lds, acc);
+    M::run(P, a0, X, b0, 0, (int)(t.pm / M::STEP), lds, acc);
     constexpr float down = 1.f / (float)(1 << kScale);
     using W = WaveStore<M>;
     char* reg = W::region(lds);
     const int r0 = a0 + M::wave_row(), c0 = b0 + M::wave_col();
     if constexpr (LAST == 0) {
-        char* to = from ? t.Xt0 : t.Xt1;
 #pragma unroll
         for (int j = 0; j < M::TN; ++j) {
             const int c = b0 + M::bcol(j);
@@ -266,11 +271,8 @@ __global__ __launch_bounds__(M::NT, 2) void ns_update_kernel(Table table, char* 
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
             auto val = [&](int i, int j, int e) -> uint16_t { return plane16(acc[i][j][e], q); };
-            W::store_cols(reg, val, [&](int c, int r, u32x4 d) {
-                if (c0 + c < t.n && kbyte<2>(r0 + r) < t.pm) *reinterpret_cast<u32x4*>(to + (int64_t)(c0 + c) * t.pm + kbyte<2>(r0 + r, q)) = d;
-            });
             W::store_rows(reg, val, [&](int r, int c, u32x4 d) {
-                if (r0 + r < t.m && kbyte<2>(c0 + c) < t.pn) *reinterpret_cast<u32x4*>(t.X + (int64_t)(r0 + r) * t.pn + kbyte<2>(c0 + c, q)) = d;
+                if (r0 + r < t.m && kbyte<2>(c0 + c) < t.pn) *reinterpret_cast<u32x4*>(t.X[1] + (int64_t)(r0 + r) * t.pn + kbyte<2>(c0 + c, q)) = d;
             });
         }
         return;
@@ -310,9 +312,10 @@ __global__ __launch_bounds__(M::NT, 2) void ns_update_kernel(Table table, char* 
     }
 }
 
-using Big = MmTile<_Float16, 2, 256, 256, 2, 4, 2>;
-using Mid = MmTile<_Float16, 2, 128, 128, 2, 2, 2>;
-using Small = MmTile<_Float16, 2, 64, 64, 2, 2, 4>;
+template <bool TB> using Big = MmTile<_Float16, 2, 256, 256, 2, 4, 2, false, TB>;
+using Tri = MmTile<_Float16, 2, 192, 192, 3, 2, 3>;      // a triangle of tiles: 253 of them cover 4096 x 4096, one per CU
+template <bool TB> using Mid = MmTile<_Float16, 2, 128, 128, 2, 2, 2, false, TB>;
+template <bool TB> using Small = MmTile<_Float16, 2, 64, 64, 2, 2, 4, false, TB>;
 
 #define SSECG_NS_LAUNCH(M, kernel, grid, st, ...)                                                                               \
     do {                                                                                                                        \
@@ -323,40 +326,53 @@ using Small = MmTile<_Float16, 2, 64, 64, 2, 2, 4>;
 
 struct Plan {
     size_t bytes;
-    int prep, gram, upd, gramTile, updTile;       // workgroups of the launches and tile sides
+    int parts, prep, gram, upd, gramTile, updTile;       // workgroups of the launches and tile sides
 };
 
 template <bool POLY>
-int launch_gram(const Table& t, const Plan& p, char* ws, const float* skip, hipStream_t st) {
-    if (p.gramTile == 256) SSECG_NS_LAUNCH(Big, (ns_gram_kernel<Big, POLY>), p.gram, st, t, ws, skip);
-    else if (p.gramTile == 128) SSECG_NS_LAUNCH(Mid, (ns_gram_kernel<Mid, POLY>), p.gram, st, t, ws, skip);
-    else SSECG_NS_LAUNCH(Small, (ns_gram_kernel<Small, POLY>), p.gram, st, t, ws, skip);
+int launch_gram(const Table& t, const Plan& p, char* ws, int from, const float* skip, hipStream_t st) {
+#define SSECG_NS_GRAM(...) do { using M = __VA_ARGS__; SSECG_NS_LAUNCH(M, (ns_gram_kernel<M, POLY>), p.gram, st, t, ws, from, skip); } while (0)
+    if (p.gramTile == 256) SSECG_NS_GRAM(Big<false>);
+    else if (p.gramTile == 192) SSECG_NS_GRAM(Tri);
+    else if (p.gramTile == 128) SSECG_NS_GRAM(Mid<false>);
+    else SSECG_NS_GRAM(Small<false>);
+#undef SSECG_NS_GRAM
     return 0;
 }
 
 template <typename S, int LAST>
 int launch_update(const Table& t, const Plan& p, char* ws, int from, const Apply& ap, const float* skip, hipStream_t st) {
-    if (p.updTile == 256) SSECG_NS_LAUNCH(Big, (ns_update_kernel<Big, S, LAST>), p.upd, st, t, ws, from, ap, skip);
-    else if (p.updTile == 128) SSECG_NS_LAUNCH(Mid, (ns_update_kernel<Mid, S, LAST>), p.upd, st, t, ws, from, ap, skip);
-    else SSECG_NS_LAUNCH(Small, (ns_update_kernel<Small, S, LAST>), p.upd, st, t, ws, from, ap, skip);
+#define SSECG_NS_UPDATE(...) \
+    do { using M = __VA_ARGS__; SSECG_NS_LAUNCH(M, (ns_update_kernel<M, S, LAST>), p.upd, st, t, ws, from, ap, skip); } while (0)
+    if (p.updTile == 256) SSECG_NS_UPDATE(Big<true>);
+    else if (p.updTile == 128) SSECG_NS_UPDATE(Mid<true>);
+    else SSECG_NS_UPDATE(Small<true>);
+#undef SSECG_NS_UPDATE
     return 0;
 }
 
 // mats: host rows {source, result or parameter, momentum, rows, cols} of at most kMost matrices
 int make_plan(const int64_t* mats, int count, Table& t, Plan& p) {
-    auto tiles = [&](int64_t side, bool gram) {
-        int64_t s = 0;
+    // the tile side that mm_time expects to be fastest: the two products of a step over a triangle of tiles, the update over all
+    int64_t largest = 0;
+    auto time = [&](int side, bool gram) {
+        MmWork along, square, whole;
         for (int k = 0; k < count; ++k) {
             const int64_t a = mats[5 * k + 3], b = mats[5 * k + 4], m = a < b ? a : b, n = a < b ? b : a;
             const int64_t tm = (m + side - 1) / side, tn = (n + side - 1) / side;
-            s += gram ? tm * (tm + 1) / 2 : tm * tn;
+            along.add(tm * (tm + 1) / 2, (n + 31) / 32);
+            square.add(tm * (tm + 1) / 2, (m + 31) / 32);
+            whole.add(tm * tn, (m + 31) / 32);
+            largest = a * b > largest ? a * b : largest;
         }
-        return s;
+        return gram ? mm_time(side, 2, along) + mm_time(side, 2, square) : mm_time(side, 2, whole);
     };
-    // the largest tile that still gives each of the 256 CUs one
-    auto pick = [&](bool gram) { return tiles(256, gram) >= 256 ? 256 : (tiles(128, gram) >= 256 ? 128 : 64); };
-    p.gramTile = pick(true);
-    p.updTile = pick(false);
+    p.gramTile = p.updTile = 64;
+    for (int side : {128, 192, 256}) {
+        if (time(side, true) < time(p.gramTile, true)) p.gramTile = side;
+        if (side != 192 && time(side, false) < time(p.updTile, false)) p.updTile = side;
+    }
+    p.parts = (int)(largest / 8192 < 1 ? 1 : largest / 8192 > kNormParts ? kNormParts : largest / 8192);
     t.count = count;
     int64_t at = up((int64_t)kMost * kNormParts * 8, 256), prep = 0, gram = 0, upd = 0;
     for (int k = 0; k < kMost; ++k) {
@@ -393,12 +409,12 @@ int run_chain(const int64_t* mats, int count, float mu, int nesterov, int steps,
     int rc = make_plan(mats, count, t, p);
     if (rc != 0) return rc;
     double* partial = reinterpret_cast<double*>(ws);
-    hipLaunchKernelGGL((ns_norm_kernel<S, MUON>), dim3(kNormParts, count), dim3(256), 0, st, t, mu, nesterov, skip, partial);
-    hipLaunchKernelGGL((ns_prep_kernel<S, MUON>), dim3((unsigned)p.prep), dim3(256), 0, st, t, ws, mu, nesterov, kNormParts, eps, skip, partial);
+    hipLaunchKernelGGL((ns_norm_kernel<S, MUON>), dim3(p.parts, count), dim3(256), 0, st, t, mu, nesterov, skip, partial);
+    hipLaunchKernelGGL((ns_prep_kernel<S, MUON>), dim3((unsigned)p.prep), dim3(256), 0, st, t, ws, mu, nesterov, p.parts, eps, skip, partial);
     rc = (int)hipGetLastError();
     for (int k = 0; k < steps && rc == 0; ++k) {
-        if ((rc = launch_gram<false>(t, p, ws, skip, st)) != 0) break;
-        if ((rc = launch_gram<true>(t, p, ws, skip, st)) != 0) break;
+        if ((rc = launch_gram<false>(t, p, ws, k & 1, skip, st)) != 0) break;
+        if ((rc = launch_gram<true>(t, p, ws, k & 1, skip, st)) != 0) break;
         if (k + 1 < steps) rc = launch_update<S, 0>(t, p, ws, k & 1, ap, skip, st);
         else rc = launch_update<S, MUON ? 2 : 1>(t, p, ws, k & 1, ap, skip, st);
     }
