@@ -147,7 +147,7 @@ __device__ __forceinline__ void tile_of(int tilesA, int tilesB, int& ta, int& tb
 }
 
 template <class M>
-__device__ __forceinline__ void logits_tile(const LogitArgs& p, int a0, int b0, char* lds, f32x16 (&acc)[M::TM][M::TN]) {
+__device__ __forceinline__ bool logits_tile(const LogitArgs& p, int a0, int b0, char* lds, f32x16 (&acc)[M::TM][M::TN]) {
     int ex = 0;
     if constexpr (M::P == 2) {
         // every thread reads the parts itself (256 words, cached); the wave's maximum is the workgroup's
@@ -165,8 +165,7 @@ __device__ __forceinline__ void logits_tile(const LogitArgs& p, int a0, int b0, 
         }
         ex = -(scale_exp(mx) + scale_exp(mw));
     }
-    M::zero(acc);
-    M::run(p.W, a0, p.X, b0, 0, p.stages, lds, acc);
+    if (!M::run(p.W, a0, p.X, b0, 0, p.stages, lds, acc)) return false;
     if constexpr (M::P == 2) {
 #pragma unroll
         for (int i = 0; i < M::TM; ++i)
@@ -199,6 +198,7 @@ __device__ __forceinline__ void logits_tile(const LogitArgs& p, int a0, int b0, 
             }
     }
     __builtin_amdgcn_sched_barrier(0);
+    return true;
 }
 
 // the label of a position as an offset from the lane's first class: register (i, e) holds it where offset == 32 i + 8 (e / 4) + e % 4
@@ -216,7 +216,7 @@ __global__ __launch_bounds__(M::NT, 2) void ce_lse_kernel(LogitArgs p) {
     tile_of<M>(p.tilesV, p.tilesN, ta, tb);
     const int a0 = ta * M::BM, b0 = tb * M::BN;
     f32x16 acc[M::TM][M::TN];
-    logits_tile<M>(p, a0, b0, lds, acc);
+    if (!logits_tile<M>(p, a0, b0, lds, acc)) return;
     const int wm = (threadIdx.x >> 6) / M::WN, h = (threadIdx.x >> 5) & 1;
 #pragma unroll
     for (int j = 0; j < M::TN; ++j) {
@@ -347,7 +347,7 @@ __global__ __launch_bounds__(M::NT, 2) void ce_grad_kernel(LogitArgs p) {
     const int a0 = ta * M::BM, b0 = tb * M::BN;
     using T = typename M::T;
     f32x16 acc[M::TM][M::TN];
-    logits_tile<M>(p, a0, b0, lds, acc);
+    if (!logits_tile<M>(p, a0, b0, lds, acc)) return;
     const int lane = threadIdx.x & 63, wn = (threadIdx.x >> 6) % M::WN;
     float lse[M::TN], g[M::TN];
     int off[M::TN];
@@ -383,7 +383,7 @@ __global__ __launch_bounds__(M::NT, 2) void ce_grad_kernel(LogitArgs p) {
     }
     if (DB) {
         __syncthreads();
-        for (int r = threadIdx.x; r < M::BM; r += M::NT) {
+        for (int r = threadIdx.x; r < M::BM; r += M::NW * 64) {
             float sum = 0.f;
 #pragma unroll
             for (int k = 0; k < M::WN; ++k) sum += part[k * M::BM + r];
@@ -395,17 +395,14 @@ __global__ __launch_bounds__(M::NT, 2) void ce_grad_kernel(LogitArgs p) {
     using W = WaveStore<M>;
     char* reg = W::region(lds);
     const int v0 = a0 + M::wave_row(), n0 = b0 + M::wave_col();
-#pragma unroll
-    for (int q = 0; q < M::P; ++q) {
-        auto val = [&](int i, int j, int e) -> uint16_t {
-            if constexpr (M::P == 2) return plane16(acc[i][j][e], q);
-            else return bits16((T)acc[i][j][e]);
-        };
-        // the pitch covers the whole tile: no condition on the class
-        W::store_cols(reg, val, [&](int n, int v, u32x4 d) {
-            if (n0 + n < p.rowsE) *reinterpret_cast<u32x4*>(p.E + (n0 + n) * p.pitchE + kbyte<M::P>(v0 + v, q)) = d;
-        });
-    }
+    auto val = [&](int i, int j, int e, int q) -> uint16_t {
+        if constexpr (M::P == 2) return plane16(acc[i][j][e], q);
+        else return bits16((T)acc[i][j][e]);
+    };
+    // the pitch covers the whole tile: no condition on the class
+    W::template store_cols<M::P>(reg, val, [&](int n, int v, int q, u32x4 d) {
+        if (n0 + n < p.rowsE) *reinterpret_cast<u32x4*>(p.E + (n0 + n) * p.pitchE + kbyte<M::P>(v0 + v, q)) = d;
+    });
 }
 
 // ---------------------------------------------------------------- products with E
@@ -430,8 +427,7 @@ __global__ __launch_bounds__(M::NT, 2) void ce_prod_kernel(ProdArgs p) {
     const int a0 = ta * M::BM, b0 = tb * M::BN;
     const int z = blockIdx.y, s0 = (int)((int64_t)p.stages * z / p.splits), s1 = (int)((int64_t)p.stages * (z + 1) / p.splits);
     f32x16 acc[M::TM][M::TN];
-    M::zero(acc);
-    M::run(p.A, a0, p.B, b0, s0, s1 - s0, lds, acc);
+    if (!M::run(p.A, a0, p.B, b0, s0, s1 - s0, lds, acc)) return;
     int ex = -kEScale;
     float f = 0.f;
     if (!p.plane) {
@@ -451,8 +447,8 @@ __global__ __launch_bounds__(M::NT, 2) void ce_prod_kernel(ProdArgs p) {
         if (!plane) {
             using W = WaveStore<M>;
             const int r0 = a0 + M::wave_row(), c0 = b0 + M::wave_col();
-            W::store_rows(W::region(lds), [&](int i, int j, int e) -> uint16_t { return bits16(finish<O>(acc[i][j][e], f, ex)); },
-                          [&](int r, int c, u32x4 d) {
+            W::template store_rows<1>(W::region(lds), [&](int i, int j, int e, int) -> uint16_t { return bits16(finish<O>(acc[i][j][e], f, ex)); },
+                          [&](int r, int c, int, u32x4 d) {
                               if (r0 + r < p.rows && c0 + c < p.cols)
                                   store_vec(reinterpret_cast<O*>(p.out) + (int64_t)(r0 + r) * p.cols, c0 + c, p.cols,
                                             __builtin_bit_cast(typename Vec<O>::type, d));
@@ -512,8 +508,8 @@ template <typename S> struct Inner { using T = S; static constexpr int P = 1; };
 template <> struct Inner<float> { using T = _Float16; static constexpr int P = 2; };
 
 template <typename T, int P, bool TA = false, bool TB = false> using Big = MmTile<T, P, 256, 256, 2, 4, 2, TA, TB>;
-template <typename T, int P, bool TA = false, bool TB = false> using Mid = MmTile<T, P, 128, 128, 2, 2, 2, TA, TB>;
-template <typename T, int P, bool TA = false, bool TB = false> using Small = MmTile<T, P, 64, 64, 2, 2, 4, TA, TB>;
+template <typename T, int P, bool TA = false, bool TB = false, int KG = 1> using Mid = MmTile<T, P, 128, 128, 2, 2, 2, TA, TB, KG>;
+template <typename T, int P, bool TA = false, bool TB = false, int KG = 1> using Small = MmTile<T, P, 64, 64, 2, 2, 4, TA, TB, KG>;
 
 inline int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
@@ -561,36 +557,40 @@ Packed plan_packed(void* base, const void* x, const void* w, int dtype, int64_t 
 
 inline int64_t tiles_of(int64_t n, int side) { return (n + side - 1) / side; }
 
-// the tile side (256, 128, 64) of a product of a x b tiles with `stages` stages, and how many workgroups share the k of a tile
-struct Choice { int side, splits; };
+// the tile side (256, 128, 64) of a product of a x b results with `stages` stages, and how many workgroups and how many groups of a
+// workgroup's waves share the k of a tile
+struct Choice { int side, splits, groups; };
 inline Choice choose(int64_t a, int64_t b, int64_t stages, int P, bool split) {
-    Choice best = {256, 1};
+    Choice best = {256, 1, 1};
     double least = 0.0;
     for (int side = 256; side >= 64; side /= 2)
         for (int s = 1; s <= (split ? 64 : 1) && (s == 1 || stages / s >= 4); s += s < 8 ? 1 : s < 16 ? 2 : 8) {
             MmWork w;
             w.add(tiles_of(a, side) * tiles_of(b, side) * s, (stages + s - 1) / s);
-            // the planes of the parts are written and read again (4 TB/s), and a launch sums them
-            const double t = mm_time(side, P, w) + (s > 1 ? 4.0 + (double)a * b * s * 8 / 4e6 : 0.0);
-            if (least == 0.0 || t < least) {
-                least = t;
-                best = {side, s};
+            for (int g = 1; g <= (side < 256 ? 2 : 1); ++g) {
+                // the planes of the parts are written and read again (4 TB/s), and a launch sums them
+                const double t = mm_time(side, P, w, g) + (s > 1 ? 4.0 + (double)a * b * s * 8 / 4e6 : 0.0);
+                if (least == 0.0 || t < least) {
+                    least = t;
+                    best = {side, s, g};
+                }
             }
         }
     return best;
 }
 
 struct FwdPlan {
-    int side, tilesV, tilesN, parts;
+    Choice c;
+    int tilesV, tilesN, parts;
     float *pm, *ps, *tl, *row;
 };
 
 FwdPlan plan_fwd(Blob& ws, int dtype, int64_t N, int64_t C, int64_t V) {
     FwdPlan p;
     const int P = dtype == kF32 ? 2 : 1;
-    p.side = choose(V, N, up(C, 64) * P / 64, P, false).side;
-    p.tilesV = (int)tiles_of(V, p.side);
-    p.tilesN = (int)tiles_of(N, p.side);
+    p.c = choose(V, N, up(C, 64) * P / 64, P, false);
+    p.tilesV = (int)tiles_of(V, p.c.side);
+    p.tilesN = (int)tiles_of(N, p.c.side);
     p.parts = p.tilesV * 2;                      // two waves of a tile along the classes
     p.pm = ws.take<float>((size_t)p.parts * N);
     p.ps = ws.take<float>((size_t)p.parts * N);
@@ -617,6 +617,16 @@ int pack(const void* src, int64_t R, int64_t C, const Counts& counts, const floa
         hipLaunchKernelGGL(kernel, grid, dim3(M::NT), 0, st, args);                                                        \
         const int rc_ = (int)hipGetLastError();                                                                                 \
         if (rc_ != 0) return rc_;                                                                                               \
+    } while (0)
+
+// the tile of a choice
+#define SSECG_CE_TILES(c, WITH, TA, TB)                                                \
+    do {                                                                               \
+        if ((c).side == 256) WITH(Big<T, P, TA, TB>);                                  \
+        else if ((c).side == 128 && (c).groups == 2) WITH(Mid<T, P, TA, TB, 2>);       \
+        else if ((c).side == 128) WITH(Mid<T, P, TA, TB>);                             \
+        else if ((c).groups == 2) WITH(Small<T, P, TA, TB, 2>);                        \
+        else WITH(Small<T, P, TA, TB>);                                                \
     } while (0)
 
 template <typename S>
@@ -646,10 +656,8 @@ int ce_fwd(const void* x, const void* w, const float* bias, const int64_t* targe
     a.stages = (int)(k.pitch / 128);
     a.target = target; a.v0 = 0;
     a.pm = p.pm; a.ps = p.ps; a.tl = p.tl;
-#define SSECG_CE_LSE(TILE) do { using M = TILE<T, P>; SSECG_CE_LAUNCH(M, ce_lse_kernel<M>, dim3(p.tilesV * p.tilesN), st, a); } while (0)
-    if (p.side == 256) SSECG_CE_LSE(Big);
-    else if (p.side == 128) SSECG_CE_LSE(Mid);
-    else SSECG_CE_LSE(Small);
+#define SSECG_CE_LSE(...) do { using M = __VA_ARGS__; SSECG_CE_LAUNCH(M, ce_lse_kernel<M>, dim3(p.tilesV * p.tilesN), st, a); } while (0)
+    SSECG_CE_TILES(p.c, SSECG_CE_LSE, false, false);
 #undef SSECG_CE_LSE
     float* row = reduction == 0 ? loss : p.row;
     hipLaunchKernelGGL(ce_join_kernel, dim3((unsigned)((N + 15) / 16)), dim3(1024), 0, st, p.pm, p.ps, p.tl, p.parts, (int)N, (int)V, target, counts,
@@ -664,8 +672,7 @@ constexpr size_t kPieceBytes = (size_t)1 << 30;  // of E
 struct BwdPlan {
     int64_t Vc, rowsE, pitchE;                   // classes per piece (a multiple of 256 unless there is one piece); E's rows and bytes
     int pieces;
-    int sideL;
-    Choice cx, cw;                               // dx, dw
+    Choice cl, cx, cw;                           // E, dx, dw
     float *coef, *fscale, *pdb, *planeX, *planeW;
     char *Xg, *E;
 };
@@ -681,12 +688,12 @@ BwdPlan plan_bwd(Blob& ws, int dtype, int64_t N, int64_t C, int64_t V, bool want
     p.Vc = pieces == 1 ? V : up((V + pieces - 1) / pieces, 256);
     p.pieces = (int)((V + p.Vc - 1) / p.Vc);
     p.pitchE = up(p.Vc, 256) * 2 * P;
-    p.sideL = choose(p.Vc, N, up(C, 64) * P / 64, P, false).side;
+    p.cl = choose(p.Vc, N, up(C, 64) * P / 64, P, false);
     p.cx = choose(N, C, up(p.Vc, BK) / BK, P, true);
     p.cw = choose(p.Vc, C, up(N, BK) / BK, P, true);
     p.coef = ws.take<float>((size_t)N);
     p.fscale = ws.take<float>(1);
-    p.pdb = ws.take<float>(want_b ? (size_t)(tiles_of(N, p.sideL) * p.Vc) : 0);
+    p.pdb = ws.take<float>(want_b ? (size_t)(tiles_of(N, p.cl.side) * p.Vc) : 0);
     p.planeX = ws.take<float>(want_x && (p.cx.splits > 1 || p.pieces > 1) ? (size_t)p.cx.splits * N * C : 0);
     p.planeW = ws.take<float>(want_w && p.cw.splits > 1 ? (size_t)p.cw.splits * p.Vc * C : 0);
     p.Xg = ws.take<char>(want_w && x_direct ? (size_t)(N * C * 2) : 0);
@@ -695,14 +702,12 @@ BwdPlan plan_bwd(Blob& ws, int dtype, int64_t N, int64_t C, int64_t V, bool want
 }
 
 template <typename S, bool TA>
-int product(const ProdArgs& q, int side, hipStream_t st) {
+int product(const ProdArgs& q, const Choice& c, hipStream_t st) {
     using T = typename Inner<S>::T;
     constexpr int P = Inner<S>::P;
     const dim3 grid((unsigned)(q.tilesA * q.tilesB), (unsigned)q.splits);
-#define SSECG_CE_PROD(TILE) do { using M = TILE<T, P, TA, true>; SSECG_CE_LAUNCH(M, (ce_prod_kernel<M, S>), grid, st, q); } while (0)
-    if (side == 256) SSECG_CE_PROD(Big);
-    else if (side == 128) SSECG_CE_PROD(Mid);
-    else SSECG_CE_PROD(Small);
+#define SSECG_CE_PROD(...) do { using M = __VA_ARGS__; SSECG_CE_LAUNCH(M, (ce_prod_kernel<M, S>), grid, st, q); } while (0)
+    SSECG_CE_TILES(c, SSECG_CE_PROD, TA, true);
 #undef SSECG_CE_PROD
     return 0;
 }
@@ -736,22 +741,20 @@ int ce_bwd(const float* dloss, const void* x, const void* w, const float* bias, 
         a.bias = bias ? bias + v0 : nullptr;
         a.amaxX = k.amaxX; a.amaxW = k.amaxW;
         a.V = (int)vn; a.N = (int)N;
-        a.tilesV = (int)tiles_of(vn, p.sideL); a.tilesN = (int)tiles_of(N, p.sideL);
+        a.tilesV = (int)tiles_of(vn, p.cl.side); a.tilesN = (int)tiles_of(N, p.cl.side);
         a.stages = (int)(k.pitch / 128);
         a.target = target; a.v0 = v0;
         a.lse = lse; a.gate = gate; a.coef = reduction == 0 ? p.coef : nullptr;
         a.E = dx || dw ? p.E : nullptr; a.pitchE = p.pitchE; a.rowsE = (int)p.rowsE;
         a.pdb = p.pdb;
         const dim3 grid(a.tilesV * a.tilesN);
-#define SSECG_CE_GRAD(TILE)                                                             \
+#define SSECG_CE_GRAD(...)                                                              \
     do {                                                                                \
-        using M = TILE<T, P>;                                                           \
+        using M = __VA_ARGS__;                                                          \
         if (db) SSECG_CE_LAUNCH(M, (ce_grad_kernel<M, true>), grid, st, a);             \
         else SSECG_CE_LAUNCH(M, (ce_grad_kernel<M, false>), grid, st, a);               \
     } while (0)
-        if (p.sideL == 256) SSECG_CE_GRAD(Big);
-        else if (p.sideL == 128) SSECG_CE_GRAD(Mid);
-        else SSECG_CE_GRAD(Small);
+        SSECG_CE_TILES(p.cl, SSECG_CE_GRAD, false, false);
 #undef SSECG_CE_GRAD
         if (db) hipLaunchKernelGGL(ce_db_kernel, dim3((unsigned)((vn + 255) / 256)), dim3(256), 0, st, p.pdb, a.tilesN, (int)vn, f, db + v0);
         if (dx) {                                // E along its rows, W across
@@ -763,7 +766,7 @@ int ce_bwd(const float* dloss, const void* x, const void* w, const float* bias, 
             q.stages = (int)(up(vn, BK) / BK); q.splits = p.cx.splits;
             q.plane = p.cx.splits > 1 || p.pieces > 1 ? p.planeX : nullptr;
             q.add = i > 0; q.out = dx; q.amax = k.amaxW; q.f = f;
-            if ((rc = product<S, false>(q, p.cx.side, st)) != 0) return rc;
+            if ((rc = product<S, false>(q, p.cx, st)) != 0) return rc;
         }
         if (dw) {                                // both across
             ProdArgs q = {};
@@ -774,7 +777,7 @@ int ce_bwd(const float* dloss, const void* x, const void* w, const float* bias, 
             q.stages = (int)(up(N, BK) / BK); q.splits = p.cw.splits;
             q.plane = p.cw.splits > 1 ? p.planeW : nullptr;
             q.out = (S*)dw + v0 * C; q.amax = k.amaxX; q.f = f;
-            if ((rc = product<S, true>(q, p.cw.side, st)) != 0) return rc;
+            if ((rc = product<S, true>(q, p.cw, st)) != 0) return rc;
             if (q.plane)
                 hipLaunchKernelGGL((ce_sum_planes_kernel<S>), dim3(grid_for(vn * C)), dim3(256), 0, st, p.planeW, p.cw.splits, vn * C,
                                    P == 2 ? k.amaxX : nullptr, f, (S*)dw + v0 * C);

@@ -17,6 +17,9 @@
 // BK rows of the tile's indices; ds_read_b64_tr_b16 gives a lane 4 consecutive k of its index, so two of them are a fragment.  The
 // chunks of a row are permuted by its row so that the 8 rows of a read fall into different banks.
 //
+// KG groups of waves, each with a ring of its own, may share a tile's k (group g takes its g-th share of the stages): half the chain
+// of stages where there are too few tiles to fill the chip.  Their sums are joined in LDS, and the first group goes on alone.
+//
 // Bounds: an index beyond a k-fast operand is clamped to its last row, a chunk beyond a k-slow one to its row's last chunk (the
 // caller masks the result).  k-fast operands are padded with zeros to a whole stage; of a k-slow operand rows beyond the last are
 // read as the last one, and the other operand holds zeros there.  Offsets within a tile are 32 bits: 256 pitch < 2^32.
@@ -62,20 +65,20 @@ template <> struct Frag<_Float16> {
     static __device__ __forceinline__ f32x16 mfma(type a, type b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 };
 
-template <typename T_, int P_, int BM_, int BN_, int WM_, int WN_, int R_, bool TA_ = false, bool TB_ = false>
+template <typename T_, int P_, int BM_, int BN_, int WM_, int WN_, int R_, bool TA_ = false, bool TB_ = false, int KG_ = 1>
 struct MmTile {
     using T = T_;
     using F = Frag<T>;
     using V8 = typename F::type;
     static constexpr int P = P_, BM = BM_, BN = BN_, WM = WM_, WN = WN_, R = R_;
     static constexpr bool TA = TA_, TB = TB_;
-    static constexpr int NW = WM * WN, NT = NW * 64;
+    static constexpr int KG = KG_, NW = WM * WN, NT = KG * NW * 64;   // waves of a group, threads of the workgroup
     static constexpr int TM = BM / WM / 32, TN = BN / WN / 32;
     static constexpr int BK = P == 1 ? 64 : 32;                 // k of a stage
     static constexpr int STEP = 128;                            // bytes of a k-fast row in a stage
     static constexpr int PA = BM / 8 / NW, PB = BN / 8 / NW, PPW = PA + PB;   // 1 KB pieces (8 rows) per wave and stage
     static constexpr int SLOT = (BM + BN) * 128;
-    static constexpr int LDS = R * SLOT;
+    static constexpr int LDS = KG * R * SLOT;
     static_assert(PA * NW * 8 == BM && PB * NW * 8 == BN, "every wave requests the same number of pieces");
     static_assert(R >= 2 && (R - 2) * PPW <= 63, "vmcnt counts to 63");
 
@@ -163,10 +166,49 @@ struct MmTile {
         }
     };
 
-    // acc += the tile at indices a0 of A and b0 of B over stages [s0, s0 + n); all waves of the workgroup call it together
-    static __device__ __forceinline__ void run(const Operand& A, int a0, const Operand& B, int b0, int s0, int n, char* lds,
+    // acc = the tile at indices a0 of A and b0 of B over stages [s0, s0 + n); all waves of the workgroup call it together.  False for
+    // the waves of the groups that are done: the tile is in the others' accumulators.
+    static __device__ __forceinline__ bool run(const Operand& A, int a0, const Operand& B, int b0, int s0, int n, char* lds,
                                                f32x16 (&acc)[TM][TN]) {
-        const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        zero(acc);
+        if constexpr (KG == 1) {
+            sweep(A, a0, B, b0, s0, n, n, lds, acc);
+            return true;
+        } else {
+            const int group = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) / NW, share = (n + KG - 1) / KG;
+            const int from = group * share < n ? group * share : n, to = from + share < n ? from + share : n;
+            sweep(A, a0, B, b0, s0 + from, to - from, share, lds + group * (R * SLOT), acc);
+            // one group after the other leaves its sums in LDS, element-wise in lane order (no bank conflict)
+            float* x = reinterpret_cast<float*>(lds) + (threadIdx.x & (NW * 64 - 1));
+#pragma unroll
+            for (int g = 1; g < KG; ++g) {
+                if (group == g) {
+#pragma unroll
+                    for (int i = 0; i < TM; ++i)
+#pragma unroll
+                        for (int j = 0; j < TN; ++j)
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) x[((i * TN + j) * 16 + e) * (NW * 64)] = acc[i][j][e];
+                }
+                __syncthreads();
+                if (group == 0) {
+#pragma unroll
+                    for (int i = 0; i < TM; ++i)
+#pragma unroll
+                        for (int j = 0; j < TN; ++j)
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) acc[i][j][e] += x[((i * TN + j) * 16 + e) * (NW * 64)];
+                }
+                __syncthreads();
+            }
+            return group == 0;
+        }
+    }
+
+    // a group's sweep over its n stages from s0; `most`: the stages of the largest group, whose barriers all waves meet
+    static __device__ __forceinline__ void sweep(const Operand& A, int a0, const Operand& B, int b0, int s0, int n, int most, char* lds,
+                                                 f32x16 (&acc)[TM][TN]) {
+        const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % NW;
         const int wm = wave / WN, wn = wave % WN, r = lane & 31, h = lane >> 5;
         const unsigned ldsbase = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
         Loader<BM, PA, TA> la(A, a0, s0, lane, wave, ldsbase);
@@ -217,9 +259,9 @@ struct MmTile {
                     for (int j = 0; j < TN; ++j)
                         acc[i][j] = F::mfma(a[set][q == 0 ? P - 1 : 0][i], b[set][q == 1 ? P - 1 : 0][j], acc[i][j]);
         };
-        if (n > 0) {
-            stage_wait<R - 2>(n - 1 < R - 2 ? n - 1 : R - 2);
-            if (AHEAD) frags(0, 0, 0);
+        if (most > 0) {
+            stage_wait<R - 2>(n < 1 ? 0 : n - 1 < R - 2 ? n - 1 : R - 2);
+            if (AHEAD && n > 0) frags(0, 0, 0);
         }
         int slot = 0;
         for (int s = 0; s < n; ++s) {
@@ -244,6 +286,7 @@ struct MmTile {
             }
             slot = next;
         }
+        for (int s = n < 1 ? 1 : n; s < most; ++s) __builtin_amdgcn_s_barrier();   // (a group with fewer stages)
         // LDS may be reused by the caller behind this point (every wave has read its last stage)
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     }
@@ -258,10 +301,10 @@ struct MmTile {
     }
     // element e of acc[i][j] is row a0 + arow(i, e), column b0 + bcol(j)
     static __device__ __forceinline__ int arow(int i, int e) {
-        const int lane = threadIdx.x & 63, wm = (threadIdx.x >> 6) / WN;
+        const int lane = threadIdx.x & 63, wm = (threadIdx.x >> 6) % NW / WN;
         return wm * TM * 32 + i * 32 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
     }
-    static __device__ __forceinline__ int wave_row() { return (__builtin_amdgcn_readfirstlane(threadIdx.x >> 6) / WN) * TM * 32; }
+    static __device__ __forceinline__ int wave_row() { return (__builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % NW / WN) * TM * 32; }
     static __device__ __forceinline__ int wave_col() { return (__builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % WN) * TN * 32; }
     static __device__ __forceinline__ int bcol(int j) {
         const int lane = threadIdx.x & 63, wn = (threadIdx.x >> 6) % WN;
@@ -272,58 +315,66 @@ struct MmTile {
 // The wave's tile as 16-bit values, 16 bytes a lane, through a region of LDS that only this wave uses (after MmTile::run): an
 // accumulator's lanes run along B and its registers along A, so stores straight from it would be 2 bytes a lane (along B) or 8
 // bytes to 32 different rows (along A).
-//   store_rows: rows of A's index, B's index fastest;  dst(row, first column, 8 values), row and column relative to the wave's tile
-//   store_cols: rows of B's index, A's index fastest;  dst(column, first row, 8 values)
+//   store_rows: rows of A's index, B's index fastest;  dst(row, first column, plane, 8 values), row and column of the wave's tile
+//   store_cols: rows of B's index, A's index fastest;  dst(column, first row, plane, 8 values)
+// val(i, j, e, plane) is the value of an accumulator.
 template <class M> struct WaveStore {
-    static constexpr int SI = M::TM > 1 ? 2 : 1;                          // 32-row blocks that store_cols takes at a time
+    static constexpr int SI = M::TM % 2 == 0 ? 2 : 1;                     // 32-row blocks that store_cols takes at a time
     static constexpr int PC = SI * 64 + 16, PR = M::TN * 64 + 16;         // bytes of a row in LDS; the pad spreads the banks
     static constexpr int BYTES = M::TN * 32 * PC > 32 * PR ? M::TN * 32 * PC : 32 * PR;
     static_assert(M::NW * BYTES <= M::LDS, "the regions of all waves fit the tile's LDS");
 
     static __device__ __forceinline__ char* region(char* lds) { return lds + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * BYTES; }
-    static __device__ __forceinline__ void fence() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
-
-    template <typename VAL, typename DST> static __device__ __forceinline__ void store_rows(char* reg, VAL val, DST dst) {
-        const int lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5;
-#pragma unroll
-        for (int i = 0; i < M::TM; ++i) {
-#pragma unroll
-            for (int e = 0; e < 16; ++e)
-#pragma unroll
-                for (int j = 0; j < M::TN; ++j)
-                    *reinterpret_cast<uint16_t*>(reg + (8 * (e >> 2) + 4 * h + (e & 3)) * PR + (j * 32 + r) * 2) = val(i, j, e);
-            fence();
-#pragma unroll
-            for (int q = 0; q < M::TN * 2; ++q) {
-                const int at = q * 64 + lane, row = at / (M::TN * 4), c = at % (M::TN * 4);
-                dst(i * 32 + row, c * 8, *reinterpret_cast<const u32x4*>(reg + row * PR + c * 16));
-            }
-            fence();
-        }
+    static __device__ __forceinline__ void fence() {   // the sched_barrier keeps the next strip's conversions out of this one's registers
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
     }
-    template <typename VAL, typename DST> static __device__ __forceinline__ void store_cols(char* reg, VAL val, DST dst) {
+
+    template <int PLANES, typename VAL, typename DST> static __device__ __forceinline__ void store_rows(char* reg, VAL val, DST dst) {
         const int lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5;
 #pragma unroll
-        for (int i0 = 0; i0 < M::TM; i0 += SI) {
+        for (int i = 0; i < M::TM; ++i)
 #pragma unroll
-            for (int i = 0; i < SI; ++i)
+            for (int p = 0; p < PLANES; ++p) {
 #pragma unroll
-                for (int j = 0; j < M::TN; ++j)
+                for (int e = 0; e < 16; ++e)
 #pragma unroll
-                    for (int g = 0; g < 4; ++g) {
-                        u32x2 v;
-                        v[0] = (unsigned)val(i0 + i, j, 4 * g) | (unsigned)val(i0 + i, j, 4 * g + 1) << 16;
-                        v[1] = (unsigned)val(i0 + i, j, 4 * g + 2) | (unsigned)val(i0 + i, j, 4 * g + 3) << 16;
-                        *reinterpret_cast<u32x2*>(reg + (j * 32 + r) * PC + (i * 32 + 8 * g + 4 * h) * 2) = v;
-                    }
-            fence();
+                    for (int j = 0; j < M::TN; ++j)
+                        *reinterpret_cast<uint16_t*>(reg + (8 * (e >> 2) + 4 * h + (e & 3)) * PR + (j * 32 + r) * 2) = val(i, j, e, p);
+                fence();
 #pragma unroll
-            for (int q = 0; q < M::TN * 2 * SI; ++q) {
-                const int at = q * 64 + lane, row = at / (SI * 4), c = at % (SI * 4);
-                dst(row, i0 * 32 + c * 8, *reinterpret_cast<const u32x4*>(reg + row * PC + c * 16));
+                for (int q = 0; q < M::TN * 2; ++q) {
+                    const int at = q * 64 + lane, row = at / (M::TN * 4), c = at % (M::TN * 4);
+                    dst(i * 32 + row, c * 8, p, *reinterpret_cast<const u32x4*>(reg + row * PR + c * 16));
+                }
+                fence();
             }
-            fence();
-        }
+    }
+    template <int PLANES, typename VAL, typename DST> static __device__ __forceinline__ void store_cols(char* reg, VAL val, DST dst) {
+        const int lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5;
+#pragma unroll
+        for (int i0 = 0; i0 < M::TM; i0 += SI)
+#pragma unroll
+            for (int p = 0; p < PLANES; ++p) {
+#pragma unroll
+                for (int i = 0; i < SI; ++i)
+#pragma unroll
+                    for (int j = 0; j < M::TN; ++j)
+#pragma unroll
+                        for (int g = 0; g < 4; ++g) {
+                            u32x2 v;
+                            v[0] = (unsigned)val(i0 + i, j, 4 * g, p) | (unsigned)val(i0 + i, j, 4 * g + 1, p) << 16;
+                            v[1] = (unsigned)val(i0 + i, j, 4 * g + 2, p) | (unsigned)val(i0 + i, j, 4 * g + 3, p) << 16;
+                            *reinterpret_cast<u32x2*>(reg + (j * 32 + r) * PC + (i * 32 + 8 * g + 4 * h) * 2) = v;
+                        }
+                fence();
+#pragma unroll
+                for (int q = 0; q < M::TN * 2 * SI; ++q) {
+                    const int at = q * 64 + lane, row = at / (SI * 4), c = at % (SI * 4);
+                    dst(row, i0 * 32 + c * 8, p, *reinterpret_cast<const u32x4*>(reg + row * PC + c * 16));
+                }
+                fence();
+            }
     }
 };
 
@@ -338,13 +389,17 @@ struct MmWork {
         longest = longest < per ? per : longest;
     }
 };
-inline double mm_time(int side, int planes, const MmWork& w) {
+// groups: two groups of waves take a tile's stages in pairs (one workgroup a CU): a pair takes 1.25 us at a side of 128 with two
+// planes and 0.42 us at 64 (ResNet18's matrices, A = X X^T over 240 tiles of 64 and 48 stages: 16 us against 21).
+inline double mm_time(int side, int planes, const MmWork& w, int groups = 1) {
     const bool two = planes == 2;
     const double full = side == 256 ? (two ? 2.4 : 1.87) : side == 192 ? (two ? 1.4 : 1.1) : side == 128 ? (two ? 1.34 : 1.2) : (two ? 0.46 : 0.39);
     const double alone = side == 256 ? (two ? 1.9 : 1.5) : side == 192 ? (two ? 1.2 : 0.9) : side == 128 ? (two ? 0.75 : 0.6) : 0.3;
-    const int64_t slots = side > 128 ? 256 : 512;
+    const double pair = side == 128 ? (two ? 1.25 : 1.1) : (two ? 0.42 : 0.36);
+    const int64_t slots = side > 128 || groups == 2 ? 256 : 512;
+    const double rounds = (double)((w.tiles + slots - 1) / slots), mean = w.tiles ? (double)w.stages / (double)w.tiles : 0.0;
+    if (groups == 2) return 4.0 + (rounds <= 1.0 ? (w.longest + 1) / 2 * pair : rounds * (mean * 0.5 * pair + 1.0));
     if (w.tiles <= 256) return 3.0 + w.longest * alone;
-    const double rounds = (double)((w.tiles + slots - 1) / slots), mean = (double)w.stages / (double)w.tiles;
     const double busy = rounds * mean * full, chain = w.longest * alone;
     return 3.0 + (busy > chain ? busy : chain);
 }

@@ -12,6 +12,8 @@
 // Precision: the iteration multiplies errors along weak directions by up to a = 3.44 per step (485 over five), so 16-bit iterates
 // would lose them.  All matrices are two fp16 planes times 2^13 - singular values stay below 1.21 and P's below 3.45, far inside
 // fp16's range, and an entry keeps 22 bits down to 2^-16 of the largest possible one - with fp32 accumulators.
+#include <initializer_list>
+#include <utility>
 #include "mm_core.h"
 #include "ssecg.h"
 
@@ -176,7 +178,7 @@ __device__ __forceinline__ void tri_tile(int q, int& ti, int& tj) {
 
 // POLY = false: A = X X^T.  POLY = true: P = a I + b A + c A A.
 template <class M, bool POLY>
-__global__ __launch_bounds__(M::NT, 2) void ns_gram_kernel(Table table, char* __restrict__ ws, int from,
+__global__ __launch_bounds__(M::NT, M::TM * M::TN > 8 ? 1 : 2) void ns_gram_kernel(Table table, char* __restrict__ ws, int from,
                                                         const float* __restrict__ skip) {
     if (skip != nullptr && skip[0] != 0.f) return;
     __shared__ __attribute__((aligned(16))) char lds[M::LDS];
@@ -188,8 +190,7 @@ __global__ __launch_bounds__(M::NT, 2) void ns_gram_kernel(Table table, char* __
     const int64_t pitch = POLY ? t.pm : t.pn;
     const Operand op = {POLY ? t.A : t.X[0], pitch, t.m};
     f32x16 acc[M::TM][M::TN];
-    M::zero(acc);
-    M::run(op, a0, op, b0, 0, (int)(pitch / M::STEP), lds, acc);
+    if (!M::run(op, a0, op, b0, 0, (int)(pitch / M::STEP), lds, acc)) return;
     char* out = POLY ? t.P : t.A;
     constexpr float down = 1.f / (float)(1 << kScale);
 #pragma unroll
@@ -222,16 +223,13 @@ __global__ __launch_bounds__(M::NT, 2) void ns_gram_kernel(Table table, char* __
     using W = WaveStore<M>;
     char* reg = W::region(lds);
     const int r0 = a0 + M::wave_row(), c0 = b0 + M::wave_col();
-#pragma unroll
-    for (int q = 0; q < 2; ++q) {
-        auto val = [&](int i, int j, int e) -> uint16_t { return plane16(acc[i][j][e], q); };
-        auto put = [&](int r, int c, u32x4 d) {
-            if (r < t.m && kbyte<2>(c) < t.pm) *reinterpret_cast<u32x4*>(out + (int64_t)r * t.pm + kbyte<2>(c, q)) = d;
-        };
-        W::store_rows(reg, val, [&](int r, int c, u32x4 d) { put(r0 + r, c0 + c, d); });
-        // below the diagonal: the mirrored tile as well
-        if (ti != tj) W::store_cols(reg, val, [&](int c, int r, u32x4 d) { put(c0 + c, r0 + r, d); });
-    }
+    auto val = [&](int i, int j, int e, int q) -> uint16_t { return plane16(acc[i][j][e], q); };
+    auto put = [&](int r, int c, int q, u32x4 d) {
+        if (r < t.m && kbyte<2>(c) < t.pm) *reinterpret_cast<u32x4*>(out + (int64_t)r * t.pm + kbyte<2>(c, q)) = d;
+    };
+    W::template store_rows<2>(reg, val, [&](int r, int c, int q, u32x4 d) { put(r0 + r, c0 + c, q, d); });
+    // below the diagonal: the mirrored tile as well
+    if (ti != tj) W::template store_cols<2>(reg, val, [&](int c, int r, int q, u32x4 d) { put(c0 + c, r0 + r, q, d); });
 }
 
 struct Apply {                                    // the optimiser's half of the last product
@@ -240,9 +238,13 @@ struct Apply {                                    // the optimiser's half of the
     const double* lr_dev;
 };
 
+__device__ __forceinline__ double update_scale(const Mat& t, int adjust) {
+    return adjust == 1 ? 0.2 * sqrt((double)t.n) : sqrt(t.rows > t.cols ? (double)t.rows / (double)t.cols : 1.0);
+}
+
 // X = P X, from X number `from` to the other, or the last one: the result / the parameter's update
 template <class M, typename S, int LAST>          // LAST: 0 = planes, 1 = result, 2 = optimiser
-__global__ __launch_bounds__(M::NT, 2) void ns_update_kernel(Table table, char* __restrict__ ws, int from, Apply ap,
+__global__ __launch_bounds__(M::NT, M::TM * M::TN > 8 ? 1 : 2) void ns_update_kernel(Table table, char* __restrict__ ws, int from, Apply ap,
                                                           const float* __restrict__ skip) {
     if (skip != nullptr && skip[0] != 0.f) return;
     __shared__ __attribute__((aligned(16))) char lds[M::LDS];
@@ -253,8 +255,7 @@ __global__ __launch_bounds__(M::NT, 2) void ns_update_kernel(Table table, char* 
     const int a0 = q % tm * M::BM, b0 = q / tm * M::BN;
     const Operand P = {t.P, t.pm, t.m}, X = {t.X[0], t.pn, t.m};
     f32x16 acc[M::TM][M::TN];
-    M::zero(acc);
-    M::run(P, a0, X, b0, 0, (int)(t.pm / M::STEP), lds, acc);
+    if (!M::run(P, a0, X, b0, 0, (int)(t.pm / M::STEP), lds, acc)) return;
     constexpr float down = 1.f / (float)(1 << kScale);
     using W = WaveStore<M>;
     char* reg = W::region(lds);
@@ -268,31 +269,28 @@ __global__ __launch_bounds__(M::NT, 2) void ns_update_kernel(Table table, char* 
 #pragma unroll
                 for (int e = 0; e < 16; ++e) acc[i][j][e] = a0 + M::arow(i, e) < t.m && c < t.n ? acc[i][j][e] * down : 0.f;
         }
-#pragma unroll
-        for (int q = 0; q < 2; ++q) {
-            auto val = [&](int i, int j, int e) -> uint16_t { return plane16(acc[i][j][e], q); };
-            W::store_rows(reg, val, [&](int r, int c, u32x4 d) {
-                if (r0 + r < t.m && kbyte<2>(c0 + c) < t.pn) *reinterpret_cast<u32x4*>(t.X[1] + (int64_t)(r0 + r) * t.pn + kbyte<2>(c0 + c, q)) = d;
-            });
-        }
+        W::template store_rows<2>(reg, [&](int i, int j, int e, int q) -> uint16_t { return plane16(acc[i][j][e], q); },
+                                  [&](int r, int c, int q, u32x4 d) {
+                                      if (r0 + r < t.m && kbyte<2>(c0 + c) < t.pn)
+                                          *reinterpret_cast<u32x4*>(t.X[1] + (int64_t)(r0 + r) * t.pn + kbyte<2>(c0 + c, q)) = d;
+                                  });
         return;
     }
     const bool tall = t.rows > t.cols;
     if constexpr (LAST == 1 && sizeof(S) == 2) {
-        auto val = [&](int i, int j, int e) -> uint16_t { return bits16((S)(acc[i][j][e] * (down * down))); };
+        auto val = [&](int i, int j, int e, int) -> uint16_t { return bits16((S)(acc[i][j][e] * (down * down))); };
         S* out = reinterpret_cast<S*>(t.dst);
         auto put = [&](int r, int c, u32x4 d) {
             if (r < t.rows && c < t.cols) store_vec(out + (int64_t)r * t.cols, c, t.cols, __builtin_bit_cast(typename Vec<S>::type, d));
         };
-        if (tall) W::store_cols(reg, val, [&](int c, int r, u32x4 d) { put(c0 + c, r0 + r, d); });
-        else W::store_rows(reg, val, [&](int r, int c, u32x4 d) { put(r0 + r, c0 + c, d); });
+        if (tall) W::template store_cols<1>(reg, val, [&](int c, int r, int, u32x4 d) { put(c0 + c, r0 + r, d); });
+        else W::template store_rows<1>(reg, val, [&](int r, int c, int, u32x4 d) { put(r0 + r, c0 + c, d); });
         return;
     }
     float step = 0.f, keep = 0.f;
     if (LAST == 2) {
         const double lr = ap.lr_dev != nullptr ? ap.lr_dev[0] : ap.lr;
-        const double s = ap.adjust == 1 ? 0.2 * sqrt((double)t.n) : sqrt(t.rows > t.cols ? (double)t.rows / (double)t.cols : 1.0);
-        step = (float)(lr * s);
+        step = (float)(lr * update_scale(t, ap.adjust));
         keep = (float)(1.0 - lr * ap.weight_decay);
     }
 #pragma unroll
@@ -312,10 +310,182 @@ __global__ __launch_bounds__(M::NT, 2) void ns_update_kernel(Table table, char* 
     }
 }
 
+// ---------------------------------------------------------------- small matrices: the whole iteration in one workgroup
+// A matrix whose X, A and P fit the LDS of a CU (160 KB) needs no launch between the steps: 17 launches of 5 us (64 x 192) become one.
+// Rows are padded by 16 bytes, so that 16 rows read at one k lie in different banks.  A: a wave takes a 32 x 32 block and its share
+// of k, the shares are joined in fixed order; P: a wave takes a block; update: a wave takes 32 columns of X, which only it reads and
+// writes, so X is updated in place.
+constexpr int kSmallWaves = 8, kSmallScratch = 7 * 4096, kSmallLds = 160 * 1024 - 256;
+inline __host__ __device__ int64_t small_lds(int64_t m, int64_t n) {
+    const int64_t mp = up(m, 32), np = up(n, 32);
+    return mp * (np * 4 + 16) + 2 * mp * (mp * 4 + 16) + kSmallScratch;
+}
+inline bool small_ok(int64_t rows, int64_t cols) {
+    const int64_t m = rows < cols ? rows : cols, n = rows < cols ? cols : rows;
+    return m <= 64 && small_lds(m, n) <= kSmallLds;
+}
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+// rows r of a block at k 16 kk + 8 h .. + 7, plane q (k fast)
+__device__ __forceinline__ f16x8 small_along(const char* base, int64_t pitch, int row, int kk, int h, int q) {
+    return *reinterpret_cast<const f16x8*>(base + row * pitch + kbyte<2>(16 * kk + 8 * h, q));
+}
+// columns 32 blk + r at rows 16 kk + 8 h .. + 7, plane q (k slow)
+__device__ __forceinline__ f16x8 small_across(const char* base, int64_t pitch, int lane, int blk, int kk, int q) {
+    const int l = lane & 15, g = lane >> 4, k = 16 * kk + 8 * (g >> 1) + (l >> 2);
+    const char* p = base + k * pitch + blk * 128 + q * 64 + 32 * (g & 1) + 8 * (l & 3);
+    const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
+    const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(p + 4 * pitch));
+    return __builtin_bit_cast(f16x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+__device__ __forceinline__ void small_put(char* base, int64_t pitch, int row, int col, float v) {
+    char* d = base + row * pitch + (col >> 5) * 128 + (col & 31) * 2;
+    *reinterpret_cast<uint16_t*>(d) = plane16(v, 0);
+    *reinterpret_cast<uint16_t*>(d + 64) = plane16(v, 1);
+}
+
+template <typename S, bool MUON>
+__global__ __launch_bounds__(kSmallWaves * 64, 2) void ns_small_kernel(Table table, float mu, int nesterov, int steps, double eps, Apply ap,
+                                                                       const float* __restrict__ skip) {
+    if (MUON && skip != nullptr && skip[0] != 0.f) return;
+    __shared__ __attribute__((aligned(16))) char lds[kSmallLds];
+    __shared__ double sums[kSmallWaves];
+    const Mat t = load_mat(table, blockIdx.x, nullptr, 0);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 31, h = lane >> 5;
+    const int mp = (int)up(t.m, 32), np = (int)up(t.n, 32), mb = mp / 32;
+    const int64_t px = np * 4 + 16, pa = mp * 4 + 16;
+    char *X = lds, *A = X + mp * px, *P = A + mp * pa;
+    float* scratch = reinterpret_cast<float*>(P + mp * pa);
+    const bool tall = t.rows > t.cols;
+    const int64_t count = (int64_t)t.rows * t.cols;
+    // norm and momentum; X's pads are zeros
+    double s = 0.0;
+    for (int64_t i = threadIdx.x; i < count; i += kSmallWaves * 64) {
+        float u;
+        if (MUON) {
+            const float g = (float)reinterpret_cast<const S*>(t.src)[i], v = mu * t.mom[i] + g;
+            t.mom[i] = v;
+            u = nesterov ? g + mu * v : v;
+        } else {
+            u = (float)reinterpret_cast<const S*>(t.src)[i];
+        }
+        s += (double)u * (double)u;
+    }
+    for (int i = threadIdx.x * 16; i < mp * px; i += kSmallWaves * 64 * 16) *reinterpret_cast<u32x4*>(X + i) = u32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+    if (lane == 0) sums[wave] = s;
+    __syncthreads();
+    s = 0.0;
+#pragma unroll
+    for (int w = 0; w < kSmallWaves; ++w) s += sums[w];
+    const float f = (float)((double)(1 << kScale) / (sqrt(s) + eps));
+    for (int64_t i = threadIdx.x; i < count; i += kSmallWaves * 64) {   // (a thread reads the momentum that it wrote)
+        const int row = (int)(i / t.cols), col = (int)(i - (int64_t)row * t.cols);
+        small_put(X, px, tall ? col : row, tall ? row : col, update_of<S, MUON>(t, i, mu, nesterov) * f);
+    }
+    __syncthreads();
+    constexpr float down = 1.f / (float)(1 << kScale);
+    const int blocks = mb * mb, share = kSmallWaves / blocks;             // 1 or 4 blocks of A; 8 or 2 waves share one's k
+    for (int step = 0; step < steps; ++step) {
+        {   // A = X X^T
+            const int b = wave % blocks, part = wave / blocks, i = b / mb, j = b % mb;
+            f32x16 acc;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[e] = 0.f;
+            for (int kk = part; kk < np / 16; kk += share) {
+                const f16x8 ah = small_along(X, px, 32 * i + r, kk, h, 0), al = small_along(X, px, 32 * i + r, kk, h, 1);
+                const f16x8 bh = small_along(X, px, 32 * j + r, kk, h, 0), bl = small_along(X, px, 32 * j + r, kk, h, 1);
+                acc = Frag<_Float16>::mfma(al, bh, acc);
+                acc = Frag<_Float16>::mfma(ah, bl, acc);
+                acc = Frag<_Float16>::mfma(ah, bh, acc);
+            }
+            if (part > 0)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) scratch[((part - 1) * blocks + b) * 1024 + e * 64 + lane] = acc[e];
+            __syncthreads();
+            if (part == 0) {
+                for (int q = 1; q < share; ++q)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) acc[e] += scratch[((q - 1) * blocks + b) * 1024 + e * 64 + lane];
+#pragma unroll
+                for (int e = 0; e < 16; ++e) small_put(A, pa, 32 * i + 8 * (e >> 2) + 4 * h + (e & 3), 32 * j + r, acc[e] * down);
+            }
+        }
+        __syncthreads();
+        if (wave < blocks) {   // P = a I + b A + c A A
+            const int i = wave / mb, j = wave % mb;
+            f32x16 acc;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[e] = 0.f;
+            for (int kk = 0; kk < mp / 16; ++kk) {
+                const f16x8 ah = small_along(A, pa, 32 * i + r, kk, h, 0), al = small_along(A, pa, 32 * i + r, kk, h, 1);
+                const f16x8 bh = small_along(A, pa, 32 * j + r, kk, h, 0), bl = small_along(A, pa, 32 * j + r, kk, h, 1);
+                acc = Frag<_Float16>::mfma(al, bh, acc);
+                acc = Frag<_Float16>::mfma(ah, bl, acc);
+                acc = Frag<_Float16>::mfma(ah, bh, acc);
+            }
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int row = 32 * i + 8 * (e >> 2) + 4 * h + (e & 3), col = 32 * j + r;
+                const char* d = A + row * pa + (col >> 5) * 128 + (col & 31) * 2;
+                const float w = (float)*reinterpret_cast<const _Float16*>(d) + (float)*reinterpret_cast<const _Float16*>(d + 64);
+                const float v = kC * (acc[e] * down) + (kB * w + (row == col ? kA * (float)(1 << kScale) : 0.f));
+                small_put(P, pa, row, col, row < t.m && col < t.m ? v : 0.f);
+            }
+        }
+        __syncthreads();
+        const bool last = step + 1 == steps;
+        float lr_step = 0.f, keep = 0.f;
+        if (MUON && last) {
+            const double lr = ap.lr_dev != nullptr ? ap.lr_dev[0] : ap.lr;
+            lr_step = (float)(lr * update_scale(t, ap.adjust));
+            keep = (float)(1.0 - lr * ap.weight_decay);
+        }
+        for (int blk = wave; blk < np / 32; blk += kSmallWaves) {   // X = P X, 32 columns
+            f32x16 acc[2];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[0][e] = acc[1][e] = 0.f;
+            for (int kk = 0; kk < mp / 16; ++kk) {
+                const f16x8 bh = small_across(X, px, lane, blk, kk, 0), bl = small_across(X, px, lane, blk, kk, 1);
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    if (i < mb) {
+                        const f16x8 ah = small_along(P, pa, 32 * i + r, kk, h, 0), al = small_along(P, pa, 32 * i + r, kk, h, 1);
+                        acc[i] = Frag<_Float16>::mfma(al, bh, acc[i]);
+                        acc[i] = Frag<_Float16>::mfma(ah, bl, acc[i]);
+                        acc[i] = Frag<_Float16>::mfma(ah, bh, acc[i]);
+                    }
+            }
+            const int c = 32 * blk + r;
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                if (i < mb)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const int row = 32 * i + 8 * (e >> 2) + 4 * h + (e & 3);
+                        if (!last) {
+                            small_put(X, px, row, c, acc[i][e] * down);
+                        } else if (row < t.m && c < t.n) {
+                            const float v = acc[i][e] * (down * down);
+                            const int64_t at = tall ? (int64_t)c * t.cols + row : (int64_t)row * t.cols + c;
+                            if constexpr (MUON) {
+                                float* p = reinterpret_cast<float*>(t.dst) + at;
+                                *p = *p * keep - lr_step * v;
+                            } else {
+                                reinterpret_cast<S*>(t.dst)[at] = (S)v;
+                            }
+                        }
+                    }
+        }
+        __syncthreads();
+    }
+}
+
 template <bool TB> using Big = MmTile<_Float16, 2, 256, 256, 2, 4, 2, false, TB>;
-using Tri = MmTile<_Float16, 2, 192, 192, 3, 2, 3>;      // a triangle of tiles: 253 of them cover 4096 x 4096, one per CU
-template <bool TB> using Mid = MmTile<_Float16, 2, 128, 128, 2, 2, 2, false, TB>;
-template <bool TB> using Small = MmTile<_Float16, 2, 64, 64, 2, 2, 4, false, TB>;
+using Tri = MmTile<_Float16, 2, 192, 192, 2, 2, 3>;      // a triangle of tiles: 253 of them cover 4096 x 4096, one per CU
+template <bool TB, int KG = 1> using Mid = MmTile<_Float16, 2, 128, 128, 2, 2, 2, false, TB, KG>;
+template <bool TB, int KG = 1> using Small = MmTile<_Float16, 2, 64, 64, 2, 2, 4, false, TB, KG>;
 
 #define SSECG_NS_LAUNCH(M, kernel, grid, st, ...)                                                                               \
     do {                                                                                                                        \
@@ -326,7 +496,7 @@ template <bool TB> using Small = MmTile<_Float16, 2, 64, 64, 2, 2, 4, false, TB>
 
 struct Plan {
     size_t bytes;
-    int parts, prep, gram, upd, gramTile, updTile;       // workgroups of the launches and tile sides
+    int parts, prep, gram, upd, gramTile, updTile, gramGroups, updGroups;   // workgroups of the launches, tile sides, groups of waves
 };
 
 template <bool POLY>
@@ -335,6 +505,7 @@ int launch_gram(const Table& t, const Plan& p, char* ws, int from, const float* 
     if (p.gramTile == 256) SSECG_NS_GRAM(Big<false>);
     else if (p.gramTile == 192) SSECG_NS_GRAM(Tri);
     else if (p.gramTile == 128) SSECG_NS_GRAM(Mid<false>);
+    else if (p.gramGroups == 2) SSECG_NS_GRAM(Small<false, 2>);
     else SSECG_NS_GRAM(Small<false>);
 #undef SSECG_NS_GRAM
     return 0;
@@ -345,6 +516,7 @@ int launch_update(const Table& t, const Plan& p, char* ws, int from, const Apply
 #define SSECG_NS_UPDATE(...) \
     do { using M = __VA_ARGS__; SSECG_NS_LAUNCH(M, (ns_update_kernel<M, S, LAST>), p.upd, st, t, ws, from, ap, skip); } while (0)
     if (p.updTile == 256) SSECG_NS_UPDATE(Big<true>);
+    else if (p.updTile == 128 && p.updGroups == 2) SSECG_NS_UPDATE(Mid<true, 2>);
     else if (p.updTile == 128) SSECG_NS_UPDATE(Mid<true>);
     else SSECG_NS_UPDATE(Small<true>);
 #undef SSECG_NS_UPDATE
@@ -355,7 +527,7 @@ int launch_update(const Table& t, const Plan& p, char* ws, int from, const Apply
 int make_plan(const int64_t* mats, int count, Table& t, Plan& p) {
     // the tile side that mm_time expects to be fastest: the two products of a step over a triangle of tiles, the update over all
     int64_t largest = 0;
-    auto time = [&](int side, bool gram) {
+    auto time = [&](int side, int groups, bool gram) {
         MmWork along, square, whole;
         for (int k = 0; k < count; ++k) {
             const int64_t a = mats[5 * k + 3], b = mats[5 * k + 4], m = a < b ? a : b, n = a < b ? b : a;
@@ -365,13 +537,17 @@ int make_plan(const int64_t* mats, int count, Table& t, Plan& p) {
             whole.add(tm * tn, (m + 31) / 32);
             largest = a * b > largest ? a * b : largest;
         }
-        return gram ? mm_time(side, 2, along) + mm_time(side, 2, square) : mm_time(side, 2, whole);
+        return gram ? mm_time(side, 2, along, groups) + mm_time(side, 2, square, groups) : mm_time(side, 2, whole, groups);
     };
-    p.gramTile = p.updTile = 64;
-    for (int side : {128, 192, 256}) {
-        if (time(side, true) < time(p.gramTile, true)) p.gramTile = side;
-        if (side != 192 && time(side, false) < time(p.updTile, false)) p.updTile = side;
-    }
+    auto pick = [&](bool gram, int& tile, int& groups, std::initializer_list<std::pair<int, int>> of) {
+        double least = 0.0;
+        for (const auto& c : of) {
+            const double t = time(c.first, c.second, gram);
+            if (least == 0.0 || t < least) { least = t; tile = c.first; groups = c.second; }
+        }
+    };
+    pick(true, p.gramTile, p.gramGroups, {{64, 1}, {64, 2}, {128, 1}, {192, 1}, {256, 1}});
+    pick(false, p.updTile, p.updGroups, {{64, 1}, {128, 1}, {128, 2}, {256, 1}});
     p.parts = (int)(largest / 8192 < 1 ? 1 : largest / 8192 > kNormParts ? kNormParts : largest / 8192);
     t.count = count;
     int64_t at = up((int64_t)kMost * kNormParts * 8, 256), prep = 0, gram = 0, upd = 0;
@@ -408,6 +584,12 @@ int run_chain(const int64_t* mats, int count, float mu, int nesterov, int steps,
     Plan p;
     int rc = make_plan(mats, count, t, p);
     if (rc != 0) return rc;
+    bool small = true;
+    for (int k = 0; k < count; ++k) small = small && small_ok(mats[5 * k + 3], mats[5 * k + 4]);
+    if (small) {
+        hipLaunchKernelGGL((ns_small_kernel<S, MUON>), dim3(count), dim3(kSmallWaves * 64), 0, st, t, mu, nesterov, steps, eps, ap, skip);
+        return (int)hipGetLastError();
+    }
     double* partial = reinterpret_cast<double*>(ws);
     hipLaunchKernelGGL((ns_norm_kernel<S, MUON>), dim3(p.parts, count), dim3(256), 0, st, t, mu, nesterov, skip, partial);
     hipLaunchKernelGGL((ns_prep_kernel<S, MUON>), dim3((unsigned)p.prep), dim3(256), 0, st, t, ws, mu, nesterov, p.parts, eps, skip, partial);
