@@ -293,36 +293,47 @@ __global__ __launch_bounds__(M::NT, M::TM * M::TN > 8 ? 1 : 2) void ns_update_ke
         step = (float)(lr * update_scale(t, ap.adjust));
         keep = (float)(1.0 - lr * ap.weight_decay);
     }
+    float* out = reinterpret_cast<float*>(t.dst);
 #pragma unroll
     for (int j = 0; j < M::TN; ++j) {
         const int c = b0 + M::bcol(j);
-        if (c >= t.n) continue;
 #pragma unroll
-        for (int i = 0; i < M::TM; ++i)
+        for (int i = 0; i < M::TM; ++i) {
+            auto at = [&](int e) { const int64_t r = a0 + M::arow(i, e); return tall ? (int64_t)c * t.cols + r : r * t.cols + c; };
+            float old[16];
+            if (LAST == 2)                              // 16 loads in flight, then the stores
+#pragma unroll
+                for (int e = 0; e < 16; ++e) old[e] = c < t.n && a0 + M::arow(i, e) < t.m ? out[at(e)] : 0.f;
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-                const int r = a0 + M::arow(i, e);
-                if (r >= t.m) continue;
                 const float v = acc[i][j][e] * (down * down);
-                float* d = reinterpret_cast<float*>(t.dst) + (tall ? (int64_t)c * t.cols + r : (int64_t)r * t.cols + c);
-                *d = LAST == 1 ? v : *d * keep - step * v;
+                if (c < t.n && a0 + M::arow(i, e) < t.m) out[at(e)] = LAST == 1 ? v : old[e] * keep - step * v;
             }
+        }
     }
 }
 
 // ---------------------------------------------------------------- small matrices: the whole iteration in one workgroup
 // A matrix whose X, A and P fit the LDS of a CU (160 KB) needs no launch between the steps: 17 launches of 5 us (64 x 192) become one.
-// Rows are padded by 16 bytes, so that 16 rows read at one k lie in different banks.  A: a wave takes a 32 x 32 block and its share
-// of k, the shares are joined in fixed order; P: a wave takes a block; update: a wave takes 32 columns of X, which only it reads and
-// writes, so X is updated in place.
-constexpr int kSmallWaves = 8, kSmallScratch = 7 * 4096, kSmallLds = 160 * 1024 - 256;
-inline __host__ __device__ int64_t small_lds(int64_t m, int64_t n) {
+// What bounds it is instructions: a phase lasts as long as its busiest wave.  So the 32 x 32 blocks of a product and shares of its k
+// go over all sixteen waves, the sums meet in LDS in fp32, and every thread joins and splits four values of the result.  Rows are
+// padded by 16 bytes, so that 16 rows read at one k lie in different banks.  X is updated in place, between two barriers.
+constexpr int kSmallWaves = 16, kSmallLds = 160 * 1024 - 256;
+constexpr int kSmallPairs = 2;                    // 32 x 32 blocks of X that a wave updates at most
+inline __host__ __device__ int64_t small_planes(int64_t m, int64_t n) {
     const int64_t mp = up(m, 32), np = up(n, 32);
-    return mp * (np * 4 + 16) + 2 * mp * (mp * 4 + 16) + kSmallScratch;
+    return mp * (np * 4 + 16) + 2 * mp * (mp * 4 + 16);
+}
+// waves that share the k of a block of A: what LDS leaves for their sums (4 KB a block each), 8 at most
+inline __host__ __device__ int small_shares(int64_t m, int64_t n) {
+    const int64_t blocks = m > 32 ? 4 : 1;
+    for (int s = m > 32 ? 4 : 8; s > 0; s /= 2)
+        if (small_planes(m, n) + s * blocks * 4096 <= kSmallLds) return s;
+    return 0;
 }
 inline bool small_ok(int64_t rows, int64_t cols) {
     const int64_t m = rows < cols ? rows : cols, n = rows < cols ? cols : rows;
-    return m <= 64 && small_lds(m, n) <= kSmallLds;
+    return m <= 64 && n <= 1024 && up(m, 32) / 32 * (up(n, 32) / 32) <= kSmallWaves * kSmallPairs && small_shares(m, n) > 0;
 }
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -345,31 +356,40 @@ __device__ __forceinline__ void small_put(char* base, int64_t pitch, int row, in
 }
 
 template <typename S, bool MUON>
-__global__ __launch_bounds__(kSmallWaves * 64, 2) void ns_small_kernel(Table table, float mu, int nesterov, int steps, double eps, Apply ap,
+__global__ __launch_bounds__(kSmallWaves * 64) void ns_small_kernel(Table table, float mu, int nesterov, int steps, double eps, Apply ap,
                                                                        const float* __restrict__ skip) {
     if (MUON && skip != nullptr && skip[0] != 0.f) return;
     __shared__ __attribute__((aligned(16))) char lds[kSmallLds];
     __shared__ double sums[kSmallWaves];
     const Mat t = load_mat(table, blockIdx.x, nullptr, 0);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 31, h = lane >> 5;
-    const int mp = (int)up(t.m, 32), np = (int)up(t.n, 32), mb = mp / 32;
+    const int mp = (int)up(t.m, 32), np = (int)up(t.n, 32), lb = mp >> 6, mb = 1 << lb;   // 32 or 64 rows: 1 or 2 blocks, lb = log2
     const int64_t px = np * 4 + 16, pa = mp * 4 + 16;
     char *X = lds, *A = X + mp * px, *P = A + mp * pa;
     float* scratch = reinterpret_cast<float*>(P + mp * pa);
     const bool tall = t.rows > t.cols;
-    const int64_t count = (int64_t)t.rows * t.cols;
     // norm and momentum; X's pads are zeros
     double s = 0.0;
-    for (int64_t i = threadIdx.x; i < count; i += kSmallWaves * 64) {
-        float u;
-        if (MUON) {
-            const float g = (float)reinterpret_cast<const S*>(t.src)[i], v = mu * t.mom[i] + g;
-            t.mom[i] = v;
-            u = nesterov ? g + mu * v : v;
+    const int count = t.rows * t.cols;                             // at most 32 blocks of 1024
+    constexpr int V = Vec<S>::N;
+    const S* src = reinterpret_cast<const S*>(t.src);
+#pragma unroll 2
+    for (int i = threadIdx.x * V; i < count; i += kSmallWaves * 64 * V) {
+        const int left = count - i < V ? count - i : V;
+        const auto g = load_vec(src + i, 0, left);
+        if constexpr (MUON) {
+            auto v = load_vec(t.mom + i, 0, left);
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                v[j] = mu * v[j] + g[j];
+                const float u = nesterov ? g[j] + mu * v[j] : v[j];
+                s += (double)u * (double)u;                        // beyond the end: zeros
+            }
+            store_vec(t.mom + i, 0, left, v);
         } else {
-            u = (float)reinterpret_cast<const S*>(t.src)[i];
+#pragma unroll
+            for (int j = 0; j < V; ++j) s += (double)(float)g[j] * (double)(float)g[j];
         }
-        s += (double)u * (double)u;
     }
     for (int i = threadIdx.x * 16; i < mp * px; i += kSmallWaves * 64 * 16) *reinterpret_cast<u32x4*>(X + i) = u32x4{0, 0, 0, 0};
 #pragma unroll
@@ -380,105 +400,138 @@ __global__ __launch_bounds__(kSmallWaves * 64, 2) void ns_small_kernel(Table tab
 #pragma unroll
     for (int w = 0; w < kSmallWaves; ++w) s += sums[w];
     const float f = (float)((double)(1 << kScale) / (sqrt(s) + eps));
-    for (int64_t i = threadIdx.x; i < count; i += kSmallWaves * 64) {   // (a thread reads the momentum that it wrote)
-        const int row = (int)(i / t.cols), col = (int)(i - (int64_t)row * t.cols);
-        small_put(X, px, tall ? col : row, tall ? row : col, update_of<S, MUON>(t, i, mu, nesterov) * f);
+#pragma unroll 2
+    for (int i = threadIdx.x * V; i < count; i += kSmallWaves * 64 * V) {   // (a thread reads the momentum that it wrote)
+        const int left = count - i < V ? count - i : V;
+        const auto g = load_vec(src + i, 0, left);
+        typename Vec<float>::type v = {};
+        if constexpr (MUON) v = load_vec(t.mom + i, 0, left);
+        int row = i / t.cols, col = i - row * t.cols;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            float u = (float)g[j];
+            if constexpr (MUON) u = nesterov ? u + mu * v[j] : v[j];
+            if (j < left) small_put(X, px, tall ? col : row, tall ? row : col, u * f);
+            if (++col == t.cols) { col = 0; ++row; }
+        }
     }
     __syncthreads();
     constexpr float down = 1.f / (float)(1 << kScale);
-    const int blocks = mb * mb, share = kSmallWaves / blocks;             // 1 or 4 blocks of A; 8 or 2 waves share one's k
+    using F = Frag<_Float16>;
+    const int blocks = mb * mb, shares = small_shares(t.m, t.n), pairs = mb * (np / 32);
+    auto zero = [](f32x16& v) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) v[e] = 0.f;
+    };
     for (int step = 0; step < steps; ++step) {
-        {   // A = X X^T
-            const int b = wave % blocks, part = wave / blocks, i = b / mb, j = b % mb;
-            f32x16 acc;
+#pragma unroll 1
+        for (int phase = 0; phase < 2; ++phase) {         // A = X X^T, then P = a I + b A + c A A
+            const char* src = phase == 0 ? X : A;
+            const int64_t pitch = phase == 0 ? px : pa;
+            const int b = wave & (blocks - 1), part = wave >> 2 * lb, i = b >> lb, j = b & (mb - 1), kks = phase == 0 ? np / 16 : mp / 16;
+            if (part < shares) {
+                f32x16 acc, low, cross;                       // one chain of products each: a chain's next product waits for its last
+                zero(acc);
+                zero(low);
+                zero(cross);
+#pragma unroll 1
+                for (int kk = part; kk < kks; kk += shares) {
+                    const f16x8 ah = small_along(src, pitch, 32 * i + r, kk, h, 0), al = small_along(src, pitch, 32 * i + r, kk, h, 1);
+                    const f16x8 bh = small_along(src, pitch, 32 * j + r, kk, h, 0), bl = small_along(src, pitch, 32 * j + r, kk, h, 1);
+                    low = F::mfma(al, bh, low);
+                    cross = F::mfma(ah, bl, cross);
+                    acc = F::mfma(ah, bh, acc);
+                }
 #pragma unroll
-            for (int e = 0; e < 16; ++e) acc[e] = 0.f;
-            for (int kk = part; kk < np / 16; kk += share) {
-                const f16x8 ah = small_along(X, px, 32 * i + r, kk, h, 0), al = small_along(X, px, 32 * i + r, kk, h, 1);
-                const f16x8 bh = small_along(X, px, 32 * j + r, kk, h, 0), bl = small_along(X, px, 32 * j + r, kk, h, 1);
-                acc = Frag<_Float16>::mfma(al, bh, acc);
-                acc = Frag<_Float16>::mfma(ah, bl, acc);
-                acc = Frag<_Float16>::mfma(ah, bh, acc);
+                for (int e = 0; e < 16; ++e) scratch[(part * blocks + b) * 1024 + e * 64 + lane] = acc[e] + (low[e] + cross[e]);
             }
-            if (part > 0)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) scratch[((part - 1) * blocks + b) * 1024 + e * 64 + lane] = acc[e];
             __syncthreads();
-            if (part == 0) {
-                for (int q = 1; q < share; ++q)
+            for (int g = threadIdx.x; g < mp * mp / 4; g += kSmallWaves * 64) {
+                const int row = g >> (3 + lb), col = (g & (mp / 4 - 1)) * 4, q = row & 31;
+                const float* at = scratch + (((row >> 5) << lb) + (col >> 5)) * 1024 + ((q >> 3) * 4 + (q & 3)) * 64 + (q >> 2 & 1) * 32 + (col & 31);
+                f32x4 v = *reinterpret_cast<const f32x4*>(at);
+                for (int k = 1; k < shares; ++k) v += *reinterpret_cast<const f32x4*>(at + k * blocks * 1024);
+                const int64_t off = row * pa + (col >> 5) * 128 + (col & 31) * 2;
+                _Float16 hi[4], lo[4];
+                if (phase == 1) {
+                    __builtin_memcpy(hi, A + off, 8);
+                    __builtin_memcpy(lo, A + off + 64, 8);
+                }
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) acc[e] += scratch[((q - 1) * blocks + b) * 1024 + e * 64 + lane];
-#pragma unroll
-                for (int e = 0; e < 16; ++e) small_put(A, pa, 32 * i + 8 * (e >> 2) + 4 * h + (e & 3), 32 * j + r, acc[e] * down);
+                for (int k = 0; k < 4; ++k) {
+                    float d = v[k] * down;
+                    if (phase == 1) d = kC * d + (kB * ((float)hi[k] + (float)lo[k]) + (row == col + k ? kA * (float)(1 << kScale) : 0.f));
+                    d = row < t.m && col + k < t.m ? d : 0.f;
+                    hi[k] = (_Float16)d;
+                    lo[k] = (_Float16)(d - (float)hi[k]);
+                }
+                char* d = (phase == 0 ? A : P) + off;
+                __builtin_memcpy(d, hi, 8);
+                __builtin_memcpy(d + 64, lo, 8);
             }
+            __syncthreads();
         }
-        __syncthreads();
-        if (wave < blocks) {   // P = a I + b A + c A A
-            const int i = wave / mb, j = wave % mb;
-            f32x16 acc;
-#pragma unroll
-            for (int e = 0; e < 16; ++e) acc[e] = 0.f;
-            for (int kk = 0; kk < mp / 16; ++kk) {
-                const f16x8 ah = small_along(A, pa, 32 * i + r, kk, h, 0), al = small_along(A, pa, 32 * i + r, kk, h, 1);
-                const f16x8 bh = small_along(A, pa, 32 * j + r, kk, h, 0), bl = small_along(A, pa, 32 * j + r, kk, h, 1);
-                acc = Frag<_Float16>::mfma(al, bh, acc);
-                acc = Frag<_Float16>::mfma(ah, bl, acc);
-                acc = Frag<_Float16>::mfma(ah, bh, acc);
-            }
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const int row = 32 * i + 8 * (e >> 2) + 4 * h + (e & 3), col = 32 * j + r;
-                const char* d = A + row * pa + (col >> 5) * 128 + (col & 31) * 2;
-                const float w = (float)*reinterpret_cast<const _Float16*>(d) + (float)*reinterpret_cast<const _Float16*>(d + 64);
-                const float v = kC * (acc[e] * down) + (kB * w + (row == col ? kA * (float)(1 << kScale) : 0.f));
-                small_put(P, pa, row, col, row < t.m && col < t.m ? v : 0.f);
-            }
-        }
-        __syncthreads();
         const bool last = step + 1 == steps;
-        float lr_step = 0.f, keep = 0.f;
-        if (MUON && last) {
-            const double lr = ap.lr_dev != nullptr ? ap.lr_dev[0] : ap.lr;
-            lr_step = (float)(lr * update_scale(t, ap.adjust));
-            keep = (float)(1.0 - lr * ap.weight_decay);
-        }
-        for (int blk = wave; blk < np / 32; blk += kSmallWaves) {   // X = P X, 32 columns
-            f32x16 acc[2];
+        f32x16 acc[kSmallPairs];                          // X = P X: block (i, blk) is pair wave + 8 n
 #pragma unroll
-            for (int e = 0; e < 16; ++e) acc[0][e] = acc[1][e] = 0.f;
+        for (int n = 0; n < kSmallPairs; ++n) {
+            const int pair = wave + kSmallWaves * n, i = pair & (mb - 1), blk = pair >> lb;
+            if (pair >= pairs) break;
+            zero(acc[n]);
+#pragma unroll 1
             for (int kk = 0; kk < mp / 16; ++kk) {
                 const f16x8 bh = small_across(X, px, lane, blk, kk, 0), bl = small_across(X, px, lane, blk, kk, 1);
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-                    if (i < mb) {
-                        const f16x8 ah = small_along(P, pa, 32 * i + r, kk, h, 0), al = small_along(P, pa, 32 * i + r, kk, h, 1);
-                        acc[i] = Frag<_Float16>::mfma(al, bh, acc[i]);
-                        acc[i] = Frag<_Float16>::mfma(ah, bl, acc[i]);
-                        acc[i] = Frag<_Float16>::mfma(ah, bh, acc[i]);
-                    }
+                const f16x8 ah = small_along(P, pa, 32 * i + r, kk, h, 0), al = small_along(P, pa, 32 * i + r, kk, h, 1);
+                acc[n] = F::mfma(al, bh, acc[n]);
+                acc[n] = F::mfma(ah, bl, acc[n]);
+                acc[n] = F::mfma(ah, bh, acc[n]);
             }
-            const int c = 32 * blk + r;
+            __builtin_amdgcn_sched_barrier(0);            // (one block's fragments at a time: registers)
+        }
+        __syncthreads();                                  // every wave has read what it needs of X
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
-                if (i < mb)
+        for (int n = 0; n < kSmallPairs; ++n) {
+            const int pair = wave + kSmallWaves * n, i = pair & (mb - 1), blk = pair >> lb;
+            if (pair >= pairs) break;
+            char* d = X + (32 * i + 4 * h) * px + blk * 128 + r * (last ? 4 : 2);
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        const int row = 32 * i + 8 * (e >> 2) + 4 * h + (e & 3);
-                        if (!last) {
-                            small_put(X, px, row, c, acc[i][e] * down);
-                        } else if (row < t.m && c < t.n) {
-                            const float v = acc[i][e] * (down * down);
-                            const int64_t at = tall ? (int64_t)c * t.cols + row : (int64_t)row * t.cols + c;
-                            if constexpr (MUON) {
-                                float* p = reinterpret_cast<float*>(t.dst) + at;
-                                *p = *p * keep - lr_step * v;
-                            } else {
-                                reinterpret_cast<S*>(t.dst)[at] = (S)v;
-                            }
-                        }
-                    }
+            for (int e = 0; e < 16; ++e) {
+                const float v = acc[n][e] * down;
+                char* q = d + (8 * (e >> 2) + (e & 3)) * px;
+                if (last) {                               // in fp32: rows of as many bytes
+                    *reinterpret_cast<float*>(q) = v * down;
+                } else {
+                    const _Float16 hi = (_Float16)v;
+                    *reinterpret_cast<_Float16*>(q) = hi;
+                    *reinterpret_cast<_Float16*>(q + 64) = (_Float16)(v - (float)hi);
+                }
+            }
         }
         __syncthreads();
+    }
+    float lr_step = 0.f, keep = 0.f;
+    if constexpr (MUON) {
+        const double lr = ap.lr_dev != nullptr ? ap.lr_dev[0] : ap.lr;
+        lr_step = (float)(lr * update_scale(t, ap.adjust));
+        keep = (float)(1.0 - lr * ap.weight_decay);
+    }
+    S* dst = reinterpret_cast<S*>(t.dst);
+#pragma unroll 2
+    for (int i = threadIdx.x * V; i < count; i += kSmallWaves * 64 * V) {
+        const int left = count - i < V ? count - i : V;
+        typename Vec<S>::type o = {};
+        if constexpr (MUON) o = load_vec(dst + i, 0, left);
+        int row = i / t.cols, col = i - row * t.cols;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            if (j < left) {
+                const float v = *reinterpret_cast<const float*>(X + (tall ? col * px + row * 4 : row * px + col * 4));
+                if constexpr (MUON) o[j] = o[j] * keep - lr_step * v;
+                else o[j] = (S)v;
+            }
+            if (++col == t.cols) { col = 0; ++row; }
+        }
+        store_vec(dst + i, 0, left, o);
     }
 }
 

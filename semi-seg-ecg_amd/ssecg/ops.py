@@ -1331,74 +1331,80 @@ def _lm(t, name, dtype=None):
     return t if t.is_contiguous() else t.contiguous()
 
 
-def _lm_vec(t, name, n, like):
-    """A parameter vector of ``n`` values as fp32 on ``like``'s device; None stays None."""
+def _lm_vec(t, name, n, device):
+    """A parameter vector of ``n`` values as fp32 on ``device``; None stays None."""
     if t is None:
         return None
     t = _lm(t, name)
-    if t.numel() != n or t.dim() != 1:
+    if t.shape != (n,):
         raise SsecgError(f"{name}: expected ({n},), got {tuple(t.shape)}")
-    _lm_device(like, **{name: t})
-    return t.float()
+    _lm_device(device, name, t)
+    return t if t.dtype == torch.float32 else t.float()
 
 
-def _lm_device(ref, **tensors):
-    for name, t in tensors.items():
-        if t is not None and t.device != ref.device:
-            raise SsecgError(f"{name}: on {t.device}, expected {ref.device}")
+def _lm_device(device, name, t):
+    if t is not None and t.device != device:
+        raise SsecgError(f"{name}: on {t.device}, expected {device}")
 
 
-def _lm_guard(t):
+_NO_GUARD = contextlib.nullcontext()
+
+
+def _lm_guard(device):
     """The launches of a call go to the current stream of ITS tensors' device."""
-    return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+    return _NO_GUARD if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def layer_norm_fwd(x, weight=None, bias=None, eps=1e-5):
     """Layer norm over the last axis of x (..., C) -> (y of x's type, mean, rstd); mean and rstd are fp32, one per row.
     ``weight`` / ``bias``: (C,), None = 1 / 0."""
-    trace("layer_norm_fwd", tuple(getattr(x, "shape", ())))
     x = _lm(x, "x")
-    if x.dim() < 1 or x.shape[-1] == 0:
+    trace("layer_norm_fwd", tuple(x.shape))
+    shape, dev, n = x.shape, x.device, x.numel()
+    if not shape or shape[-1] == 0:
         raise SsecgError("layer_norm: x must be (..., C) with C > 0")
     if not eps >= 0:
         raise SsecgError("layer_norm: eps must not be negative")
-    C = x.shape[-1]
-    rows = x.numel() // C
-    weight, bias = _lm_vec(weight, "weight", C, x), _lm_vec(bias, "bias", C, x)
+    C = shape[-1]
+    rows = n // C
+    weight, bias = _lm_vec(weight, "weight", C, dev), _lm_vec(bias, "bias", C, dev)
     y = torch.empty_like(x)
-    mean, rstd = torch.empty((2, rows), device=x.device, dtype=torch.float32).unbind(0)
+    mean = torch.empty(rows, device=dev, dtype=torch.float32)
+    rstd = torch.empty(rows, device=dev, dtype=torch.float32)
     if rows:
-        with _lm_guard(x), _Timed("ln_fwd_kernel", 0.0, 2.0 * x.numel() * x.element_size()):
-            check(lib().ssecg_layer_norm_fwd(_p(x), _p(weight), _p(bias), _LM_DTYPE[x.dtype], rows, C, float(eps), _p(y), _p(mean),
-                                             _p(rstd), _stream()), "ssecg_layer_norm_fwd")
+        with _lm_guard(dev), _Timed("ln_fwd_kernel", 0.0, 2.0 * n * x.element_size()):
+            check(lib().ssecg_layer_norm_fwd(x.data_ptr(), _p(weight), _p(bias), _LM_DTYPE[x.dtype], rows, C, eps, y.data_ptr(),
+                                             mean.data_ptr(), rstd.data_ptr(), _stream()), "ssecg_layer_norm_fwd")
     return y, mean, rstd
 
 
 def layer_norm_bwd(dy, x, mean, rstd, weight=None, want_params=True):
     """-> (dx of x's type, dweight, dbias in fp32 or None): the backward pass of ``layer_norm_fwd``."""
-    trace("layer_norm_bwd", tuple(getattr(x, "shape", ())))
     x = _lm(x, "x")
     dy = _lm(dy, "dy", x.dtype)
-    if dy.shape != x.shape or x.dim() < 1 or x.shape[-1] == 0:
+    trace("layer_norm_bwd", tuple(x.shape))
+    shape, dev, n = x.shape, x.device, x.numel()
+    if dy.shape != shape or not shape or shape[-1] == 0:
         raise SsecgError("layer_norm_bwd: dy and x must both be (..., C)")
-    C = x.shape[-1]
-    rows = x.numel() // C
+    C = shape[-1]
+    rows = n // C
     mean, rstd = _req(mean, "mean"), _req(rstd, "rstd")
     if mean.numel() != rows or rstd.numel() != rows:
         raise SsecgError("layer_norm_bwd: mean and rstd must hold one value per row")
-    _lm_device(x, dy=dy, mean=mean, rstd=rstd)
-    weight = _lm_vec(weight, "weight", C, x)
+    _lm_device(dev, "dy", dy), _lm_device(dev, "mean", mean), _lm_device(dev, "rstd", rstd)
+    weight = _lm_vec(weight, "weight", C, dev)
     dx = torch.empty_like(x)
-    dw = db = ws = None
+    dw = db = None
     if want_params:
-        dw, db = (torch.empty if rows else torch.zeros)((2, C), device=x.device, dtype=torch.float32).unbind(0)
+        make = torch.empty if rows else torch.zeros
+        dw, db = make(C, device=dev, dtype=torch.float32), make(C, device=dev, dtype=torch.float32)
     if rows:
         Lb, code = lib(), _LM_DTYPE[x.dtype]
-        with _lm_guard(x), _Timed("ln_bwd_kernel", 0.0, 3.0 * x.numel() * x.element_size()):
-            if want_params:
-                ws = torch.empty((Lb.ssecg_layer_norm_bwd_workspace(code, rows, C),), device=x.device, dtype=torch.uint8)
-            check(Lb.ssecg_layer_norm_bwd(_p(dy), _p(x), _p(mean), _p(rstd), _p(weight), code, rows, C, _p(dx), _p(dw), _p(db), _p(ws),
-                                          ws.numel() if ws is not None else 0, _stream()), "ssecg_layer_norm_bwd")
+        with _lm_guard(dev), _Timed("ln_bwd_kernel", 0.0, 3.0 * n * x.element_size()):
+            nbytes = Lb.ssecg_layer_norm_bwd_workspace(code, rows, C) if want_params else 0
+            ws = torch.empty(nbytes, device=dev, dtype=torch.uint8) if nbytes else None
+            check(Lb.ssecg_layer_norm_bwd(dy.data_ptr(), x.data_ptr(), mean.data_ptr(), rstd.data_ptr(), _p(weight), code, rows, C,
+                                          dx.data_ptr(), _p(dw), _p(db), _p(ws), nbytes, _stream()), "ssecg_layer_norm_bwd")
     return dx, dw, db
 
 
@@ -1434,19 +1440,21 @@ def linear_ce_fwd(x, weight, target, bias=None, conf=None, thresh=0.0, ignore_in
     if target.shape != x.shape[:-1]:
         raise SsecgError("linear_ce: target must have x's shape without its last axis")
     (V, C), N, mode = weight.shape, target.numel(), _REDUCTION[reduction]
-    bias = _lm_vec(bias, "bias", V, x)
+    dev = x.device
+    bias = _lm_vec(bias, "bias", V, dev)
     if conf is not None:
         conf = _req(conf, "conf")
         if conf.shape != target.shape:
             raise SsecgError("linear_ce: conf must have target's shape")
-    _lm_device(x, weight=weight, target=target, conf=conf)
+    _lm_device(dev, "weight", weight), _lm_device(dev, "target", target), _lm_device(dev, "conf", conf)
     loss = torch.empty(target.shape if mode == 0 else (), device=x.device, dtype=torch.float32)
-    lse, gate = torch.empty((2, N), device=x.device, dtype=torch.float32).unbind(0)
-    count = torch.empty((1,), device=x.device, dtype=torch.float32)
+    lse = torch.empty(N, device=dev, dtype=torch.float32)
+    gate = torch.empty(N, device=dev, dtype=torch.float32)
+    count = torch.empty(1, device=dev, dtype=torch.float32)
     packed = None
     if N:
         Lb, code = lib(), _LM_DTYPE[x.dtype]
-        with _lm_guard(x), _Timed("ce_lse_kernel", 2.0 * N * C * V, (N + V) * C * x.element_size()):
+        with _lm_guard(x.device), _Timed("ce_lse_kernel", 2.0 * N * C * V, (N + V) * C * x.element_size()):
             keep = Lb.ssecg_linear_ce_packed_bytes(_p(x), _p(weight), code, N, C, V)
             packed = torch.empty((keep,), device=x.device, dtype=torch.uint8) if keep else None
             ws = torch.empty((Lb.ssecg_linear_ce_fwd_workspace(code, N, C, V),), device=x.device, dtype=torch.uint8)
@@ -1471,7 +1479,7 @@ def linear_ce_bwd(saved, dloss=None, want_dx=True, want_dweight=True, want_dbias
     dloss = _req(dloss, "dloss")
     if dloss.numel() != (N if mode == 0 else 1):
         raise SsecgError(f"linear_ce_bwd: dloss must be {tuple(shape)}, got {tuple(dloss.shape)}")
-    _lm_device(x, dloss=dloss)
+    _lm_device(x.device, "dloss", dloss)
     want_dbias = want_dbias and bias is not None
     make = torch.empty if N else torch.zeros
     dx = torch.empty_like(x) if want_dx else None
@@ -1480,7 +1488,7 @@ def linear_ce_bwd(saved, dloss=None, want_dx=True, want_dweight=True, want_dbias
     if N and (want_dx or want_dweight or want_dbias):
         Lb, code = lib(), _LM_DTYPE[x.dtype]
         flops = 2.0 * N * C * V * (1 + bool(want_dx) + bool(want_dweight))
-        with _lm_guard(x), _Timed("ce_grad_kernel + ce_prod_kernel", flops, 2.0 * (N + V) * C * x.element_size()):
+        with _lm_guard(x.device), _Timed("ce_grad_kernel + ce_prod_kernel", flops, 2.0 * (N + V) * C * x.element_size()):
             ws = torch.empty((Lb.ssecg_linear_ce_bwd_workspace(code, N, C, V, int(want_dx), int(want_dweight), int(want_dbias)),),
                              device=x.device, dtype=torch.uint8)
             check(Lb.ssecg_linear_ce_bwd(_p(dloss), _p(x), _p(weight), _p(bias), _p(target), _p(lse), _p(gate), _p(count), code, N, C, V, mode,
@@ -1510,12 +1518,12 @@ def orthogonalize(matrices, steps=5, eps=1e-7):
     for m in mats:
         if m.dim() != 2:
             raise SsecgError(f"orthogonalize: expected matrices, got {tuple(m.shape)}")
-        _lm_device(mats[0], matrix=m)
+        _lm_device(mats[0].device, "matrix", m)
     out = [torch.empty_like(m) for m in mats]
     rows = [(m.data_ptr(), o.data_ptr(), 0, m.shape[0], m.shape[1]) for m, o in zip(mats, out) if m.numel()]
     if rows:
         Lb, arr = lib(), _mats(rows)
-        with _lm_guard(mats[0]), _Timed("ns_gram_kernel + ns_update_kernel", _ortho_flops(rows, steps),
+        with _lm_guard(mats[0].device), _Timed("ns_gram_kernel + ns_update_kernel", _ortho_flops(rows, steps),
                                         2.0 * mats[0].element_size() * sum(m.numel() for m in mats)):
             nbytes = Lb.ssecg_orthogonalize_workspace(arr, len(rows))
             ws = torch.empty((max(nbytes, 256),), device=mats[0].device, dtype=torch.uint8)
