@@ -81,11 +81,18 @@ __device__ __forceinline__ int amax_exp(const float* __restrict__ parts) {
     return scale_exp(fmaxf(fmaxf(sh[0], sh[1]), fmaxf(sh[2], sh[3])));
 }
 
-// src (R, C) as an operand: its planes, zeros up to the pitch, and zeros for a row that does not count.  One thread: 8 values.
+// src (R, C) as an operand: its planes, zeros up to the pitch, and zeros for a row that does not count.  One thread: 8 values; one
+// launch for all of a pass (blockIdx.y).
+struct PackJob { const void* src; int64_t R; Counts counts; const float* amax; char* dst; };
+struct PackJobs { PackJob job[2]; };
 template <typename S, typename T, int P>
-__global__ __launch_bounds__(256) void ce_pack_kernel(const S* __restrict__ src, int64_t R, int C, Counts counts, const float* __restrict__ amax,
-                                                      char* __restrict__ dst, int64_t pitch) {
-    const int ex = P == 2 ? amax_exp(amax) : 0;
+__global__ __launch_bounds__(256) void ce_pack_kernel(PackJobs jobs, int C, int64_t pitch) {
+    const PackJob& job = jobs.job[blockIdx.y];
+    const S* __restrict__ src = reinterpret_cast<const S*>(job.src);
+    char* __restrict__ dst = job.dst;
+    const Counts counts = job.counts;
+    const int64_t R = job.R;
+    const int ex = P == 2 ? amax_exp(job.amax) : 0;
     const int per = (int)(pitch / (16 * P));               // threads of a row
     for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < R * per; at += (int64_t)gridDim.x * 256) {
         const int64_t r = at / per;
@@ -119,6 +126,12 @@ __global__ __launch_bounds__(256) void ce_pack_kernel(const S* __restrict__ src,
     }
 }
 
+// f: upstream / count (mean), upstream (sum), or the power of two that ce_coef_kernel chose
+struct Factor {
+    const float* up; const float* count;
+    __device__ __forceinline__ float operator()() const { return count ? up[0] / count[0] : up[0]; }
+};
+
 // ---------------------------------------------------------------- logits
 struct LogitArgs {
     Operand W, X;                                // vocabulary rows (of the piece), position rows
@@ -134,6 +147,7 @@ struct LogitArgs {
     char* E; int64_t pitchE;
     int rowsE;
     float* pdb;
+    float* db; Factor f;                         // db itself where one tile holds all positions, times f
 };
 
 template <class M>
@@ -311,12 +325,6 @@ __global__ __launch_bounds__(1024) void ce_total_kernel(const float* __restrict_
 }
 
 // ---------------------------------------------------------------- gradient
-// f: upstream / count (mean), upstream (sum), or the power of two that ce_coef_kernel chose
-struct Factor {
-    const float* up; const float* count;
-    __device__ __forceinline__ float operator()() const { return count ? up[0] / count[0] : up[0]; }
-};
-
 // Not reduced: coef[n] = g_n dloss[n] / s with s a power of two >= max |g dloss| (so that E stays in [-1, 1]); fscale[0] = s.
 __global__ __launch_bounds__(1024) void ce_coef_kernel(const float* __restrict__ dloss, const float* __restrict__ gate, int N,
                                                        float* __restrict__ coef, float* __restrict__ fscale) {
@@ -387,7 +395,10 @@ __global__ __launch_bounds__(M::NT, 2) void ce_grad_kernel(LogitArgs p) {
             float sum = 0.f;
 #pragma unroll
             for (int k = 0; k < M::WN; ++k) sum += part[k * M::BM + r];
-            if (a0 + r < p.V) p.pdb[(int64_t)tb * p.V + a0 + r] = sum;
+            if (a0 + r < p.V) {
+                if (p.db) p.db[a0 + r] = sum * p.f();
+                else p.pdb[(int64_t)tb * p.V + a0 + r] = sum;
+            }
         }
         __syncthreads();
     }
@@ -523,9 +534,13 @@ struct Blob {                                    // carves a workspace; a first 
     }
 };
 
-constexpr int64_t kMaxN = 1 << 21, kMaxV = 1 << 24, kMaxC = 1 << 16;   // rows of operands stay below kMaxPitch
+constexpr int64_t kMaxN = 1 << 21, kMaxV = 1 << 24, kMaxC = 1 << 16;
+constexpr int64_t kMaxPiece = 1 << 21;           // classes of a piece
+static_assert(kMaxC * 4 <= kMaxPitch && kMaxPiece * 4 <= kMaxPitch, "rows of every operand");
+constexpr int64_t kMaxTiles = 1 << 22;           // of a launch: its 512 kMaxTiles threads stay below 2^32
+inline int64_t tiles_of(int64_t n, int side) { return (n + side - 1) / side; }
 inline bool shape_ok(int64_t N, int64_t C, int64_t V) {
-    return N > 0 && C > 0 && V > 0 && N <= kMaxN && V <= kMaxV && C <= kMaxC && (N / 128 + 1) * (V / 128 + 1) < INT32_MAX;
+    return N > 0 && C > 0 && V > 0 && N <= kMaxN && V <= kMaxV && C <= kMaxC && tiles_of(N, 256) * tiles_of(V, 256) <= kMaxTiles;
 }
 
 // Is the matrix an operand as it lies (16-bit, whole stages of k, aligned)?
@@ -555,15 +570,13 @@ Packed plan_packed(void* base, const void* x, const void* w, int dtype, int64_t 
     return p;
 }
 
-inline int64_t tiles_of(int64_t n, int side) { return (n + side - 1) / side; }
-
 // the tile side (256, 128, 64) of a product of a x b results with `stages` stages, and how many workgroups and how many groups of a
 // workgroup's waves share the k of a tile
 struct Choice { int side, splits, groups; };
 inline Choice choose(int64_t a, int64_t b, int64_t stages, int P, bool split) {
     Choice best = {256, 1, 1};
     double least = 0.0;
-    for (int side = 256; side >= 64; side /= 2)
+    for (int side = 256; side >= 64 && tiles_of(a, side) * tiles_of(b, side) <= kMaxTiles; side /= 2)
         for (int s = 1; s <= (split ? 64 : 1) && (s == 1 || stages / s >= 4); s += s < 8 ? 1 : s < 16 ? 2 : 8) {
             MmWork w;
             w.add(tiles_of(a, side) * tiles_of(b, side) * s, (stages + s - 1) / s);
@@ -605,10 +618,12 @@ inline unsigned grid_for(int64_t n) {
 }
 
 template <typename S>
-int pack(const void* src, int64_t R, int64_t C, const Counts& counts, const float* amax, char* dst, int64_t pitch, hipStream_t st) {
+int pack(const PackJobs& jobs, int count, int64_t C, int64_t pitch, hipStream_t st) {
     constexpr int P = Inner<S>::P;
-    hipLaunchKernelGGL((ce_pack_kernel<S, typename Inner<S>::T, P>), dim3(grid_for(R * (pitch / (16 * P)))), dim3(256), 0, st, (const S*)src, R, (int)C,
-                       counts, amax, dst, pitch);
+    int64_t rows = jobs.job[0].R;
+    if (count == 2 && jobs.job[1].R > rows) rows = jobs.job[1].R;
+    hipLaunchKernelGGL((ce_pack_kernel<S, typename Inner<S>::T, P>), dim3(grid_for(rows * (pitch / (16 * P))), count), dim3(256), 0, st, jobs, (int)C,
+                       pitch);
     return (int)hipGetLastError();
 }
 
@@ -647,8 +662,11 @@ int ce_fwd(const void* x, const void* w, const float* bias, const int64_t* targe
         a.amaxX = k.amaxX;
         a.amaxW = k.amaxW;
     }
-    if (k.Xp && (rc = pack<S>(x, N, C, counts, k.amaxX, k.Xp, k.pitch, st)) != 0) return rc;
-    if (k.Wp && (rc = pack<S>(w, V, C, Counts{}, k.amaxW, k.Wp, k.pitch, st)) != 0) return rc;
+    PackJobs jobs = {};
+    int copies = 0;
+    if (k.Xp) jobs.job[copies++] = {x, N, counts, k.amaxX, k.Xp};
+    if (k.Wp) jobs.job[copies++] = {w, V, Counts{}, k.amaxW, k.Wp};
+    if (copies && (rc = pack<S>(jobs, copies, C, k.pitch, st)) != 0) return rc;
     a.X = {k.Xp ? k.Xp : (const char*)x, k.pitch, (int)N};
     a.W = {k.Wp ? k.Wp : (const char*)w, k.pitch, (int)V};
     a.bias = bias;
@@ -683,7 +701,7 @@ BwdPlan plan_bwd(Blob& ws, int dtype, int64_t N, int64_t C, int64_t V, bool want
     p.rowsE = up(N, 64);
     int64_t most = (int64_t)(kPieceBytes / (size_t)(p.rowsE * 2 * P)) / 256 * 256;
     if (most < 256) most = 256;
-    if (most > (1 << 21)) most = 1 << 21;        // a row of E stays below the operand's largest pitch
+    if (most > kMaxPiece) most = kMaxPiece;
     const int64_t pieces = (V + most - 1) / most;
     p.Vc = pieces == 1 ? V : up((V + pieces - 1) / pieces, 256);
     p.pieces = (int)((V + p.Vc - 1) / p.Vc);
@@ -730,7 +748,8 @@ int ce_bwd(const float* dloss, const void* x, const void* w, const float* bias, 
     }
     const char* Xw = X;                          // of dw: rows that do not count are zeros (a copy made by the forward pass has them so)
     if (dw && !k.Xp) {
-        if ((rc = pack<S>(x, N, C, Counts{gate, nullptr, 0, nullptr, 0.f}, nullptr, p.Xg, k.pitch, st)) != 0) return rc;
+        const PackJobs jobs = {{{x, N, Counts{gate, nullptr, 0, nullptr, 0.f}, nullptr, p.Xg}}};
+        if ((rc = pack<S>(jobs, 1, C, k.pitch, st)) != 0) return rc;
         Xw = p.Xg;
     }
     for (int i = 0; i < p.pieces; ++i) {
@@ -747,6 +766,8 @@ int ce_bwd(const float* dloss, const void* x, const void* w, const float* bias, 
         a.lse = lse; a.gate = gate; a.coef = reduction == 0 ? p.coef : nullptr;
         a.E = dx || dw ? p.E : nullptr; a.pitchE = p.pitchE; a.rowsE = (int)p.rowsE;
         a.pdb = p.pdb;
+        a.db = db && a.tilesN == 1 ? db + v0 : nullptr;
+        a.f = f;
         const dim3 grid(a.tilesV * a.tilesN);
 #define SSECG_CE_GRAD(...)                                                              \
     do {                                                                                \
@@ -756,7 +777,8 @@ int ce_bwd(const float* dloss, const void* x, const void* w, const float* bias, 
     } while (0)
         SSECG_CE_TILES(p.cl, SSECG_CE_GRAD, false, false);
 #undef SSECG_CE_GRAD
-        if (db) hipLaunchKernelGGL(ce_db_kernel, dim3((unsigned)((vn + 255) / 256)), dim3(256), 0, st, p.pdb, a.tilesN, (int)vn, f, db + v0);
+        if (db && !a.db)
+            hipLaunchKernelGGL(ce_db_kernel, dim3((unsigned)((vn + 255) / 256)), dim3(256), 0, st, p.pdb, a.tilesN, (int)vn, f, db + v0);
         if (dx) {                                // E along its rows, W across
             ProdArgs q = {};
             q.A = {p.E, p.pitchE, (int)N};

@@ -16,7 +16,6 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 enum { kF32 = 0, kB16 = 1, kF16 = 2 };
 inline bool dtype_ok(int t) { return t == kF32 || t == kB16 || t == kF16; }
-inline size_t dtype_size(int t) { return t == kF32 ? 4 : 2; }
 
 // 16 bytes of elements, at any alignment that the element itself has (the hardware takes unaligned global accesses)
 template <typename T> struct Vec;

@@ -430,10 +430,4 @@ __device__ __forceinline__ uint16_t plane16(float v, int q) {
     return __builtin_isinf(f) ? 0 : bits16((_Float16)(v - f));   // an infinity stays one instead of inf - inf
 }
 
-__device__ __forceinline__ void split16(float v, _Float16& hi, _Float16& lo) {
-    hi = (_Float16)v;
-    const float f = (float)hi;
-    lo = __builtin_isinf(f) ? (_Float16)0.f : (_Float16)(v - f);   // an infinity stays one instead of inf - inf
-}
-
 }  // namespace ssecg_lm

@@ -207,6 +207,13 @@ class FusedMuon(FusedAdamW):
             raise ValueError("invalid Muon hyper-parameter")
         super().add_param_group(param_group)
 
+    def load_state_dict(self, state_dict):
+        """A state of ``FusedAdamW`` or torch.optim.AdamW loads too: the matrices start with no momentum."""
+        super().load_state_dict(state_dict)
+        for group in self.param_groups:
+            for k, v in self._muon_defaults.items():
+                group.setdefault(k, v)
+
     @torch.no_grad()
     def step(self, closure=None, found_inf=None):
         """``found_inf``: device float tensor; non-zero -> this update is skipped inside the kernels (no host sync)."""
