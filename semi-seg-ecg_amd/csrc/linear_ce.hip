@@ -274,21 +274,33 @@ __device__ __forceinline__ void join_lse(float& m, float& s, float m2, float s2)
     m = mt;
 }
 
-// joins the parts of a row: lse, g and the row's loss.  A workgroup: 16 rows x 64 strands of parts.
+// joins the parts of a row: lse, g and the row's loss.  A workgroup: ROWS rows, 1024 / ROWS strands of parts each.
+template <int ROWS>
 __global__ __launch_bounds__(1024) void ce_join_kernel(const float* __restrict__ pm, const float* __restrict__ ps, const float* __restrict__ tl,
                                                        int parts, int N, int V, const int64_t* __restrict__ target, Counts counts,
                                                        float* __restrict__ lse, float* __restrict__ gate, float* __restrict__ row_loss) {
-    __shared__ float sm[16][17], ss[16][17];
-    const int c = threadIdx.x & 15, k = threadIdx.x >> 4, n = blockIdx.x * 16 + c;
+    __shared__ float sm[16][ROWS + 1], ss[16][ROWS + 1];
+    constexpr int K = 1024 / ROWS;
+    const int c = threadIdx.x % ROWS, k = threadIdx.x / ROWS, n = blockIdx.x * ROWS + c;
     float m = -INFINITY, s = 0.f;
     if (n < N)
-        for (int p = k; p < parts; p += 64) join_lse(m, s, pm[(int64_t)p * N + n], ps[(int64_t)p * N + n]);
+        for (int p = k; p < parts; p += 4 * K) {          // 4 loads in flight
+            float m2[4], s2[4];
 #pragma unroll
-    for (int o = 16; o < 64; o *= 2) {                    // the wave's 4 strands
+            for (int j = 0; j < 4; ++j) {
+                const bool in = p + j * K < parts;
+                m2[j] = in ? pm[(int64_t)(p + j * K) * N + n] : -INFINITY;
+                s2[j] = in ? ps[(int64_t)(p + j * K) * N + n] : 0.f;
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) join_lse(m, s, m2[j], s2[j]);
+        }
+#pragma unroll
+    for (int o = ROWS; o < 64; o *= 2) {                  // the wave's strands
         const float m2 = __shfl_xor(m, o, 64), s2 = __shfl_xor(s, o, 64);
         join_lse(m, s, m2, s2);
     }
-    if ((threadIdx.x & 63) < 16) { sm[threadIdx.x >> 6][c] = m; ss[threadIdx.x >> 6][c] = s; }
+    if ((threadIdx.x & 63) < ROWS) { sm[threadIdx.x >> 6][c] = m; ss[threadIdx.x >> 6][c] = s; }
     __syncthreads();
     if (k != 0 || n >= N) return;
     for (int q = 1; q < 16; ++q) join_lse(m, s, sm[q][c], ss[q][c]);
@@ -371,6 +383,7 @@ __global__ __launch_bounds__(M::NT, 2) void ce_grad_kernel(LogitArgs p) {
     float* part = reinterpret_cast<float*>(lds);          // DB: column sums [WN][BM] of the waves
 #pragma unroll
     for (int i = 0; i < M::TM; ++i) {
+        float sums[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
             float sum = 0.f;
@@ -381,11 +394,22 @@ __global__ __launch_bounds__(M::NT, 2) void ce_grad_kernel(LogitArgs p) {
                 acc[i][j][e] = q * (float)(1 << kEScale);
                 sum += q;
             }
-            if (DB) {                                                // column sum over the wave's positions
+            sums[e] = sum;
+        }
+        if (DB) {
+            // column sums over the wave's 32 positions: at each exchange a lane keeps half of its sums and hands the others over (16
+            // exchanges; 80 for one sum after the other).  Lane l ends with register (l / 2) % 16.
 #pragma unroll
-                for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
-                if ((lane & 31) == 0) part[wn * M::BM + M::arow(i, e)] = sum;
+            for (int half = 8; half > 0; half >>= 1) {
+                const bool upper = (lane & 2 * half) != 0;
+#pragma unroll
+                for (int k = 0; k < half; ++k) {
+                    const float give = upper ? sums[k] : sums[k + half], keep = upper ? sums[k + half] : sums[k];
+                    sums[k] = keep + __shfl_xor(give, 2 * half, 64);
+                }
             }
+            sums[0] += __shfl_xor(sums[0], 1, 64);
+            if ((lane & 1) == 0) part[wn * M::BM + M::arow(i, (lane >> 1) & 15)] = sums[0];
         }
         __builtin_amdgcn_sched_barrier(0);
     }
@@ -678,8 +702,13 @@ int ce_fwd(const void* x, const void* w, const float* bias, const int64_t* targe
     SSECG_CE_TILES(p.c, SSECG_CE_LSE, false, false);
 #undef SSECG_CE_LSE
     float* row = reduction == 0 ? loss : p.row;
-    hipLaunchKernelGGL(ce_join_kernel, dim3((unsigned)((N + 15) / 16)), dim3(1024), 0, st, p.pm, p.ps, p.tl, p.parts, (int)N, (int)V, target, counts,
-                       lse, gate, row);
+    // few rows: more strands each (8 rows of 1024 parts: 8.0 us with 16 rows to a workgroup); many: whole sectors of their parts
+    if (N < 1024)
+        hipLaunchKernelGGL(ce_join_kernel<2>, dim3((unsigned)((N + 1) / 2)), dim3(1024), 0, st, p.pm, p.ps, p.tl, p.parts, (int)N, (int)V, target,
+                           counts, lse, gate, row);
+    else
+        hipLaunchKernelGGL(ce_join_kernel<16>, dim3((unsigned)((N + 15) / 16)), dim3(1024), 0, st, p.pm, p.ps, p.tl, p.parts, (int)N, (int)V, target,
+                           counts, lse, gate, row);
     hipLaunchKernelGGL(ce_total_kernel, dim3(1), dim3(1024), 0, st, row, target, ignore, (int)N, reduction == 1 ? 1 : 0,
                        reduction == 0 ? nullptr : loss, count);
     return (int)hipGetLastError();
