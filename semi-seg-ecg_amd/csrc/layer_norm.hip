@@ -3,12 +3,14 @@
 //   mu = mean(x), r = 1 / sqrt(mean((x - mu)^2) + eps), xh = (x - mu) r, y = xh w + b
 //   g = dy w,  dx = r (g - mean(g) - xh mean(g xh)),  dw = sum_rows dy xh,  db = sum_rows dy
 //
-// Both passes are bound by HBM: forward reads x and writes y, backward reads x and dy and writes dx - each byte once.  A row
-// stays in the registers of the threads that own it (64 to 1024 of them), so the
-// variance is the two-pass one (the sum of squared differences from the mean, no cancellation) without a second read.  A thread
-// owns the same columns of every row its workgroup takes: w and b are loaded once, and the column sums dw / db grow in its
-// registers; the row groups of a workgroup are joined in LDS, the workgroups by a second launch in fixed order (no atomics:
-// results do not change from run to run).  Statistics, sums and parameter gradients are fp32; y and dx are rounded once.
+// Both passes are bound by HBM: forward reads x and writes y, backward reads x and dy and writes dx - each byte once.  32768 x 4096
+// bf16: 90 us and 174 us (6.0 and 4.6 TB/s; a large copy reaches 5.0), and 5 us for the parameters' gradients.  Below a few
+// megabytes latency counts: 1008 x 512 fp32 takes 3.9 us, and 6.3 + 4.4 us backward.  A row stays in the registers of the threads
+// that own it (64 to 1024 of them), so the variance is the two-pass one (the sum of squared differences from the mean, no
+// cancellation) without a second read.  A thread owns the same columns of every row its workgroup takes: w and b are loaded once,
+// and the column sums dw / db grow in its registers; the row groups of a workgroup are joined in LDS, the workgroups by a second
+// launch in fixed order (no atomics: results do not change from run to run).  Statistics, sums and parameter gradients are fp32; y
+// and dx are rounded once.
 #include "lm_common.h"
 #include "ssecg.h"
 
@@ -370,6 +372,9 @@ __global__ __launch_bounds__(1024) void ln_param_grads_kernel(const float* __res
 
 // Threads per row and 16-byte vectors per thread: the fewest threads whose registers hold the row beside the parameters (and, in the
 // backward pass, the column sums and the next row: 128 registers a thread at 1024 threads).  One wave per row needs no barrier.
+// Longer rows take the kernels that read a row two or three times.  Those cost 131 us forward and 155 us backward at 2000 x 16384
+// bf16 where the registers take 26 and 114 (with 141 values spilled); at 2000 x 16384 fp32 they take 153 us backward, where four
+// vectors a thread (251 spilled) took 181.
 struct LnShape { int tpr, nch; };
 inline LnShape ln_shape(int C, int V, bool bwd) {
     const int64_t vecs = ((int64_t)C + V - 1) / V;
@@ -377,7 +382,7 @@ inline LnShape ln_shape(int C, int V, bool bwd) {
     for (int tpr = 64; tpr <= 1024; tpr *= V == 8 || bwd ? 2 : 4)
         for (int n = 1; n <= most; n *= 2)
             if (vecs <= (int64_t)tpr * n) return {tpr, n};
-    if (bwd && vecs <= 2048 * most) return {1024, 2 * most};
+    if (bwd && V == 8 && vecs <= 2048) return {1024, 2};
     return {0, 0};
 }
 
@@ -390,33 +395,32 @@ int launch_fwd(const void* x, const float* w, const float* b, void* y, float* me
     return (int)hipGetLastError();
 }
 
-// Workgroups of the backward pass: 1024 threads, one per CU, if that gives every CU one; else as few threads as a row takes (256 at
-// least), so that few rows still reach many CUs.
+// Workgroups of the backward pass: 1024 threads, one per CU, if that gives every CU one (16384 x 1024 bf16: 28.7 us; 512 of 256
+// threads 31.4, 256 of them 44.3) or a row takes 512 threads (300 x 4096 fp32: 11.3 us; one row a workgroup, with twice the partial
+// sums, 13.6); else 256 threads, so that few rows still reach many CUs (1008 x 512 bf16: 9.4 us; 1024 threads 11.2).
 struct LnGrid { int nt, parts; };
 inline LnGrid ln_grid(int64_t rows, int C, int dtype) {
     const LnShape s = ln_shape(C, dtype == kF32 ? 4 : 8, true);
     if (!s.tpr) return {1024, (int)(rows < 32 ? rows : 32)};           // very long rows: few slabs bound the workspace
     const int64_t g = 1024 / s.tpr, wide = (rows + g - 1) / g;
-    if (s.tpr == 1024 || wide >= 256) return {1024, (int)(wide < 256 ? wide : 256)};
-    const int nt = s.tpr < 256 ? 256 : s.tpr;
-    return {nt, (int)((rows * s.tpr + nt - 1) / nt)};
+    if (s.tpr >= 512 || wide >= 256) return {1024, (int)(wide < 256 ? wide : 256)};
+    return {256, (int)((rows * s.tpr + 255) / 256)};
 }
 
+template <typename T, int TPR, int NT, int NCH>
+int launch_bwd_of(const void* dy, const void* x, const float* mean, const float* rstd, const float* w, void* dx, float* partial, int64_t rows,
+                  int C, int parts, hipStream_t st) {
+    const size_t lds = partial && TPR < NT ? (size_t)(NT / TPR / 2) * C * sizeof(float) : 0;
+    hipLaunchKernelGGL((ln_bwd_kernel<T, TPR, NT, NCH>), dim3((unsigned)parts), dim3(NT), lds, st, (const T*)dy, (const T*)x, mean, rstd, w, (T*)dx,
+                       partial, rows, C);
+    return (int)hipGetLastError();
+}
 template <typename T, int TPR, int NCH>
 int launch_bwd(const void* dy, const void* x, const float* mean, const float* rstd, const float* w, void* dx, float* partial, int64_t rows,
                int C, const LnGrid& g, hipStream_t st) {
-    if (TPR < 1024 && g.nt < 1024) {
-        constexpr int NT = TPR < 256 ? 256 : TPR;
-        const size_t lds = partial && TPR < NT ? (size_t)(NT / TPR / 2) * C * sizeof(float) : 0;
-        hipLaunchKernelGGL((ln_bwd_kernel<T, TPR, NT, NCH>), dim3((unsigned)g.parts), dim3(NT), lds, st, (const T*)dy, (const T*)x, mean, rstd, w,
-                           (T*)dx, partial, rows, C);
-    } else {
-        constexpr int NT = 1024;
-        const size_t lds = partial && TPR < NT ? (size_t)(NT / TPR / 2) * C * sizeof(float) : 0;
-        hipLaunchKernelGGL((ln_bwd_kernel<T, TPR, NT, NCH>), dim3((unsigned)g.parts), dim3(NT), lds, st, (const T*)dy, (const T*)x, mean, rstd, w,
-                           (T*)dx, partial, rows, C);
-    }
-    return (int)hipGetLastError();
+    if constexpr (TPR <= 256)
+        if (g.nt == 256) return launch_bwd_of<T, TPR, 256, NCH>(dy, x, mean, rstd, w, dx, partial, rows, C, g.parts, st);
+    return launch_bwd_of<T, TPR, 1024, NCH>(dy, x, mean, rstd, w, dx, partial, rows, C, g.parts, st);
 }
 
 template <typename T>
@@ -442,7 +446,7 @@ int ln_bwd(const void* dy, const void* x, const float* mean, const float* rstd, 
 #define SSECG_LN_CASE(TPR, NCH) if (s.tpr == TPR && s.nch == NCH) return launch_bwd<T, TPR, NCH>(dy, x, mean, rstd, w, dx, partial, rows, C, g, st)
     SSECG_LN_CASE(64, 1); SSECG_LN_CASE(1024, 2);
     if constexpr (Vec<T>::N == 4) {
-        SSECG_LN_CASE(64, 2); SSECG_LN_CASE(128, 2); SSECG_LN_CASE(256, 2); SSECG_LN_CASE(512, 2); SSECG_LN_CASE(1024, 4);
+        SSECG_LN_CASE(64, 2); SSECG_LN_CASE(128, 2); SSECG_LN_CASE(256, 2); SSECG_LN_CASE(512, 2);
     } else {
         SSECG_LN_CASE(128, 1); SSECG_LN_CASE(256, 1); SSECG_LN_CASE(512, 1); SSECG_LN_CASE(1024, 1);
     }
