@@ -1342,6 +1342,12 @@ def _lm_vec(t, name, n, device):
     return t if t.dtype == torch.float32 else t.float()
 
 
+def _lm_aligned(t):
+    """On a 16-byte boundary, as everything from the allocator is: whether an operand is copied then depends on its type and sizes
+    alone, in the backward pass as in the forward one."""
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
 def _lm_device(device, name, t):
     if t is not None and t.device != device:
         raise SsecgError(f"{name}: on {t.device}, expected {device}")
@@ -1441,6 +1447,7 @@ def linear_ce_fwd(x, weight, target, bias=None, conf=None, thresh=0.0, ignore_in
         raise SsecgError("linear_ce: target must have x's shape without its last axis")
     (V, C), N, mode = weight.shape, target.numel(), _REDUCTION[reduction]
     dev = x.device
+    x, weight = _lm_aligned(x), _lm_aligned(weight)
     bias = _lm_vec(bias, "bias", V, dev)
     if conf is not None:
         conf = _req(conf, "conf")
@@ -1471,6 +1478,7 @@ def linear_ce_bwd(saved, dloss=None, want_dx=True, want_dweight=True, want_dbias
     """-> (dx, dweight of their operands' type, dbias in fp32): gradients of ``linear_ce_fwd``'s loss times ``dloss`` (a device scalar,
     or one value per position for reduction "none"; None = 1).  What is not wanted (or has no bias) is None."""
     x, weight, bias, target, lse, gate, count, packed, mode = saved
+    x, weight = _lm_aligned(x), _lm_aligned(weight)
     trace("linear_ce_bwd", tuple(x.shape), tuple(weight.shape))
     (V, C), N = weight.shape, target.numel()
     shape = target.shape if mode == 0 else ()

@@ -194,8 +194,6 @@ class FusedMuon(FusedAdamW):
 
     def __init__(self, params, lr=1e-3, momentum=0.95, nesterov=True, weight_decay=0.1, ns_steps=5, ns_eps=1e-7,
                  adjust_lr="match_rms_adamw", betas=(0.9, 0.999), eps=1e-8):
-        if not 0.0 <= momentum < 1.0 or not 1 <= int(ns_steps) <= 100 or not ns_eps >= 0.0 or adjust_lr not in self.ADJUST:
-            raise ValueError("invalid Muon hyper-parameter")
         self._muon_defaults = dict(momentum=momentum, nesterov=bool(nesterov), ns_steps=int(ns_steps), ns_eps=ns_eps, adjust_lr=adjust_lr,
                                    muon=True)
         super().__init__(params, lr=lr, betas=betas, eps=eps, weight_decay=weight_decay)
@@ -203,9 +201,15 @@ class FusedMuon(FusedAdamW):
     def add_param_group(self, param_group):
         for k, v in self._muon_defaults.items():
             param_group.setdefault(k, v)
-        if param_group["adjust_lr"] not in self.ADJUST:
+        if (not 0.0 <= param_group["momentum"] < 1.0 or not 1 <= int(param_group["ns_steps"]) <= 100 or not param_group["ns_eps"] >= 0.0
+                or param_group["adjust_lr"] not in self.ADJUST):
             raise ValueError("invalid Muon hyper-parameter")
         super().add_param_group(param_group)
+        group = self.param_groups[-1]
+        for p in group["params"] if group["muon"] else ():
+            if p.dim() >= 2 and p.numel() and max(p.shape[0], p.numel() // p.shape[0]) > 1 << 20:
+                self.param_groups.pop()
+                raise ValueError(f"FusedMuon: a matrix of {tuple(p.shape)} has more than 2^20 rows or columns: give it a group with muon=False")
 
     def load_state_dict(self, state_dict):
         """A state of ``FusedAdamW`` or torch.optim.AdamW loads too: the matrices start with no momentum."""
