@@ -84,3 +84,32 @@ def test_muon_hyper_parameters():
     p.grad = torch.zeros(4, 4)
     with pytest.raises(SsecgError):
         opt.step()                   # a CPU parameter
+
+
+def test_limits_are_refused_before_anything_is_sized():
+    from ssecg.lib import lib
+    from ssecg.optim import FusedMuon
+    L = lib()
+    assert L.ssecg_linear_ce_fwd_workspace(1, 1 << 21, 64, 1 << 17) > 0
+    for N, C, V in ((1 << 21, 64, (1 << 17) + 1), ((1 << 21) + 1, 64, 8), (8, (1 << 16) + 1, 8), (8, 8, (1 << 24) + 1)):
+        assert L.ssecg_linear_ce_fwd_workspace(1, N, C, V) == 0 == L.ssecg_linear_ce_bwd_workspace(1, N, C, V, 1, 1, 1)
+        assert L.ssecg_linear_ce_fwd(256, 256, None, 256, None, 0.0, -100, 1, N, C, V, 1, 256, 256, 256, 256, None, 0, 256, 1 << 40, None) == -1
+    assert L.ssecg_layer_norm_bwd_workspace(0, 4, (1 << 24) + 1) == 0
+    assert L.ssecg_orthogonalize_workspace(_i64(0, 0, 0, (1 << 20) + 1, 4), 1) == 0
+    big, small = torch.nn.Parameter(torch.empty((1 << 20) + 1, 2)), torch.nn.Parameter(torch.empty(4, 2))
+    with pytest.raises(ValueError):
+        FusedMuon([big])
+    opt = FusedMuon([{"params": [big], "muon": False}, {"params": [small]}])
+    for bad in (dict(ns_steps=101), dict(momentum=-0.1), dict(ns_eps=float("nan")), dict(adjust_lr=1)):
+        with pytest.raises(ValueError):
+            opt.add_param_group(dict(params=[torch.nn.Parameter(torch.empty(2, 2))], **bad))
+    assert len(opt.param_groups) == 2
+
+
+def test_every_piece_of_the_vocabulary_is_covered_once():
+    """The backward workspace holds a bounded piece of the gradient of the logits, whatever the vocabulary."""
+    from ssecg.lib import lib
+    L = lib()
+    whole = L.ssecg_linear_ce_bwd_workspace(1, 8192, 1024, 65536, 1, 1, 0)
+    assert (1 << 30) <= whole < (1 << 30) + (1 << 28)
+    assert L.ssecg_linear_ce_bwd_workspace(1, 8192, 1024, 1 << 20, 1, 1, 0) < 2 * whole

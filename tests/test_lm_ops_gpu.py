@@ -563,3 +563,126 @@ def test_fixmatch_trains_with_muon():
         assert torch.isfinite(p).all() and not torch.equal(p, before[k]), k
     convs = [p for p in model.parameters() if p.dim() >= 2]
     assert all("momentum_buffer" in opt.state[p] for p in convs) and all("exp_avg" in opt.state[p] for p in model.parameters() if p.dim() < 2)
+
+
+# ------------------------------------------------------------------------------------------------ calls at once, other callers' habits
+def test_two_streams_and_two_graphs_share_nothing():
+    """The same operators on two streams at once and in two captured graphs replayed in turn: every result is the one alone."""
+    from ssecg import ops
+    cases = [_ce_case(40 + k, 200 + 31 * k, 96, 700, torch.bfloat16, True, True) for k in range(2)]
+    mats = [_normal(_gen(42 + k), 130 + k, 260) for k in range(2)]
+
+    def work(k):
+        x, w, b, t, conf = cases[k]
+        loss, saved = ops.linear_ce_fwd(x, w, t, b, conf, 0.3)
+        y, mean, rstd = ops.layer_norm_fwd(x)
+        return (loss, *ops.linear_ce_bwd(saved), y, *ops.layer_norm_bwd(x, x, mean, rstd), ops.orthogonalize(mats[k]))
+    alone = [work(k) for k in range(2)]
+    torch.cuda.synchronize()
+    streams, both = [torch.cuda.Stream() for _ in range(2)], [None, None]
+    for _ in range(4):
+        for k, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                both[k] = work(k)
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, q) for k in range(2) for p, q in zip(both[k], alone[k]))
+    graphs, held = [], []
+    for k in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            held.append(work(k))
+        graphs.append(g)
+    for _ in range(3):
+        for k in (1, 0):
+            for p in held[k]:
+                p.zero_()
+            graphs[k].replay()
+            work(1 - k)
+            torch.cuda.synchronize()
+            assert all(torch.equal(p, q) for p, q in zip(held[k], alone[k]))
+
+
+def test_linear_ce_summed_per_position_and_twice_backward():
+    from ssecg import functional as SF
+    x, w, b, t, conf = _ce_case(50, 33, 64, 129, torch.float32, True, True)
+    x.requires_grad_(True), w.requires_grad_(True)
+    per = SF.masked_linear_cross_entropy(x, w, t, conf, 0.4, bias=b, reduction="none")
+    total = SF.masked_linear_cross_entropy(x, w, t, conf, 0.4, bias=b, reduction="sum")
+    first = torch.autograd.grad(per.sum(), (x, w), retain_graph=True)      # dloss arrives expanded, stride 0
+    again = torch.autograd.grad(per.sum(), (x, w))
+    assert all(torch.equal(p, q) for p, q in zip(first, again))
+    want, bound = R.linear_ce(x.detach(), w.detach(), t, b, conf, 0.4, reduction="sum")
+    for got, v, e, what in zip((total.detach(), *first), want, bound, ("loss", "dx", "dw")):
+        R.within(got, v, e, what)
+    with pytest.raises(RuntimeError):
+        g = torch.autograd.grad(total, x, create_graph=True)[0]
+        g.sum().backward()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_linear_ce_saved_tensors_may_move(dtype):
+    """Saved tensors that come back elsewhere in memory, off a 16-byte boundary too (offloading hooks)."""
+    from ssecg import functional as SF
+    x, w, b, t, _ = _ce_case(51, 40, 64, 100, dtype, True, False)
+    x = torch.empty(40 * 64 + 1, dtype=dtype, device="cuda")[1:].view(40, 64).copy_(x).requires_grad_(True)
+    w.requires_grad_(True)
+    plain = torch.autograd.grad(SF.linear_cross_entropy(x, w, t, bias=b), (x, w))
+
+    def moved(s):
+        return torch.empty(s.numel() + 1, dtype=s.dtype, device=s.device)[1:].view(s.shape).copy_(s)
+    with torch.autograd.graph.saved_tensors_hooks(lambda s: s.detach().clone(), moved):
+        loss = SF.linear_cross_entropy(x, w, t, bias=b)
+    assert all(torch.equal(p, q) for p, q in zip(torch.autograd.grad(loss, (x, w)), plain))
+
+
+def test_linear_ce_wants_only_what_is_asked_for():
+    from ssecg import ops
+    x, w, b, t, _ = _ce_case(52, 70, 48, 90, torch.bfloat16, True, False)
+    _, saved = ops.linear_ce_fwd(x, w, t, b)
+    whole = ops.linear_ce_bwd(saved)
+    for k in range(3):
+        want = [k == i for i in range(3)]
+        part = ops.linear_ce_bwd(saved, None, *want)
+        assert [p is not None for p in part] == want and torch.equal(part[k], whole[k])
+    assert ops.linear_ce_bwd(saved, None, False, False, False) == (None, None, None)
+
+
+def test_refusals_on_the_device():
+    from ssecg import ops
+    from ssecg.lib import SsecgError
+    x, w, b, t, conf = _ce_case(53, 12, 64, 30, torch.float32, True, True)
+    y, mean, rstd = ops.layer_norm_fwd(x)
+    for call in (lambda: ops.linear_ce_fwd(x, w.bfloat16(), t), lambda: ops.linear_ce_fwd(x, w[:, :32], t), lambda: ops.linear_ce_fwd(x, w, t[:5]),
+                 lambda: ops.linear_ce_fwd(x, w, t.int()), lambda: ops.linear_ce_fwd(x, w, t, b[:3]), lambda: ops.linear_ce_fwd(x, w, t, b.cpu()),
+                 lambda: ops.linear_ce_fwd(x, w, t, conf=conf[:2]), lambda: ops.linear_ce_fwd(x, w, t, conf=conf.half()),
+                 lambda: ops.linear_ce_fwd(x, w, t, reduction="avg"), lambda: ops.linear_ce_fwd(x.double(), w.double(), t),
+                 lambda: ops.linear_ce_bwd(ops.linear_ce_fwd(x, w, t)[1], torch.ones(12, device="cuda")),
+                 lambda: ops.linear_ce_bwd(ops.linear_ce_fwd(x, w, t, reduction="none")[1], torch.ones(1, device="cuda")),
+                 lambda: ops.layer_norm_fwd(x, w[0][:5]), lambda: ops.layer_norm_fwd(x, eps=-1.0), lambda: ops.layer_norm_fwd(x[:, :0]),
+                 lambda: ops.layer_norm_bwd(y.half(), x, mean, rstd), lambda: ops.layer_norm_bwd(y[:5], x, mean, rstd),
+                 lambda: ops.layer_norm_bwd(y, x, mean[:5], rstd), lambda: ops.layer_norm_bwd(y, x, mean.double(), rstd),
+                 lambda: ops.orthogonalize(x[0]), lambda: ops.orthogonalize([x, x.half()]), lambda: ops.orthogonalize(x, eps=-1.0),
+                 lambda: ops.orthogonalize(x, steps=101), lambda: ops.orthogonalize([x, x.cpu()])):
+        with pytest.raises(SsecgError):
+            call()
+
+
+def test_muon_takes_an_adamw_state():
+    from ssecg.optim import FusedAdamW, FusedMuon
+    g = _gen(54)
+    make = lambda: [torch.nn.Parameter(t.clone()) for t in tensors]   # noqa: E731
+    tensors = [_normal(g, 30, 20), _normal(g, 9)]
+    a, b = make(), make()
+    adam, muon = FusedAdamW(a, lr=1e-2), FusedMuon(b, lr=0.3)
+    for p in a:
+        p.grad = torch.ones_like(p)
+    adam.step()
+    muon.load_state_dict(copy.deepcopy(adam.state_dict()))
+    with torch.no_grad():
+        for p, q in zip(b, a):
+            p.copy_(q)
+    for p, q in zip(a, b):
+        p.grad, q.grad = torch.ones_like(p), torch.ones_like(q)
+    adam.step(), muon.step()
+    assert torch.equal(a[1], b[1]) and not torch.equal(a[0], b[0])     # the vector continues AdamW, the matrix starts its momentum
+    assert torch.equal(muon.state[b[0]]["momentum_buffer"], torch.ones_like(b[0]))
