@@ -148,21 +148,25 @@ struct MmTile {
                 }
             }
         }
+        __device__ __forceinline__ void piece(int slot, int i, unsigned back = 0) {
+            lds_dma16(uniform(base), off[i] - back, __builtin_amdgcn_readfirstlane(dst + i * 1024 + slot * SLOT));
+        }
+        __device__ __forceinline__ void advance() {
+            base += step;
+            if (SLOW) left -= BK;
+        }
         __device__ __forceinline__ void issue(int slot) {
-            const char* u = uniform(base);
             if (SLOW && left < BK) {           // the last stage: rows that do not exist are read as the last one
 #pragma unroll
                 for (int i = 0; i < PC; ++i) {
                     const int k = row0 + i * RPP;
-                    const unsigned back = k < left ? 0u : (unsigned)(k - left + 1) * pitch;
-                    lds_dma16(u, off[i] - back, __builtin_amdgcn_readfirstlane(dst + i * 1024 + slot * SLOT));
+                    piece(slot, i, k < left ? 0u : (unsigned)(k - left + 1) * pitch);
                 }
             } else {
 #pragma unroll
-                for (int i = 0; i < PC; ++i) lds_dma16(u, off[i], __builtin_amdgcn_readfirstlane(dst + i * 1024 + slot * SLOT));
+                for (int i = 0; i < PC; ++i) piece(slot, i);
             }
-            base += step;
-            if (SLOW) left -= BK;
+            advance();
         }
     };
 
@@ -227,66 +231,93 @@ struct MmTile {
         constexpr int KK = P == 1 ? 4 : 2;                      // k steps of 16 in a stage
         constexpr bool AHEAD = !(P == 2 && TA && TB && TM * TN > 4);   // (there a second set of fragments would spill)
         V8 a[2][P][TM], b[2][P][TN];                            // two sets: one is multiplied while the other is read
-        auto frags = [&](int set, int slot, int kk) {
-#pragma unroll
-            for (int q = 0; q < P; ++q) {
-                const int c = slot * SLOT + ((4 * q + 2 * kk + h) ^ swz) * 16;
-#pragma unroll
-                for (int i = 0; i < TM; ++i) {
-                    if constexpr (TA)
-                        a[set][q][i] = read_tr(fa + slot * SLOT + Slow<BM>::at(lane, wm * TM + i, kk, 0, q),
-                                               fa + slot * SLOT + Slow<BM>::at(lane, wm * TM + i, kk, 1, q));
-                    else
-                        a[set][q][i] = *reinterpret_cast<const V8*>(fa + i * 4096 + c);
-                }
-#pragma unroll
-                for (int j = 0; j < TN; ++j) {
-                    if constexpr (TB)
-                        b[set][q][j] = read_tr(fb + slot * SLOT + Slow<BN>::at(lane, wn * TN + j, kk, 0, q),
-                                               fb + slot * SLOT + Slow<BN>::at(lane, wn * TN + j, kk, 1, q));
-                    else
-                        b[set][q][j] = *reinterpret_cast<const V8*>(fb + j * 4096 + c);
-                }
+        constexpr int NF = P * (TM + TN);                       // fragments of a k step: in the order of their use, a k-slow B's last
+        auto frag = [&](int set, int slot, int kk, int f) {
+            const int q = f / (TM + TN), at = f % (TM + TN), i = TB || at == 0 ? at : at - TN, j = TB ? at - TM : at - 1;
+            const int c = slot * SLOT + ((4 * q + 2 * kk + h) ^ swz) * 16;
+            if (TB ? at < TM : at == 0 || at > TN) {
+                if constexpr (TA)
+                    a[set][q][i] = read_tr(fa + slot * SLOT + Slow<BM>::at(lane, wm * TM + i, kk, 0, q),
+                                           fa + slot * SLOT + Slow<BM>::at(lane, wm * TM + i, kk, 1, q));
+                else
+                    a[set][q][i] = *reinterpret_cast<const V8*>(fa + i * 4096 + c);
+            } else {
+                if constexpr (TB)
+                    b[set][q][j] = read_tr(fb + slot * SLOT + Slow<BN>::at(lane, wn * TN + j, kk, 0, q),
+                                           fb + slot * SLOT + Slow<BN>::at(lane, wn * TN + j, kk, 1, q));
+                else
+                    b[set][q][j] = *reinterpret_cast<const V8*>(fb + j * 4096 + c);
             }
         };
-        auto multiply = [&](int set) {
-            // two planes: the small products first, each product over all blocks: no accumulator is used twice in a row
+        // Where a wave has its SIMD to itself, what else it issues is spread between the products of a k step, each of which keeps the
+        // pipe busy for 32 cycles (A = X X^T at 4096: 230 -> 205 us); two waves cover for each other, and requests that leave
+        // early count for more (8192 x 1024 x 65536 bf16: dx 951 us, 986 spread).
+        constexpr bool SPREAD = TM * TN > 8;
+        static_assert(!SPREAD || (!TA && !TB), "the spread requests are those of k-fast operands");
+        auto multiply = [&](int set, int extra, auto other) {
+            constexpr int NM = (P == 1 ? 1 : 3) * TM * TN;
 #pragma unroll
-            for (int q = P == 1 ? 2 : 0; q < 3; ++q)
+            for (int m = 0; m < NM; ++m) {
+                // two planes: the small products first, each product over all blocks: no accumulator is used twice in a row
+                const int q = P == 1 ? 2 : m / (TM * TN), i = m % (TM * TN) / TN, j = m % TN;
+                acc[i][j] = F::mfma(a[set][q == 0 ? P - 1 : 0][i], b[set][q == 1 ? P - 1 : 0][j], acc[i][j]);
+                if (SPREAD) {
 #pragma unroll
-                for (int i = 0; i < TM; ++i)
-#pragma unroll
-                    for (int j = 0; j < TN; ++j)
-                        acc[i][j] = F::mfma(a[set][q == 0 ? P - 1 : 0][i], b[set][q == 1 ? P - 1 : 0][j], acc[i][j]);
+                    for (int x = m * extra / NM; x < (m + 1) * extra / NM; ++x) other(x);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
         };
         if (most > 0) {
             stage_wait<R - 2>(n < 1 ? 0 : n - 1 < R - 2 ? n - 1 : R - 2);
-            if (AHEAD && n > 0) frags(0, 0, 0);
+            if (AHEAD && n > 0)
+#pragma unroll
+                for (int f = 0; f < NF; ++f) frag(0, 0, 0, f);
         }
-        int slot = 0;
-        for (int s = 0; s < n; ++s) {
-            const int next = slot + 1 == R ? 0 : slot + 1;
-            // the stage that is requested R - 1 ahead goes into the slot of the stage before this one: every wave has read that one
-            // (it passed the barrier below with no LDS read outstanding)
-            if (s + R - 1 < n) issue(slot == 0 ? R - 1 : slot - 1);
+        int slot = 0, s = 0;
+        for (; s < n; ++s) {
+            // a stage is requested R - 1 ahead, into the slot of the stage before this one: every wave has read that one (it passed the
+            // barrier below with no LDS read outstanding)
+            const bool more = s + R - 1 < n;
+            const int next = slot + 1 == R ? 0 : slot + 1, into = slot == 0 ? R - 1 : slot - 1;
+            if (!SPREAD && more) issue(into);
 #pragma unroll
             for (int kk = 0; kk < KK; ++kk) {
-                if (!AHEAD) frags(kk & 1, slot, kk);
-                if (kk + 1 < KK) {
-                    if (AHEAD) frags((kk + 1) & 1, slot, kk + 1);
+                if (!AHEAD)
+#pragma unroll
+                    for (int f = 0; f < NF; ++f) frag(kk & 1, slot, kk, f);
+                const bool within = kk + 1 < KK;
+                // a fragment of the next k step (spread, behind the last stage: not used)
+                auto read = [&](int f) { frag((kk + 1) & 1, within ? slot : next, within ? kk + 1 : 0, f); };
+                auto read_all = [&]() {
+                    if (AHEAD && !SPREAD)
+#pragma unroll
+                        for (int f = 0; f < NF; ++f) read(f);
+                };
+                if (within) {
+                    read_all();
                 } else if (s + 1 < n) {
                     // the next stage has landed when only the pieces of the stages requested after it are outstanding
                     const int ahead = n - 2 - s < R - 2 ? n - 2 - s : R - 2;
                     stage_wait<R - 2>(ahead);
-                    if (AHEAD) frags((kk + 1) & 1, next, 0);
+                    read_all();
                 }
+                const int pieces = kk == 0 ? PPW : 0;
                 __builtin_amdgcn_sched_barrier(0);   // the reads above travel under the products below
-                multiply(kk & 1);
-                __builtin_amdgcn_sched_barrier(0);
+                multiply(kk & 1, NF + pieces, [&](int x) {
+                    if (x >= pieces) read(x - pieces);
+                    else if (more && x < PA) la.piece(into, x);
+                    else if (more) lb.piece(into, x - PA);
+                });
+                if (SPREAD && more && kk == 0) {
+                    la.advance();
+                    lb.advance();
+                }
             }
             slot = next;
         }
-        for (int s = n < 1 ? 1 : n; s < most; ++s) __builtin_amdgcn_s_barrier();   // (a group with fewer stages)
+        for (s = n < 1 ? 1 : n; s < most; ++s) __builtin_amdgcn_s_barrier();   // (a group with fewer stages)
         // LDS may be reused by the caller behind this point (every wave has read its last stage)
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     }

@@ -13,8 +13,8 @@
 // would lose them.  All matrices are two fp16 planes times 2^13 - singular values stay below 1.21 and P's below 3.45, far inside
 // fp16's range, and an entry keeps 22 bits down to 2^-16 of the largest possible one - with fp32 accumulators.
 //
-// Large matrices are bound by the matrix pipe: 4096 x 4096 takes 3.67 ms for five steps; an update's product 327 us (1.26 PFLOP/s of
-// fp16 products; a large library product reaches 1.3 to 1.6), a symmetric one 223 us (0.92 of those that count: 253 tiles of one
+// Large matrices are bound by the matrix pipe: 4096 x 4096 takes 3.5 ms for five steps; an update's product 340 us (1.21 PFLOP/s of
+// fp16 products; a large library product reaches 1.3 to 1.6), a symmetric one 204 to 215 us (1.0 of those that count: 253 tiles of one
 // workgroup each, four waves, fill the 256 CUs once).  A model's matrices are bound by the chain: the optimiser step of a 1D
 // ResNet18 (21 matrices up to 512 x 1536) takes 260 us over 17 launches of 5 to 35 us, each a few dozen stages of latency.
 #include <initializer_list>
