@@ -279,13 +279,31 @@ __device__ __forceinline__ void join_lse(float& m, float& s, float m2, float s2)
     m = mt;
 }
 
-// joins the parts of a row: lse, g and the row's loss.  A workgroup: ROWS rows, 1024 / ROWS strands of parts each.
-template <int ROWS>
+struct Joined { float *lse, *gate, *row, *loss, *count; };
+// loss (mean / sum; null: not reduced) and count from the sums of a workgroup of 1024; fixed order, fp64
+__device__ __forceinline__ void ce_total(double s, int k, int mean, const Joined& out) {
+    __shared__ double sh[16];
+    __shared__ int shc[16];
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) { s += __shfl_xor(s, o, 64); k += __shfl_xor(k, o, 64); }
+    if ((threadIdx.x & 63) == 0) { sh[threadIdx.x >> 6] = s; shc[threadIdx.x >> 6] = k; }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < 16; ++w) { s += sh[w]; k += shc[w]; }
+        const int c = k > 0 ? k : 1;
+        out.count[0] = (float)c;
+        if (out.loss) out.loss[0] = (float)(mean ? s / (double)c : s);
+    }
+}
+
+// joins the parts of a row: lse, g and the row's loss.  A workgroup: ROWS rows, 1024 / ROWS strands of parts each.  WHOLE: it has all
+// rows, and the total as well.
+template <int ROWS, bool WHOLE>
 __global__ __launch_bounds__(1024) void ce_join_kernel(const float* __restrict__ pm, const float* __restrict__ ps, const float* __restrict__ tl,
-                                                       int parts, int N, int V, const int64_t* __restrict__ target, Counts counts,
-                                                       float* __restrict__ lse, float* __restrict__ gate, float* __restrict__ row_loss) {
-    __shared__ float sm[16][ROWS + 1], ss[16][ROWS + 1];
-    constexpr int K = 1024 / ROWS;
+                                                       int parts, int N, int V, const int64_t* __restrict__ target, Counts counts, int mean,
+                                                       Joined out) {
+    constexpr int K = 1024 / ROWS, SPAN = ROWS < 64 ? 64 : ROWS, S = 1024 / SPAN;   // strands; threads whose strands meet in one wave
+    __shared__ float sm[S][ROWS + 1], ss[S][ROWS + 1];
     const int c = threadIdx.x % ROWS, k = threadIdx.x / ROWS, n = blockIdx.x * ROWS + c;
     float m = -INFINITY, s = 0.f;
     if (n < N)
@@ -305,40 +323,33 @@ __global__ __launch_bounds__(1024) void ce_join_kernel(const float* __restrict__
         const float m2 = __shfl_xor(m, o, 64), s2 = __shfl_xor(s, o, 64);
         join_lse(m, s, m2, s2);
     }
-    if ((threadIdx.x & 63) < ROWS) { sm[threadIdx.x >> 6][c] = m; ss[threadIdx.x >> 6][c] = s; }
+    if (threadIdx.x % SPAN < ROWS) { sm[threadIdx.x / SPAN][c] = m; ss[threadIdx.x / SPAN][c] = s; }
     __syncthreads();
-    if (k != 0 || n >= N) return;
-    for (int q = 1; q < 16; ++q) join_lse(m, s, sm[q][c], ss[q][c]);
-    const int64_t t = target[n];
-    const bool bad = t != counts.ignore && (t < 0 || t >= V);
-    const float l = bad || m == -INFINITY ? NAN : m + logf(s);     // a label outside the vocabulary poisons its row: no silent loss
-    const float g = counts(n) ? 1.f : 0.f;
-    lse[n] = l;
-    gate[n] = g;
-    row_loss[n] = g != 0.f ? l - (bad ? 0.f : tl[n]) : 0.f;
+    double loss = 0.0;
+    int kept = 0;
+    if (k == 0 && n < N) {
+        for (int q = 1; q < S; ++q) join_lse(m, s, sm[q][c], ss[q][c]);
+        const int64_t t = target[n];
+        const bool bad = t != counts.ignore && (t < 0 || t >= V);
+        const float l = bad || m == -INFINITY ? NAN : m + logf(s);     // a label outside the vocabulary poisons its row: no silent loss
+        const float g = counts(n) ? 1.f : 0.f, row = g != 0.f ? l - (bad ? 0.f : tl[n]) : 0.f;
+        out.lse[n] = l;
+        out.gate[n] = g;
+        out.row[n] = row;
+        loss = (double)row;
+        kept = t != counts.ignore ? 1 : 0;
+    }
+    if (WHOLE) ce_total(loss, kept, mean, out);
 }
 
-// out[0] = sum of the row losses (/ count for the mean), count[0] = max(1, positions that are not ignored); fixed order, fp64
-__global__ __launch_bounds__(1024) void ce_total_kernel(const float* __restrict__ row_loss, const int64_t* __restrict__ target, int64_t ignore,
-                                                        int N, int mean, float* __restrict__ out, float* __restrict__ count) {
-    __shared__ double sh[16];
-    __shared__ int shc[16];
+__global__ __launch_bounds__(1024) void ce_total_kernel(const int64_t* __restrict__ target, int64_t ignore, int N, int mean, Joined out) {
     double s = 0.0;
     int k = 0;
     for (int i = threadIdx.x; i < N; i += 1024) {
-        s += (double)row_loss[i];
+        s += (double)out.row[i];
         k += target[i] != ignore ? 1 : 0;
     }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) { s += __shfl_xor(s, o, 64); k += __shfl_xor(k, o, 64); }
-    if ((threadIdx.x & 63) == 0) { sh[threadIdx.x >> 6] = s; shc[threadIdx.x >> 6] = k; }
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int w = 1; w < 16; ++w) { s += sh[w]; k += shc[w]; }
-        const int c = k > 0 ? k : 1;
-        count[0] = (float)c;
-        if (out) out[0] = (float)(mean ? s / (double)c : s);
-    }
+    ce_total(s, k, mean, out);
 }
 
 // ---------------------------------------------------------------- gradient
@@ -513,34 +524,32 @@ __global__ __launch_bounds__(M::NT, 2) void ce_prod_kernel(ProdArgs p) {
         }
 }
 
-// out = f 2^ex sum of the planes, in their order
+// out = f 2^ex sum of the planes, in their order; one launch for the results of a piece (blockIdx.y): dx and dweight of type O, dbias
+// in fp32 (its planes are the tiles' column sums)
+struct SumJob { const float* planes; int splits; int64_t n; int scaled; const float* amax; void* out; };   // scaled: O, from E and amax' planes
+struct SumJobs { SumJob job[3]; };
 template <typename O>
-__global__ __launch_bounds__(256) void ce_sum_planes_kernel(const float* __restrict__ planes, int splits, int64_t n, const float* __restrict__ amax,
-                                                            Factor factor, O* __restrict__ out) {
-    int ex = -kEScale;
-    if (amax) ex -= amax_exp(amax);
+__global__ __launch_bounds__(256) void ce_sum_kernel(SumJobs jobs, Factor factor) {
+    const SumJob& job = jobs.job[blockIdx.y];
+    int ex = job.scaled ? -kEScale : 0;
+    if (job.amax) ex -= amax_exp(job.amax);
     const float f = factor();
+    const float* __restrict__ planes = job.planes;
+    const int64_t n = job.n;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
         float s = 0.f;
         int k = 0;
-        for (; k + 8 <= splits; k += 8) {                 // 8 loads in flight
+        for (; k + 8 <= job.splits; k += 8) {             // 8 loads in flight
             float v[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[j] = planes[(int64_t)(k + j) * n + i];
 #pragma unroll
             for (int j = 0; j < 8; ++j) s += v[j];
         }
-        for (; k < splits; ++k) s += planes[(int64_t)k * n + i];
-        out[i] = finish<O>(s, f, ex);
+        for (; k < job.splits; ++k) s += planes[(int64_t)k * n + i];
+        if (job.scaled) reinterpret_cast<O*>(job.out)[i] = finish<O>(s, f, ex);
+        else reinterpret_cast<float*>(job.out)[i] = s * f;
     }
-}
-
-__global__ __launch_bounds__(256) void ce_db_kernel(const float* __restrict__ pdb, int parts, int V, Factor factor, float* __restrict__ db) {
-    const int v = blockIdx.x * 256 + threadIdx.x;
-    if (v >= V) return;
-    float s = 0.f;
-    for (int p = 0; p < parts; ++p) s += pdb[(int64_t)p * V + v];
-    db[v] = s * factor();
 }
 
 // ---------------------------------------------------------------- host side
@@ -706,17 +715,26 @@ int ce_fwd(const void* x, const void* w, const float* bias, const int64_t* targe
 #define SSECG_CE_LSE(...) do { using M = __VA_ARGS__; SSECG_CE_LAUNCH(M, ce_lse_kernel<M>, dim3(p.tilesV * p.tilesN), st, a); } while (0)
     SSECG_CE_TILES(p.c, SSECG_CE_LSE, false, false);
 #undef SSECG_CE_LSE
-    float* row = reduction == 0 ? loss : p.row;
-    // few rows: more strands each (8 x 1024 x 32768 fp16: the forward pass takes 19.7 us, 21.2 with 16 rows a workgroup); more: whole
-    // sectors of their parts (126 rows: the same; 2000 x 768 x 32000 bf16: 104 us against 109)
-    if (N <= 64)
-        hipLaunchKernelGGL(ce_join_kernel<2>, dim3((unsigned)((N + 1) / 2)), dim3(1024), 0, st, p.pm, p.ps, p.tl, p.parts, (int)N, (int)V, target,
-                           counts, lse, gate, row);
-    else
-        hipLaunchKernelGGL(ce_join_kernel<16>, dim3((unsigned)((N + 15) / 16)), dim3(1024), 0, st, p.pm, p.ps, p.tl, p.parts, (int)N, (int)V, target,
-                           counts, lse, gate, row);
-    hipLaunchKernelGGL(ce_total_kernel, dim3(1), dim3(1024), 0, st, row, target, ignore, (int)N, reduction == 1 ? 1 : 0,
-                       reduction == 0 ? nullptr : loss, count);
+    const Joined out = {lse, gate, reduction == 0 ? loss : p.row, reduction == 0 ? nullptr : loss, count};
+    const int mean = reduction == 1 ? 1 : 0;
+#define SSECG_CE_JOIN(ROWS, WHOLE)                                                                                                        \
+    hipLaunchKernelGGL((ce_join_kernel<ROWS, WHOLE>), dim3((unsigned)((N + ROWS - 1) / ROWS)), dim3(1024), 0, st, p.pm, p.ps, p.tl, p.parts, \
+                       (int)N, (int)V, target, counts, mean, out)
+    // few rows whose parts one workgroup reads in a few rounds: the total in the same launch.  Else few rows: more strands each (8 x 1024
+    // x 32768 fp16: the forward pass takes 19.7 us, 21.2 with 16 rows a workgroup), many: whole sectors of their parts (126 rows: the
+    // same; 2000 x 768 x 32000 bf16: 104 us against 109).
+    if (N <= 8 && p.parts <= 2048) {
+        SSECG_CE_JOIN(8, true);
+        return (int)hipGetLastError();
+    }
+    if (N <= 128 && p.parts <= 128) {
+        SSECG_CE_JOIN(128, true);
+        return (int)hipGetLastError();
+    }
+    if (N <= 64) SSECG_CE_JOIN(2, false);
+    else SSECG_CE_JOIN(16, false);
+#undef SSECG_CE_JOIN
+    hipLaunchKernelGGL(ce_total_kernel, dim3(1), dim3(1024), 0, st, target, ignore, (int)N, mean, out);
     return (int)hipGetLastError();
 }
 
@@ -812,8 +830,9 @@ int ce_bwd(const float* dloss, const void* x, const void* w, const float* bias, 
     } while (0)
         SSECG_CE_TILES(p.cl, SSECG_CE_GRAD, false, false);
 #undef SSECG_CE_GRAD
-        if (db && !a.db)
-            hipLaunchKernelGGL(ce_db_kernel, dim3((unsigned)((vn + 255) / 256)), dim3(256), 0, st, p.pdb, a.tilesN, (int)vn, f, db + v0);
+        SumJobs jobs = {};
+        int sums = 0;
+        if (db && !a.db) jobs.job[sums++] = {p.pdb, a.tilesN, vn, 0, nullptr, db + v0};
         if (dx) {                                // E along its rows, W across
             ProdArgs q = {};
             q.A = {p.E, p.pitchE, (int)N};
@@ -835,14 +854,15 @@ int ce_bwd(const float* dloss, const void* x, const void* w, const float* bias, 
             q.plane = p.cw.splits > 1 ? p.planeW : nullptr;
             q.out = (S*)dw + v0 * C; q.amax = k.amaxX; q.f = f;
             if ((rc = product<S, true>(q, p.cw, st)) != 0) return rc;
-            if (q.plane)
-                hipLaunchKernelGGL((ce_sum_planes_kernel<S>), dim3(grid_for(vn * C)), dim3(256), 0, st, p.planeW, p.cw.splits, vn * C,
-                                   P == 2 ? k.amaxX : nullptr, f, (S*)dw + v0 * C);
+            if (q.plane) jobs.job[sums++] = {p.planeW, p.cw.splits, vn * C, 1, k.amaxX, (S*)dw + v0 * C};
+        }
+        if (dx && i + 1 == p.pieces && (p.cx.splits > 1 || p.pieces > 1)) jobs.job[sums++] = {p.planeX, p.cx.splits, N * C, 1, k.amaxW, dx};
+        if (sums) {
+            int64_t most = 0;
+            for (int n = 0; n < sums; ++n) most = jobs.job[n].n > most ? jobs.job[n].n : most;
+            hipLaunchKernelGGL((ce_sum_kernel<S>), dim3(grid_for(most), sums), dim3(256), 0, st, jobs, f);
         }
     }
-    if (dx && (p.cx.splits > 1 || p.pieces > 1))
-        hipLaunchKernelGGL((ce_sum_planes_kernel<S>), dim3(grid_for(N * C)), dim3(256), 0, st, p.planeX, p.cx.splits, N * C,
-                           P == 2 ? k.amaxW : nullptr, f, (S*)dx);
     return (int)hipGetLastError();
 }
 

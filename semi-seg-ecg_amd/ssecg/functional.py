@@ -808,7 +808,7 @@ class _LinearCEFn(torch.autograd.Function):
     def forward(ctx, x, weight, bias, target, conf, thresh, ignore_index, reduction):
         loss, saved = ops.linear_ce_fwd(x, weight, target, bias, conf, thresh, ignore_index, reduction)
         # the operands as the kernels read them (a contiguous copy where the caller's is strided), with what was made of them
-        ctx.save_for_backward(x, weight, bias, *saved[3:7])
+        ctx.save_for_backward(x, weight, bias, saved.target, saved.stats)
         ctx.made = (saved.x if saved.x is not x else None, saved.weight if saved.weight is not weight else None, saved.bias, saved.packed)
         ctx.reduction = saved.reduction
         return loss
@@ -816,9 +816,9 @@ class _LinearCEFn(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dloss):
-        x, weight, bias, target, lse, gate, count = ctx.saved_tensors
+        x, weight, bias, target, stats = ctx.saved_tensors
         xc, wc, f32_bias, packed = ctx.made
-        saved = ops.LinearCE(x if xc is None else xc, weight if wc is None else wc, f32_bias, target, lse, gate, count, packed, ctx.reduction)
+        saved = ops.LinearCE(x if xc is None else xc, weight if wc is None else wc, f32_bias, target, stats, packed, ctx.reduction)
         need = ctx.needs_input_grad
         dx, dw, db = ops.linear_ce_bwd(saved, dloss, need[0], need[1], need[2])
         return dx, dw, db.to(bias.dtype) if db is not None else None, None, None, None, None, None

@@ -1415,15 +1415,13 @@ def layer_norm_bwd(dy, x, mean, rstd, weight=None, want_params=True):
 
 
 class LinearCE(NamedTuple):
-    """What ``linear_ce_bwd`` needs of ``linear_ce_fwd``: the operands, log-sum-exp and gate per position, and (fp32, or C not a
-    multiple of 64) the operands as the matrix pipe reads them."""
+    """What ``linear_ce_bwd`` needs of ``linear_ce_fwd``: the operands, log-sum-exp and gate per position and the count behind them
+    (``stats``: 2 N + 1 values), and (fp32, or C not a multiple of 64) the operands as the matrix pipe reads them."""
     x: torch.Tensor
     weight: torch.Tensor
     bias: Optional[torch.Tensor]
     target: torch.Tensor
-    lse: torch.Tensor
-    gate: torch.Tensor
-    count: torch.Tensor
+    stats: torch.Tensor
     packed: Optional[torch.Tensor]
     reduction: int
 
@@ -1455,9 +1453,7 @@ def linear_ce_fwd(x, weight, target, bias=None, conf=None, thresh=0.0, ignore_in
             raise SsecgError("linear_ce: conf must have target's shape")
     _lm_device(dev, "weight", weight), _lm_device(dev, "target", target), _lm_device(dev, "conf", conf)
     loss = torch.empty(target.shape if mode == 0 else (), device=x.device, dtype=torch.float32)
-    lse = torch.empty(N, device=dev, dtype=torch.float32)
-    gate = torch.empty(N, device=dev, dtype=torch.float32)
-    count = torch.empty(1, device=dev, dtype=torch.float32)
+    stats = torch.empty(2 * N + 1, device=dev, dtype=torch.float32)
     packed = None
     if N:
         Lb, code = lib(), _LM_DTYPE[x.dtype]
@@ -1466,18 +1462,23 @@ def linear_ce_fwd(x, weight, target, bias=None, conf=None, thresh=0.0, ignore_in
             packed = torch.empty((keep,), device=x.device, dtype=torch.uint8) if keep else None
             ws = torch.empty((Lb.ssecg_linear_ce_fwd_workspace(code, N, C, V),), device=x.device, dtype=torch.uint8)
             check(Lb.ssecg_linear_ce_fwd(_p(x), _p(weight), _p(bias), _p(target), _p(conf), float(thresh), int(ignore_index), code, N, C, V,
-                                         mode, _p(loss), _p(lse), _p(gate), _p(count), _p(packed), keep, _p(ws), ws.numel(), _stream()),
+                                         mode, _p(loss), *_ce_stats(stats, N), _p(packed), keep, _p(ws), ws.numel(), _stream()),
                   "ssecg_linear_ce_fwd")
     else:
         loss.zero_()
-        count.fill_(1)
-    return loss, LinearCE(x, weight, bias, target, lse, gate, count, packed, mode)
+    return loss, LinearCE(x, weight, bias, target, stats, packed, mode)
+
+
+def _ce_stats(stats, N):
+    """lse, gate and count in ``stats``"""
+    at = stats.data_ptr()
+    return at, at + 4 * N, at + 8 * N
 
 
 def linear_ce_bwd(saved, dloss=None, want_dx=True, want_dweight=True, want_dbias=True):
     """-> (dx, dweight of their operands' type, dbias in fp32): gradients of ``linear_ce_fwd``'s loss times ``dloss`` (a device scalar,
     or one value per position for reduction "none"; None = 1).  What is not wanted (or has no bias) is None."""
-    x, weight, bias, target, lse, gate, count, packed, mode = saved
+    x, weight, bias, target, stats, packed, mode = saved
     x, weight = _lm_aligned(x), _lm_aligned(weight)
     trace("linear_ce_bwd", tuple(x.shape), tuple(weight.shape))
     (V, C), N = weight.shape, target.numel()
@@ -1499,7 +1500,7 @@ def linear_ce_bwd(saved, dloss=None, want_dx=True, want_dweight=True, want_dbias
         with _lm_guard(x.device), _Timed("ce_grad_kernel + ce_prod_kernel", flops, 2.0 * (N + V) * C * x.element_size()):
             ws = torch.empty((Lb.ssecg_linear_ce_bwd_workspace(code, N, C, V, int(want_dx), int(want_dweight), int(want_dbias)),),
                              device=x.device, dtype=torch.uint8)
-            check(Lb.ssecg_linear_ce_bwd(_p(dloss), _p(x), _p(weight), _p(bias), _p(target), _p(lse), _p(gate), _p(count), code, N, C, V, mode,
+            check(Lb.ssecg_linear_ce_bwd(_p(dloss), _p(x), _p(weight), _p(bias), _p(target), *_ce_stats(stats, N), code, N, C, V, mode,
                                          _p(dx), _p(dw), _p(db), _p(packed), packed.numel() if packed is not None else 0, _p(ws), ws.numel(),
                                          _stream()), "ssecg_linear_ce_bwd")
     return dx, dw, db
