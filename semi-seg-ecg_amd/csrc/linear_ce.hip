@@ -18,8 +18,8 @@
 //
 // Many positions are bound by the matrix pipe: 8192 x 1024 x 65536 bf16 takes 1.13 ms forward (0.97 PFLOP/s) and 3.4 ms backward: E
 // 1.43 ms, of which 0.3 for its 1 GiB and its exponentials, dx 0.94 (1.17 PFLOP/s), dw 0.99.  Few positions are bound by the weights,
-// read three times and written once: 8 x 1024 x 32768 fp16 takes 78 us, each pass over them 13 to 20 us (4.7 to 3.4 TB/s).  The
-// smallest calls are bound by their launches: 126 x 512 x 1000 fp32, 10 of them, 55 us.
+// read three times and written once: 8 x 1024 x 32768 fp16 takes 76 us, each pass over them 13 to 20 us (4.7 to 3.4 TB/s).  The
+// smallest calls are bound by their launches: 126 x 512 x 1000 fp32, 8 of them, 48 us.
 #include "mm_core.h"
 #include "ssecg.h"
 
