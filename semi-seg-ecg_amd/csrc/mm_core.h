@@ -409,9 +409,10 @@ template <class M> struct WaveStore {
     }
 };
 
-// The time of a launch in microseconds, to choose a tile side by.  One stage of one workgroup takes `alone` us where it has its CU to
-// itself and `full` us where the chip is full (two workgroups a CU up to 128); measured on products of 4096 x 4096 x 4096 (full:
-// 120 / 155 / 200 us with one plane, 308 / 344 / 466 us with two, for sides of 256 / 128 / 64) and 512 x 1536 x 512 (alone).
+// The time of a launch in microseconds, to choose a tile side by.  One stage of one workgroup takes `alone` us where it has the chip to
+// itself and `full` us where the chip is full (two workgroups a CU up to 128), measured on products of 4096 x 4096 x 4096 (full:
+// 120 / 155 / 200 us with one plane, 308 / 344 / 466 us with two, for sides of 256 / 128 / 64; a triangle of 192: 204) and 512 x 1536
+// x 512 (alone; 128 with two planes, whose operands leave the L2 first: 2000 x 6000); between them it grows with the workgroups.
 struct MmWork {
     int64_t tiles = 0, stages = 0, longest = 0;      // workgroups, their stages together, the most stages of one
     void add(int64_t n, int64_t per) {
@@ -421,16 +422,17 @@ struct MmWork {
     }
 };
 // groups: two groups of waves take a tile's stages in pairs (one workgroup a CU): a pair takes 1.25 us at a side of 128 with two
-// planes and 0.42 us at 64 (ResNet18's matrices, A = X X^T over 240 tiles of 64 and 48 stages: 16 us against 21).
+// planes and 0.42 us at 64 (ResNet18's matrices, A = X X^T over 240 tiles of 64 and 48 stages: 16 us against 21), and 1.45 times that
+// where the tiles take more than one round (the iteration at 3000 x 3500: 2471 us by pairs, 2345 without, 2176 at a side of 128).
 inline double mm_time(int side, int planes, const MmWork& w, int groups = 1) {
     const bool two = planes == 2;
-    const double full = side == 256 ? (two ? 2.4 : 1.87) : side == 192 ? (two ? 1.4 : 1.1) : side == 128 ? (two ? 1.34 : 1.2) : (two ? 0.46 : 0.39);
-    const double alone = side == 256 ? (two ? 1.9 : 1.5) : side == 192 ? (two ? 1.2 : 0.9) : side == 128 ? (two ? 0.75 : 0.6) : 0.3;
+    const double full = side == 256 ? (two ? 2.4 : 1.87) : side == 192 ? (two ? 1.65 : 1.3) : side == 128 ? (two ? 1.34 : 1.2) : (two ? 0.46 : 0.39);
+    const double alone = side == 256 ? (two ? 1.9 : 1.5) : side == 192 ? (two ? 1.2 : 0.9) : side == 128 ? (two ? 0.9 : 0.6) : 0.3;
     const double pair = side == 128 ? (two ? 1.25 : 1.1) : (two ? 0.42 : 0.36);
     const int64_t slots = side > 128 || groups == 2 ? 256 : 512;
     const double rounds = (double)((w.tiles + slots - 1) / slots), mean = w.tiles ? (double)w.stages / (double)w.tiles : 0.0;
-    if (groups == 2) return 4.0 + (rounds <= 1.0 ? (w.longest + 1) / 2 * pair : rounds * (mean * 0.5 * pair + 1.0));
-    if (w.tiles <= 256) return 3.0 + w.longest * alone;
+    if (groups == 2) return 4.0 + (rounds <= 1.0 ? (w.longest + 1) / 2 * pair : rounds * (mean * 0.5 * 1.45 * pair + 1.0));
+    if (rounds <= 1.0) return 3.0 + w.longest * (alone + (full - alone) * (double)w.tiles / (double)slots);
     const double busy = rounds * mean * full, chain = w.longest * alone;
     return 3.0 + (busy > chain ? busy : chain);
 }
