@@ -686,3 +686,25 @@ def test_muon_takes_an_adamw_state():
     adam.step(), muon.step()
     assert torch.equal(a[1], b[1]) and not torch.equal(a[0], b[0])     # the vector continues AdamW, the matrix starts its momentum
     assert torch.equal(muon.state[b[0]]["momentum_buffer"], torch.ones_like(b[0]))
+
+
+# ------------------------------------------------------------------------------------------------ sizes at which other tiles are chosen
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("N,C,V", [(2990, 1501, 3001), (4500, 2100, 301), (301, 2101, 4501), (601, 209, 4091), (2500, 130, 9001), (2001, 511, 8193)])
+def test_linear_ce_larger(N, C, V, dtype):
+    from ssecg import ops
+    x, w, b, t, conf = _ce_case(N + C + V, N, C, V, dtype, True, True)
+    loss, saved = ops.linear_ce_fwd(x, w, t, b, conf, 0.3)
+    got = (loss, *ops.linear_ce_bwd(saved))
+    want, bound = R.linear_ce(x, w, t, b, conf, 0.3)
+    for p, v, e, what in zip(got, want, bound, ("loss", "dx", "dw", "db")):
+        R.within(p, v, e, what)
+
+
+@pytest.mark.parametrize("shapes", [[(2600, 2750)], [(3500, 3001)], [(4090, 4097)], [(5200, 5100)], [(1024, 1030)] * 8])
+def test_orthogonalize_larger(shapes):
+    from ssecg import ops
+    g = _gen(sum(m * 1000 + n for m, n in shapes))
+    mats = [_normal(g, m, n) for m, n in shapes]
+    for m, o in zip(mats[:2], ops.orthogonalize(mats)):
+        _near(o, m, tuple(m.shape))
