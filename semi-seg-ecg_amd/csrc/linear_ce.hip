@@ -12,6 +12,11 @@
 // along its rows, one across (mm_core.h reads an operand either way, so no operand is transposed in memory).  8 N V C
 // multiplications and additions against the 6 N V C that keeping N V logits would need.
 //
+// Roundings to fewer bits: E, to the operands' type (fp32: two planes, 22 bits), so that its products run at one 16-bit product's
+// rate like those of x and w; two planes for 16-bit inputs too would write twice the bytes and triple dx's and dw's time.  The
+// gradients' relative error against 64 bits is 1.7e-3 to 2.2e-3 in bf16 (1.7e-3 of it their own rounding at the end), 2.1e-4 to
+// 2.8e-4 in fp16.
+//
 // 32-bit inputs travel as two fp16 planes (mm_core.h), scaled by a power of two that the largest finite value sets: exact, and an
 // entry 2^-17 of the largest still has all its bits.  E lies in [-1, 1] and is held times 2^14 for fp16's sake.  Rows whose g_n is
 // zero enter nothing: neither their values (which may be infinite or NaN) nor their products.

@@ -13,7 +13,7 @@
 // would lose them.  All matrices are two fp16 planes times 2^13 - singular values stay below 1.21 and P's below 3.45, far inside
 // fp16's range, and an entry keeps 22 bits down to 2^-16 of the largest possible one - with fp32 accumulators.
 //
-// Large matrices are bound by the matrix pipe: 4096 x 4096 takes 3.5 ms for five steps; an update's product 340 us (1.21 PFLOP/s of
+// Large matrices are bound by the matrix pipe: 4096 x 4096 takes 3.6 ms for five steps; an update's product 340 us (1.21 PFLOP/s of
 // fp16 products; a large library product reaches 1.3 to 1.6), a symmetric one 204 to 215 us (1.0 of those that count: 253 tiles of one
 // workgroup each, four waves, fill the 256 CUs once).  A model's matrices are bound by the chain: the optimiser step of a 1D
 // ResNet18 (21 matrices up to 512 x 1536) takes 260 us over 17 launches of 5 to 35 us, each a few dozen stages of latency.
@@ -182,8 +182,8 @@ __device__ __forceinline__ void tri_tile(int q, int& ti, int& tj) {
 }
 
 // The same triangle of T rows of tiles in blocks of S x S tiles, so that the tiles of one XCD, which follow each other, share few rows of
-// the operand: those of one row of tiles would each read different ones (ResNet18's matrices: 266 -> 253 us; 4096 x 4096 in tiles of 64:
-// 5053 -> 4633).  S = 1 is the order by rows: tiles of 192, which all run at once, are as well off with it (3767 us; 3838 in blocks of 6).
+// the operand: those of one row of tiles would each read different ones (4096 x 4096 in tiles of 64:
+// 5.05 -> 4.63 ms, of 256: 4.63 -> 4.39; small matrices: the same).  S = 1 is the order by rows: tiles of 192, which all run at once, are as well off with it (3767 us; 3838 in blocks of 6).
 template <int S>
 __device__ __forceinline__ void tri_block(int q, int T, int& ti, int& tj) {
     tri_tile(q, ti, tj);
