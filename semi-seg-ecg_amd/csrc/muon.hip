@@ -182,8 +182,9 @@ __device__ __forceinline__ void tri_tile(int q, int& ti, int& tj) {
 }
 
 // The same triangle of T rows of tiles in blocks of S x S tiles, so that the tiles of one XCD, which follow each other, share few rows of
-// the operand: those of one row of tiles would each read different ones (4096 x 4096 in tiles of 64:
-// 5.05 -> 4.63 ms, of 256: 4.63 -> 4.39; small matrices: the same).  S = 1 is the order by rows: tiles of 192, which all run at once, are as well off with it (3767 us; 3838 in blocks of 6).
+// the operand: those of one row of tiles would each read different ones (4096 x 4096 in tiles of 64: 5.05 -> 4.63 ms, of 256: 4.63 ->
+// 4.39; small matrices: the same).  S = 1 is the order by rows: tiles of 192, which all run at once, are as well off with it (3767 us;
+// 3838 in blocks of 6).
 template <int S>
 __device__ __forceinline__ void tri_block(int q, int T, int& ti, int& tj) {
     tri_tile(q, ti, tj);

@@ -708,3 +708,26 @@ def test_orthogonalize_larger(shapes):
     mats = [_normal(g, m, n) for m, n in shapes]
     for m, o in zip(mats[:2], ops.orthogonalize(mats)):
         _near(o, m, tuple(m.shape))
+
+
+def test_layer_norm_beyond_2_31_elements():
+    from ssecg import ops
+    C, rows = 4096, (1 << 19) + 9
+    g = _gen(60)
+    x = torch.empty(rows, C, dtype=torch.bfloat16, device="cuda")
+    piece = _normal(g, 1 << 14, C, dtype=torch.bfloat16)
+    for r in range(0, rows, 1 << 14):
+        x[r:r + (1 << 14)] = piece[:min(1 << 14, rows - r)]
+    w = 1 + _normal(g, C, scale=0.1)
+    y, mean, rstd = ops.layer_norm_fwd(x, w)
+    dx, dw, db = ops.layer_norm_bwd(x, x, mean, rstd, w)
+    few, m, r = ops.layer_norm_fwd(piece[:9], w)
+    assert torch.equal(y[-9:], few) and torch.equal(y[:9], few) and torch.equal(mean[-9:], m) and torch.equal(rstd[-9:], r)
+    assert torch.equal(dx[-9:], ops.layer_norm_bwd(piece[:9], piece[:9], m, r, w)[0])
+    p = piece.double()
+    xh = (p - p.mean(1, keepdim=True)) / torch.sqrt(p.var(1, unbiased=False, keepdim=True) + 1e-5)
+    for got, terms in ((dw, p * xh), (db, p)):
+        want = 32 * terms.sum(0) + terms[:9].sum(0)
+        # at most 2049 rows one after the other (of 256 workgroups, or more of them), then their partial sums; the terms' own errors
+        bound = R.U * (2049 + 512) * (32 * terms.abs().sum(0) + terms[:9].abs().sum(0))
+        R.within(got, want, bound, "column sums")
