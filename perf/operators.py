@@ -147,12 +147,10 @@ def run(state):
     return {"ortho": _run_ortho, "muon": _run_muon, "ln": _run_ln, "ce": _run_ce}[state["op"]](state)
 
 
-_SRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "semi-seg-ecg_amd")
-
-
 def _ssecg():
-    if _SRC not in sys.path:
-        sys.path.insert(1, _SRC)
+    src = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "semi-seg-ecg_amd")
+    if src not in sys.path:
+        sys.path.insert(1, src)
     from ssecg import ops
     return ops
 
