@@ -233,6 +233,14 @@ __device__ __forceinline__ int label_offset(int64_t t, int a0) {
 }
 __device__ __forceinline__ constexpr int reg_offset(int i, int e) { return 32 * i + 8 * (e >> 2) + (e & 3); }
 
+// (m, s): a maximum and the sum of exp(z - m), joined with another's.  Each is weighted by exp(m - max): 0 for a side without a finite
+// logit (m = -inf, s = 0), whatever the other side's maximum is.  A NaN sum stays one.
+__device__ __forceinline__ void join_lse(float& m, float& s, float m2, float s2) {
+    const float mt = fmaxf(m, m2), mz = mt == -INFINITY ? 0.f : mt;
+    s = s * exp2_fast((m - mz) * kLog2e) + s2 * exp2_fast((m2 - mz) * kLog2e);
+    m = mt;
+}
+
 template <class M>
 __global__ __launch_bounds__(M::NT, 2) void ce_lse_kernel(LogitArgs p) {
     __shared__ __attribute__((aligned(16))) char lds[M::LDS];
@@ -267,21 +275,13 @@ __global__ __launch_bounds__(M::NT, 2) void ce_lse_kernel(LogitArgs p) {
         if (off >= 0 && (off & 4) == 0 && a0 + M::arow(0, 0) + off < p.V) p.tl[n] = hit;
         // the lane's other half of the rows
         const float m2 = __shfl_xor(m, 32, 64), s2 = __shfl_xor(s, 32, 64);
-        const float mt = fmaxf(m, m2), mz = mt == -INFINITY ? 0.f : mt;
-        const float mm2 = m2 == -INFINITY ? 0.f : m2;
-        s = s * exp2_fast((mm - mz) * kLog2e) + s2 * exp2_fast((mm2 - mz) * kLog2e);
+        join_lse(m, s, m2, s2);
         if (h == 0 && n < p.N) {
             const int64_t part = (int64_t)ta * M::WM + wm;
-            p.pm[part * p.N + n] = mt;
+            p.pm[part * p.N + n] = m;
             p.ps[part * p.N + n] = s;
         }
     }
-}
-
-__device__ __forceinline__ void join_lse(float& m, float& s, float m2, float s2) {
-    const float mt = fmaxf(m, m2), mz = mt == -INFINITY ? 0.f : mt;
-    s = s * exp2_fast(((m == -INFINITY ? 0.f : m) - mz) * kLog2e) + s2 * exp2_fast(((m2 == -INFINITY ? 0.f : m2) - mz) * kLog2e);
-    m = mt;
 }
 
 struct Joined { float *lse, *gate, *row, *loss, *count; };
