@@ -146,7 +146,7 @@ class FusedAdamW(_FusedOptimizer):
         """One launch: AdamW on ``plist``, parameters of group ``gi``."""
         for p in plist:
             st = self.state[p]
-            if len(st) == 0:
+            if "exp_avg" not in st:
                 st["step"] = torch.tensor(0.0, dtype=torch.float32)
                 st["exp_avg"] = torch.zeros_like(p, memory_format=torch.preserve_format)
                 st["exp_avg_sq"] = torch.zeros_like(p, memory_format=torch.preserve_format)
@@ -198,25 +198,43 @@ class FusedMuon(FusedAdamW):
                                    muon=True)
         super().__init__(params, lr=lr, betas=betas, eps=eps, weight_decay=weight_decay)
 
+    def _check_group(self, group, params):
+        if (not 0.0 <= group["momentum"] < 1.0 or not 1 <= int(group["ns_steps"]) <= 100 or not group["ns_eps"] >= 0.0
+                or group["adjust_lr"] not in self.ADJUST):
+            raise ValueError("invalid Muon hyper-parameter")
+        for p in params if group["muon"] else ():
+            if p.dim() >= 2 and p.numel() and max(p.shape[0], p.numel() // p.shape[0]) > 1 << 20:
+                raise ValueError(f"FusedMuon: a matrix of {tuple(p.shape)} has more than 2^20 rows or columns: give it a group with muon=False")
+
     def add_param_group(self, param_group):
         for k, v in self._muon_defaults.items():
             param_group.setdefault(k, v)
-        if (not 0.0 <= param_group["momentum"] < 1.0 or not 1 <= int(param_group["ns_steps"]) <= 100 or not param_group["ns_eps"] >= 0.0
-                or param_group["adjust_lr"] not in self.ADJUST):
-            raise ValueError("invalid Muon hyper-parameter")
+        self._check_group(param_group, ())
         super().add_param_group(param_group)
         group = self.param_groups[-1]
-        for p in group["params"] if group["muon"] else ():
-            if p.dim() >= 2 and p.numel() and max(p.shape[0], p.numel() // p.shape[0]) > 1 << 20:
-                self.param_groups.pop()
-                raise ValueError(f"FusedMuon: a matrix of {tuple(p.shape)} has more than 2^20 rows or columns: give it a group with muon=False")
+        try:
+            self._check_group(group, group["params"])
+        except ValueError:
+            self.param_groups.pop()
+            raise
 
     def load_state_dict(self, state_dict):
-        """A state of ``FusedAdamW`` or torch.optim.AdamW loads too: the matrices start with no momentum."""
+        """A state of ``FusedAdamW`` or torch.optim.AdamW loads too: a group keeps its own settings where the state has none for them
+        (``muon: False`` among them), and the matrices start with no momentum."""
+        keys = tuple(self._muon_defaults)
+        own = [{k: group[k] for k in keys} for group in self.param_groups]
+        saved = state_dict["param_groups"]
+        if len(saved) == len(own):                               # (otherwise torch refuses the state)
+            for group, mine, theirs in zip(self.param_groups, own, saved):
+                mine.update({k: theirs[k] for k in keys if k in theirs})
+                self._check_group(mine, group["params"])         # before anything is replaced
         super().load_state_dict(state_dict)
-        for group in self.param_groups:
-            for k, v in self._muon_defaults.items():
-                group.setdefault(k, v)
+        for group, settings in zip(self.param_groups, own):
+            group.update(settings)
+            for p in group["params"] if group["muon"] else ():
+                if p.dim() >= 2:
+                    for k in ("step", "exp_avg", "exp_avg_sq"):  # a matrix's AdamW state is of no use here
+                        self.state.get(p, {}).pop(k, None)
 
     @torch.no_grad()
     def step(self, closure=None, found_inf=None):

@@ -80,3 +80,33 @@ def test_linear_ce_nan_logits_are_not_hidden_by_ruled_out_classes():
         w2[at, 3] = float("nan")
         assert torch.isnan(ops.linear_ce_fwd(x, w2, t, b)[0])
     assert torch.isnan(ops.linear_ce_fwd(x, w, t, torch.full_like(b, float("-inf")))[0])       # no class is left: 0 / 0, as a softmax has it
+
+
+# ------------------------------------------------------------------------------------------------ the optimiser's states
+def test_muon_excluded_group_continues_adamw_after_a_load():
+    from ssecg.optim import FusedAdamW, FusedMuon
+    import copy
+    g = _gen(120)
+    tensors = [_normal(g, 30, 20), _normal(g, 9), _normal(g, 50, 30)]
+    make = lambda: [torch.nn.Parameter(t.clone()) for t in tensors]   # noqa: E731
+    a, b = make(), make()
+    adam = FusedAdamW([{"params": a[:2]}, {"params": a[2:]}], lr=1e-2)
+    muon = FusedMuon([{"params": b[:2]}, {"params": b[2:], "muon": False}], lr=0.3)
+    for p in a:
+        p.grad = torch.ones_like(p)
+    adam.step()
+    muon.load_state_dict(copy.deepcopy(adam.state_dict()))
+    with torch.no_grad():
+        for p, q in zip(b, a):
+            p.copy_(q)
+    for _ in range(2):
+        for p, q in zip(a, b):
+            p.grad = _normal(g, *p.shape)
+            q.grad = p.grad.clone()
+        adam.step(), muon.step()
+    assert torch.equal(a[1], b[1]) and torch.equal(a[2], b[2]) and not torch.equal(a[0], b[0])
+    assert set(muon.state[b[0]]) == {"momentum_buffer"}
+    muon.param_groups[0]["muon"] = False                     # from now on AdamW for the matrix too: its own first step
+    del muon.state[b[1]]
+    muon.step()
+    assert {"step", "exp_avg", "exp_avg_sq"} <= set(muon.state[b[0]])
