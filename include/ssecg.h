@@ -553,8 +553,10 @@ int ssecg_layer_norm_bwd(const void *dy, const void *x, const float *mean, const
  *   count   = max(1, positions whose target is not ignore_index)
  *   loss    : reduction 0: (N) gate (lse - z_target); 1: their sum / count; 2: their sum
  * A position whose gate is 0 contributes nothing, whatever x holds there.
- *  packed: what the backward pass reuses - the scales and copies of operands that are none as they lie (fp32, C not a multiple of
+ *  packed: what the backward pass reuses - copies of operands that are none as they lie (fp32: 6 bytes a value; C not a multiple of
  *  64, not 16-byte aligned); 0 bytes otherwise.  x and weight must stay where they are until then.
+ *  fp32 products are as precise as 32-bit ones for values of any size (three bf16 parts, six products).  bf16 / fp16: the gradient of the
+ *  logits is rounded to the type before its products; fp16 holds probabilities below 2^-29 with fewer bits and none below 2^-40.
  */
 size_t ssecg_linear_ce_packed_bytes(const void *x, const void *weight, int dtype, int64_t N, int64_t C, int64_t V);
 size_t ssecg_linear_ce_fwd_workspace(int dtype, int64_t N, int64_t C, int64_t V);

@@ -12,19 +12,21 @@
 // along its rows, one across (mm_core.h reads an operand either way, so no operand is transposed in memory).  8 N V C
 // multiplications and additions against the 6 N V C that keeping N V logits would need.
 //
-// Roundings to fewer bits: E, to the operands' type (fp32: two planes, 22 bits), so that its products run at one 16-bit product's
-// rate like those of x and w; two planes for 16-bit inputs too would write twice the bytes and triple dx's and dw's time.  The
-// gradients' relative error against 64 bits is 1.7e-3 to 2.2e-3 in bf16 (1.7e-3 of it their own rounding at the end), 2.1e-4 to
-// 2.8e-4 in fp16.
+// 32-bit operands, and E between them, travel as three bf16 planes (mm_core.h): exact at every element's own exponent, so a row beside
+// one 10^30 times larger, a class of probability 10^-30 and a position of a tiny upstream gradient are as precise as in a 32-bit
+// product.  (Two fp16 planes and one scale per tensor took half the time, 231 us against 421 at 2000 x 512 x 8192, and lost them.)
 //
-// 32-bit inputs travel as two fp16 planes (mm_core.h), scaled by a power of two that the largest finite value sets: exact, and an
-// entry 2^-17 of the largest still has all its bits.  E lies in [-1, 1] and is held times 2^14 for fp16's sake.  Rows whose g_n is
-// zero enter nothing: neither their values (which may be infinite or NaN) nor their products.
+// Roundings to fewer bits: for 16-bit operands E is held in their type, so that its products run at one 16-bit product's rate like those
+// of x and w; more planes would write twice the bytes and triple dx's and dw's time.  The gradients' relative error against 64 bits is
+// 1.7e-3 to 2.2e-3 in bf16 (1.7e-3 of it their own rounding at the end), 2.1e-4 to 2.8e-4 in fp16.  fp16 has no values below
+// 2^-24: E, in [-1, 1], is held times 2^15, has fewer bits below 2^-29 and is zero below 2^-40 (of the largest |upstream gradient| where the
+// loss is not reduced) - as f E x itself is in fp16 at a loss scale of 2^16.  Rows whose g_n is zero enter nothing: neither their values (which may be infinite or NaN) nor their products.
 //
 // Many positions are bound by the matrix pipe: 8192 x 1024 x 65536 bf16 takes 1.13 ms forward (0.97 PFLOP/s) and 3.4 ms backward: E
 // 1.43 ms, of which 0.3 for its 1 GiB and its exponentials, dx 0.94 (1.17 PFLOP/s), dw 0.99.  Few positions are bound by the weights,
 // read three times and written once: 8 x 1024 x 32768 fp16 takes 76 us, each pass over them 13 to 20 us (4.7 to 3.4 TB/s).  The
 // smallest calls are bound by their launches: 126 x 512 x 1000 fp32, 8 of them, 48 us.
+#include <type_traits>
 #include "mm_core.h"
 #include "ssecg.h"
 
@@ -32,8 +34,8 @@ namespace {
 using namespace ssecg_lm;
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kEScale = 14;                       // E is held times 2^14
-constexpr int kAmaxParts = 256;
+// E is held times 2^15 where its type has few exponents
+template <typename T> constexpr int kEScale = std::is_same<T, _Float16>::value ? 15 : 0;
 
 __device__ __forceinline__ float exp2_fast(float v) { return __builtin_amdgcn_exp2f(v); }
 
@@ -48,68 +50,24 @@ struct Counts {                                   // which rows count: by the ga
     }
 };
 
-// largest finite |x| of the rows that count (blockIdx.y = 0) and of W (1), per workgroup (a maximum: any order gives the same); a
-// wave per row
-__global__ __launch_bounds__(1024) void ce_amax_kernel(const float* __restrict__ x, int64_t N, const float* __restrict__ w, int64_t V, int C,
-                                                       Counts counts, float* __restrict__ out) {
-    float m = 0.f;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const bool first = blockIdx.y == 0;
-    const float* src = first ? x : w;
-    const int64_t rows = first ? N : V;
-    for (int64_t r = (int64_t)blockIdx.x * 16 + wave; r < rows; r += (int64_t)kAmaxParts * 16) {
-        if (first && !counts(r)) continue;
-        for (int c = lane * 4; c < C; c += 256) {
-            const auto q = load_vec(src + r * C, c, C);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const float v = fabsf(q[k]);
-                m = v < INFINITY ? fmaxf(m, v) : m;
-            }
-        }
-    }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-    __shared__ float sh[16];
-    if (lane == 0) sh[wave] = m;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int k = 1; k < 16; ++k) m = fmaxf(m, sh[k]);
-        out[blockIdx.y * kAmaxParts + blockIdx.x] = m;
-    }
-}
-
-// -> the scale's exponent, the same in every thread of a 256-thread workgroup
-__device__ __forceinline__ int amax_exp(const float* __restrict__ parts) {
-    __shared__ float sh[4];
-    float m = parts[threadIdx.x & (kAmaxParts - 1)];
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) sh[(threadIdx.x >> 6) & 3] = m;
-    __syncthreads();
-    return scale_exp(fmaxf(fmaxf(sh[0], sh[1]), fmaxf(sh[2], sh[3])));
-}
-
 // src (R, C) as an operand: its planes, zeros up to the pitch, and zeros for a row that does not count.  One thread: 8 values; one
 // launch for all of a pass (blockIdx.y).
-struct PackJob { const void* src; int64_t R; Counts counts; const float* amax; char* dst; };
+struct PackJob { const void* src; int64_t R; Counts counts; char* dst; };
 struct PackJobs { PackJob job[2]; };
-template <typename S, typename T, int P>
+template <typename S, int P>
 __global__ __launch_bounds__(256) void ce_pack_kernel(PackJobs jobs, int C, int64_t pitch) {
     const PackJob& job = jobs.job[blockIdx.y];
     const S* __restrict__ src = reinterpret_cast<const S*>(job.src);
     char* __restrict__ dst = job.dst;
     const Counts counts = job.counts;
     const int64_t R = job.R;
-    const int ex = P == 2 ? amax_exp(job.amax) : 0;
-    const int per = (int)(pitch / (16 * P));               // threads of a row
+    const int per = (int)(pitch / 16);                     // threads of a row
+    const int64_t plane = R * pitch;
     for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < R * per; at += (int64_t)gridDim.x * 256) {
         const int64_t r = at / per;
         const int k = (int)(at - r * per) * 8;
         const bool live = counts(r);
-        float v[8];
-        uint16_t q[2][8];
+        uint16_t q[8][P];
         constexpr int V = Vec<S>::N;
 #pragma unroll
         for (int i = 0; i < 8; i += V) {
@@ -117,21 +75,16 @@ __global__ __launch_bounds__(256) void ce_pack_kernel(PackJobs jobs, int C, int6
             if (live && k + i < C) t = load_vec(src + r * C, k + i, C);
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                if constexpr (P == 2) {
-                    v[i + j] = ldexpf((float)t[j], ex);
-                    q[0][i + j] = plane16(v[i + j], 0);
-                    q[1][i + j] = plane16(v[i + j], 1);
-                } else {
-                    q[0][i + j] = bits16(t[j]);
-                }
+                if constexpr (P == 3) split3(t[j], q[i + j]);
+                else q[i + j][0] = bits16(t[j]);
             }
         }
 #pragma unroll
         for (int p = 0; p < P; ++p) {
             u32x4 d;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) d[j] = (unsigned)q[p][2 * j] | (unsigned)q[p][2 * j + 1] << 16;
-            *reinterpret_cast<u32x4*>(dst + r * pitch + kbyte<P>(k, p)) = d;
+            for (int j = 0; j < 4; ++j) d[j] = (unsigned)q[2 * j][p] | (unsigned)q[2 * j + 1][p] << 16;
+            *reinterpret_cast<u32x4*>(dst + p * plane + r * pitch + k * 2) = d;
         }
     }
 }
@@ -146,7 +99,6 @@ struct Factor {
 struct LogitArgs {
     Operand W, X;                                // vocabulary rows (of the piece), position rows
     const float* bias;                           // of the piece, or null
-    const float* amaxX; const float* amaxW;      // scale parts (two planes) or null
     int V, N, tilesV, tilesN, stages;
     const int64_t* target;                       // class indices; v0 is the piece's first class
     int64_t v0;
@@ -154,7 +106,7 @@ struct LogitArgs {
     float* pm; float* ps; float* tl;
     // gradient: lse and g per row, E [rowsE][pitchE] (rows from N on are zeros), partial db [tilesN][V]
     const float* lse; const float* gate; const float* coef;
-    char* E; int64_t pitchE;
+    char* E; int64_t pitchE, planeE;
     int rowsE;
     float* pdb;
     float* db; Factor f;                         // db itself where one tile holds all positions, times f
@@ -172,32 +124,7 @@ __device__ __forceinline__ void tile_of(int tilesA, int tilesB, int& ta, int& tb
 
 template <class M>
 __device__ __forceinline__ bool logits_tile(const LogitArgs& p, int a0, int b0, char* lds, f32x16 (&acc)[M::TM][M::TN]) {
-    int ex = 0;
-    if constexpr (M::P == 2) {
-        // every thread reads the parts itself (256 words, cached); the wave's maximum is the workgroup's
-        float mx = 0.f, mw = 0.f;
-        const int lane = threadIdx.x & 63;
-#pragma unroll
-        for (int k = 0; k < kAmaxParts / 64; ++k) {
-            mx = fmaxf(mx, p.amaxX[lane + 64 * k]);
-            mw = fmaxf(mw, p.amaxW[lane + 64 * k]);
-        }
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) {
-            mx = fmaxf(mx, __shfl_xor(mx, o, 64));
-            mw = fmaxf(mw, __shfl_xor(mw, o, 64));
-        }
-        ex = -(scale_exp(mx) + scale_exp(mw));
-    }
     if (!M::run(p.W, a0, p.X, b0, 0, p.stages, lds, acc)) return false;
-    if constexpr (M::P == 2) {
-#pragma unroll
-        for (int i = 0; i < M::TM; ++i)
-#pragma unroll
-            for (int j = 0; j < M::TN; ++j)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) acc[i][j][e] = ldexpf(acc[i][j][e], ex);
-    }
     if (p.bias) {
 #pragma unroll
         for (int i = 0; i < M::TM; ++i) {
@@ -412,7 +339,7 @@ __global__ __launch_bounds__(M::NT, 2) void ce_grad_kernel(LogitArgs p) {
             for (int j = 0; j < M::TN; ++j) {
                 const float pr = exp2_fast((acc[i][j][e] - lse[j]) * kLog2e) - (reg_offset(i, e) == off[j] ? 1.f : 0.f);
                 const float q = g[j] != 0.f ? pr * g[j] : 0.f;      // a row that does not count enters as zero, whatever it holds
-                acc[i][j][e] = q * (float)(1 << kEScale);
+                acc[i][j][e] = q * (float)(1 << kEScale<T>);
                 sum += q;
             }
             sums[e] = sum;
@@ -452,12 +379,17 @@ __global__ __launch_bounds__(M::NT, 2) void ce_grad_kernel(LogitArgs p) {
     char* reg = W::region(lds);
     const int v0 = a0 + M::wave_row(), n0 = b0 + M::wave_col();
     auto val = [&](int i, int j, int e, int q) -> uint16_t {
-        if constexpr (M::P == 2) return plane16(acc[i][j][e], q);
-        else return bits16((T)acc[i][j][e]);
+        if constexpr (M::P == 3) {
+            uint16_t b[3];
+            split3(acc[i][j][e], b);
+            return b[q];
+        } else {
+            return bits16((T)acc[i][j][e]);
+        }
     };
     // the pitch covers the whole tile: no condition on the class
     W::template store_cols<M::P>(reg, val, [&](int n, int v, int q, u32x4 d) {
-        if (n0 + n < p.rowsE) *reinterpret_cast<u32x4*>(p.E + (n0 + n) * p.pitchE + kbyte<M::P>(v0 + v, q)) = d;
+        if (n0 + n < p.rowsE) *reinterpret_cast<u32x4*>(p.E + q * p.planeE + (n0 + n) * p.pitchE + (v0 + v) * 2) = d;
     });
 }
 
@@ -468,12 +400,11 @@ struct ProdArgs {
     float* plane;                                // partial planes [splits][rows][cols], or null: write out
     int add;                                     // plane += instead of plane =
     void* out;                                   // (rows, cols) of the result's type
-    const float* amax;                           // scale parts of operand B, or null
     Factor f;
 };
 
 template <typename O>
-__device__ __forceinline__ O finish(float v, float f, int ex) { return (O)ldexpf(v * f, ex); }
+__device__ __forceinline__ O finish(float v, float f) { return (O)(v * f * (1.f / (float)(1 << kEScale<O>))); }
 
 template <class M, typename O>
 __global__ __launch_bounds__(M::NT, 2) void ce_prod_kernel(ProdArgs p) {
@@ -484,26 +415,13 @@ __global__ __launch_bounds__(M::NT, 2) void ce_prod_kernel(ProdArgs p) {
     const int z = blockIdx.y, s0 = (int)((int64_t)p.stages * z / p.splits), s1 = (int)((int64_t)p.stages * (z + 1) / p.splits);
     f32x16 acc[M::TM][M::TN];
     if (!M::run(p.A, a0, p.B, b0, s0, s1 - s0, lds, acc)) return;
-    int ex = -kEScale;
-    float f = 0.f;
-    if (!p.plane) {
-        f = p.f();
-        if constexpr (M::P == 2) {
-            float m = 0.f;
-            const int lane = threadIdx.x & 63;
-#pragma unroll
-            for (int k = 0; k < kAmaxParts / 64; ++k) m = fmaxf(m, p.amax[lane + 64 * k]);
-#pragma unroll
-            for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-            ex -= scale_exp(m);
-        }
-    }
+    const float f = p.plane ? 0.f : p.f();
     float* plane = p.plane ? p.plane + (int64_t)z * p.rows * p.cols : nullptr;
     if constexpr (sizeof(O) == 2) {
         if (!plane) {
             using W = WaveStore<M>;
             const int r0 = a0 + M::wave_row(), c0 = b0 + M::wave_col();
-            W::template store_rows<1>(W::region(lds), [&](int i, int j, int e, int) -> uint16_t { return bits16(finish<O>(acc[i][j][e], f, ex)); },
+            W::template store_rows<1>(W::region(lds), [&](int i, int j, int e, int) -> uint16_t { return bits16(finish<O>(acc[i][j][e], f)); },
                           [&](int r, int c, int, u32x4 d) {
                               if (r0 + r < p.rows && c0 + c < p.cols)
                                   store_vec(reinterpret_cast<O*>(p.out) + (int64_t)(r0 + r) * p.cols, c0 + c, p.cols,
@@ -524,20 +442,18 @@ __global__ __launch_bounds__(M::NT, 2) void ce_prod_kernel(ProdArgs p) {
                 if (c >= p.cols) continue;
                 const int64_t at = r * p.cols + c;
                 if (plane) plane[at] = p.add ? plane[at] + acc[i][j][e] : acc[i][j][e];
-                else reinterpret_cast<O*>(p.out)[at] = finish<O>(acc[i][j][e], f, ex);
+                else reinterpret_cast<O*>(p.out)[at] = finish<O>(acc[i][j][e], f);
             }
         }
 }
 
-// out = f 2^ex sum of the planes, in their order; one launch for the results of a piece (blockIdx.y): dx and dweight of type O, dbias
+// out = f (E's scale) sum of the planes, in their order; one launch for the results of a piece (blockIdx.y): dx and dweight of type O, dbias
 // in fp32 (its planes are the tiles' column sums)
-struct SumJob { const float* planes; int splits; int64_t n; int scaled; const float* amax; void* out; };   // scaled: O, from E and amax' planes
+struct SumJob { const float* planes; int splits; int64_t n; int scaled; void* out; };   // scaled: O, from E
 struct SumJobs { SumJob job[3]; };
 template <typename O>
 __global__ __launch_bounds__(256) void ce_sum_kernel(SumJobs jobs, Factor factor) {
     const SumJob& job = jobs.job[blockIdx.y];
-    int ex = job.scaled ? -kEScale : 0;
-    if (job.amax) ex -= amax_exp(job.amax);
     const float f = factor();
     const float* __restrict__ planes = job.planes;
     const int64_t n = job.n;
@@ -552,20 +468,23 @@ __global__ __launch_bounds__(256) void ce_sum_kernel(SumJobs jobs, Factor factor
             for (int j = 0; j < 8; ++j) s += v[j];
         }
         for (; k < job.splits; ++k) s += planes[(int64_t)k * n + i];
-        if (job.scaled) reinterpret_cast<O*>(job.out)[i] = finish<O>(s, f, ex);
+        if (job.scaled) reinterpret_cast<O*>(job.out)[i] = finish<O>(s, f);
         else reinterpret_cast<float*>(job.out)[i] = s * f;
     }
 }
 
 // ---------------------------------------------------------------- host side
 template <typename S> struct Inner { using T = S; static constexpr int P = 1; };
-template <> struct Inner<float> { using T = _Float16; static constexpr int P = 2; };
+template <> struct Inner<float> { using T = __bf16; static constexpr int P = 3; };
+inline int planes_of(int dtype) { return dtype == kF32 ? 3 : 1; }
 
 template <typename T, int P, bool TA = false, bool TB = false> using Big = MmTile<T, P, 256, 256, 2, 4, 2, TA, TB>;
 template <typename T, int P, bool TA = false, bool TB = false, int KG = 1> using Mid = MmTile<T, P, 128, 128, 2, 2, 2, TA, TB, KG>;
 template <typename T, int P, bool TA = false, bool TB = false, int KG = 1> using Small = MmTile<T, P, 64, 64, 2, 2, 4, TA, TB, KG>;
 
 inline int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
+// stages of a product over k
+inline int64_t stages_of(int64_t k, int planes) { return up(k, 64) / 64 * (planes == 3 ? kTerms : 1); }
 
 struct Blob {                                    // carves a workspace; a first pass with base 0 sizes it
     char* base; size_t at = 0;
@@ -579,7 +498,7 @@ struct Blob {                                    // carves a workspace; a first 
 
 constexpr int64_t kMaxN = 1 << 21, kMaxV = 1 << 24, kMaxC = 1 << 16;
 constexpr int64_t kMaxPiece = 1 << 21;           // classes of a piece
-static_assert(kMaxC * 4 <= kMaxPitch && kMaxPiece * 4 <= kMaxPitch, "rows of every operand");
+static_assert(kMaxC * 2 <= kMaxPitch && kMaxPiece * 2 <= kMaxPitch, "rows of every operand");
 constexpr int64_t kMaxTiles = 1 << 22;           // of a launch: its 512 kMaxTiles threads stay below 2^32
 inline int64_t tiles_of(int64_t n, int side) { return (n + side - 1) / side; }
 inline bool shape_ok(int64_t N, int64_t C, int64_t V) {
@@ -589,10 +508,8 @@ inline bool shape_ok(int64_t N, int64_t C, int64_t V) {
 // Is the matrix an operand as it lies (16-bit, whole stages of k, aligned)?
 inline bool direct(int dtype, const void* p, int64_t C) { return dtype != kF32 && C % 64 == 0 && ((uintptr_t)p & 15) == 0; }
 
-// What forward leaves for backward beside the statistics: the scales' parts and the operands that had to be copied (two planes, or
-// k padded to a stage).
+// What forward leaves for backward beside the statistics: the operands that had to be copied (three planes, or k padded to a stage).
 struct Packed {
-    float *amaxX, *amaxW;                        // null for 16-bit types
     char *Xp, *Wp;                               // null where the tensor is an operand as it lies
     int64_t pitch;
     size_t bytes;
@@ -601,14 +518,10 @@ struct Packed {
 Packed plan_packed(void* base, const void* x, const void* w, int dtype, int64_t N, int64_t C, int64_t V) {
     Blob b(base);
     Packed p = {};
-    const int P = dtype == kF32 ? 2 : 1;
-    p.pitch = up(C, 64) * 2 * P;
-    if (P == 2) {
-        p.amaxX = b.take<float>(2 * kAmaxParts);
-        p.amaxW = p.amaxX + kAmaxParts;
-    }
-    if (!direct(dtype, x, C)) p.Xp = b.take<char>((size_t)(N * p.pitch));
-    if (!direct(dtype, w, C)) p.Wp = b.take<char>((size_t)(V * p.pitch));
+    const int P = planes_of(dtype);
+    p.pitch = up(C, 64) * 2;
+    if (!direct(dtype, x, C)) p.Xp = b.take<char>((size_t)(N * p.pitch * P));
+    if (!direct(dtype, w, C)) p.Wp = b.take<char>((size_t)(V * p.pitch * P));
     p.bytes = b.at;
     return p;
 }
@@ -616,7 +529,7 @@ Packed plan_packed(void* base, const void* x, const void* w, int dtype, int64_t 
 // the tile side (256, 128, 64) of a product of a x b results with `stages` stages, and how many workgroups and how many groups of a
 // workgroup's waves share the k of a tile
 struct Choice { int side, splits, groups; };
-inline Choice choose(int64_t a, int64_t b, int64_t stages, int P, bool split) {
+inline Choice choose(int64_t a, int64_t b, int64_t stages, bool split) {
     Choice best = {256, 1, 1};
     double least = 0.0;
     for (int side = 256; side >= 64 && tiles_of(a, side) * tiles_of(b, side) <= kMaxTiles; side /= 2)
@@ -625,7 +538,7 @@ inline Choice choose(int64_t a, int64_t b, int64_t stages, int P, bool split) {
             w.add(tiles_of(a, side) * tiles_of(b, side) * s, (stages + s - 1) / s);
             for (int g = 1; g <= (side < 256 ? 2 : 1); ++g) {
                 // the planes of the parts are written and read again (4 TB/s), and a launch sums them
-                const double t = mm_time(side, P, w, g) + (s > 1 ? 4.0 + (double)a * b * s * 8 / 4e6 : 0.0);
+                const double t = mm_time(side, 1, w, g) + (s > 1 ? 4.0 + (double)a * b * s * 8 / 4e6 : 0.0);
                 if (least == 0.0 || t < least) {
                     least = t;
                     best = {side, s, g};
@@ -643,8 +556,7 @@ struct FwdPlan {
 
 FwdPlan plan_fwd(Blob& ws, int dtype, int64_t N, int64_t C, int64_t V) {
     FwdPlan p;
-    const int P = dtype == kF32 ? 2 : 1;
-    p.c = choose(V, N, up(C, 64) * P / 64, P, false);
+    p.c = choose(V, N, stages_of(C, planes_of(dtype)), false);
     p.tilesV = (int)tiles_of(V, p.c.side);
     p.tilesN = (int)tiles_of(N, p.c.side);
     p.parts = p.tilesV * 2;                      // two waves of a tile along the classes
@@ -665,7 +577,7 @@ int pack(const PackJobs& jobs, int count, int64_t C, int64_t pitch, hipStream_t 
     constexpr int P = Inner<S>::P;
     int64_t rows = jobs.job[0].R;
     if (count == 2 && jobs.job[1].R > rows) rows = jobs.job[1].R;
-    hipLaunchKernelGGL((ce_pack_kernel<S, typename Inner<S>::T, P>), dim3(grid_for(rows * (pitch / (16 * P))), count), dim3(256), 0, st, jobs, (int)C,
+    hipLaunchKernelGGL((ce_pack_kernel<S, P>), dim3(grid_for(rows * (pitch / 16)), count), dim3(256), 0, st, jobs, (int)C,
                        pitch);
     return (int)hipGetLastError();
 }
@@ -699,22 +611,16 @@ int ce_fwd(const void* x, const void* w, const float* bias, const int64_t* targe
     const Counts counts = {nullptr, target, ignore, conf, thresh};
     LogitArgs a = {};
     int rc = 0;
-    if constexpr (P == 2) {
-        hipLaunchKernelGGL(ce_amax_kernel, dim3(kAmaxParts, 2), dim3(1024), 0, st, (const float*)x, N, (const float*)w, V, (int)C,
-                           counts, k.amaxX);
-        a.amaxX = k.amaxX;
-        a.amaxW = k.amaxW;
-    }
     PackJobs jobs = {};
     int copies = 0;
-    if (k.Xp) jobs.job[copies++] = {x, N, counts, k.amaxX, k.Xp};
-    if (k.Wp) jobs.job[copies++] = {w, V, Counts{}, k.amaxW, k.Wp};
+    if (k.Xp) jobs.job[copies++] = {x, N, counts, k.Xp};
+    if (k.Wp) jobs.job[copies++] = {w, V, Counts{}, k.Wp};
     if (copies && (rc = pack<S>(jobs, copies, C, k.pitch, st)) != 0) return rc;
-    a.X = {k.Xp ? k.Xp : (const char*)x, k.pitch, (int)N};
-    a.W = {k.Wp ? k.Wp : (const char*)w, k.pitch, (int)V};
+    a.X = {k.Xp ? k.Xp : (const char*)x, k.pitch, (int)N, N * k.pitch};
+    a.W = {k.Wp ? k.Wp : (const char*)w, k.pitch, (int)V, V * k.pitch};
     a.bias = bias;
     a.V = (int)V; a.N = (int)N; a.tilesV = p.tilesV; a.tilesN = p.tilesN;
-    a.stages = (int)(k.pitch / 128);
+    a.stages = (int)stages_of(C, P);
     a.target = target; a.v0 = 0;
     a.pm = p.pm; a.ps = p.ps; a.tl = p.tl;
 #define SSECG_CE_LSE(...) do { using M = __VA_ARGS__; SSECG_CE_LAUNCH(M, ce_lse_kernel<M>, dim3(p.tilesV * p.tilesN), st, a); } while (0)
@@ -746,7 +652,7 @@ int ce_fwd(const void* x, const void* w, const float* bias, const int64_t* targe
 constexpr size_t kPieceBytes = (size_t)1 << 30;  // of E
 
 struct BwdPlan {
-    int64_t Vc, rowsE, pitchE;                   // classes per piece (a multiple of 256 unless there is one piece); E's rows and bytes
+    int64_t Vc, rowsE, pitchE, planeE;           // classes per piece (a multiple of 256 unless there is one piece); E's rows and bytes
     int pieces;
     Choice cl, cx, cw;                           // E, dx, dw
     float *coef, *fscale, *pdb, *planeX, *planeW;
@@ -755,7 +661,7 @@ struct BwdPlan {
 
 BwdPlan plan_bwd(Blob& ws, int dtype, int64_t N, int64_t C, int64_t V, bool want_x, bool want_w, bool want_b, bool x_direct) {
     BwdPlan p;
-    const int P = dtype == kF32 ? 2 : 1, BK = P == 1 ? 64 : 32;
+    const int P = planes_of(dtype);
     p.rowsE = up(N, 64);
     int64_t most = (int64_t)(kPieceBytes / (size_t)(p.rowsE * 2 * P)) / 256 * 256;
     if (most < 256) most = 256;
@@ -763,17 +669,18 @@ BwdPlan plan_bwd(Blob& ws, int dtype, int64_t N, int64_t C, int64_t V, bool want
     const int64_t pieces = (V + most - 1) / most;
     p.Vc = pieces == 1 ? V : up((V + pieces - 1) / pieces, 256);
     p.pieces = (int)((V + p.Vc - 1) / p.Vc);
-    p.pitchE = up(p.Vc, 256) * 2 * P;
-    p.cl = choose(p.Vc, N, up(C, 64) * P / 64, P, false);
-    p.cx = choose(N, C, up(p.Vc, BK) / BK, P, true);
-    p.cw = choose(p.Vc, C, up(N, BK) / BK, P, true);
+    p.pitchE = up(p.Vc, 256) * 2;
+    p.planeE = p.rowsE * p.pitchE;
+    p.cl = choose(p.Vc, N, stages_of(C, P), false);
+    p.cx = choose(N, C, stages_of(p.Vc, P), true);
+    p.cw = choose(p.Vc, C, stages_of(N, P), true);
     p.coef = ws.take<float>((size_t)N);
     p.fscale = ws.take<float>(1);
     p.pdb = ws.take<float>(want_b ? (size_t)(tiles_of(N, p.cl.side) * p.Vc) : 0);
     p.planeX = ws.take<float>(want_x && (p.cx.splits > 1 || p.pieces > 1) ? (size_t)p.cx.splits * N * C : 0);
     p.planeW = ws.take<float>(want_w && p.cw.splits > 1 ? (size_t)p.cw.splits * p.Vc * C : 0);
     p.Xg = ws.take<char>(want_w && x_direct ? (size_t)(N * C * 2) : 0);
-    p.E = ws.take<char>(want_x || want_w ? (size_t)(p.rowsE * p.pitchE) : 0);
+    p.E = ws.take<char>(want_x || want_w ? (size_t)(P * p.planeE) : 0);
     return p;
 }
 
@@ -793,7 +700,7 @@ int ce_bwd(const float* dloss, const void* x, const void* w, const float* bias, 
            const float* count, int dtype, int64_t N, int64_t C, int64_t V, int reduction, void* dx, void* dw, float* db, void* packed, void* ws,
            hipStream_t st) {
     using T = typename Inner<S>::T;
-    constexpr int P = Inner<S>::P, BK = P == 1 ? 64 : 32;
+    constexpr int P = Inner<S>::P;
     Blob blob(ws);
     const Packed k = plan_packed(packed, x, w, dtype, N, C, V);
     const BwdPlan p = plan_bwd(blob, dtype, N, C, V, dx != nullptr, dw != nullptr, db != nullptr, !k.Xp);
@@ -806,23 +713,22 @@ int ce_bwd(const float* dloss, const void* x, const void* w, const float* bias, 
     }
     const char* Xw = X;                          // of dw: rows that do not count are zeros (a copy made by the forward pass has them so)
     if (dw && !k.Xp) {
-        const PackJobs jobs = {{{x, N, Counts{gate, nullptr, 0, nullptr, 0.f}, nullptr, p.Xg}}};
+        const PackJobs jobs = {{{x, N, Counts{gate, nullptr, 0, nullptr, 0.f}, p.Xg}}};
         if ((rc = pack<S>(jobs, 1, C, k.pitch, st)) != 0) return rc;
         Xw = p.Xg;
     }
     for (int i = 0; i < p.pieces; ++i) {
         const int64_t v0 = i * p.Vc, vn = V - v0 < p.Vc ? V - v0 : p.Vc;
         LogitArgs a = {};
-        a.X = {X, k.pitch, (int)N};
-        a.W = {W + v0 * k.pitch, k.pitch, (int)vn};
+        a.X = {X, k.pitch, (int)N, N * k.pitch};
+        a.W = {W + v0 * k.pitch, k.pitch, (int)vn, V * k.pitch};
         a.bias = bias ? bias + v0 : nullptr;
-        a.amaxX = k.amaxX; a.amaxW = k.amaxW;
         a.V = (int)vn; a.N = (int)N;
         a.tilesV = (int)tiles_of(vn, p.cl.side); a.tilesN = (int)tiles_of(N, p.cl.side);
-        a.stages = (int)(k.pitch / 128);
+        a.stages = (int)stages_of(C, P);
         a.target = target; a.v0 = v0;
         a.lse = lse; a.gate = gate; a.coef = reduction == 0 ? p.coef : nullptr;
-        a.E = dx || dw ? p.E : nullptr; a.pitchE = p.pitchE; a.rowsE = (int)p.rowsE;
+        a.E = dx || dw ? p.E : nullptr; a.pitchE = p.pitchE; a.planeE = p.planeE; a.rowsE = (int)p.rowsE;
         a.pdb = p.pdb;
         a.db = db && a.tilesN == 1 ? db + v0 : nullptr;
         a.f = f;
@@ -837,31 +743,31 @@ int ce_bwd(const float* dloss, const void* x, const void* w, const float* bias, 
 #undef SSECG_CE_GRAD
         SumJobs jobs = {};
         int sums = 0;
-        if (db && !a.db) jobs.job[sums++] = {p.pdb, a.tilesN, vn, 0, nullptr, db + v0};
+        if (db && !a.db) jobs.job[sums++] = {p.pdb, a.tilesN, vn, 0, db + v0};
         if (dx) {                                // E along its rows, W across
             ProdArgs q = {};
-            q.A = {p.E, p.pitchE, (int)N};
-            q.B = {W + v0 * k.pitch, k.pitch, (int)vn};
+            q.A = {p.E, p.pitchE, (int)N, p.planeE};
+            q.B = {W + v0 * k.pitch, k.pitch, (int)vn, V * k.pitch};
             q.rows = (int)N; q.cols = (int)C;
             q.tilesA = (int)tiles_of(N, p.cx.side); q.tilesB = (int)tiles_of(C, p.cx.side);
-            q.stages = (int)(up(vn, BK) / BK); q.splits = p.cx.splits;
+            q.stages = (int)stages_of(vn, P); q.splits = p.cx.splits;
             q.plane = p.cx.splits > 1 || p.pieces > 1 ? p.planeX : nullptr;
-            q.add = i > 0; q.out = dx; q.amax = k.amaxW; q.f = f;
+            q.add = i > 0; q.out = dx; q.f = f;
             if ((rc = product<S, false>(q, p.cx, st)) != 0) return rc;
         }
         if (dw) {                                // both across
             ProdArgs q = {};
-            q.A = {p.E, p.pitchE, (int)p.rowsE};
-            q.B = {Xw, k.pitch, (int)N};
+            q.A = {p.E, p.pitchE, (int)p.rowsE, p.planeE};
+            q.B = {Xw, k.pitch, (int)N, N * k.pitch};
             q.rows = (int)vn; q.cols = (int)C;
             q.tilesA = (int)tiles_of(vn, p.cw.side); q.tilesB = (int)tiles_of(C, p.cw.side);
-            q.stages = (int)(up(N, BK) / BK); q.splits = p.cw.splits;
+            q.stages = (int)stages_of(N, P); q.splits = p.cw.splits;
             q.plane = p.cw.splits > 1 ? p.planeW : nullptr;
-            q.out = (S*)dw + v0 * C; q.amax = k.amaxX; q.f = f;
+            q.out = (S*)dw + v0 * C; q.f = f;
             if ((rc = product<S, true>(q, p.cw, st)) != 0) return rc;
-            if (q.plane) jobs.job[sums++] = {p.planeW, p.cw.splits, vn * C, 1, k.amaxX, (S*)dw + v0 * C};
+            if (q.plane) jobs.job[sums++] = {p.planeW, p.cw.splits, vn * C, 1, (S*)dw + v0 * C};
         }
-        if (dx && i + 1 == p.pieces && (p.cx.splits > 1 || p.pieces > 1)) jobs.job[sums++] = {p.planeX, p.cx.splits, N * C, 1, k.amaxW, dx};
+        if (dx && i + 1 == p.pieces && (p.cx.splits > 1 || p.pieces > 1)) jobs.job[sums++] = {p.planeX, p.cx.splits, N * C, 1, dx};
         if (sums) {
             int64_t most = 0;
             for (int n = 0; n < sums; ++n) most = jobs.job[n].n > most ? jobs.job[n].n : most;

@@ -1,11 +1,16 @@
 // The matrix product under linear_ce.hip and muon.hip: D[i][j] = sum_k A[i][k] B[j][k] on the bf16 / fp16 matrix pipe, both
 // operands with k fastest.
 //
-// An operand is one or two PLANES of 16-bit values.  One plane: the data itself (bf16 or fp16).  Two planes (fp16): a 32-bit value
-// v, scaled by a power of two into fp16's normal range, as hi = fp16(v) and lo = fp16(v - hi) - 22 to 23 significant bits - and
-// D = hi hi + hi lo + lo hi in fp32 accumulators (the dropped lo lo is 2^-22 of the product and of random sign).  Three 16-bit
-// products run at 1/3 of 2.5 PFLOP/s; the fp32 matrix pipe's peak is 0.157.  Two planes lie interleaved, 32 hi then 32 lo, so that
-// a stage of a row is 128 consecutive bytes either way: 64 k of one plane or 32 k of both.
+// An operand is one to three PLANES of 16-bit values.
+//   One: the data itself (bf16 or fp16).
+//   Two (fp16), for values of a known range: v, scaled by a power of two into fp16's normal range, as hi = fp16(v) and
+// lo = fp16(v - hi) - 22 to 23 significant bits - and D = hi hi + hi lo + lo hi in fp32 accumulators (the dropped lo lo is 2^-22 of
+// the product and of random sign).  They lie interleaved, 32 hi then 32 lo, so that a stage of a row is 128 consecutive bytes: 32 k.
+//   Three (bf16), for any 32-bit values: b0 = bf16(v), b1 = bf16(v - b0), b2 = v - b0 - b1.  8 + 8 + 8 bits hold v exactly, and at
+// its own exponent: no scale, no floor, each row and each element is as precise as in a 32-bit product whatever else the operand
+// holds.  D is the six products down to 2^-18; the three dropped are at most 2^-26 of |a||b|.  The planes lie one behind the other, each
+// like an operand of one plane, and a stage of 64 k is six stages, one per product.
+// Three 16-bit products run at 1/3 of 2.5 PFLOP/s, six at 1/6; the fp32 matrix pipe's peak is 0.157.
 //
 // Tile BM x BN by WM x WN waves, v_mfma_f32_32x32x16.  Stages travel by LDS-DMA (16 bytes a lane, no registers) into a ring of R
 // slots, requested R - 1 stages ahead with counted waits and one barrier per stage; the fragments of a k step are read while the
@@ -32,13 +37,19 @@ struct Operand {
     const char* base;    // 16-byte aligned
     int64_t pitch;       // bytes of a row, a multiple of 128, below 2^24
     int rows;            // rows in memory: indices, or k of a k-slow operand
+    int64_t plane = 0;   // three planes: bytes from one to the next
 };
 constexpr int64_t kMaxPitch = (1 << 24) - 1;
 
-// bytes of element k (a multiple of 8 within its 16 bytes) in plane q of a row
+// bytes of element k (a multiple of 8 within its 16 bytes) in plane q of a row (three planes: in each of them)
 template <int P> __host__ __device__ __forceinline__ int64_t kbyte(int64_t k, int q = 0) {
-    return P == 1 ? k * 2 : (k >> 5) * 128 + q * 64 + (k & 31) * 2;
+    return P != 2 ? k * 2 : (k >> 5) * 128 + q * 64 + (k & 31) * 2;
 }
+
+// Three planes: the products of a stage of 64 k, by the plane of A and of B; consecutive ones share a plane where they can.
+constexpr int kTerms = 6;
+constexpr unsigned kTermsA = 0u | 0u << 2 | 0u << 4 | 1u << 6 | 1u << 8 | 2u << 10;
+constexpr unsigned kTermsB = 0u | 1u << 2 | 2u << 4 | 0u << 6 | 1u << 8 | 0u << 10;
 
 // LDS-DMA: the lane's 16 bytes at base + off land at lds_wave_base + 16 lane.  From inline asm, so that hipcc's wait counts do not
 // drain the queue before every LDS read; no register is written by the load, and the waits are MmTile::stage_wait's.
@@ -71,10 +82,11 @@ struct MmTile {
     using F = Frag<T>;
     using V8 = typename F::type;
     static constexpr int P = P_, BM = BM_, BN = BN_, WM = WM_, WN = WN_, R = R_;
+    static constexpr int FP = P == 2 ? 2 : 1;                   // planes of a stage
     static constexpr bool TA = TA_, TB = TB_;
     static constexpr int KG = KG_, NW = WM * WN, NT = KG * NW * 64;   // waves of a group, threads of the workgroup
     static constexpr int TM = BM / WM / 32, TN = BN / WN / 32;
-    static constexpr int BK = P == 1 ? 64 : 32;                 // k of a stage
+    static constexpr int BK = FP == 1 ? 64 : 32;                // k of a stage
     static constexpr int STEP = 128;                            // bytes of a k-fast row in a stage
     static constexpr int PA = BM / 8 / NW, PB = BN / 8 / NW, PPW = PA + PB;   // 1 KB pieces (8 rows) per wave and stage
     static constexpr int SLOT = (BM + BN) * 128;
@@ -91,13 +103,13 @@ struct MmTile {
 
     // k-slow stage: BK rows of ROW bytes (SIDE indices); position of chunk c of row k
     template <int SIDE> struct Slow {
-        static constexpr int ROW = SIDE * 2 * P, CH = ROW / 16;
+        static constexpr int ROW = SIDE * 2 * FP, CH = ROW / 16;
         static __device__ __forceinline__ int swz(int k) { return ((k & 3) << 2 | (k >> 2 & 3)) & (CH - 1); }
         // lane's 4 indices x 4 k of the read that gives lane (r, h) the k 16 kk + 8 h + 4 part .. + 3 of index 32 blk + r, plane q
         static __device__ __forceinline__ int at(int lane, int blk, int kk, int part, int q) {
             const int l = lane & 15, g = lane >> 4;
             const int k = kk * 16 + 8 * (g >> 1) + 4 * part + (l >> 2);
-            const int c = (blk * P + q) * 4 + 2 * (g & 1) + ((l & 3) >> 1);
+            const int c = (blk * FP + q) * 4 + 2 * (g & 1) + ((l & 3) >> 1);
             return k * ROW + ((c ^ swz(k)) << 4) + 8 * (l & 1);
         }
     };
@@ -110,9 +122,12 @@ struct MmTile {
     }
 
     // one operand's pieces of a stage: this wave's PC pieces of 1 KB, SIDE indices from i0
-    template <int SIDE, int PC, bool SLOW> struct Loader {
+    template <int SIDE, int PC, bool SLOW, unsigned TERMS> struct Loader {
         unsigned off[PC];
         const char* base;                      // of the stage that is requested next
+        const char* stage;                     // three planes: of its 64 k in the first plane
+        int64_t plane;
+        int term;
         unsigned dst;
         int64_t step;
         int left;                              // k-slow: rows from the stage that is requested next
@@ -122,6 +137,11 @@ struct MmTile {
         __device__ __forceinline__ Loader(const Operand& o, int i0, int s0, int lane, int wave, unsigned lds) {
             dst = lds + wave * PC * 1024;
             pitch = (unsigned)o.pitch;
+            if constexpr (P == 3) {
+                term = s0 % kTerms;
+                s0 /= kTerms;
+                plane = o.plane;
+            }
             if constexpr (!SLOW) {
                 base = o.base + i0 * o.pitch + (int64_t)s0 * STEP;
                 step = STEP;
@@ -138,7 +158,7 @@ struct MmTile {
                 step = BK * o.pitch;
                 base = o.base + s0 * step;
                 left = o.rows - s0 * BK;
-                const unsigned first = (unsigned)i0 * 2 * P, most = pitch - 16;
+                const unsigned first = (unsigned)i0 * 2 * FP, most = pitch - 16;
                 row0 = wave * PC * RPP + lane * 16 / S::ROW;
 #pragma unroll
                 for (int i = 0; i < PC; ++i) {
@@ -147,13 +167,26 @@ struct MmTile {
                     off[i] = (unsigned)k * pitch + (c < most ? c : most);
                 }
             }
+            if constexpr (P == 3) {
+                stage = base;
+                base = stage + (TERMS >> 2 * term & 3) * plane;
+            }
         }
         __device__ __forceinline__ void piece(int slot, int i, unsigned back = 0) {
             lds_dma16(uniform(base), off[i] - back, __builtin_amdgcn_readfirstlane(dst + i * 1024 + slot * SLOT));
         }
         __device__ __forceinline__ void advance() {
-            base += step;
-            if (SLOW) left -= BK;
+            if constexpr (P == 3) {
+                if (++term == kTerms) {
+                    term = 0;
+                    stage += step;
+                    if (SLOW) left -= BK;
+                }
+                base = stage + (TERMS >> 2 * term & 3) * plane;
+            } else {
+                base += step;
+                if (SLOW) left -= BK;
+            }
         }
         __device__ __forceinline__ void issue(int slot) {
             if (SLOW && left < BK) {           // the last stage: rows that do not exist are read as the last one
@@ -215,8 +248,8 @@ struct MmTile {
         const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % NW;
         const int wm = wave / WN, wn = wave % WN, r = lane & 31, h = lane >> 5;
         const unsigned ldsbase = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
-        Loader<BM, PA, TA> la(A, a0, s0, lane, wave, ldsbase);
-        Loader<BN, PB, TB> lb(B, b0, s0, lane, wave, ldsbase + BM * 128);
+        Loader<BM, PA, TA, kTermsA> la(A, a0, s0, lane, wave, ldsbase);
+        Loader<BN, PB, TB, kTermsB> lb(B, b0, s0, lane, wave, ldsbase + BM * 128);
         auto issue = [&](int slot) {
             la.issue(slot);
             lb.issue(slot);
@@ -228,10 +261,10 @@ struct MmTile {
         const int swz = r >> 1 & 7;
         const char* fa = lds + (TA ? 0 : (wm * TM * 32 + r) * 128);
         const char* fb = lds + BM * 128 + (TB ? 0 : (wn * TN * 32 + r) * 128);
-        constexpr int KK = P == 1 ? 4 : 2;                      // k steps of 16 in a stage
+        constexpr int KK = BK / 16;                             // k steps of 16 in a stage
         constexpr bool AHEAD = !(P == 2 && TA && TB && TM * TN > 4);   // (there a second set of fragments would spill)
-        V8 a[2][P][TM], b[2][P][TN];                            // two sets: one is multiplied while the other is read
-        constexpr int NF = P * (TM + TN);                       // fragments of a k step: in the order of their use, a k-slow B's last
+        V8 a[2][FP][TM], b[2][FP][TN];                          // two sets: one is multiplied while the other is read
+        constexpr int NF = FP * (TM + TN);                       // fragments of a k step: in the order of their use, a k-slow B's last
         auto frag = [&](int set, int slot, int kk, int f) {
             const int q = f / (TM + TN), at = f % (TM + TN), i = TB || at == 0 ? at : at - TN, j = TB ? at - TM : at - 1;
             const int c = slot * SLOT + ((4 * q + 2 * kk + h) ^ swz) * 16;
@@ -255,12 +288,12 @@ struct MmTile {
         constexpr bool SPREAD = TM * TN > 8;
         static_assert(!SPREAD || (!TA && !TB), "the spread requests are those of k-fast operands");
         auto multiply = [&](int set, int extra, auto other) {
-            constexpr int NM = (P == 1 ? 1 : 3) * TM * TN;
+            constexpr int NM = (FP == 1 ? 1 : 3) * TM * TN;
 #pragma unroll
             for (int m = 0; m < NM; ++m) {
                 // two planes: the small products first, each product over all blocks: no accumulator is used twice in a row
-                const int q = P == 1 ? 2 : m / (TM * TN), i = m % (TM * TN) / TN, j = m % TN;
-                acc[i][j] = F::mfma(a[set][q == 0 ? P - 1 : 0][i], b[set][q == 1 ? P - 1 : 0][j], acc[i][j]);
+                const int q = FP == 1 ? 2 : m / (TM * TN), i = m % (TM * TN) / TN, j = m % TN;
+                acc[i][j] = F::mfma(a[set][q == 0 ? FP - 1 : 0][i], b[set][q == 1 ? FP - 1 : 0][j], acc[i][j]);
                 if (SPREAD) {
 #pragma unroll
                     for (int x = m * extra / NM; x < (m + 1) * extra / NM; ++x) other(x);
@@ -444,14 +477,6 @@ __device__ __forceinline__ int xcd_tile(int bid, int n) {
     return x * q + (x < rem ? x : rem) + i;
 }
 
-// The power of two that brings |amax| to [2^14, 2^15): its exponent
-__device__ __forceinline__ int scale_exp(float amax) {
-    if (!(amax > 0.f)) return 0;
-    int e;
-    frexpf(amax, &e);                       // amax = m 2^e, m in [0.5, 1)
-    return 15 - e;
-}
-
 __device__ __forceinline__ uint16_t bits16(_Float16 v) { return __builtin_bit_cast(uint16_t, v); }
 __device__ __forceinline__ uint16_t bits16(__bf16 v) { return __builtin_bit_cast(uint16_t, v); }
 
@@ -461,6 +486,17 @@ __device__ __forceinline__ uint16_t plane16(float v, int q) {
     if (q == 0) return bits16(hi);
     const float f = (float)hi;
     return __builtin_isinf(f) ? 0 : bits16((_Float16)(v - f));   // an infinity stays one instead of inf - inf
+}
+
+// v as three bf16 values that add up to it.  What rounds to infinity is cut off instead; infinities and NaN are in the first alone.
+__device__ __forceinline__ void split3(float v, uint16_t (&q)[3]) {
+    const __bf16 r = (__bf16)v;
+    const bool finite = fabsf(v) < INFINITY;
+    q[0] = finite && __builtin_isinf((float)r) ? (uint16_t)(__builtin_bit_cast(uint32_t, v) >> 16) : bits16(r);
+    const float d = finite ? v - __builtin_bit_cast(float, (uint32_t)q[0] << 16) : 0.f;   // exact: at most 16 bits are left
+    const __bf16 r1 = (__bf16)d;
+    q[1] = bits16(r1);
+    q[2] = bits16((__bf16)(d - (float)r1));                                               // exact: at most 8
 }
 
 }  // namespace ssecg_lm

@@ -1416,7 +1416,7 @@ def layer_norm_bwd(dy, x, mean, rstd, weight=None, want_params=True):
 
 class LinearCE(NamedTuple):
     """What ``linear_ce_bwd`` needs of ``linear_ce_fwd``: the operands, log-sum-exp and gate per position and the count behind them
-    (``stats``: 2 N + 1 values), and (fp32, or C not a multiple of 64) the operands as the matrix pipe reads them."""
+    (``stats``: 2 N + 1 values), and (fp32, or C not a multiple of 64) the operands as the matrix pipe reads them (fp32: 6 bytes a value)."""
     x: torch.Tensor
     weight: torch.Tensor
     bias: Optional[torch.Tensor]

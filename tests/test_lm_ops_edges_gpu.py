@@ -110,3 +110,56 @@ def test_muon_excluded_group_continues_adamw_after_a_load():
     del muon.state[b[1]]
     muon.step()
     assert {"step", "exp_avg", "exp_avg_sq"} <= set(muon.state[b[0]])
+
+
+# ------------------------------------------------------------------------------------------------ fp32 operands of very different sizes
+@pytest.mark.parametrize("big", [1e6, 1e12, 1e30])
+@pytest.mark.parametrize("N,C,V", [(40, 64, 300), (300, 771, 2003)])
+def test_linear_ce_fp32_one_large_row_leaves_the_others_alone(N, C, V, big):
+    """A position (and a class) far larger than the others: every other row of the logits, the loss and the gradients keeps its own bound."""
+    x, w, t = _ce_case(130 + N, N, C, V, torch.float32)
+    x[7] *= big
+    w[:, :] /= big if big > 1e20 else 1                      # keep the large row's logits finite
+    b = torch.zeros(V, device="cuda")
+    dloss = torch.ones(N, device="cuda")
+    _ce_check(x, w, t, b, dloss, "none", what="row")
+    x, w, t = _ce_case(131 + N, N, C, V, torch.float32)
+    w[11] *= -big                                            # a class whose logits are huge and negative or positive
+    x[:, 1:] = 0
+    x[:, 0] = x[:, 0].abs() + 0.5
+    w[:, 0] = w[:, 0].abs() + 0.1
+    w[11, 0] = -big
+    t[t == 11] = 12
+    _ce_check(x, w, t, b, dloss, "none", what="class")
+
+
+def test_linear_ce_fp32_largest_and_smallest_values():
+    g = _gen(132)
+    x, w, t = _ce_case(132, 20, 64, 130, torch.float32)
+    x[3, 5], w[:, 5] = torch.finfo(torch.float32).max, 0.0   # rounds to infinity in 16 bits, counts for nothing here
+    x[4] = _normal(g, 64, scale=1e-30)
+    w[9] = _normal(g, 64, scale=1e-30)
+    _ce_check(x, w, t, None, torch.ones(20, device="cuda"), "none")
+
+
+@pytest.mark.parametrize("dtype,low", [(torch.float32, -20.0), (torch.float32, -30.0), (torch.float32, -60.0), (torch.bfloat16, -30.0),
+                                       (torch.bfloat16, -60.0), (torch.float16, -12.0)])
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_linear_ce_rare_classes_keep_their_precision(reduction, dtype, low):
+    """Classes that are no label and have a probability of e^low in every position: their rows of dW to their own bound (fp16: as far as
+    its exponents go)."""
+    N, C, V = 90, 64, 700
+    x, w, t = _ce_case(133, N, C, V, dtype)
+    b = torch.zeros(V, device="cuda")
+    b[200:520] = low
+    t = torch.where((t >= 200) & (t < 520), t % 200, t)
+    scale = 2.0 ** 12 if dtype == torch.float16 else 1.0
+    _ce_check(x, w, t, b, torch.full((N,) if reduction == "none" else (), scale, device="cuda"), reduction)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_linear_ce_small_upstream_gradients_beside_large_ones(dtype):
+    N = 60
+    x, w, t = _ce_case(134, N, 64, 300, dtype)
+    dloss = torch.logspace(0, -18, N, device="cuda")[torch.randperm(N, generator=_gen(135), device="cuda")]
+    _ce_check(x, w, t, torch.zeros(300, device="cuda"), dloss, "none")
