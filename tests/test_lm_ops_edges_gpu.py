@@ -163,3 +163,18 @@ def test_linear_ce_small_upstream_gradients_beside_large_ones(dtype):
     x, w, t = _ce_case(134, N, 64, 300, dtype)
     dloss = torch.logspace(0, -18, N, device="cuda")[torch.randperm(N, generator=_gen(135), device="cuda")]
     _ce_check(x, w, t, torch.zeros(300, device="cuda"), dloss, "none")
+
+
+# ------------------------------------------------------------------------------------------------ several pieces of the vocabulary
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_linear_ce_in_pieces_with_bias(reduction, dtype):
+    """More classes than a piece of the gradient of the logits holds (1 GiB: 10922 classes in fp32, 32768 in 16 bits at 16384 positions):
+    every class of dW and db and every position of dx against 64 bits."""
+    N, C, V = 16384, 64, (24001 if dtype == torch.float32 else 40001)
+    x, w, t = _ce_case(136, N, C, V, dtype)
+    t[::5] = V - 1 - torch.arange(len(t[::5]), device="cuda") % 9000        # labels in the last piece too
+    t[100:300] = -100
+    b = _normal(_gen(137), V, scale=0.3)
+    dloss = torch.rand(N, generator=_gen(138), device="cuda") if reduction == "none" else torch.tensor(256.0, device="cuda")
+    _ce_check(x, w, t, b, dloss, reduction)
