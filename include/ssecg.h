@@ -583,6 +583,10 @@ int ssecg_orthogonalize_multi(const int64_t *mats, int count, int dtype, int ste
 int ssecg_muon_multi(const int64_t *mats, int count, double lr, double momentum, int nesterov, double weight_decay, int adjust,
                      int steps, double eps, const float *skip_flag, const double *lr_dev, void *workspace, size_t workspace_bytes,
                      void *stream);
+/* The same step with scalars_dev = {lr, weight_decay, momentum} on the device: every replay of a captured launch reads them anew.
+ * 0 <= momentum < 1 is the caller's to keep. */
+int ssecg_muon_multi_scalars(const int64_t *mats, int count, const double *scalars_dev, int nesterov, int adjust, int steps, double eps,
+                             const float *skip_flag, void *workspace, size_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

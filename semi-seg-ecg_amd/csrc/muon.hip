@@ -84,6 +84,17 @@ __device__ __forceinline__ int find_mat(const Table& table, int w, int q, int& f
     return k;
 }
 
+struct Apply {                                    // the step's scalars; where they are on the device, a captured launch reads them anew
+    double lr, weight_decay;
+    int adjust;                                   // 0: sqrt(max(1, rows / cols)); 1: 0.2 sqrt(max(rows, cols))
+    float momentum;
+    const double* lr_dev;
+    const double* scalars;                        // {lr, weight_decay, momentum}, or null
+    __device__ __forceinline__ float mu() const { return scalars != nullptr ? (float)scalars[2] : momentum; }
+    __device__ __forceinline__ double rate() const { return scalars != nullptr ? scalars[0] : lr_dev != nullptr ? lr_dev[0] : lr; }
+    __device__ __forceinline__ double decay() const { return scalars != nullptr ? scalars[1] : weight_decay; }
+};
+
 // U of element i (momentum already advanced): Nesterov g + mu v, else v; without momentum g
 template <typename S, bool MUON>
 __device__ __forceinline__ float update_of(const Mat& t, int64_t i, float mu, int nesterov) {
@@ -95,9 +106,10 @@ __device__ __forceinline__ float update_of(const Mat& t, int64_t i, float mu, in
 
 // momentum and the partial sums of |U|^2 (fp64: no gradient's scale overflows it); partial [count][gridDim.x]
 template <typename S, bool MUON>
-__global__ __launch_bounds__(256) void ns_norm_kernel(Table table, float mu, int nesterov, const float* __restrict__ skip,
+__global__ __launch_bounds__(256) void ns_norm_kernel(Table table, Apply ap, int nesterov, const float* __restrict__ skip,
                                                       double* __restrict__ partial) {
     if (MUON && skip != nullptr && skip[0] != 0.f) return;
+    const float mu = MUON ? ap.mu() : 0.f;
     const Mat t = load_mat(table, blockIdx.y, nullptr, 0);
     const int64_t n = (int64_t)t.rows * t.cols;
     constexpr int V = Vec<S>::N;
@@ -130,9 +142,10 @@ __global__ __launch_bounds__(256) void ns_norm_kernel(Table table, float mu, int
 
 // U / (norm + eps) as an operand, the shorter side first; one workgroup: 64 x 64 elements, zeros up to the pitch
 template <typename S, bool MUON>
-__global__ __launch_bounds__(256) void ns_prep_kernel(Table table, char* __restrict__ ws, float mu, int nesterov,
+__global__ __launch_bounds__(256) void ns_prep_kernel(Table table, char* __restrict__ ws, Apply ap, int nesterov,
                                                       int parts, double eps, const float* __restrict__ skip, const double* __restrict__ partial) {
     if (MUON && skip != nullptr && skip[0] != 0.f) return;
+    const float mu = MUON ? ap.mu() : 0.f;
     __shared__ uint32_t tile[64][65];
     int first;
     const int k = find_mat(table, wPrep, blockIdx.x, first);
@@ -256,12 +269,6 @@ __global__ __launch_bounds__(M::NT, M::TM * M::TN > 8 ? 1 : 2) void ns_gram_kern
     if (ti != tj) W::template store_cols<2>(reg, val, [&](int c, int r, int q, u32x4 d) { put(c0 + c, r0 + r, q, d); });
 }
 
-struct Apply {                                    // the optimiser's half of the last product
-    double lr, weight_decay;
-    int adjust;                                   // 0: sqrt(max(1, rows / cols)); 1: 0.2 sqrt(max(rows, cols))
-    const double* lr_dev;
-};
-
 __device__ __forceinline__ double update_scale(const Mat& t, int adjust) {
     return adjust == 1 ? 0.2 * sqrt((double)t.n) : sqrt(t.rows > t.cols ? (double)t.rows / (double)t.cols : 1.0);
 }
@@ -313,9 +320,9 @@ __global__ __launch_bounds__(M::NT, M::TM * M::TN > 8 ? 1 : 2) void ns_update_ke
     }
     float step = 0.f, keep = 0.f;
     if (LAST == 2) {
-        const double lr = ap.lr_dev != nullptr ? ap.lr_dev[0] : ap.lr;
+        const double lr = ap.rate();
         step = (float)(lr * update_scale(t, ap.adjust));
-        keep = (float)(1.0 - lr * ap.weight_decay);
+        keep = (float)(1.0 - lr * ap.decay());
     }
     float* out = reinterpret_cast<float*>(t.dst);
 #pragma unroll
@@ -382,9 +389,10 @@ __device__ __forceinline__ void small_put(char* base, int64_t pitch, int row, in
 }
 
 template <typename S, bool MUON>
-__global__ __launch_bounds__(kSmallWaves * 64) void ns_small_kernel(Table table, float mu, int nesterov, int steps, double eps, Apply ap,
+__global__ __launch_bounds__(kSmallWaves * 64) void ns_small_kernel(Table table, int nesterov, int steps, double eps, Apply ap,
                                                                        const float* __restrict__ skip) {
     if (MUON && skip != nullptr && skip[0] != 0.f) return;
+    const float mu = MUON ? ap.mu() : 0.f;
     __shared__ __attribute__((aligned(16))) char lds[kSmallLds];
     __shared__ double sums[kSmallWaves];
     const Mat t = load_mat(table, blockIdx.x, nullptr, 0);
@@ -537,9 +545,9 @@ __global__ __launch_bounds__(kSmallWaves * 64) void ns_small_kernel(Table table,
     }
     float lr_step = 0.f, keep = 0.f;
     if constexpr (MUON) {
-        const double lr = ap.lr_dev != nullptr ? ap.lr_dev[0] : ap.lr;
+        const double lr = ap.rate();
         lr_step = (float)(lr * update_scale(t, ap.adjust));
-        keep = (float)(1.0 - lr * ap.weight_decay);
+        keep = (float)(1.0 - lr * ap.decay());
     }
     S* dst = reinterpret_cast<S*>(t.dst);
 #pragma unroll 2
@@ -657,7 +665,7 @@ int make_plan(const int64_t* mats, int count, Table& t, Plan& p) {
 }
 
 template <typename S, bool MUON>
-int run_chain(const int64_t* mats, int count, float mu, int nesterov, int steps, double eps, const Apply& ap, const float* skip, char* ws,
+int run_chain(const int64_t* mats, int count, int nesterov, int steps, double eps, const Apply& ap, const float* skip, char* ws,
               hipStream_t st) {
     Table t;
     Plan p;
@@ -666,12 +674,12 @@ int run_chain(const int64_t* mats, int count, float mu, int nesterov, int steps,
     bool small = true;
     for (int k = 0; k < count; ++k) small = small && small_ok(mats[5 * k + 3], mats[5 * k + 4]);
     if (small) {
-        hipLaunchKernelGGL((ns_small_kernel<S, MUON>), dim3(count), dim3(kSmallWaves * 64), 0, st, t, mu, nesterov, steps, eps, ap, skip);
+        hipLaunchKernelGGL((ns_small_kernel<S, MUON>), dim3(count), dim3(kSmallWaves * 64), 0, st, t, nesterov, steps, eps, ap, skip);
         return (int)hipGetLastError();
     }
     double* partial = reinterpret_cast<double*>(ws);
-    hipLaunchKernelGGL((ns_norm_kernel<S, MUON>), dim3(p.parts, count), dim3(256), 0, st, t, mu, nesterov, skip, partial);
-    hipLaunchKernelGGL((ns_prep_kernel<S, MUON>), dim3((unsigned)p.prep), dim3(256), 0, st, t, ws, mu, nesterov, p.parts, eps, skip, partial);
+    hipLaunchKernelGGL((ns_norm_kernel<S, MUON>), dim3(p.parts, count), dim3(256), 0, st, t, ap, nesterov, skip, partial);
+    hipLaunchKernelGGL((ns_prep_kernel<S, MUON>), dim3((unsigned)p.prep), dim3(256), 0, st, t, ws, ap, nesterov, p.parts, eps, skip, partial);
     rc = (int)hipGetLastError();
     for (int k = 0; k < steps && rc == 0; ++k) {
         if ((rc = launch_gram<false>(t, p, ws, k & 1, skip, st)) != 0) break;
@@ -719,8 +727,22 @@ int ssecg_orthogonalize_multi(const int64_t* mats, int count, int dtype, int ste
     const Apply ap = {};
     for (int k = 0; k < count; k += kMost) {
         int rc = 0;
-        SSECG_LM_DTYPE(dtype, S, rc = (run_chain<S, false>(mats + 5 * (size_t)k, count - k < kMost ? count - k : kMost, 0.f, 0, steps, eps, ap, nullptr,
+        SSECG_LM_DTYPE(dtype, S, rc = (run_chain<S, false>(mats + 5 * (size_t)k, count - k < kMost ? count - k : kMost, 0, steps, eps, ap, nullptr,
                                                           (char*)workspace, (hipStream_t)stream)));
+        if (rc != 0) return rc;
+    }
+    return 0;
+}
+
+static int muon_multi(const int64_t* mats, int count, const Apply& ap, int nesterov, int steps, double eps, const float* skip_flag, void* workspace,
+                      size_t workspace_bytes, void* stream) {
+    if (!mats_ok(mats, count, true, true) || steps < 1 || steps > 100 || !(eps >= 0.0) || ap.adjust < 0 || ap.adjust > 1 || !workspace ||
+        ((uintptr_t)workspace & 255))
+        return SSECG_E_INVAL;
+    if (workspace_bytes < ssecg_orthogonalize_workspace(mats, count)) return SSECG_E_WORKSPACE;
+    for (int k = 0; k < count; k += kMost) {
+        const int rc = run_chain<float, true>(mats + 5 * (size_t)k, count - k < kMost ? count - k : kMost, nesterov != 0, steps, eps, ap, skip_flag,
+                                              (char*)workspace, (hipStream_t)stream);
         if (rc != 0) return rc;
     }
     return 0;
@@ -728,17 +750,15 @@ int ssecg_orthogonalize_multi(const int64_t* mats, int count, int dtype, int ste
 
 int ssecg_muon_multi(const int64_t* mats, int count, double lr, double momentum, int nesterov, double weight_decay, int adjust, int steps, double eps,
                      const float* skip_flag, const double* lr_dev, void* workspace, size_t workspace_bytes, void* stream) {
-    if (!mats_ok(mats, count, true, true) || steps < 1 || steps > 100 || !(eps >= 0.0) || !(momentum >= 0.0 && momentum < 1.0) || adjust < 0 ||
-        adjust > 1 || !workspace || ((uintptr_t)workspace & 255))
-        return SSECG_E_INVAL;
-    if (workspace_bytes < ssecg_orthogonalize_workspace(mats, count)) return SSECG_E_WORKSPACE;
-    const Apply ap = {lr, weight_decay, adjust, lr_dev};
-    for (int k = 0; k < count; k += kMost) {
-        const int rc = run_chain<float, true>(mats + 5 * (size_t)k, count - k < kMost ? count - k : kMost, (float)momentum, nesterov != 0, steps, eps, ap,
-                                              skip_flag, (char*)workspace, (hipStream_t)stream);
-        if (rc != 0) return rc;
-    }
-    return 0;
+    if (!(momentum >= 0.0 && momentum < 1.0)) return SSECG_E_INVAL;
+    return muon_multi(mats, count, {lr, weight_decay, adjust, (float)momentum, lr_dev, nullptr}, nesterov, steps, eps, skip_flag, workspace, workspace_bytes,
+                      stream);
+}
+
+int ssecg_muon_multi_scalars(const int64_t* mats, int count, const double* scalars_dev, int nesterov, int adjust, int steps, double eps,
+                             const float* skip_flag, void* workspace, size_t workspace_bytes, void* stream) {
+    if (!scalars_dev) return SSECG_E_INVAL;
+    return muon_multi(mats, count, {0.0, 0.0, adjust, 0.f, nullptr, scalars_dev}, nesterov, steps, eps, skip_flag, workspace, workspace_bytes, stream);
 }
 
 }  // extern "C"

@@ -86,6 +86,7 @@ class StepScalars:
         self.used = 0
         self.refreshers = []          # (kind, offset, callable) in capture order
         self.keep = []                # tensors whose addresses the captured launches use (ops.keep_for_graph)
+        self.checks = []              # run before every replay's refresh: what a captured launch holds fixed must not have changed
         self.aborts = []              # undo callables of host bookkeeping done during the capture (run if it fails)
         # pointer tables built while the step is captured (optimiser, EMA, weight operands: their tensors move into the graph's
         # memory pool): slices of ONE pinned block and ONE device block allocated before the capture starts; append-only, so the
@@ -136,6 +137,14 @@ class StepScalars:
         self.refreshers.append(("lr", k, refresh))
         return self.dev.data_ptr() + 8 * k
 
+    def muon_slot(self, lr, weight_decay, momentum, refresh=None):
+        if refresh is None:
+            raise SsecgError("a captured Muon launch needs its optimiser's refresh hook")
+        k = self._take(3)
+        self.host[k], self.host[k + 1], self.host[k + 2] = float(lr), float(weight_decay), float(momentum)
+        self.refreshers.append(("muon", k, refresh))
+        return self.dev.data_ptr() + 8 * k
+
     def seed_slot(self, seed, refresh=None):
         k = self._take(1)
         self.host_i[k] = _as_i64(seed)
@@ -144,6 +153,8 @@ class StepScalars:
 
     # ---- before a replay
     def refresh(self):
+        for check_fixed in self.checks:               # before any host bookkeeping moves
+            check_fixed()
         self.slot = (self.slot + 1) % self.RING
         if self.events[self.slot] is not None:
             self.events[self.slot].synchronize()      # its last upload (RING steps ago) has long completed; never blocks in practice
@@ -155,6 +166,8 @@ class StepScalars:
                 self._put_adamw(k, *v)
             elif kind == "lr":
                 self.host[k] = float(v)
+            elif kind == "muon":
+                self.host[k], self.host[k + 1], self.host[k + 2] = (float(x) for x in v)
             else:
                 self.host_i[k] = _as_i64(v)
 

@@ -122,6 +122,7 @@ SIGNATURES = {
     "ssecg_orthogonalize_workspace": (_sz, [_vp, _i]),
     "ssecg_orthogonalize_multi": (_i, [_vp, _i, _i, _i, _d, _vp, _sz, _vp]),
     "ssecg_muon_multi": (_i, [_vp, _i, _d, _d, _i, _d, _i, _i, _d, _vp, _vp, _vp, _sz, _vp]),
+    "ssecg_muon_multi_scalars": (_i, [_vp, _i, _vp, _i, _i, _i, _d, _vp, _vp, _sz, _vp]),
 }
 
 _lib = None

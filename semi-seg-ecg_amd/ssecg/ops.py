@@ -1550,15 +1550,19 @@ def _ortho_flops(rows, steps):
 
 def muon_multi(rows, device, lr, momentum, nesterov, weight_decay, adjust, steps, eps, skip_flag=None, refresh=None):
     """One step of ``ssecg_muon_multi`` on rows {gradient, parameter, momentum, rows, cols} (fp32, contiguous).  ``skip_flag``: as in
-    ``adamw_multi``."""
+    ``adamw_multi``.  ``refresh`` (captured steps): -> this step's (lr, weight_decay, momentum)."""
     weights_changed()
     trace("muon_multi", len(rows))
     Lb, arr = lib(), _mats(rows)
-    lr_dev = STEP_SCALARS.lr_slot(lr, refresh) if STEP_SCALARS is not None else None
     ws = torch.empty((max(Lb.ssecg_orthogonalize_workspace(arr, len(rows)), 256),), device=device, dtype=torch.uint8)
     with _Timed("ns_gram_kernel + ns_update_kernel", _ortho_flops(rows, steps), 20.0 * sum(r[3] * r[4] for r in rows)):
-        check(Lb.ssecg_muon_multi(arr, len(rows), float(lr), float(momentum), int(bool(nesterov)), float(weight_decay), int(adjust), int(steps),
-                                  float(eps), _p(skip_flag), lr_dev, _p(ws), ws.numel(), _stream()), "ssecg_muon_multi")
+        if STEP_SCALARS is not None:
+            scalars = STEP_SCALARS.muon_slot(lr, weight_decay, momentum, refresh)
+            check(Lb.ssecg_muon_multi_scalars(arr, len(rows), scalars, int(bool(nesterov)), int(adjust), int(steps), float(eps), _p(skip_flag),
+                                              _p(ws), ws.numel(), _stream()), "ssecg_muon_multi_scalars")
+        else:
+            check(Lb.ssecg_muon_multi(arr, len(rows), float(lr), float(momentum), int(bool(nesterov)), float(weight_decay), int(adjust), int(steps),
+                                      float(eps), _p(skip_flag), None, _p(ws), ws.numel(), _stream()), "ssecg_muon_multi")
 
 
 # ----------------------------------------------------------------------------- record pipeline (SURVEY.md 8f N1)

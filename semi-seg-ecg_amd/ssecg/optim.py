@@ -187,8 +187,9 @@ class FusedMuon(FusedAdamW):
     parameters share lr and weight_decay -, "original": s = sqrt(max(1, rows / cols)).  Vectors (norms, biases) take AdamW's update
     with ``betas`` and ``eps``.  A group with ``muon: False`` takes AdamW for everything (a classifier, an embedding).
 
-    State: ``momentum_buffer`` per matrix, torch.optim.AdamW's entries for the others.  Skipped steps (``found_inf``), checkpoints and
-    captured steps behave as in ``FusedAdamW``."""
+    State: ``momentum_buffer`` per matrix, torch.optim.AdamW's entries for the others.  Skipped steps (``found_inf``) and checkpoints
+    behave as in ``FusedAdamW``.  Under a captured step lr, weight_decay and momentum may change between replays; another setting that
+    changes is refused."""
 
     ADJUST = {"original": 0, "match_rms_adamw": 1}
 
@@ -246,6 +247,8 @@ class FusedMuon(FusedAdamW):
                 loss = closure()
         for gi, group in enumerate(self.param_groups):
             plist = [p for p in self._plist(group) if p.numel()]
+            if ops.STEP_SCALARS is not None and plist:
+                ops.STEP_SCALARS.checks.append(self._captured_check(group))
             matrices = [p for p in plist if p.dim() >= 2] if group["muon"] else []
             others = [p for p in plist if p.dim() < 2] if group["muon"] else plist
             if others:
@@ -266,8 +269,19 @@ class FusedMuon(FusedAdamW):
             with torch.cuda.device(matrices[0].device):
                 ops.muon_multi(rows, matrices[0].device, group["lr"], group["momentum"], group["nesterov"], group["weight_decay"],
                                self.ADJUST[group["adjust_lr"]], group["ns_steps"], group["ns_eps"], skip_flag=found_inf,
-                               refresh=lambda group=group: float(group["lr"]))
+                               refresh=lambda group=group: (group["lr"], group["weight_decay"], group["momentum"]))
         return loss
+
+    def _captured_check(self, group):
+        """A replay reads lr, weight_decay and momentum anew; the rest is part of the captured launches."""
+        fixed = ("muon", "nesterov", "ns_steps", "ns_eps", "adjust_lr", "betas", "eps")
+        held = {k: group[k] for k in fixed}
+
+        def check():
+            self._check_group(group, ())
+            if any(group[k] != v for k, v in held.items()):
+                raise SsecgError(f"FusedMuon: {', '.join(fixed)} cannot change under a captured step: {held} was captured")
+        return check
 
 
 class FusedSGD(_FusedOptimizer):

@@ -60,3 +60,18 @@ def test_a_state_that_a_group_cannot_take_is_refused_whole():
     state["param_groups"].pop()
     with pytest.raises(ValueError):
         opt.load_state_dict(state)
+
+
+def test_muon_entry_with_its_scalars_on_the_device_refuses_bad_arguments():
+    import ctypes
+    from ssecg.lib import lib
+    L = lib()
+    one = (ctypes.c_int64 * 5)(256, 256, 256, 64, 192)
+    n = L.ssecg_orthogonalize_workspace(one, 1)
+    ok = [one, 1, 256, 1, 1, 5, 1e-7, None, 256, n, None]
+    for at, bad in ((0, None), (1, 0), (2, None), (4, 2), (4, -1), (5, 0), (5, 101), (6, -1.0), (6, float("nan")), (8, None), (8, 264)):
+        args = list(ok)
+        args[at] = bad
+        assert L.ssecg_muon_multi_scalars(*args) == -1, at
+    assert L.ssecg_muon_multi_scalars(*(ok[:9] + [n - 1, None])) == -2
+    assert L.ssecg_muon_multi_scalars(*([(ctypes.c_int64 * 5)(256, 256, 0, 64, 192)] + ok[1:])) == -1      # no momentum

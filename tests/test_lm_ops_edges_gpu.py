@@ -178,3 +178,46 @@ def test_linear_ce_in_pieces_with_bias(reduction, dtype):
     b = _normal(_gen(137), V, scale=0.3)
     dloss = torch.rand(N, generator=_gen(138), device="cuda") if reduction == "none" else torch.tensor(256.0, device="cuda")
     _ce_check(x, w, t, b, dloss, reduction)
+
+
+@pytest.mark.parametrize("shapes", [[(40, 20), (7,)], [(200, 300), (64, 64), (7,)]])
+def test_captured_muon_step_follows_its_hyper_parameters(shapes):
+    """lr, weight decay and momentum that change between replays; the settings that a captured launch holds are refused."""
+    from ssecg.graph import StepGraph
+    from ssecg.lib import SsecgError
+    from ssecg.optim import FusedMuon
+    start = [_normal(_gen(140 + k), *s) for k, s in enumerate(shapes)]
+    grads = [[_normal(_gen(150 + 10 * n + k), *s) for k, s in enumerate(shapes)] for n in range(8)]
+
+    def build():
+        ps = [torch.nn.Parameter(t.clone()) for t in start]
+        opt = FusedMuon(ps, lr=1e-2)
+
+        def step(*gs):
+            for p, g in zip(ps, gs):
+                p.grad = g * 1.0
+            opt.step()
+            opt.zero_grad()
+            return (ps[0].detach().sum(),)
+        return ps, opt, step
+    ps_e, opt_e, step_e = build()
+    ps_g, opt_g, step_g = build()
+    graph = StepGraph(step_g)
+    for n, gs in enumerate(grads):
+        for o in (opt_e, opt_g):
+            o.param_groups[0].update(lr=1e-2 / (n + 1), weight_decay=0.02 * n, momentum=0.5 + 0.06 * n)
+        step_e(*gs), graph(*gs)
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(ps_e, ps_g)), n
+    assert graph.replays >= 5 and not graph.disabled
+    steps = float(opt_g.state[ps_g[-1]]["step"])
+    for change in (dict(nesterov=False), dict(ns_steps=4), dict(ns_eps=1e-3), dict(adjust_lr="original"), dict(muon=False), dict(momentum=1.0),
+                   dict(betas=(0.8, 0.99)), dict(eps=1e-6)):
+        old = {k: opt_g.param_groups[0][k] for k in change}
+        opt_g.param_groups[0].update(change)
+        with pytest.raises((SsecgError, ValueError)):
+            graph(*grads[0])
+        opt_g.param_groups[0].update(old)
+    step_e(*grads[0]), graph(*grads[0])                      # a refused call has moved nothing
+    assert float(opt_g.state[ps_g[-1]]["step"]) == steps + 1
+    assert all(torch.equal(p, q) for p, q in zip(ps_e, ps_g))
