@@ -1361,14 +1361,17 @@ def _lm_guard(device):
     return _NO_GUARD if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
+_LN_MOST = 1 << 24    # columns; more would not fit the C ABI's int either
+
+
 def layer_norm_fwd(x, weight=None, bias=None, eps=1e-5):
     """Layer norm over the last axis of x (..., C) -> (y of x's type, mean, rstd); mean and rstd are fp32, one per row.
     ``weight`` / ``bias``: (C,), None = 1 / 0."""
     x = _lm(x, "x")
     trace("layer_norm_fwd", tuple(x.shape))
     shape, dev, n = x.shape, x.device, x.numel()
-    if not shape or shape[-1] == 0:
-        raise SsecgError("layer_norm: x must be (..., C) with C > 0")
+    if not shape or not 0 < shape[-1] <= _LN_MOST:
+        raise SsecgError(f"layer_norm: x must be (..., C) with 0 < C <= {_LN_MOST}, got {tuple(shape)}")
     if not eps >= 0:
         raise SsecgError("layer_norm: eps must not be negative")
     C = shape[-1]
@@ -1390,8 +1393,8 @@ def layer_norm_bwd(dy, x, mean, rstd, weight=None, want_params=True):
     dy = _lm(dy, "dy", x.dtype)
     trace("layer_norm_bwd", tuple(x.shape))
     shape, dev, n = x.shape, x.device, x.numel()
-    if dy.shape != shape or not shape or shape[-1] == 0:
-        raise SsecgError("layer_norm_bwd: dy and x must both be (..., C)")
+    if dy.shape != shape or not shape or not 0 < shape[-1] <= _LN_MOST:
+        raise SsecgError(f"layer_norm_bwd: dy and x must both be (..., C) with 0 < C <= {_LN_MOST}, got {tuple(dy.shape)} and {tuple(shape)}")
     C = shape[-1]
     rows = n // C
     mean, rstd = _req(mean, "mean"), _req(rstd, "rstd")

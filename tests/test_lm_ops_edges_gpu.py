@@ -221,3 +221,18 @@ def test_captured_muon_step_follows_its_hyper_parameters(shapes):
     step_e(*grads[0]), graph(*grads[0])                      # a refused call has moved nothing
     assert float(opt_g.state[ps_g[-1]]["step"]) == steps + 1
     assert all(torch.equal(p, q) for p, q in zip(ps_e, ps_g))
+
+
+# ------------------------------------------------------------------------------------------------ layer norm: sizes and values
+def test_layer_norm_refuses_rows_longer_than_it_counts():
+    """2^24 columns are the limit; 2^32 + 512 is not 512."""
+    from ssecg import ops
+    from ssecg.lib import SsecgError
+    one = torch.zeros(1, device="cuda")
+    for C in ((1 << 24) + 1, (1 << 32) + 512):
+        x = torch.empty(1, C, dtype=torch.bfloat16, device="cuda")
+        with pytest.raises(SsecgError):
+            ops.layer_norm_fwd(x)
+        with pytest.raises(SsecgError):
+            ops.layer_norm_bwd(x, x, one, one)
+        del x
