@@ -17,6 +17,8 @@ def get_optimizer_from_config(config: dict, param_groups):
             betas = tuple(betas)
         return FusedAdamW(param_groups, lr=lr, betas=betas, eps=kwargs.get('eps', 1e-8), weight_decay=weight_decay)
     if opt_name == "muon":
-        known = {k: kwargs[k] for k in ('momentum', 'nesterov', 'ns_steps', 'ns_eps', 'adjust_lr', 'eps') if k in kwargs}
-        return FusedMuon(param_groups, lr=lr, weight_decay=weight_decay, betas=tuple(kwargs.get('betas', (0.9, 0.999))), **known)
+        known = ('momentum', 'nesterov', 'ns_steps', 'ns_eps', 'adjust_lr', 'betas', 'eps')
+        if set(kwargs) - set(known):
+            raise ValueError(f"muon: unknown optimizer_kwargs {sorted(set(kwargs) - set(known))}, expected some of {known}")
+        return FusedMuon(param_groups, lr=lr, weight_decay=weight_decay, **{**kwargs, 'betas': tuple(kwargs.get('betas', (0.9, 0.999)))})
     raise ValueError(f"Unknown optimizer: {opt_name}")

@@ -75,3 +75,17 @@ def test_muon_entry_with_its_scalars_on_the_device_refuses_bad_arguments():
         assert L.ssecg_muon_multi_scalars(*args) == -1, at
     assert L.ssecg_muon_multi_scalars(*(ok[:9] + [n - 1, None])) == -2
     assert L.ssecg_muon_multi_scalars(*([(ctypes.c_int64 * 5)(256, 256, 0, 64, 192)] + ok[1:])) == -1      # no momentum
+
+
+def test_muon_refuses_settings_it_does_not_know():
+    """A misspelt setting of the YAML is an error, not the default."""
+    from utils.optimizer import get_optimizer_from_config
+    conf = {"optimizer": "muon", "lr": 1e-3, "weight_decay": 0.05}
+    known = {"momentum": 0.9, "nesterov": False, "ns_steps": 4, "ns_eps": 1e-6, "adjust_lr": "original", "betas": [0.8, 0.9], "eps": 1e-6}
+    group = get_optimizer_from_config({**conf, "optimizer_kwargs": known}, _params()).param_groups[0]
+    assert {k: group[k] for k in known} == {**known, "betas": (0.8, 0.9)}
+    for name in ("momentun", "muon", "adjust"):
+        with pytest.raises(ValueError, match=name):
+            get_optimizer_from_config({**conf, "optimizer_kwargs": {name: 0.5}}, _params())
+    for empty in ({}, None):
+        assert get_optimizer_from_config({**conf, "optimizer_kwargs": empty}, _params()).param_groups[0]["momentum"] == 0.95
