@@ -807,21 +807,20 @@ class _LinearCEFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, target, conf, thresh, ignore_index, reduction):
         loss, saved = ops.linear_ce_fwd(x, weight, target, bias, conf, thresh, ignore_index, reduction)
-        # the operands as the kernels read them (a contiguous copy where the caller's is strided), with what was made of them
-        ctx.save_for_backward(x, weight, bias, saved.target, saved.stats)
-        ctx.made = (saved.x if saved.x is not x else None, saved.weight if saved.weight is not weight else None, saved.bias, saved.packed)
+        # the operands as the kernels read them (a contiguous copy where the caller's is strided), with what was made of them: all of
+        # it as saved tensors, so that it goes when they go and hooks see it
+        ctx.save_for_backward(saved.x, saved.weight, saved.bias, saved.target, saved.stats, saved.packed)
         ctx.reduction = saved.reduction
+        ctx.bias_dtype = None if bias is None else bias.dtype
         return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dloss):
-        x, weight, bias, target, stats = ctx.saved_tensors
-        xc, wc, f32_bias, packed = ctx.made
-        saved = ops.LinearCE(x if xc is None else xc, weight if wc is None else wc, f32_bias, target, stats, packed, ctx.reduction)
+        saved = ops.LinearCE(*ctx.saved_tensors, ctx.reduction)
         need = ctx.needs_input_grad
         dx, dw, db = ops.linear_ce_bwd(saved, dloss, need[0], need[1], need[2])
-        return dx, dw, db.to(bias.dtype) if db is not None else None, None, None, None, None, None
+        return dx, dw, db.to(ctx.bias_dtype) if db is not None else None, None, None, None, None, None
 
 
 def linear_cross_entropy(x, weight, target, bias=None, ignore_index=-100, reduction="mean"):

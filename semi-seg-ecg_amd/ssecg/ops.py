@@ -1483,6 +1483,8 @@ def linear_ce_bwd(saved, dloss=None, want_dx=True, want_dweight=True, want_dbias
     or one value per position for reduction "none"; None = 1).  What is not wanted (or has no bias) is None."""
     x, weight, bias, target, stats, packed, mode = saved
     x, weight = _lm_aligned(x), _lm_aligned(weight)
+    if packed is not None and packed.data_ptr() % 256:       # (a saved tensor that came back elsewhere in memory)
+        packed = packed.clone()
     trace("linear_ce_bwd", tuple(x.shape), tuple(weight.shape))
     (V, C), N = weight.shape, target.numel()
     shape = target.shape if mode == 0 else ()

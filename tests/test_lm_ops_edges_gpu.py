@@ -236,3 +236,41 @@ def test_layer_norm_refuses_rows_longer_than_it_counts():
         with pytest.raises(SsecgError):
             ops.layer_norm_bwd(x, x, one, one)
         del x
+
+
+# ------------------------------------------------------------------------------------------------ what autograd keeps
+@pytest.mark.parametrize("dtype", TYPES)
+def test_linear_ce_keeps_everything_as_saved_tensors(dtype):
+    """Hooks see every byte that the node keeps, wherever they put it back (off any boundary too), and nothing is left after the backward
+    pass."""
+    from ssecg import functional as SF
+    N, C, V = 512, 200, 4096                                 # C is no whole stage: copies in every type
+    x, w, t = _ce_case(160, N, C, V, dtype)
+    x.requires_grad_(True), w.requires_grad_(True)
+    b = torch.zeros(V, device="cuda", dtype=dtype, requires_grad=True)
+    plain = torch.autograd.grad(SF.linear_cross_entropy(x, w, t, bias=b), (x, w, b))
+    torch.cuda.synchronize()
+    start = torch.cuda.memory_allocated()
+
+    def moved(s):
+        return torch.empty(s.numel() + 1, dtype=s.dtype, device=s.device)[1:].view(s.shape).copy_(s)
+    with torch.autograd.graph.saved_tensors_hooks(lambda s: s.detach().cpu(), lambda s: moved(s.cuda())):
+        loss = SF.linear_cross_entropy(x, w, t, bias=b)
+    assert torch.cuda.memory_allocated() - start <= 4096     # the loss; all else went with the hooks
+    assert all(torch.equal(p, q) for p, q in zip(torch.autograd.grad(loss, (x, w, b)), plain))
+    loss = SF.linear_cross_entropy(x, w, t, bias=b)
+    assert torch.cuda.memory_allocated() - start >= (N + V) * 256 * 2
+    grads = torch.autograd.grad(loss, (x, w, b))
+    del grads
+    assert torch.cuda.memory_allocated() - start <= 8192     # the node still lives with the loss, what it kept does not
+
+
+def test_linear_ce_notices_operands_that_changed():
+    from ssecg import functional as SF
+    x, w, t = _ce_case(161, 16, 64, 50, torch.float32)
+    w.requires_grad_(True)
+    loss = SF.linear_cross_entropy(x, w, t)
+    with torch.no_grad():
+        w.mul_(2)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
