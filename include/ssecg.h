@@ -541,7 +541,8 @@ int ssecg_amp_wgrad(const void *dy, const void *x, float *dw, int N, int Cin, in
 /* y = (x - mean) rstd weight + bias over the last axis of x (rows, C); weight / bias may be NULL (1 / 0); mean, rstd: (rows) */
 int ssecg_layer_norm_fwd(const void *x, const float *weight, const float *bias, int dtype, int64_t rows, int C, double eps, void *y,
                          float *mean, float *rstd, void *stream);
-/* dx and, where not NULL, dweight[c] = sum_rows dy xhat, dbias[c] = sum_rows dy (deterministic; they need the workspace) */
+/* dx, dweight[c] = sum_rows dy xhat, dbias[c] = sum_rows dy, each where not NULL, not all NULL (deterministic; dweight and dbias need the
+ * workspace) */
 size_t ssecg_layer_norm_bwd_workspace(int dtype, int64_t rows, int C);
 int ssecg_layer_norm_bwd(const void *dy, const void *x, const float *mean, const float *rstd, const float *weight, int dtype,
                          int64_t rows, int C, void *dx, float *dweight, float *dbias, float *workspace, size_t workspace_bytes,

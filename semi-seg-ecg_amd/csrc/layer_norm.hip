@@ -226,7 +226,7 @@ __global__ __launch_bounds__(NT) void ln_bwd_kernel(const T* __restrict__ dy, co
             }
         row_sum<TPR, 2>(s, sh, flip);
         const float c1 = s[0] * invC, c2 = s[1] * invC;
-        if (live) {
+        if (live && dx != nullptr) {
 #pragma unroll
             for (int j = 0; j < NCH; ++j) {
                 const int c0 = (t + TPR * j) * V;
@@ -451,8 +451,9 @@ int ln_bwd(const void* dy, const void* x, const float* mean, const float* rstd, 
         SSECG_LN_CASE(128, 1); SSECG_LN_CASE(256, 1); SSECG_LN_CASE(512, 1); SSECG_LN_CASE(1024, 1);
     }
 #undef SSECG_LN_CASE
-    hipLaunchKernelGGL((ln_bwd_long_kernel<T>), dim3((unsigned)(rows < 512 ? rows : 512)), dim3(1024), 0, st, (const T*)dy, (const T*)x, mean,
-                       rstd, w, (T*)dx, rows, C);
+    if (dx)
+        hipLaunchKernelGGL((ln_bwd_long_kernel<T>), dim3((unsigned)(rows < 512 ? rows : 512)), dim3(1024), 0, st, (const T*)dy, (const T*)x, mean,
+                           rstd, w, (T*)dx, rows, C);
     if (partial)
         hipLaunchKernelGGL((ln_bwd_cols_kernel<T>), dim3((unsigned)((C + 255) / 256), (unsigned)g.parts), dim3(256), 0, st, (const T*)dy,
                            (const T*)x, mean, rstd, partial, rows, C);
@@ -478,8 +479,8 @@ size_t ssecg_layer_norm_bwd_workspace(int dtype, int64_t rows, int C) {
 
 int ssecg_layer_norm_bwd(const void* dy, const void* x, const float* mean, const float* rstd, const float* weight, int dtype, int64_t rows,
                          int C, void* dx, float* dweight, float* dbias, float* workspace, size_t workspace_bytes, void* stream) {
-    if (!dy || !x || !mean || !rstd || !dx || !dtype_ok(dtype) || rows <= 0 || C <= 0 || C > kMaxC) return SSECG_E_INVAL;
     const bool params = dweight || dbias;
+    if (!dy || !x || !mean || !rstd || !(dx || params) || !dtype_ok(dtype) || rows <= 0 || C <= 0 || C > kMaxC) return SSECG_E_INVAL;
     if (params && (!workspace || workspace_bytes < ssecg_layer_norm_bwd_workspace(dtype, rows, C))) return SSECG_E_WORKSPACE;
     const LnGrid g = ln_grid(rows, C, dtype);
     float* partial = params ? workspace : nullptr;

@@ -696,7 +696,7 @@ class LayerNormFn(torch.autograd.Function):
     def backward(ctx, dy):
         x, mean, rstd, weight, bias = ctx.saved_tensors
         params = ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
-        dx, dw, db = ops.layer_norm_bwd(dy, x, mean, rstd, weight, want_params=params)
+        dx, dw, db = ops.layer_norm_bwd(dy, x, mean, rstd, weight, want_params=params, want_dx=ctx.needs_input_grad[0])
         dw = dw.to(weight.dtype) if ctx.needs_input_grad[1] else None
         db = db.to(bias.dtype) if ctx.needs_input_grad[2] else None
         return dx, dw, db, None

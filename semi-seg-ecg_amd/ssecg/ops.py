@@ -1387,8 +1387,8 @@ def layer_norm_fwd(x, weight=None, bias=None, eps=1e-5):
     return y, mean, rstd
 
 
-def layer_norm_bwd(dy, x, mean, rstd, weight=None, want_params=True):
-    """-> (dx of x's type, dweight, dbias in fp32 or None): the backward pass of ``layer_norm_fwd``."""
+def layer_norm_bwd(dy, x, mean, rstd, weight=None, want_params=True, want_dx=True):
+    """-> (dx of x's type, dweight, dbias in fp32): the backward pass of ``layer_norm_fwd``.  What is not wanted is None."""
     x = _lm(x, "x")
     dy = _lm(dy, "dy", x.dtype)
     trace("layer_norm_bwd", tuple(x.shape))
@@ -1402,18 +1402,18 @@ def layer_norm_bwd(dy, x, mean, rstd, weight=None, want_params=True):
         raise SsecgError("layer_norm_bwd: mean and rstd must hold one value per row")
     _lm_device(dev, "dy", dy), _lm_device(dev, "mean", mean), _lm_device(dev, "rstd", rstd)
     weight = _lm_vec(weight, "weight", C, dev)
-    dx = torch.empty_like(x)
+    dx = torch.empty_like(x) if want_dx else None
     dw = db = None
     if want_params:
         make = torch.empty if rows else torch.zeros
         dw, db = make(C, device=dev, dtype=torch.float32), make(C, device=dev, dtype=torch.float32)
-    if rows:
+    if rows and (want_dx or want_params):
         Lb, code = lib(), _LM_DTYPE[x.dtype]
-        with _lm_guard(dev), _Timed("ln_bwd_kernel", 0.0, 3.0 * n * x.element_size()):
+        with _lm_guard(dev), _Timed("ln_bwd_kernel", 0.0, (2.0 + bool(want_dx)) * n * x.element_size()):
             nbytes = Lb.ssecg_layer_norm_bwd_workspace(code, rows, C) if want_params else 0
             ws = torch.empty(nbytes, device=dev, dtype=torch.uint8) if nbytes else None
             check(Lb.ssecg_layer_norm_bwd(dy.data_ptr(), x.data_ptr(), mean.data_ptr(), rstd.data_ptr(), _p(weight), code, rows, C,
-                                          dx.data_ptr(), _p(dw), _p(db), _p(ws), nbytes, _stream()), "ssecg_layer_norm_bwd")
+                                          _p(dx), _p(dw), _p(db), _p(ws), nbytes, _stream()), "ssecg_layer_norm_bwd")
     return dx, dw, db
 
 

@@ -89,3 +89,10 @@ def test_muon_refuses_settings_it_does_not_know():
             get_optimizer_from_config({**conf, "optimizer_kwargs": {name: 0.5}}, _params())
     for empty in ({}, None):
         assert get_optimizer_from_config({**conf, "optimizer_kwargs": empty}, _params()).param_groups[0]["momentum"] == 0.95
+
+
+def test_layer_norm_backward_entry_needs_something_to_make():
+    from ssecg.lib import lib
+    L = lib()
+    assert L.ssecg_layer_norm_bwd(8, 8, 8, 8, None, 0, 4, 8, None, None, None, None, 0, None) == -1
+    assert L.ssecg_layer_norm_bwd(8, 8, 8, 8, None, 0, 4, 8, None, 8, None, None, 0, None) == -2          # dweight alone: its workspace is missing

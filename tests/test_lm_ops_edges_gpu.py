@@ -274,3 +274,28 @@ def test_linear_ce_notices_operands_that_changed():
         w.mul_(2)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         loss.backward()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,C", [(300, 64), (70, 777), (5, 20001)])
+def test_layer_norm_makes_only_the_gradients_that_are_wanted(rows, C, dtype):
+    from ssecg import functional as SF, ops
+    g = _gen(170)
+    x, dy = _normal(g, rows, C, dtype=dtype), _normal(g, rows, C, dtype=dtype)
+    w, b = (1 + _normal(g, C, scale=0.2)).requires_grad_(True), _normal(g, C).requires_grad_(True)
+    _, mean, rstd = ops.layer_norm_fwd(x, w.detach(), b.detach())
+    dx, dw, db = ops.layer_norm_bwd(dy, x, mean, rstd, w.detach())
+    part = ops.layer_norm_bwd(dy, x, mean, rstd, w.detach(), want_dx=False)
+    assert part[0] is None and torch.equal(part[1], dw) and torch.equal(part[2], db)
+    part = ops.layer_norm_bwd(dy, x, mean, rstd, w.detach(), want_params=False)
+    assert torch.equal(part[0], dx) and part[1] is None and part[2] is None
+    assert ops.layer_norm_bwd(dy, x, mean, rstd, w.detach(), want_params=False, want_dx=False) == (None, None, None)
+    y = SF.layer_norm(x, w, b)                               # the data need no gradient
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    start = torch.cuda.memory_allocated()
+    got = torch.autograd.grad(y, (w, b), dy)
+    assert torch.equal(got[0], dw) and torch.equal(got[1], db)
+    if rows == 300:                                          # (the others' column sums need more than dx)
+        nbytes = ops.lib().ssecg_layer_norm_bwd_workspace({torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}[dtype], rows, C)
+        assert torch.cuda.max_memory_allocated() - start <= nbytes + 3 * 1024
