@@ -7,7 +7,9 @@
 // bf16: 90 us and 174 us (6.0 and 4.6 TB/s; a large copy reaches 5.0), and 5 us for the parameters' gradients.  Below a few
 // megabytes latency counts: 1008 x 512 fp32 takes 3.9 us, and 6.3 + 4.4 us backward.  A row stays in the registers of the threads
 // that own it (64 to 1024 of them), so the variance is the two-pass one (the sum of squared differences from the mean, no
-// cancellation) without a second read.  A thread owns the same columns of every row its workgroup takes: w and b are loaded once,
+// cancellation) without a second read.  The differences are summed beside their squares and correct the mean: a sum's roundings leave
+// it a few steps of x off, which for rows of nearly equal large values is as much as they differ (a constant row gave 0.93
+// instead of 0).  A thread owns the same columns of every row its workgroup takes: w and b are loaded once,
 // and the column sums dw / db grow in its registers; the row groups of a workgroup are joined in LDS, the workgroups by a second
 // launch in fixed order (no atomics: results do not change from run to run).  Statistics, sums and parameter gradients are fp32; y
 // and dx are rounded once.
@@ -40,6 +42,19 @@ __device__ __forceinline__ void row_sum(float (&v)[K], float* sh, int& flip) {
             v[k] = t;
         }
     }
+}
+
+// a b, rounded: left to itself the compiler fuses the product into the differences from it and not into the mean
+__device__ __forceinline__ float product(float a, float b) {
+#pragma clang fp contract(off)
+    return a * b;
+}
+
+// mean and 1 / deviation from an approximate mean and the means of the differences from it and of their squares
+__device__ __forceinline__ void row_stats(float near, float d, float d2, float eps, float& mu, float& rs) {
+    const float var = d2 - d * d;                     // d2 >= d^2 but for roundings
+    mu = near + d;
+    rs = 1.f / sqrtf((var < 0.f ? 0.f : var) + eps);  // (a NaN stays one)
 }
 
 // a thread's share of a parameter vector (absent or beyond C: `none`)
@@ -80,7 +95,7 @@ __global__ __launch_bounds__(NT) void ln_fwd_kernel(const T* __restrict__ x, con
                                                     T* __restrict__ y, float* __restrict__ mean, float* __restrict__ rstd,
                                                     int64_t rows, int C, float eps) {
     constexpr int V = Vec<T>::N, G = NT / TPR;
-    __shared__ float sh[2 * 16];
+    __shared__ float sh[2 * 32];
     int flip = 0;
     const int t = threadIdx.x % TPR, grp = threadIdx.x / TPR;
     const int64_t step = (int64_t)gridDim.x * G;
@@ -103,17 +118,18 @@ __global__ __launch_bounds__(NT) void ln_fwd_kernel(const T* __restrict__ x, con
 #pragma unroll
             for (int i = 0; i < V; ++i) s[0] += (float)cur[j][i];
         row_sum<TPR, 1>(s, sh, flip);
-        const float mu = s[0] * invC;
-        float q[1] = {0.f};
+        const float near = product(s[0], invC);
+        float q[2] = {0.f, 0.f};
 #pragma unroll
         for (int j = 0; j < NCH; ++j)
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                const float d = (float)cur[j][i] - mu;
-                if ((t + TPR * j) * V + i < C) q[0] += d * d;
+                const float d = (float)cur[j][i] - near;
+                if ((t + TPR * j) * V + i < C) { q[0] += d; q[1] += d * d; }
             }
-        row_sum<TPR, 1>(q, sh, flip);
-        const float rs = 1.f / sqrtf(q[0] * invC + eps);
+        row_sum<TPR, 2>(q, sh, flip);
+        float mu, rs;
+        row_stats(near, q[0] * invC, q[1] * invC, eps, mu, rs);
         if (live) {
             if (t == 0) { mean[row] = mu; rstd[row] = rs; }
 #pragma unroll
@@ -138,7 +154,7 @@ __global__ __launch_bounds__(1024) void ln_fwd_long_kernel(const T* __restrict__
                                                            T* __restrict__ y, float* __restrict__ mean, float* __restrict__ rstd,
                                                            int64_t rows, int C, float eps) {
     constexpr int V = Vec<T>::N;
-    __shared__ float sh[2 * 16];
+    __shared__ float sh[2 * 32];
     int flip = 0;
     for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
         const T* xr = x + row * C;
@@ -149,18 +165,19 @@ __global__ __launch_bounds__(1024) void ln_fwd_long_kernel(const T* __restrict__
             for (int i = 0; i < V; ++i) s[0] += (float)q[i];
         }
         row_sum<1024, 1>(s, sh, flip);
-        const float mu = s[0] / (float)C;
-        float d2[1] = {0.f};
+        const float near = s[0] / (float)C;
+        float q2[2] = {0.f, 0.f};
         for (int64_t c0 = (int64_t)threadIdx.x * V; c0 < C; c0 += 1024 * V) {
             const auto q = load_vec(xr, (int)c0, C);
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                const float d = (float)q[i] - mu;
-                if (c0 + i < C) d2[0] += d * d;
+                const float d = (float)q[i] - near;
+                if (c0 + i < C) { q2[0] += d; q2[1] += d * d; }
             }
         }
-        row_sum<1024, 1>(d2, sh, flip);
-        const float rs = 1.f / sqrtf(d2[0] / (float)C + eps);
+        row_sum<1024, 2>(q2, sh, flip);
+        float mu, rs;
+        row_stats(near, q2[0] / (float)C, q2[1] / (float)C, eps, mu, rs);
         if (threadIdx.x == 0) { mean[row] = mu; rstd[row] = rs; }
         for (int64_t c0 = (int64_t)threadIdx.x * V; c0 < C; c0 += 1024 * V) {
             const auto q = load_vec(xr, (int)c0, C);

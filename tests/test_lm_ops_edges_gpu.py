@@ -299,3 +299,31 @@ def test_layer_norm_makes_only_the_gradients_that_are_wanted(rows, C, dtype):
     if rows == 300:                                          # (the others' column sums need more than dx)
         nbytes = ops.lib().ssecg_layer_norm_bwd_workspace({torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}[dtype], rows, C)
         assert torch.cuda.max_memory_allocated() - start <= nbytes + 3 * 1024
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("C", [7, 49, 100, 777, 2049, 6000, 20001])
+def test_layer_norm_of_rows_of_equal_and_nearly_equal_large_values(C, dtype):
+    """Equal values: no deviation, y = bias exactly and the mean is the value.  Nearly equal ones, a step apart: fp32's mean may be half a
+    step of x off, no more."""
+    from ssecg import ops
+    top = 6e4 if dtype == torch.float16 else 3e7
+    v = torch.tensor([3.0, 1000.3, 12345.6, 60000.0, 123456.7, 1e6, 3e7, -1e6], device="cuda").clamp(max=top, min=-top).to(dtype)
+    x = v[:, None].expand(-1, C).contiguous()
+    b = _normal(_gen(180), C)
+    y, mean, rstd = ops.layer_norm_fwd(x, None, b)
+    assert torch.equal(mean, v.float()) and torch.equal(y, b.to(dtype).expand_as(y))
+    dx, dw, db = ops.layer_norm_bwd(torch.ones_like(x), x, mean, rstd)
+    assert not dw.any() and torch.isfinite(dx).all()
+    if dtype == torch.float32:
+        step = 2.0 ** -23 * 2.0 ** torch.floor(torch.log2(v.abs()))
+        x = x + step[:, None] * torch.randint(-3, 4, (8, C), generator=_gen(181), device="cuda")
+        y, mean, rstd = ops.layer_norm_fwd(x)
+        x64 = x.double()
+        mu, var = x64.mean(1, keepdim=True), x64.var(1, unbiased=False, keepdim=True)
+        rs = 1 / torch.sqrt(var + 1e-5)
+        assert ((mean.double() - mu[:, 0]).abs() <= 0.5 * 1.001 * step.double()).all()
+        # the mean half a step off (and once more where rstd's variance takes it in: at most (step / 2)^2 of it), then fp32's roundings
+        off = 0.5 * 1.001 * step[:, None].double() * rs
+        R.within(y, (x64 - mu) * rs, off + 32 * R.U * ((x64 - mu) * rs).abs() + 32 * R.U, "y")
+        R.within(rstd, rs[:, 0], 64 * R.U * rs[:, 0], "rstd")
