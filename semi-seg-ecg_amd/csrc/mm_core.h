@@ -287,13 +287,26 @@ struct MmTile {
         // early count for more (8192 x 1024 x 65536 bf16: dx 951 us, 986 spread).
         constexpr bool SPREAD = TM * TN > 8;
         static_assert(!SPREAD || (!TA && !TB), "the spread requests are those of k-fast operands");
+        // Two planes: the small products have accumulators of their own where registers allow it, so that the large one takes one rounding
+        // per k step instead of three.
+        constexpr bool APART = P == 2 && TM * TN <= 4;
+        f32x16 low[APART ? TM : 1][APART ? TN : 1];
+        if constexpr (APART) {
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int j = 0; j < TN; ++j)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) low[i][j][e] = 0.f;
+        }
         auto multiply = [&](int set, int extra, auto other) {
             constexpr int NM = (FP == 1 ? 1 : 3) * TM * TN;
 #pragma unroll
             for (int m = 0; m < NM; ++m) {
                 // two planes: the small products first, each product over all blocks: no accumulator is used twice in a row
                 const int q = FP == 1 ? 2 : m / (TM * TN), i = m % (TM * TN) / TN, j = m % TN;
-                acc[i][j] = F::mfma(a[set][q == 0 ? FP - 1 : 0][i], b[set][q == 1 ? FP - 1 : 0][j], acc[i][j]);
+                f32x16& to = APART && q < 2 ? low[APART ? i : 0][APART ? j : 0] : acc[i][j];
+                to = F::mfma(a[set][q == 0 ? FP - 1 : 0][i], b[set][q == 1 ? FP - 1 : 0][j], to);
                 if (SPREAD) {
 #pragma unroll
                     for (int x = m * extra / NM; x < (m + 1) * extra / NM; ++x) other(x);
@@ -349,6 +362,12 @@ struct MmTile {
                 }
             }
             slot = next;
+        }
+        if constexpr (APART) {
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int j = 0; j < TN; ++j) acc[i][j] += low[i][j];
         }
         for (s = n < 1 ? 1 : n; s < most; ++s) __builtin_amdgcn_s_barrier();   // (a group with fewer stages)
         // LDS may be reused by the caller behind this point (every wave has read its last stage)

@@ -327,3 +327,28 @@ def test_layer_norm_of_rows_of_equal_and_nearly_equal_large_values(C, dtype):
         off = 0.5 * 1.001 * step[:, None].double() * rs
         R.within(y, (x64 - mu) * rs, off + 32 * R.U * ((x64 - mu) * rs).abs() + 32 * R.U, "y")
         R.within(rstd, rs[:, 0], 64 * R.U * rs[:, 0], "rstd")
+
+
+@pytest.mark.parametrize("chain", [False, True])
+def test_orthogonalize_is_as_near_to_64_bits_as_32_bit_products(chain):
+    """300 matrices of up to 64 rows, alone and beside a larger one (which sends them through the chain of launches): against the plain form
+    in 32 bits.  Both errors are a few roundings that the iteration amplifies, so either form is the nearer one by chance.  Where one is
+    1.5 times as far off as the other (and beyond 1e-6), a fair coin decides which: of n such matrices the kernel has at most
+    n / 2 + 3 sqrt(n) / 2."""
+    import math
+    import random
+    from ssecg import ops
+    rng = random.Random(5)
+    larger = _normal(_gen(199), 300, 400)
+    further = nearer = 0
+    for k in range(300):
+        m, n = (int(round(math.exp(rng.uniform(0, math.log(top))))) for top in (64, 4096))
+        g, r = _gen(k), max(1, min(m, n) // 8)
+        x = ((_normal(g, m, r) @ _normal(g, r, n)) / math.sqrt(r) + _normal(g, m, n, scale=0.5)) * 1e-3
+        want, plain = R.orthogonal(x), R.orthogonal(x, dtype=torch.float32)
+        got = ops.orthogonalize([x, larger])[0] if chain else ops.orthogonalize(x)
+        own, off = ((v.double() - want).norm() / want.norm() for v in (plain, got))
+        further += int(off > max(1e-6, 1.5 * own))
+        nearer += int(own > max(1e-6, 1.5 * off))
+    count = further + nearer
+    assert further <= count / 2 + 1.5 * math.sqrt(count), (further, nearer)
