@@ -631,9 +631,12 @@ int ce_fwd(const void* x, const void* w, const float* bias, const int64_t* targe
 #define SSECG_CE_JOIN(ROWS, WHOLE)                                                                                                        \
     hipLaunchKernelGGL((ce_join_kernel<ROWS, WHOLE>), dim3((unsigned)((N + ROWS - 1) / ROWS)), dim3(1024), 0, st, p.pm, p.ps, p.tl, p.parts, \
                        (int)N, (int)V, target, counts, mean, out)
-    // few rows whose parts one workgroup reads in a few rounds: the total in the same launch.  Else few rows: more strands each (8 x 1024
-    // x 32768 fp16: the forward pass takes 19.7 us, 21.2 with 16 rows a workgroup), many: whole sectors of their parts (126 rows: the
-    // same; 2000 x 768 x 32000 bf16: 104 us against 109).
+    // Few rows whose parts one workgroup reads in a few rounds: the total in the same launch.  Forward passes over 64 columns in fp16, one
+    // workgroup for all against many and a second launch: 8 rows and 500 / 2000 / 4096 parts 7.2 / 10.8 / 17.0 us against 9.4 / 12.1 / 17.3, 2 rows
+    // and 2000 / 4096 parts 11.1 / 17.2 against 10.8 / 14.3; 16 to 128 rows and 32 / 126 / 500 parts 6.9 / 8.6 / 16.8 against 8.9 / 9.0 / 10.3.
+    // Else up to 64 rows: more strands each (2 rows a workgroup against 16, 8 rows and 2000 / 4096 parts 12.1 / 17.3 us against 15.1 /
+    // 23.4, 32 rows 15.2 / 23.6 against 16.0 / 25.7, 64 rows 16.4 / 26.4 against 16.7 / 26.0); more rows: whole sectors of their parts
+    // (128 rows 14.2 / 20.7 against 14.8 / 22.5; 256 rows 17.4 / 26.7 against 18.3 / 28.3).
     if (N <= 8 && p.parts <= 2048) {
         SSECG_CE_JOIN(8, true);
         return (int)hipGetLastError();

@@ -5,7 +5,9 @@
 //   One: the data itself (bf16 or fp16).
 //   Two (fp16), for values of a known range: v, scaled by a power of two into fp16's normal range, as hi = fp16(v) and
 // lo = fp16(v - hi) - 22 to 23 significant bits - and D = hi hi + hi lo + lo hi in fp32 accumulators (the dropped lo lo is 2^-22 of
-// the product and of random sign).  They lie interleaved, 32 hi then 32 lo, so that a stage of a row is 128 consecutive bytes: 32 k.
+// the product and of random sign but on a Gram matrix's diagonal).  FULL tiles, of up to 4 blocks a wave, form lo lo too and sum the three
+// small products apart, so that the large one takes one rounding per k step instead of three; beyond, registers do not allow it, and
+// the roundings of longer sums count for more.  The planes lie interleaved, 32 hi then 32 lo, so that a stage of a row is 128 consecutive bytes: 32 k.
 //   Three (bf16), for any 32-bit values: b0 = bf16(v), b1 = bf16(v - b0), b2 = v - b0 - b1.  8 + 8 + 8 bits hold v exactly, and at
 // its own exponent: no scale, no floor, each row and each element is as precise as in a 32-bit product whatever else the operand
 // holds.  D is the six products down to 2^-18; the three dropped are at most 2^-26 of |a||b|.  The planes lie one behind the other, each
@@ -76,7 +78,7 @@ template <> struct Frag<_Float16> {
     static __device__ __forceinline__ f32x16 mfma(type a, type b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 };
 
-template <typename T_, int P_, int BM_, int BN_, int WM_, int WN_, int R_, bool TA_ = false, bool TB_ = false, int KG_ = 1>
+template <typename T_, int P_, int BM_, int BN_, int WM_, int WN_, int R_, bool TA_ = false, bool TB_ = false, int KG_ = 1, bool FULL_ = false>
 struct MmTile {
     using T = T_;
     using F = Frag<T>;
@@ -86,6 +88,7 @@ struct MmTile {
     static constexpr bool TA = TA_, TB = TB_;
     static constexpr int KG = KG_, NW = WM * WN, NT = KG * NW * 64;   // waves of a group, threads of the workgroup
     static constexpr int TM = BM / WM / 32, TN = BN / WN / 32;
+    static constexpr bool FULL = FULL_, APART = FULL && P == 2 && TM * TN <= 4;
     static constexpr int BK = FP == 1 ? 64 : 32;                // k of a stage
     static constexpr int STEP = 128;                            // bytes of a k-fast row in a stage
     static constexpr int PA = BM / 8 / NW, PB = BN / 8 / NW, PPW = PA + PB;   // 1 KB pieces (8 rows) per wave and stage
@@ -287,9 +290,6 @@ struct MmTile {
         // early count for more (8192 x 1024 x 65536 bf16: dx 951 us, 986 spread).
         constexpr bool SPREAD = TM * TN > 8;
         static_assert(!SPREAD || (!TA && !TB), "the spread requests are those of k-fast operands");
-        // Two planes: the small products have accumulators of their own where registers allow it, so that the large one takes one rounding
-        // per k step instead of three.
-        constexpr bool APART = P == 2 && TM * TN <= 4;
         f32x16 low[APART ? TM : 1][APART ? TN : 1];
         if constexpr (APART) {
 #pragma unroll
@@ -300,13 +300,13 @@ struct MmTile {
                     for (int e = 0; e < 16; ++e) low[i][j][e] = 0.f;
         }
         auto multiply = [&](int set, int extra, auto other) {
-            constexpr int NM = (FP == 1 ? 1 : 3) * TM * TN;
+            constexpr int NM = (FP == 1 ? 1 : APART ? 4 : 3) * TM * TN;
 #pragma unroll
             for (int m = 0; m < NM; ++m) {
                 // two planes: the small products first, each product over all blocks: no accumulator is used twice in a row
-                const int q = FP == 1 ? 2 : m / (TM * TN), i = m % (TM * TN) / TN, j = m % TN;
+                const int q = FP == 1 ? 2 : m / (TM * TN) - (APART ? 1 : 0), i = m % (TM * TN) / TN, j = m % TN;
                 f32x16& to = APART && q < 2 ? low[APART ? i : 0][APART ? j : 0] : acc[i][j];
-                to = F::mfma(a[set][q == 0 ? FP - 1 : 0][i], b[set][q == 1 ? FP - 1 : 0][j], to);
+                to = F::mfma(a[set][q <= 0 ? FP - 1 : 0][i], b[set][q == 1 || q < 0 ? FP - 1 : 0][j], to);
                 if (SPREAD) {
 #pragma unroll
                     for (int x = m * extra / NM; x < (m + 1) * extra / NM; ++x) other(x);
@@ -464,7 +464,9 @@ template <class M> struct WaveStore {
 // The time of a launch in microseconds, to choose a tile side by.  One stage of one workgroup takes `alone` us where it has the chip to
 // itself and `full` us where the chip is full (two workgroups a CU up to 128), measured on products of 4096 x 4096 x 4096 (full:
 // 120 / 155 / 200 us with one plane, 308 / 344 / 466 us with two, for sides of 256 / 128 / 64; a triangle of 192: 204) and 512 x 1536
-// x 512 (alone; 128 with two planes, whose operands leave the L2 first: 2000 x 6000); between them it grows with the workgroups.
+// x 512 (alone; 128 with two planes, whose operands leave the L2 first: 2000 x 6000); between them it grows with the workgroups.  Three
+// planes are timed as six stages of one: the side chosen so is within 3 % of the best of the three at eight shapes from 126 x 512 x 1000
+// to 8192 x 512 x 16384.
 struct MmWork {
     int64_t tiles = 0, stages = 0, longest = 0;      // workgroups, their stages together, the most stages of one
     void add(int64_t n, int64_t per) {
@@ -505,6 +507,13 @@ __device__ __forceinline__ uint16_t plane16(float v, int q) {
     if (q == 0) return bits16(hi);
     const float f = (float)hi;
     return __builtin_isinf(f) ? 0 : bits16((_Float16)(v - f));   // an infinity stays one instead of inf - inf
+}
+
+// both planes of v + rest, |rest| a few units of v's last place (hi in the lower half)
+__device__ __forceinline__ uint32_t planes16(float v, float rest) {
+    const _Float16 hi = (_Float16)v;
+    const float f = (float)hi;
+    return (uint32_t)bits16(hi) | (__builtin_isinf(f) ? 0u : (uint32_t)bits16((_Float16)((v - f) + rest)) << 16);
 }
 
 // v as three bf16 values that add up to it.  What rounds to infinity is cut off instead; infinities and NaN are in the first alone.

@@ -11,13 +11,16 @@
 //
 // Precision: the iteration multiplies errors along weak directions by up to a = 3.44 per step (485 over five), so 16-bit iterates
 // would lose them.  All matrices are two fp16 planes times 2^13 - singular values stay below 1.21 and P's below 3.45, far inside
-// fp16's range, and an entry keeps 22 bits down to 2^-16 of the largest possible one - with fp32 accumulators.
+// fp16's range - with fp32 accumulators.  An entry of a matrix whose norm is 1 keeps 22 to 23 bits down to 2^-16, fewer below, none below
+// 2^-38: entries of 10^-9 have 7 bits left, in a direction that ends as 5e-7 of the result.  Results in fp32 are as far from
+// 64 bits as 32-bit products are (300 matrices of up to 64 rows: the one or the other by chance; 4096 x 4096: 3.7e-6 against 3.6e-6).
 //
 // Large matrices are bound by the matrix pipe: 4096 x 4096 takes 3.6 ms for five steps; an update's product 340 us (1.21 PFLOP/s of
 // fp16 products; a large library product reaches 1.3 to 1.6), a symmetric one 204 to 215 us (1.0 of those that count: 253 tiles of one
 // workgroup each, four waves, fill the 256 CUs once).  A model's matrices are bound by the chain: the optimiser step of a 1D
 // ResNet18 (21 matrices up to 512 x 1536) takes 260 us over 17 launches of 5 to 35 us, each a few dozen stages of latency.
 #include <initializer_list>
+#include <type_traits>
 #include <utility>
 #include "mm_core.h"
 #include "ssecg.h"
@@ -25,8 +28,48 @@
 namespace {
 using namespace ssecg_lm;
 
-constexpr float kA = 3.4445f, kB = -4.7750f, kC = 2.0315f;
+constexpr double kA = 3.4445, kB = -4.7750, kC = 2.0315;
 constexpr int kScale = 13;
+
+// Both planes of kC v + kB w (+ kA on the diagonal), all times 2^13.  The three cancel to a fifth of the largest.  FULL: the sums' roundings
+// and the coefficients' own (2^-25, the same in every entry and step) are carried along; what is left is the planes' rounding.
+template <bool FULL>
+__device__ __forceinline__ uint32_t poly_planes(float v, float w, bool diagonal) {
+    if constexpr (!FULL) {
+        return planes16((float)kC * v + ((float)kB * w + (diagonal ? (float)kA * (float)(1 << kScale) : 0.f)), 0.f);
+    } else {
+#pragma clang fp contract(off)
+        constexpr float b = (float)kB, bl = (float)(kB - (double)b), c = (float)kC, cl = (float)(kC - (double)c);
+        constexpr double a64 = kA * (double)(1 << kScale);
+        constexpr float a = (float)a64, al = (float)(a64 - (double)a);
+        const float p = b * w, r = c * v, one = diagonal ? a : 0.f;
+        const float s = p + r, sp = s - p, se = (p - (s - sp)) + (r - sp);
+        const float d = one + s, ds = d - one, de = (one - (d - ds)) + (s - ds);
+        const float rest = ((__builtin_fmaf(b, w, -p) + __builtin_fmaf(c, v, -r)) + (se + de)) + (__builtin_fmaf(bl, w, cl * v) + (diagonal ? al : 0.f));
+        return planes16(d, rest);
+    }
+}
+
+// a number as the sum of two in fp32
+struct Two {
+    float h, l;
+    explicit __device__ __forceinline__ Two(double v) : h((float)v), l((float)(v - (double)h)) {
+        if (__builtin_isinf(h)) l = 0.f;
+    }
+    // both planes of u times it
+    template <bool FULL> __device__ __forceinline__ uint32_t planes(float u) const {
+        if constexpr (!FULL) {
+            return planes16(u * h, 0.f);
+        } else {
+#pragma clang fp contract(off)
+            const float p = u * h;
+            return planes16(p, __builtin_fmaf(u, h, -p) + u * l);
+        }
+    }
+};
+
+// A result in fp32 is held to what 32-bit products give; in 16 bits its rounding, in the optimiser the parameter's is far larger.
+template <typename S, bool MUON> constexpr bool kFull = std::is_same<S, float>::value && !MUON;
 constexpr int kNormParts = 1024;                  // most workgroups that share one matrix's norm
 constexpr int kMost = 32;                         // matrices of one chain of launches: their table travels in the kernel arguments
 
@@ -155,16 +198,13 @@ __global__ __launch_bounds__(256) void ns_prep_kernel(Table table, char* __restr
     for (int p = lane; p < parts; p += 64) s += partial[(int64_t)k * parts + p];
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
-    const float f = (float)((double)(1 << kScale) / (sqrt(s) + eps));
+    const Two f((double)(1 << kScale) / (sqrt(s) + eps));
     const int tiles = (int)((up(t.cols, 32) + 63) / 64), q0 = blockIdx.x - first;
     const int64_t rb = (int64_t)(q0 / tiles) * 64, cb = (int64_t)(q0 % tiles) * 64;
     for (int i = strand; i < 64; i += 4) {
         const int64_t r = rb + i, c = cb + lane;
         uint32_t q = 0;
-        if (r < t.rows && c < t.cols) {
-            const float u = update_of<S, MUON>(t, r * t.cols + c, mu, nesterov) * f;
-            q = (uint32_t)plane16(u, 0) | (uint32_t)plane16(u, 1) << 16;
-        }
+        if (r < t.rows && c < t.cols) q = f.planes<kFull<S, MUON>>(update_of<S, MUON>(t, r * t.cols + c, mu, nesterov));
         tile[i][lane] = q;
     }
     __syncthreads();
@@ -196,8 +236,8 @@ __device__ __forceinline__ void tri_tile(int q, int& ti, int& tj) {
 
 // The same triangle of T rows of tiles in blocks of S x S tiles, so that the tiles of one XCD, which follow each other, share few rows of
 // the operand: those of one row of tiles would each read different ones (4096 x 4096 in tiles of 64: 5.05 -> 4.63 ms, of 256: 4.63 ->
-// 4.39; small matrices: the same).  S = 1 is the order by rows: tiles of 192, which all run at once, are as well off with it (3767 us;
-// 3838 in blocks of 6).
+// 4.39; small matrices: the same).  S = 1 is the order by rows: tiles of 192 are better off with it at every size (five steps at 1500 /
+// 3000 / 4096 / 6000 square: 866 / 2022 / 3647 / 13827 us; in blocks of 6: 903 / 2094 / 3706 / 14171).
 template <int S>
 __device__ __forceinline__ void tri_block(int q, int T, int& ti, int& tj) {
     tri_tile(q, ti, tj);
@@ -250,17 +290,20 @@ __global__ __launch_bounds__(M::NT, M::TM * M::TN > 8 ? 1 : 2) void ns_gram_kern
                     for (int k = 0; k < 4; ++k) w[k] = (float)hi[k] + (float)lo[k];
                 }
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    float d = acc[i][j][e + k] * down;
-                    if (POLY) d = kC * d + (kB * w[k] + (r + k == c ? kA * (float)(1 << kScale) : 0.f));
-                    acc[i][j][e + k] = r + k < t.m && c < t.m ? d : 0.f;
+                for (int k = 0; k < 4; ++k) {                // from here on both planes of the value, in its register
+                    const float d = acc[i][j][e + k] * down;
+                    const uint32_t q = POLY ? poly_planes<M::FULL>(d, w[k], r + k == c) : planes16(d, 0.f);
+                    acc[i][j][e + k] = __builtin_bit_cast(float, r + k < t.m && c < t.m ? q : 0u);
                 }
             }
     }
     using W = WaveStore<M>;
     char* reg = W::region(lds);
     const int r0 = a0 + M::wave_row(), c0 = b0 + M::wave_col();
-    auto val = [&](int i, int j, int e, int q) -> uint16_t { return plane16(acc[i][j][e], q); };
+    auto val = [&](int i, int j, int e, int q) -> uint16_t {
+        const float both = acc[i][j][e];
+        return (uint16_t)(__builtin_bit_cast(uint32_t, both) >> 16 * q);
+    };
     auto put = [&](int r, int c, int q, u32x4 d) {
         if (r < t.m && kbyte<2>(c) < t.pm) *reinterpret_cast<u32x4*>(out + (int64_t)r * t.pm + kbyte<2>(c, q)) = d;
     };
@@ -382,10 +425,10 @@ __device__ __forceinline__ f16x8 small_across(const char* base, int64_t pitch, i
     const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(p + 4 * pitch));
     return __builtin_bit_cast(f16x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
 }
-__device__ __forceinline__ void small_put(char* base, int64_t pitch, int row, int col, float v) {
+__device__ __forceinline__ void small_put(char* base, int64_t pitch, int row, int col, uint32_t q) {   // both planes
     char* d = base + row * pitch + (col >> 5) * 128 + (col & 31) * 2;
-    *reinterpret_cast<uint16_t*>(d) = plane16(v, 0);
-    *reinterpret_cast<uint16_t*>(d + 64) = plane16(v, 1);
+    *reinterpret_cast<uint16_t*>(d) = (uint16_t)q;
+    *reinterpret_cast<uint16_t*>(d + 64) = (uint16_t)(q >> 16);
 }
 
 template <typename S, bool MUON>
@@ -395,6 +438,7 @@ __global__ __launch_bounds__(kSmallWaves * 64) void ns_small_kernel(Table table,
     const float mu = MUON ? ap.mu() : 0.f;
     __shared__ __attribute__((aligned(16))) char lds[kSmallLds];
     __shared__ double sums[kSmallWaves];
+    constexpr bool FULL = kFull<S, MUON>;
     const Mat t = load_mat(table, blockIdx.x, nullptr, 0);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 31, h = lane >> 5;
     const int mp = (int)up(t.m, 32), np = (int)up(t.n, 32), lb = mp >> 6, mb = 1 << lb;   // 32 or 64 rows: 1 or 2 blocks, lb = log2
@@ -433,7 +477,7 @@ __global__ __launch_bounds__(kSmallWaves * 64) void ns_small_kernel(Table table,
     s = 0.0;
 #pragma unroll
     for (int w = 0; w < kSmallWaves; ++w) s += sums[w];
-    const float f = (float)((double)(1 << kScale) / (sqrt(s) + eps));
+    const Two f((double)(1 << kScale) / (sqrt(s) + eps));
 #pragma unroll 2
     for (int i = threadIdx.x * V; i < count; i += kSmallWaves * 64 * V) {   // (a thread reads the momentum that it wrote)
         const int left = count - i < V ? count - i : V;
@@ -445,7 +489,7 @@ __global__ __launch_bounds__(kSmallWaves * 64) void ns_small_kernel(Table table,
         for (int j = 0; j < V; ++j) {
             float u = (float)g[j];
             if constexpr (MUON) u = nesterov ? u + mu * v[j] : v[j];
-            if (j < left) small_put(X, px, tall ? col : row, tall ? row : col, u * f);
+            if (j < left) small_put(X, px, tall ? col : row, tall ? row : col, f.planes<FULL>(u));
             if (++col == t.cols) { col = 0; ++row; }
         }
     }
@@ -472,9 +516,10 @@ __global__ __launch_bounds__(kSmallWaves * 64) void ns_small_kernel(Table table,
                 for (int kk = part; kk < kks; kk += shares) {
                     const f16x8 ah = small_along(src, pitch, 32 * i + r, kk, h, 0), al = small_along(src, pitch, 32 * i + r, kk, h, 1);
                     const f16x8 bh = small_along(src, pitch, 32 * j + r, kk, h, 0), bl = small_along(src, pitch, 32 * j + r, kk, h, 1);
-                    low = F::mfma(al, bh, low);
+                    if (FULL) low = F::mfma(al, bl, low);
                     cross = F::mfma(ah, bl, cross);
                     acc = F::mfma(ah, bh, acc);
+                    low = F::mfma(al, bh, low);
                 }
 #pragma unroll
                 for (int e = 0; e < 16; ++e) scratch[(part * blocks + b) * 1024 + e * 64 + lane] = acc[e] + (low[e] + cross[e]);
@@ -493,11 +538,11 @@ __global__ __launch_bounds__(kSmallWaves * 64) void ns_small_kernel(Table table,
                 }
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    float d = v[k] * down;
-                    if (phase == 1) d = kC * d + (kB * ((float)hi[k] + (float)lo[k]) + (row == col + k ? kA * (float)(1 << kScale) : 0.f));
-                    d = row < t.m && col + k < t.m ? d : 0.f;
-                    hi[k] = (_Float16)d;
-                    lo[k] = (_Float16)(d - (float)hi[k]);
+                    const float d = v[k] * down;
+                    uint32_t q = phase == 1 ? poly_planes<FULL>(d, (float)hi[k] + (float)lo[k], row == col + k) : planes16(d, 0.f);
+                    q = row < t.m && col + k < t.m ? q : 0u;
+                    hi[k] = __builtin_bit_cast(_Float16, (uint16_t)q);
+                    lo[k] = __builtin_bit_cast(_Float16, (uint16_t)(q >> 16));
                 }
                 char* d = (phase == 0 ? A : P) + off;
                 __builtin_memcpy(d, hi, 8);
@@ -506,7 +551,7 @@ __global__ __launch_bounds__(kSmallWaves * 64) void ns_small_kernel(Table table,
             __syncthreads();
         }
         const bool last = step + 1 == steps;
-        f32x16 acc[kSmallPairs];                          // X = P X: block (i, blk) is pair wave + 8 n
+        f32x16 acc[kSmallPairs];                          // X = P X: block (i, blk) is pair wave + 16 n
 #pragma unroll
         for (int n = 0; n < kSmallPairs; ++n) {
             const int pair = wave + kSmallWaves * n, i = pair & (mb - 1), blk = pair >> lb;
@@ -516,6 +561,7 @@ __global__ __launch_bounds__(kSmallWaves * 64) void ns_small_kernel(Table table,
             for (int kk = 0; kk < mp / 16; ++kk) {
                 const f16x8 bh = small_across(X, px, lane, blk, kk, 0), bl = small_across(X, px, lane, blk, kk, 1);
                 const f16x8 ah = small_along(P, pa, 32 * i + r, kk, h, 0), al = small_along(P, pa, 32 * i + r, kk, h, 1);
+                if (FULL) acc[n] = F::mfma(al, bl, acc[n]);
                 acc[n] = F::mfma(al, bh, acc[n]);
                 acc[n] = F::mfma(ah, bl, acc[n]);
                 acc[n] = F::mfma(ah, bh, acc[n]);
@@ -569,10 +615,10 @@ __global__ __launch_bounds__(kSmallWaves * 64) void ns_small_kernel(Table table,
     }
 }
 
-template <bool TB> using Big = MmTile<_Float16, 2, 256, 256, 2, 4, 2, false, TB>;
-using Tri = MmTile<_Float16, 2, 192, 192, 2, 2, 3>;      // a triangle of tiles: 253 of them cover 4096 x 4096, one per CU
-template <bool TB, int KG = 1> using Mid = MmTile<_Float16, 2, 128, 128, 2, 2, 2, false, TB, KG>;
-template <bool TB, int KG = 1> using Small = MmTile<_Float16, 2, 64, 64, 2, 2, 4, false, TB, KG>;
+template <bool FULL, bool TB> using Big = MmTile<_Float16, 2, 256, 256, 2, 4, 2, false, TB, 1, FULL>;
+template <bool FULL> using Tri = MmTile<_Float16, 2, 192, 192, 2, 2, 3, false, false, 1, FULL>;   // 253 of them cover a triangle of 4096, one per CU
+template <bool FULL, bool TB, int KG = 1> using Mid = MmTile<_Float16, 2, 128, 128, 2, 2, 2, false, TB, KG, FULL>;
+template <bool FULL, bool TB, int KG = 1> using Small = MmTile<_Float16, 2, 64, 64, 2, 2, 4, false, TB, KG, FULL>;
 
 #define SSECG_NS_LAUNCH(M, kernel, grid, st, ...)                                                                               \
     do {                                                                                                                        \
@@ -586,26 +632,26 @@ struct Plan {
     int parts, prep, gram, upd, gramTile, updTile, gramGroups, updGroups;   // workgroups of the launches, tile sides, groups of waves
 };
 
-template <bool POLY>
+template <bool POLY, bool FULL>
 int launch_gram(const Table& t, const Plan& p, char* ws, int from, const float* skip, hipStream_t st) {
 #define SSECG_NS_GRAM(...) do { using M = __VA_ARGS__; SSECG_NS_LAUNCH(M, (ns_gram_kernel<M, POLY>), p.gram, st, t, ws, from, skip); } while (0)
-    if (p.gramTile == 256) SSECG_NS_GRAM(Big<false>);
-    else if (p.gramTile == 192) SSECG_NS_GRAM(Tri);
-    else if (p.gramTile == 128) SSECG_NS_GRAM(Mid<false>);
-    else if (p.gramGroups == 2) SSECG_NS_GRAM(Small<false, 2>);
-    else SSECG_NS_GRAM(Small<false>);
+    if (p.gramTile == 256) SSECG_NS_GRAM(Big<FULL, false>);
+    else if (p.gramTile == 192) SSECG_NS_GRAM(Tri<FULL>);
+    else if (p.gramTile == 128) SSECG_NS_GRAM(Mid<FULL, false>);
+    else if (p.gramGroups == 2) SSECG_NS_GRAM(Small<FULL, false, 2>);
+    else SSECG_NS_GRAM(Small<FULL, false>);
 #undef SSECG_NS_GRAM
     return 0;
 }
 
-template <typename S, int LAST>
+template <typename S, int LAST, bool FULL>
 int launch_update(const Table& t, const Plan& p, char* ws, int from, const Apply& ap, const float* skip, hipStream_t st) {
 #define SSECG_NS_UPDATE(...) \
     do { using M = __VA_ARGS__; SSECG_NS_LAUNCH(M, (ns_update_kernel<M, S, LAST>), p.upd, st, t, ws, from, ap, skip); } while (0)
-    if (p.updTile == 256) SSECG_NS_UPDATE(Big<true>);
-    else if (p.updTile == 128 && p.updGroups == 2) SSECG_NS_UPDATE(Mid<true, 2>);
-    else if (p.updTile == 128) SSECG_NS_UPDATE(Mid<true>);
-    else SSECG_NS_UPDATE(Small<true>);
+    if (p.updTile == 256) SSECG_NS_UPDATE(Big<FULL, true>);
+    else if (p.updTile == 128 && p.updGroups == 2) SSECG_NS_UPDATE(Mid<FULL, true, 2>);
+    else if (p.updTile == 128) SSECG_NS_UPDATE(Mid<FULL, true>);
+    else SSECG_NS_UPDATE(Small<FULL, true>);
 #undef SSECG_NS_UPDATE
     return 0;
 }
@@ -682,10 +728,11 @@ int run_chain(const int64_t* mats, int count, int nesterov, int steps, double ep
     hipLaunchKernelGGL((ns_prep_kernel<S, MUON>), dim3((unsigned)p.prep), dim3(256), 0, st, t, ws, ap, nesterov, p.parts, eps, skip, partial);
     rc = (int)hipGetLastError();
     for (int k = 0; k < steps && rc == 0; ++k) {
-        if ((rc = launch_gram<false>(t, p, ws, k & 1, skip, st)) != 0) break;
-        if ((rc = launch_gram<true>(t, p, ws, k & 1, skip, st)) != 0) break;
-        if (k + 1 < steps) rc = launch_update<S, 0>(t, p, ws, k & 1, ap, skip, st);
-        else rc = launch_update<S, MUON ? 2 : 1>(t, p, ws, k & 1, ap, skip, st);
+        constexpr bool FULL = kFull<S, MUON>;
+        if ((rc = launch_gram<false, FULL>(t, p, ws, k & 1, skip, st)) != 0) break;
+        if ((rc = launch_gram<true, FULL>(t, p, ws, k & 1, skip, st)) != 0) break;
+        if (k + 1 < steps) rc = launch_update<S, 0, FULL>(t, p, ws, k & 1, ap, skip, st);
+        else rc = launch_update<S, MUON ? 2 : 1, FULL>(t, p, ws, k & 1, ap, skip, st);
     }
     return rc;
 }
