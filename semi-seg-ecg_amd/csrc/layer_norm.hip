@@ -4,12 +4,13 @@
 //   g = dy w,  dx = r (g - mean(g) - xh mean(g xh)),  dw = sum_rows dy xh,  db = sum_rows dy
 //
 // Both passes are bound by HBM: forward reads x and writes y, backward reads x and dy and writes dx - each byte once.  32768 x 4096
-// bf16: 90 us and 174 us (6.0 and 4.6 TB/s; a large copy reaches 5.0), and 5 us for the parameters' gradients.  Below a few
-// megabytes latency counts: 1008 x 512 fp32 takes 3.9 us, and 6.3 + 4.4 us backward.  A row stays in the registers of the threads
+// bf16: 103 us and 177 us (5.2 and 4.6 TB/s; a large copy reaches 5.0), and 5 us for the parameters' gradients.  Below a few
+// megabytes latency counts: 1008 x 512 fp32 takes 3.9 us, and 5.9 + 4.6 us backward.  Rows beyond the registers (below) run at 1.0 to
+// 2.7 TB/s.  A row stays in the registers of the threads
 // that own it (64 to 1024 of them), so the variance is the two-pass one (the sum of squared differences from the mean, no
 // cancellation) without a second read.  The differences are summed beside their squares and correct the mean: a sum's roundings leave
 // it a few steps of x off, which for rows of nearly equal large values is as much as they differ (a constant row gave 0.93
-// instead of 0).  A thread owns the same columns of every row its workgroup takes: w and b are loaded once,
+// instead of 0; forward 90 us without it).  A thread owns the same columns of every row its workgroup takes: w and b are loaded once,
 // and the column sums dw / db grow in its registers; the row groups of a workgroup are joined in LDS, the workgroups by a second
 // launch in fixed order (no atomics: results do not change from run to run).  Statistics, sums and parameter gradients are fp32; y
 // and dx are rounded once.
@@ -53,7 +54,7 @@ __device__ __forceinline__ float product(float a, float b) {
 // mean and 1 / deviation from an approximate mean and the means of the differences from it and of their squares
 __device__ __forceinline__ void row_stats(float near, float d, float d2, float eps, float& mu, float& rs) {
     const float var = d2 - d * d;                     // d2 >= d^2 but for roundings
-    mu = near + d;
+    mu = d == d ? near + d : near;                    // (a row with an infinity: its mean is infinite)
     rs = 1.f / sqrtf((var < 0.f ? 0.f : var) + eps);  // (a NaN stays one)
 }
 

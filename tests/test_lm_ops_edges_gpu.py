@@ -238,6 +238,15 @@ def test_layer_norm_refuses_rows_longer_than_it_counts():
         del x
 
 
+def test_layer_norm_of_infinite_and_nan_rows_keeps_their_mean():
+    from ssecg import ops
+    x = _normal(_gen(182), 4, 300)
+    x[0, 3], x[1, 4], x[2, 5] = float("inf"), float("-inf"), float("nan")
+    y, mean, rstd = ops.layer_norm_fwd(x)
+    assert mean[0] == float("inf") and mean[1] == float("-inf") and torch.isnan(mean[2])
+    assert torch.isnan(y[:3]).all() and torch.isnan(rstd[:3]).all() and torch.isfinite(y[3]).all()
+
+
 # ------------------------------------------------------------------------------------------------ what autograd keeps
 @pytest.mark.parametrize("dtype", TYPES)
 def test_linear_ce_keeps_everything_as_saved_tensors(dtype):
