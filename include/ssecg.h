@@ -574,7 +574,8 @@ int ssecg_linear_ce_bwd(const float *dloss, const void *x, const void *weight, c
                         size_t workspace_bytes, void *stream);
 
 /* Newton-Schulz orthogonalisation of `count` matrices.  mats is a HOST array of rows {source, result, momentum, rows, cols} (device
- * pointers as integers; momentum unused here); it is read during the call only.  At most 2^20 rows / columns each. */
+ * pointers as integers; momentum unused here); it is read during the call only.  At most 2^20 rows / columns each.  fp32 results are as
+ * near to 64 bits as 32-bit products are; entries below 2^-16 of the norm keep fewer bits, below 2^-38 none. */
 size_t ssecg_orthogonalize_workspace(const int64_t *mats, int count);
 int ssecg_orthogonalize_multi(const int64_t *mats, int count, int dtype, int steps, double eps, void *workspace,
                               size_t workspace_bytes, void *stream);

@@ -20,12 +20,14 @@
 // of x and w; more planes would write twice the bytes and triple dx's and dw's time.  The gradients' relative error against 64 bits is
 // 1.7e-3 to 2.2e-3 in bf16 (1.7e-3 of it their own rounding at the end), 2.1e-4 to 2.8e-4 in fp16.  fp16 has no values below
 // 2^-24: E, in [-1, 1], is held times 2^15, has fewer bits below 2^-29 and is zero below 2^-40 (of the largest |upstream gradient| where the
-// loss is not reduced) - as f E x itself is in fp16 at a loss scale of 2^16.  Rows whose g_n is zero enter nothing: neither their values (which may be infinite or NaN) nor their products.
+// loss is not reduced) - as f E x itself is in fp16 at a loss scale of 2^16.  Rows whose g_n is zero enter nothing: neither their values
+// (which may be infinite or NaN) nor their products.
 //
-// Many positions are bound by the matrix pipe: 8192 x 1024 x 65536 bf16 takes 1.13 ms forward (0.97 PFLOP/s) and 3.4 ms backward: E
-// 1.43 ms, of which 0.3 for its 1 GiB and its exponentials, dx 0.94 (1.17 PFLOP/s), dw 0.99.  Few positions are bound by the weights,
-// read three times and written once: 8 x 1024 x 32768 fp16 takes 76 us, each pass over them 13 to 20 us (4.7 to 3.4 TB/s).  The
-// smallest calls are bound by their launches: 126 x 512 x 1000 fp32, 8 of them, 48 us.
+// Many positions are bound by the products' main loop, which keeps the matrix pipe busy 48 to 61 % of the cycles: 8192 x 1024 x 65536 bf16
+// takes 1.13 ms forward (0.97 PFLOP/s) and 3.4 ms backward: E 1.42 ms, of which 0.3 for its 1 GiB and its exponentials, dx 0.95 (1.15
+// PFLOP/s), dw 1.03.  fp32 is six such products each: 2000 x 512 x 8192 takes 93, 115, 135 and 144 us for the four (0.7 to 1.1 PFLOP/s).  Few
+// positions are bound by the weights, read three times and written once: 8 x 1024 x 32768 fp16 takes 77 us, each pass over them 13
+// to 20 us (4.7 to 3.4 TB/s).  The smallest calls are bound by their launches: 126 x 512 x 1000 fp32, 7 of them, 59 us.
 #include <type_traits>
 #include "mm_core.h"
 #include "ssecg.h"

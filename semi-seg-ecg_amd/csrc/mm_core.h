@@ -7,7 +7,8 @@
 // lo = fp16(v - hi) - 22 to 23 significant bits - and D = hi hi + hi lo + lo hi in fp32 accumulators (the dropped lo lo is 2^-22 of
 // the product and of random sign but on a Gram matrix's diagonal).  FULL tiles, of up to 4 blocks a wave, form lo lo too and sum the three
 // small products apart, so that the large one takes one rounding per k step instead of three; beyond, registers do not allow it, and
-// the roundings of longer sums count for more.  The planes lie interleaved, 32 hi then 32 lo, so that a stage of a row is 128 consecutive bytes: 32 k.
+// the roundings of longer sums count for more.  The planes lie interleaved, 32 hi then 32 lo, so that a stage of a row is 128
+// consecutive bytes: 32 k.
 //   Three (bf16), for any 32-bit values: b0 = bf16(v), b1 = bf16(v - b0), b2 = v - b0 - b1.  8 + 8 + 8 bits hold v exactly, and at
 // its own exponent: no scale, no floor, each row and each element is as precise as in a 32-bit product whatever else the operand
 // holds.  D is the six products down to 2^-18; the three dropped are at most 2^-26 of |a||b|.  The planes lie one behind the other, each

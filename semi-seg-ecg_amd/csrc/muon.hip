@@ -12,13 +12,15 @@
 // Precision: the iteration multiplies errors along weak directions by up to a = 3.44 per step (485 over five), so 16-bit iterates
 // would lose them.  All matrices are two fp16 planes times 2^13 - singular values stay below 1.21 and P's below 3.45, far inside
 // fp16's range - with fp32 accumulators.  An entry of a matrix whose norm is 1 keeps 22 to 23 bits down to 2^-16, fewer below, none below
-// 2^-38: entries of 10^-9 have 7 bits left, in a direction that ends as 5e-7 of the result.  Results in fp32 are as far from
-// 64 bits as 32-bit products are (300 matrices of up to 64 rows: the one or the other by chance; 4096 x 4096: 3.7e-6 against 3.6e-6).
+// 2^-38: entries of 10^-9 have 7 bits left, in a direction that ends as 5e-7 of the result.  For results in fp32 the tiles form
+// every product and the polynomial's roundings are carried along (kFull): over 300 matrices of up to 64 rows the median error is 0.67 of
+// that of 32-bit products; at 4096 x 4096, where long sums count for most, 3.7e-6 against 3.6e-6.
 //
-// Large matrices are bound by the matrix pipe: 4096 x 4096 takes 3.6 ms for five steps; an update's product 340 us (1.21 PFLOP/s of
-// fp16 products; a large library product reaches 1.3 to 1.6), a symmetric one 204 to 215 us (1.0 of those that count: 253 tiles of one
-// workgroup each, four waves, fill the 256 CUs once).  A model's matrices are bound by the chain: the optimiser step of a 1D
-// ResNet18 (21 matrices up to 512 x 1536) takes 260 us over 17 launches of 5 to 35 us, each a few dozen stages of latency.
+// Large matrices are bound by the products' main loop: 4096 x 4096 takes 3.65 to 3.8 ms for five steps; an update's product 340 to 360 us
+// (1.15 to 1.21 PFLOP/s of fp16 products; a large library product reaches 1.3 to 1.6), a symmetric one 204 to 227 us (0.95 to 1.0 of those
+// that count: 253 tiles of one workgroup each, four waves, fill the 256 CUs once).  A model's matrices are bound by the chain: the
+// optimiser step of a 1D ResNet18 (21 matrices up to 512 x 1536) takes 270 to 285 us over 17 launches of 10 to 35 us, each as long as its longest
+// tile, a few dozen stages of latency; its update has 111 tiles for 256 CUs.
 #include <initializer_list>
 #include <type_traits>
 #include <utility>
@@ -45,7 +47,8 @@ __device__ __forceinline__ uint32_t poly_planes(float v, float w, bool diagonal)
         const float p = b * w, r = c * v, one = diagonal ? a : 0.f;
         const float s = p + r, sp = s - p, se = (p - (s - sp)) + (r - sp);
         const float d = one + s, ds = d - one, de = (one - (d - ds)) + (s - ds);
-        const float rest = ((__builtin_fmaf(b, w, -p) + __builtin_fmaf(c, v, -r)) + (se + de)) + (__builtin_fmaf(bl, w, cl * v) + (diagonal ? al : 0.f));
+        const float rest = ((__builtin_fmaf(b, w, -p) + __builtin_fmaf(c, v, -r)) + (se + de)) +
+                           (__builtin_fmaf(bl, w, cl * v) + (diagonal ? al : 0.f));
         return planes16(d, rest);
     }
 }
@@ -389,8 +392,9 @@ __global__ __launch_bounds__(M::NT, M::TM * M::TN > 8 ? 1 : 2) void ns_update_ke
 
 // ---------------------------------------------------------------- small matrices: the whole iteration in one workgroup
 // A matrix whose X, A and P fit the LDS of a CU (160 KB) needs no launch between the steps: 17 launches become one.  Five steps take
-// 36 us at 64 x 192 (78 by the chain of launches), 53 at 64 x 400 (87), 50 at 32 x 1024 (100), 21 at 8 x 8 (52), and 37 for thirty of
-// 64 x 192 (80).  One matrix that does not fit sends all of a call's through the chain, where they cost nothing beside it.
+// 40 us at 64 x 192 (84 by the chain of launches), 59 at 64 x 400 (95), 53 at 32 x 1024 (109), 23 at 8 x 8 (58), and 41 for thirty of
+// 64 x 192 (88); 16-bit results and the optimiser, which need no full precision, 36 at 64 x 192.  One matrix that does not fit sends all
+// of a call's through the chain, where they cost nothing beside it.
 // What bounds it is instructions: a phase lasts as long as its busiest wave.  So the 32 x 32 blocks of a product and shares of its k
 // go over all sixteen waves, the sums meet in LDS in fp32, and every thread joins and splits four values of the result.  Rows are
 // padded by 16 bytes, so that 16 rows read at one k lie in different banks.  X is updated in place, between two barriers.
@@ -798,14 +802,15 @@ static int muon_multi(const int64_t* mats, int count, const Apply& ap, int neste
 int ssecg_muon_multi(const int64_t* mats, int count, double lr, double momentum, int nesterov, double weight_decay, int adjust, int steps, double eps,
                      const float* skip_flag, const double* lr_dev, void* workspace, size_t workspace_bytes, void* stream) {
     if (!(momentum >= 0.0 && momentum < 1.0)) return SSECG_E_INVAL;
-    return muon_multi(mats, count, {lr, weight_decay, adjust, (float)momentum, lr_dev, nullptr}, nesterov, steps, eps, skip_flag, workspace, workspace_bytes,
-                      stream);
+    return muon_multi(mats, count, {lr, weight_decay, adjust, (float)momentum, lr_dev, nullptr}, nesterov, steps, eps, skip_flag, workspace,
+                      workspace_bytes, stream);
 }
 
 int ssecg_muon_multi_scalars(const int64_t* mats, int count, const double* scalars_dev, int nesterov, int adjust, int steps, double eps,
                              const float* skip_flag, void* workspace, size_t workspace_bytes, void* stream) {
     if (!scalars_dev) return SSECG_E_INVAL;
-    return muon_multi(mats, count, {0.0, 0.0, adjust, 0.f, nullptr, scalars_dev}, nesterov, steps, eps, skip_flag, workspace, workspace_bytes, stream);
+    return muon_multi(mats, count, {0.0, 0.0, adjust, 0.f, nullptr, scalars_dev}, nesterov, steps, eps, skip_flag, workspace, workspace_bytes,
+                      stream);
 }
 
 }  // extern "C"

@@ -1520,7 +1520,8 @@ def _mats(rows):
 def orthogonalize(matrices, steps=5, eps=1e-7):
     """The Newton-Schulz iterate of each matrix near its orthogonal factor (singular values about 0.7 .. 1.2), of the matrix's type.
     ``matrices``: one (m, n) tensor or a list of them, all of one type on one device; a list is one chain of launches per 32
-    matrices.  X = G / (|G|_F + eps), ``steps`` times X = a X + (b A + c A A) X with A = X X^T."""
+    matrices.  X = G / (|G|_F + eps), ``steps`` times X = a X + (b A + c A A) X with A = X X^T.  fp32 results are as near to 64 bits as
+    32-bit products are; entries below 2^-38 of the norm count as zeros."""
     one = isinstance(matrices, torch.Tensor)
     mats = [matrices] if one else list(matrices)
     trace("orthogonalize", [tuple(getattr(m, "shape", ())) for m in mats])
