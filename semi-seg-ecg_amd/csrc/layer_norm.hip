@@ -6,7 +6,7 @@
 // Both passes are bound by HBM: forward reads x and writes y, backward reads x and dy and writes dx - each byte once.  32768 x 4096
 // bf16: 103 us and 177 us (5.2 and 4.6 TB/s; a large copy reaches 5.0), and 5 us for the parameters' gradients.  Below a few
 // megabytes latency counts: 1008 x 512 fp32 takes 3.9 us, and 5.9 + 4.6 us backward.  Rows beyond the registers (below) run at 1.0 to
-// 2.7 TB/s.  A row stays in the registers of the threads
+// 2.8 TB/s.  A row stays in the registers of the threads
 // that own it (64 to 1024 of them), so the variance is the two-pass one (the sum of squared differences from the mean, no
 // cancellation) without a second read.  The differences are summed beside their squares and correct the mean: a sum's roundings leave
 // it a few steps of x off, which for rows of nearly equal large values is as much as they differ (a constant row gave 0.93
@@ -391,7 +391,7 @@ __global__ __launch_bounds__(1024) void ln_param_grads_kernel(const float* __res
 // Threads per row and 16-byte vectors per thread: the fewest threads whose registers hold the row beside the parameters (and, in the
 // backward pass, the column sums and the next row: 128 registers a thread at 1024 threads).  One wave per row needs no barrier.
 // Longer rows take the kernels that read a row two or three times.  Those cost 131 us forward and 155 us backward at 2000 x 16384
-// bf16 where the registers take 26 and 114 (with 141 values spilled); at 2000 x 16384 fp32 they take 153 us backward, where four
+// bf16 where the registers take 30 and 97 (with 141 values spilled); at 2000 x 16384 fp32 they take 152 us backward, where four
 // vectors a thread (251 spilled) took 181.
 struct LnShape { int tpr, nch; };
 inline LnShape ln_shape(int C, int V, bool bwd) {
