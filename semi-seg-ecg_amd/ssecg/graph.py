@@ -67,7 +67,7 @@ def _nccl_group_active() -> bool:
         return True
 
 
-_WORDS = 512  # 8-byte words per block (4 KB): an AdamW group takes 5, a seed or a learning rate 1 - ~100 param groups
+_WORDS = 512  # 8-byte words per block (4 KB): an AdamW group takes 5, a Muon group 3 more, a seed or a learning rate 1 - ~100 param groups
 _TABLE_WORDS = 1 << 15   # int64 words for the pointer tables built during the capture (a ResNet18 step needs ~2 k)
 
 
